@@ -117,6 +117,40 @@ int wq8_gemv_lines(const void* x, int64_t ldx, const int8_t* w, const float* sw,
 int wq8_gemv_line_act(const void* x, int act, const void* act_weight, float eps, const int8_t* w, const float* sw, const void* bias,
                       const void* residual, const void* rscale, void* y, int n, int k, int dtype, wq8_stream_t stream);
 
+/* Rotary positions, no counterpart in the reference. count (1 to 4) tensors of rows (tokens, heads, head_dim) of one dtype (0-2), unit
+ * channel stride, 16-byte aligned rows: shapes holds per tensor {heads, token stride and head stride of x, of y} in elements (xs, ys
+ * and shapes are host arrays); ys[i] may be xs[i]. positions: int32, or int64 with wide, element (token, axis) at token *
+ * pos_token + axis * pos_axis. Pair i (of pairs; 2 pairs <= head_dim, a multiple of 8) turns by position * turns[i] / 2^64 turns, position
+ * on axis[i] (int32); style 0: channels 2 i, 2 i + 1; 1: i, i + pairs; the others are copied. inverse turns back. */
+int wq8_rotary(const void* const* xs, void* const* ys, const long long* shapes, int count, const void* positions, int64_t pos_token, int64_t pos_axis,
+               int wide, int64_t tokens, const long long* turns, const void* axis, int pairs, int head_dim, int style, int inverse, int dtype,
+               wq8_stream_t stream);
+
+/* The paged 8-bit key/value cache, no counterpart in the reference: codes (pages, heads, block, head_dim) int8, scales (pages, heads) f32.
+ * kv_plan: past, fresh (requests) and pages (pages_count), used (1) int32; tables rows of `width` int32, table_stride apart, completed in
+ * place; slots and positions (tokens), starts (requests + 1), lens (requests), used_out and missing (1) are written. */
+int wq8_kv_plan(const void* past, const void* fresh, int32_t* tables, int64_t table_stride, const void* pages, int pages_count, const void* used,
+                int requests, int width, int block, int64_t tokens, int64_t* slots, int32_t* positions, int32_t* starts, int32_t* lens, int32_t* used_out,
+                int32_t* missing, wq8_stream_t stream);
+
+/* Rows (tokens, heads, head_dim) of dtype 0-2 into the cache at slots; strides (host): {token, head} of k, of v, in elements; rows 16-byte
+ * aligned; block up to 128, head_dim a multiple of 8 up to 1024; owner: pages * block int32 of scratch, never cleared. */
+int wq8_kv_write(const void* k, const void* v, const long long* strides, const long long* slots, int64_t tokens, int8_t* k_codes, float* k_scales,
+                 int8_t* v_codes, float* v_scales, int64_t pages, int heads, int block, int head_dim, int dtype, int32_t* owner, wq8_stream_t stream);
+
+/* The values at slots: k, v (tokens, heads, head_dim) contiguous, of dtype 0-2; zeros for slots outside the cache. */
+int wq8_kv_read(const int8_t* k_codes, const float* k_scales, const int8_t* v_codes, const float* v_scales, const long long* slots, int64_t tokens, void* k,
+                void* v, int64_t pages, int heads, int block, int head_dim, int dtype, wq8_stream_t stream);
+
+/* Attention of q (tokens, heads * group, head_dim), dtype 0-1, over the cache: request r has rows starts[r] to starts[r + 1] and the
+ * first lens[r] tokens of its row of tables (int32; width entries, table_stride apart); strides (host): {token, head} of q, of out;
+ * head_dim 64, 128 or 256; block 16, 32, 64 or 128; workspace: of the bytes that the query gives for `keys` = width * block (sizes[1] is 0). */
+int wq8_kv_attention(const void* q, void* out, const long long* strides, const int8_t* k_codes, const float* k_scales, const int8_t* v_codes,
+                     const float* v_scales, const void* tables, int64_t table_stride, int width, const void* lens, const void* starts, int tokens,
+                     int requests, int heads, int group, int head_dim, int block, int64_t pages, float scale, int causal, int window, int dtype, int sms,
+                     void* workspace, wq8_stream_t stream);
+void wq8_kv_attention_workspace(int tokens, int requests, int heads, int group, int head_dim, int64_t keys, int sms, int64_t* sizes);
+
 /* Cold-cache timing: reads `bytes` of a library-owned buffer on `stream` (nonzero if it cannot be allocated);
  * release frees it. Replace K8:1997-2016; bound at I:77-78. */
 int wq8_l2_flush(int device, int64_t bytes, wq8_stream_t stream);

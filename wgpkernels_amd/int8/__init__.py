@@ -19,6 +19,10 @@ Paths:
 - 'block': one INT8 pass, one FP32 scale per token and 128-element K block.
 - 'row': one scale per token (W8A8), on request only.
 linear() picks a path per GPU, shape and token-count bucket by timing the candidates once (see choose_path()).
+
+Next to the linears stands the attention side of a step (no counterpart in the reference): rotary() turns queries and keys
+by positions on one to three axes (_rotary.py), and a paged cache holds keys and values in 8 bits (_kvcache.py): kv_plan(),
+kv_write(), kv_read(), kv_attention().
 """
 import ctypes
 import functools
@@ -611,4 +615,6 @@ def linear(x, weight, scale, bias=None, group=0, precise=False, mode=None, act=N
     return _run_path(path, x, weight, scale, bias, group, act, act_weight, eps, residual, residual_scale, out)
 
 
+from ._rotary import RotaryPlan, rotary, rotary_plan  # noqa: E402,F401
+from ._kvcache import KVCache, KVPlan, kv_attention, kv_plan, kv_read, kv_write  # noqa: E402,F401
 from ._selftest import reference_linear as _reference, reference_rotation as _reference_rotation, selftest  # noqa: E402,F401

@@ -1,0 +1,194 @@
+"""The paged 8-bit key/value cache on MI355X: planned on the GPU from request lengths, written, read and attended over.
+
+Keys and values are held as INT8 codes (pages, heads, block, head_dim) with one FP32 scale per page and head: a value is
+code * scale, scale = the largest magnitude of the page's tokens / 127. A slot is page * block + the place in the page. A
+request's tokens lie on the pages that its row of a block table names, in order.
+
+    plan = kv_plan(past, new, tables, free, used, block, tokens)      # slots, positions, block tables of a step
+    kv_write(cache, k, v, plan.slots)                                  # append the step's keys and values
+    out = kv_attention(q, cache, tables, plan.lens, plan.starts)       # the step's queries over the cache
+
+None of these waits for the GPU or reads lengths on the host: a step can be captured in a HIP graph.
+"""
+import ctypes
+from typing import NamedTuple
+
+import torch
+
+from . import DTYPES, _native, library
+from ._rotary import _check_device, _check_rows
+
+BLOCKS = (16, 32, 64, 128)
+ATTENTION_HEAD_DIMS = (64, 128, 256)
+
+
+class KVPlan(NamedTuple):
+    """What kv_plan() gives for a step of `tokens` tokens and R requests."""
+    slots: torch.Tensor      # (tokens,) int64: where each token goes, -1 for those that go nowhere
+    positions: torch.Tensor  # (tokens,) int32: its position in its request
+    starts: torch.Tensor     # (R + 1,) int32: each request's first token in the step
+    lens: torch.Tensor       # (R,) int32: each request's length after the step
+    used: torch.Tensor       # (1,) int32: pages of the free list taken so far
+    missing: torch.Tensor    # (1,) int32: requests that found no room
+
+
+class KVCache:
+    """An empty cache of `pages` pages of `block` tokens (16, 32, 64 or 128) on a GPU."""
+    __slots__ = ("k_codes", "k_scales", "v_codes", "v_scales", "owner")
+
+    def __init__(self, pages, heads, head_dim, block=64, device="cuda"):
+        codes = lambda: torch.zeros(pages, heads, block, head_dim, dtype=torch.int8, device=device)
+        scales = lambda: torch.zeros(pages, heads, dtype=torch.float32, device=device)
+        self._take(codes(), scales(), codes(), scales())
+
+    @classmethod
+    def from_codes(cls, k_codes, k_scales, v_codes, v_scales):
+        """A cache over existing codes (pages, heads, block, head_dim) int8 and scales (pages, heads) float32, not copied. Scales
+        are finite and not negative; where one is zero, so are its codes."""
+        cache = cls.__new__(cls)
+        cache._take(k_codes, k_scales, v_codes, v_scales)
+        return cache
+
+    def _take(self, k_codes, k_scales, v_codes, v_scales):
+        if k_codes.dim() != 4 or k_codes.shape != v_codes.shape or k_codes.shape[2] not in BLOCKS or k_codes.shape[3] % 8 or not 8 <= k_codes.shape[3] <= 1024:
+            raise ValueError(f"cache codes must be (pages, heads, {' / '.join(map(str, BLOCKS))} tokens, a multiple of 8 channels), the same for keys and values")
+        if k_codes.dtype != torch.int8 or v_codes.dtype != torch.int8 or k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32:
+            raise ValueError("cache codes must be INT8, their scales FP32")
+        if k_scales.shape != k_codes.shape[:2] or v_scales.shape != k_codes.shape[:2]:
+            raise ValueError("cache scales must be (pages, heads)")
+        parts = (k_codes, k_scales, v_codes, v_scales)
+        if not all(t.is_contiguous() for t in parts) or k_codes.data_ptr() % 16 or v_codes.data_ptr() % 16:
+            raise ValueError("cache codes and scales must be contiguous, the codes 16-byte aligned")
+        if any(t.device != k_codes.device for t in parts):
+            raise ValueError("cache codes and scales must be on one device")
+        self.k_codes, self.k_scales, self.v_codes, self.v_scales = parts
+        # which token of a kv_write() call each slot takes: scratch of that call (entries are checked, never cleared)
+        self.owner = torch.empty(k_codes.shape[0] * k_codes.shape[2], dtype=torch.int32, device=k_codes.device)
+
+    pages = property(lambda self: self.k_codes.shape[0])
+    heads = property(lambda self: self.k_codes.shape[1])
+    block = property(lambda self: self.k_codes.shape[2])
+    head_dim = property(lambda self: self.k_codes.shape[3])
+
+
+def _check_ints(t, name, dtype=torch.int32, dim=1):
+    if t.dtype != dtype or t.dim() != dim or (t.numel() and not t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous {dim}-D {str(dtype).removeprefix('torch.')} tensor")
+
+
+def _check_tables(tables):
+    if tables.dtype != torch.int32 or tables.dim() != 2 or (tables.shape[1] > 1 and tables.stride(1) != 1):
+        raise ValueError("block tables must be (requests, pages) int32 with unit column stride")
+
+
+def kv_plan(past, new, tables, free, used, block, tokens):
+    """Slots, positions and block tables of a step in which request r, with past[r] tokens cached, brings new[r] more: new tokens
+    stand one request after another in rows of the step's `tokens` (padding beyond their sum gets slot -1, position 0).
+
+    past, new: (R,) int32 (negative counts as 0). tables: (R, width) int32, completed in place with the pages that the new tokens
+    begin: free[used], free[used + 1], ... in the order of requests and tokens. free: (F,) int32; used: (1,) int32. A request that
+    the table's width, `tokens` or the free pages left cannot hold gets no page, slots -1 and its old length, and so does
+    every later one that needs a page where the free list ran out. Everything is int32 / int64 on the GPU; nothing is read
+    on the host."""
+    _check_ints(past, "past")
+    _check_ints(new, "new")
+    _check_ints(free, "free")
+    _check_tables(tables)
+    if used.dtype != torch.int32 or used.numel() != 1:
+        raise ValueError("used must be one int32")
+    requests = past.shape[0]
+    if new.shape[0] != requests or tables.shape[0] != requests:
+        raise ValueError(f"past, new and tables must be of as many requests, not {requests}, {new.shape[0]} and {tables.shape[0]}")
+    if block < 1 or not 0 <= tokens < 2 ** 31:
+        raise ValueError("a block of at least one token and a token count are wanted")
+    _check_device(past.get_device(), new=new, tables=tables, free=free, used=used)
+    state = _native.gpu(past)
+    slots = torch.empty(tokens, dtype=torch.int64, device=past.device)
+    positions, starts, lens, used_out, missing = torch.empty(tokens + 2 * requests + 3, dtype=torch.int32, device=past.device).split(
+        [tokens, requests + 1, requests, 1, 1])
+    library().call("wq8_kv_plan", past.data_ptr(), new.data_ptr(), tables.data_ptr(), tables.stride(0), free.data_ptr(), free.shape[0], used.data_ptr(),
+                   requests, tables.shape[1], block, tokens, slots.data_ptr(), positions.data_ptr(), starts.data_ptr(), lens.data_ptr(),
+                   used_out.data_ptr(), missing.data_ptr(), state.stream())
+    return KVPlan(slots, positions, starts, lens, used_out, missing)
+
+
+def kv_write(cache, k, v, slots):
+    """Keys and values (tokens, heads, head_dim), BF16, FP16 or FP32, into the cache at `slots` (int64; any order, each at most once;
+    those outside the cache, as -1, are left out). A page's scale grows to its largest value, and tokens that it holds are then
+    coded again; a write to its first slot begins it anew. NaN is held as 0 and infinities as the largest finite number."""
+    _check_rows(k, "keys")
+    _check_rows(v, "values")
+    _check_ints(slots, "slots", torch.int64)
+    codes = cache.k_codes
+    pages, heads, block, head_dim = codes.shape
+    if k.shape != v.shape or k.dtype != v.dtype or k.shape[1:] != (heads, head_dim) or slots.shape[0] != k.shape[0]:
+        raise ValueError(f"keys and values must be (tokens, {heads}, {head_dim}), of one type, with a slot each")
+    device = codes.get_device()
+    _check_device(device, keys=k, values=v, slots=slots)
+    sk, sv = k.stride(), v.stride()
+    library().call("wq8_kv_write", k.data_ptr(), v.data_ptr(), (ctypes.c_longlong * 4)(sk[0], sk[1], sv[0], sv[1]), slots.data_ptr(), k.shape[0],
+                   codes.data_ptr(), cache.k_scales.data_ptr(), cache.v_codes.data_ptr(), cache.v_scales.data_ptr(), pages, heads, block, head_dim,
+                   DTYPES[k.dtype], cache.owner.data_ptr(), _native.gpu(codes).stream())
+
+
+def kv_read(cache, slots, dtype=torch.bfloat16):
+    """The keys and values at `slots` (int64; zeros outside the cache), rounded once to dtype: two (tokens, heads, head_dim) tensors."""
+    _check_ints(slots, "slots", torch.int64)
+    if dtype not in DTYPES:
+        raise ValueError(f"dtype must be FP16, BF16 or FP32, not {dtype}")
+    codes = cache.k_codes
+    pages, heads, block, head_dim = codes.shape
+    _check_device(codes.get_device(), slots=slots)
+    tokens = slots.shape[0]
+    k, v = (torch.empty(tokens, heads, head_dim, dtype=dtype, device=codes.device) for _ in range(2))
+    library().call("wq8_kv_read", codes.data_ptr(), cache.k_scales.data_ptr(), cache.v_codes.data_ptr(), cache.v_scales.data_ptr(), slots.data_ptr(), tokens,
+                   k.data_ptr(), v.data_ptr(), pages, heads, block, head_dim, DTYPES[dtype], _native.gpu(codes).stream())
+    return k, v
+
+
+_sizes = (ctypes.c_int64 * 2)()
+
+
+def kv_attention(q, cache, tables, lens, starts, causal=True, window=0, scale=None, out=None):
+    """Attention of the step's queries over the cache: q (tokens, query heads, head_dim) BF16 or FP16, head_dim 64, 128 or 256, each key/value
+    head serving query heads / heads of them, in order. Request r owns rows starts[r] to starts[r + 1] (int32, not
+    decreasing) and sees the first lens[r] (int32) tokens of its row of `tables`, its own rows being the last of them.
+
+    causal: a row sees the tokens up to itself, otherwise all of its request's; window > 0: of those, the ones after
+    position - window. scale: of the scores, 1 / sqrt(head_dim) by default. Rows that see nothing are zero; pages outside the cache are
+    hidden; rows of no request are not written. Returns (tokens, query heads, head_dim) in q's dtype. Sums and the softmax's
+    statistics are FP32, its weights FP16 relative to the largest."""
+    _check_rows(q, "queries")
+    _check_ints(lens, "lens")
+    _check_ints(starts, "starts")
+    _check_tables(tables)
+    codes = cache.k_codes
+    pages, heads, block, head_dim = codes.shape
+    tokens, q_heads, width = q.shape
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"queries must be FP16 or BF16, not {q.dtype}")
+    if width != head_dim or head_dim not in ATTENTION_HEAD_DIMS or not q_heads or q_heads % heads:
+        raise ValueError(f"queries must have heads of {head_dim} channels ({', '.join(map(str, ATTENTION_HEAD_DIMS))}), a multiple of the cache's {heads}")
+    requests = lens.shape[0]
+    if tables.shape[0] != requests or starts.shape[0] != requests + 1:
+        raise ValueError(f"tables and starts must be of {requests} requests")
+    if window < 0 or window >= 2 ** 31:
+        raise ValueError("the window must not be negative")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _check_rows(out, "outputs")
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError("outputs do not match the queries")
+    device = codes.get_device()
+    _check_device(device, queries=q, tables=tables, lens=lens, starts=starts, outputs=out)
+    lib, state = library(), _native.gpu(codes)
+    group, columns = q_heads // heads, tables.shape[1]
+    lib.wq8_kv_attention_workspace(tokens, requests, heads, group, head_dim, columns * block, state.cus, _sizes)
+    workspace = torch.empty(_sizes[0], dtype=torch.uint8, device=q.device) if _sizes[0] else None
+    sq, so = q.stride(), out.stride()
+    lib.call("wq8_kv_attention", q.data_ptr(), out.data_ptr(), (ctypes.c_longlong * 4)(sq[0], sq[1], so[0], so[1]), codes.data_ptr(), cache.k_scales.data_ptr(),
+             cache.v_codes.data_ptr(), cache.v_scales.data_ptr(), tables.data_ptr(), tables.stride(0), columns, lens.data_ptr(), starts.data_ptr(), tokens,
+             requests, heads, group, head_dim, block, pages, head_dim ** -0.5 if scale is None else scale, causal, window, DTYPES[q.dtype], state.cus,
+             _native.ptr(workspace), state.stream())
+    return out

@@ -38,11 +38,18 @@ SIGNATURES = {
     "wq8_small_workspace": ("-", "iiii" "p"),
     "wq8_gemv_lines": ("i", "plpppppp" "iiii" "p"),
     "wq8_gemv_line_act": ("i", "pipf" "pppppp" "iii" "p"),
+    "wq8_rotary": ("i", "pppi" "plli" "l" "pp" "iiiii" "p"),
+    "wq8_kv_plan": ("i", "ppplpip" "iiil" "pppppp" "p"),
+    "wq8_kv_write": ("i", "pppp" "lpppp" "liiii" "pp"),
+    "wq8_kv_read": ("i", "ppppp" "lpp" "liiii" "p"),
+    "wq8_kv_attention": ("i", "ppp" "pppp" "plipp" "iiiiiil" "fiii" "ip" "p"),
+    "wq8_kv_attention_workspace": ("-", "iiiii" "li" "p"),
     "wq8_l2_flush": ("i", "il" "p"),
     "wq8_l2_flush_release": ("-", ""),
 }
 # entry points an older or foreign build may lack: bound when present (segments_supported() reports the first)
-OPTIONAL = {"wq8_gemm_segments", "wq8_gemm_noalloc", "wq8_quantize_at", "wq8_quantize_blocks_at", "wq8_gemm_at", "wq8_gemv_line_act"}
+OPTIONAL = {"wq8_gemm_segments", "wq8_gemm_noalloc", "wq8_quantize_at", "wq8_quantize_blocks_at", "wq8_gemm_at", "wq8_gemv_line_act",
+            "wq8_rotary", "wq8_kv_plan", "wq8_kv_write", "wq8_kv_read", "wq8_kv_attention", "wq8_kv_attention_workspace"}
 # the test library's entry points (include/wq8_test.h; libwgp_int8_test.so, not part of the product library)
 TEST_SIGNATURES = {
     "wq8_debug_block_sums": ("i", "ppp" "iii" "i" "p"),
@@ -85,7 +92,10 @@ class Library:
 
     def call(self, name, *args):
         """Calls entry point `name`; a nonzero return raises RuntimeError (there is no fallback path)."""
-        code = getattr(self, name)(*args)
+        fn = getattr(self, name, None)
+        if fn is None:
+            raise RuntimeError(f"INT8 library {self.path} lacks {name}; rebuild it")
+        code = fn(*args)
         if code:
             raise_code(code, name)
 

@@ -1,0 +1,120 @@
+"""Rotary positions with one or several axes on MI355X: the queries and keys of one projection rotated in one launch.
+
+Channels come in pairs (a, b) that turn by the angle position * frequency,
+
+    a' = a cos - b sin,   b' = a sin + b cos,
+
+where every pair belongs to one of up to three axes (time, height, width) and takes that axis's position. Turning back
+(inverse=True) is the transpose: it is also the gradient of a rotation with respect to its input.
+"""
+import ctypes
+import math
+
+import torch
+
+from . import DTYPES, _native, library
+
+STYLES = {"pairs": 0, "halves": 1}
+MAX_AXES, MAX_TENSORS = 3, 4
+
+
+class RotaryPlan:
+    """Which pairs turn, about which axis and how fast, on one GPU (rotary_plan()). Made once per model."""
+    __slots__ = ("sections", "style", "pairs", "turns", "axis")
+
+    def __init__(self, sections, style, turns, axis):
+        self.sections, self.style, self.pairs, self.turns, self.axis = sections, style, sum(sections), turns, axis
+
+
+def rotary_plan(sections, ladder="axis", style="pairs", base=10000.0, frequencies=None, device="cuda"):
+    """A plan of sum(sections) rotated pairs a head, sections[a] of them on axis a, in that order.
+
+    ladder 'axis': pair i of a section of n turns by base ** (-i / n) a position, each axis with a ladder of its own; 'joint':
+    pair i of all n by base ** (-i / n), one ladder cut into the sections. frequencies (one a pair) replaces both.
+    style 'pairs': pair i is channels 2 i and 2 i + 1; 'halves': channels i and i + sum(sections). Channels past the
+    rotated ones pass through."""
+    sections = tuple(int(s) for s in sections)
+    pairs = sum(sections)
+    if not 1 <= len(sections) <= MAX_AXES or min(sections) < 1:
+        raise ValueError(f"rotary sections must be 1 to {MAX_AXES} positive pair counts, not {sections}")
+    if style not in STYLES:
+        raise ValueError(f"unknown rotary style {style!r}")
+    if frequencies is not None:
+        frequencies = [float(f) for f in frequencies]
+        if len(frequencies) != pairs or not all(map(math.isfinite, frequencies)):
+            raise ValueError(f"{pairs} finite rotary frequencies are wanted, one a pair")
+    else:
+        if ladder not in ("axis", "joint"):
+            raise ValueError(f"unknown rotary ladder {ladder!r}")
+        if not (base > 0 and math.isfinite(base)):
+            raise ValueError("the rotary base must be positive and finite")
+        steps = [i / n for n in sections for i in range(n)] if ladder == "axis" else [i / pairs for i in range(pairs)]
+        frequencies = [float(base) ** -s for s in steps]
+    # turns a position, modulo one, as a fraction of 2^64 in two's complement: a position times it wraps at whole turns
+    turns = [round(math.fmod(f / (2 * math.pi), 1.0) * 2.0 ** 64) for f in frequencies]
+    turns = [(t + 2 ** 63) % 2 ** 64 - 2 ** 63 for t in turns]
+    axis = [a for a, n in enumerate(sections) for _ in range(n)]
+    return RotaryPlan(sections, style, torch.tensor(turns, dtype=torch.int64, device=device), torch.tensor(axis, dtype=torch.int32, device=device))
+
+
+def _check_rows(x, name):
+    """(token, head, channel) rows with unit channel stride, 16-byte aligned, heads of a multiple of 8 channels."""
+    if x.dim() != 3 or (x.shape[2] > 1 and x.stride(2) != 1):
+        raise ValueError(f"{name} must be (tokens, heads, channels) with unit channel stride")
+    if x.dtype not in DTYPES:
+        raise ValueError(f"{name} must be FP16, BF16 or FP32, not {x.dtype}")
+    if x.shape[2] % 8:
+        raise ValueError(f"{name} must have heads of a multiple of 8 channels, not {x.shape[2]}")
+    size = x.element_size()
+    if (x.data_ptr() % 16 or (x.shape[0] > 1 and x.stride(0) * size % 16) or (x.shape[1] > 1 and x.stride(1) * size % 16)):
+        raise ValueError(f"rows of {name} must be 16-byte aligned")
+
+
+def _check_device(device, **tensors):
+    """Every tensor on GPU `device` (an index; the kernels take raw pointers)."""
+    if device < 0:
+        raise ValueError("tensors must be on the GPU")
+    for name, t in tensors.items():
+        if t.get_device() != device:
+            raise ValueError(f"{name} must be on the same GPU as the other tensors")
+
+
+def rotary(xs, positions, plan, inverse=False, out=None):
+    """Rows (tokens, heads, head_dim) of BF16, FP16 or FP32 turned by their positions: a tensor, or a tuple of up to four of one
+    type, token count and head width (queries and keys; views of a packed projection). positions: (tokens, axes) int32 or
+    int64, or (tokens,) with one axis; any value. inverse turns back. Angles are exact at far positions: they are reduced to
+    parts of a turn as 64-bit integers. out: tensors of the same shapes, which may be the inputs themselves and overlap
+    them in no other way."""
+    many = not isinstance(xs, torch.Tensor)
+    tensors = tuple(xs) if many else (xs,)
+    if not 1 <= len(tensors) <= MAX_TENSORS:
+        raise ValueError(f"rotary takes 1 to {MAX_TENSORS} tensors")
+    outs = tuple(torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in tensors) if out is None else (tuple(out) if many else (out,))
+    if len(outs) != len(tensors):
+        raise ValueError("rotary outputs do not match its inputs")
+    first = tensors[0]
+    shapes = []
+    for x, y in zip(tensors, outs):
+        _check_rows(x, "rotary rows")
+        if x.dtype != first.dtype or x.shape[0] != first.shape[0] or x.shape[2] != first.shape[2]:
+            raise ValueError("rotary tensors must agree in type, tokens and head width")
+        if out is not None:
+            _check_rows(y, "rotary outputs")
+            if y.shape != x.shape or y.dtype != x.dtype:
+                raise ValueError("rotary outputs do not match its inputs")
+        sx, sy = x.stride(), y.stride()
+        shapes += (x.shape[1], sx[0], sx[1], sy[0], sy[1])
+    tokens, _, head_dim = first.shape
+    axes = len(plan.sections)
+    if 2 * plan.pairs > head_dim:
+        raise ValueError(f"the plan turns {2 * plan.pairs} channels, the heads have {head_dim}")
+    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in ((tokens, axes), (tokens,) if axes == 1 else (tokens, axes)):
+        raise ValueError(f"rotary positions must be ({tokens}, {axes}) int32 or int64, not {tuple(positions.shape)} {positions.dtype}")
+    _check_device(first.get_device(), positions=positions, plan=plan.turns, **{f"rows {i}": t for i, t in enumerate(tensors + outs)})
+    count = len(tensors)
+    pointers = ctypes.c_void_p * count
+    library().call("wq8_rotary", pointers(*[x.data_ptr() for x in tensors]), pointers(*[y.data_ptr() for y in outs]), (ctypes.c_longlong * (5 * count))(*shapes),
+                   count, positions.data_ptr(), positions.stride(0), positions.stride(1) if positions.dim() == 2 else 0, positions.dtype == torch.int64,
+                   tokens, plan.turns.data_ptr(), plan.axis.data_ptr(), plan.pairs, head_dim, STYLES[plan.style], inverse, DTYPES[first.dtype],
+                   _native.gpu(first).stream())
+    return outs if many else outs[0]

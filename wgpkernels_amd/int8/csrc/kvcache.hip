@@ -1,0 +1,349 @@
+// The paged 8-bit key/value cache on gfx950: block tables and slots from request lengths, writes, and reads.
+//
+// Codes (pages, heads, block, head_dim) int8 and one FP32 scale per (page, head): value = code * scale, scale = amax / 127
+// over the page's tokens. Slot s is token s % block of page s / block.
+#include "wq8_common.h"
+#include "wq8_abi.h"
+#include <algorithm>
+
+namespace wq8 {
+
+// ---- block tables and slots ----------------------------------------------------------------------------------------
+struct PlanArgs {
+    const int *past, *fresh, *pages, *used;
+    int* tables;
+    int64_t table_stride, tokens;
+    int pages_count, requests, width, block;
+    int64_t* slots;
+    int *positions, *starts, *lens, *used_out, *missing;
+};
+
+WQ8_DEVICE int64_t scan256(int64_t v, int64_t* lds4, int64_t& total) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int64_t o = __shfl_up(v, d);
+        if (int(threadIdx.x & 63) >= d) v += o;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) lds4[threadIdx.x >> 6] = v;
+    __syncthreads();
+    int64_t before = 0;
+    total = 0;
+    for (int w = 0; w < 4; ++w) {
+        if (w < int(threadIdx.x >> 6)) before += lds4[w];
+        total += lds4[w];
+    }
+    return v + before;
+}
+
+// Pages in order of the free list: requests in order, each taking ceil((past + new) / block) - ceil(past / block). A request
+// that the tokens, its table's width or the free pages cannot hold takes none; nor then does any later one that needs pages.
+// Every workgroup walks the requests, 256 at a time, and serves PLAN_TOKENS tokens: the walk is a few hundred
+// nanoseconds, less than a launch of its own. A page's first token writes its table entry.
+constexpr int PLAN_TOKENS = 1024;
+__global__ void __launch_bounds__(256) kv_plan_tokens(PlanArgs p) {
+    __shared__ int64_t lds4[4], ends[256];
+    __shared__ int64_t source[256];  // free-list index of the request's first new page
+    __shared__ int pasts[256], oks[256], haves[256];
+    const int64_t t0 = blockIdx.x * int64_t(PLAN_TOKENS), t1 = min(p.tokens, t0 + PLAN_TOKENS);
+    const int tid = threadIdx.x;
+    const int64_t used = *p.used;
+    int64_t upto_ends = 0, upto_need = 0, granted = 0, refused = 0;
+    for (int base = 0; base < p.requests; base += 256) {
+        const int r = base + tid;
+        const bool live = r < p.requests;
+        const int64_t past = live ? max(0, p.past[r]) : 0, fresh = live ? max(0, p.fresh[r]) : 0;
+        const int64_t have = (past + p.block - 1) / p.block, want = (past + fresh + p.block - 1) / p.block;
+        int64_t total;
+        const int64_t end = upto_ends + scan256(fresh, lds4, total);
+        const bool fits = live && want <= p.width && end <= p.tokens;
+        const int64_t need = fits ? want - have : 0;
+        int64_t total_need;
+        const int64_t upto = upto_need + scan256(need, lds4, total_need);
+        const bool ok = fits && (!need || (used + upto <= p.pages_count && used + upto - need >= 0));
+        ends[tid] = end;
+        source[tid] = used + upto - need;
+        pasts[tid] = int(past);
+        haves[tid] = int(have);
+        oks[tid] = ok;
+        __syncthreads();
+        if (blockIdx.x == 0 && live) {
+            if (!r) p.starts[0] = 0;
+            p.starts[r + 1] = int(min(end, p.tokens));
+            p.lens[r] = int(ok ? past + fresh : past);
+            granted += ok ? need : 0;
+            refused += !ok;
+        }
+        const int count = min(256, p.requests - base);
+        const int64_t low = max(t0, upto_ends), high = min(t1, upto_ends + total);
+        for (int64_t t = low + tid; t < high; t += 256) {
+            int a = 0, b = count - 1;  // the first request whose end is past t
+            while (a < b) {
+                const int m = (a + b) >> 1;
+                if (ends[m] > t) b = m; else a = m + 1;
+            }
+            const int64_t begin = a ? ends[a - 1] : upto_ends;
+            const int64_t position = pasts[a] + (t - begin);
+            int64_t slot = -1;
+            if (oks[a]) {
+                const int64_t column = position / p.block;
+                int* entry = p.tables + (base + a) * p.table_stride + column;
+                int page;
+                if (column >= haves[a]) {
+                    page = p.pages[source[a] + column - haves[a]];
+                    if (position % p.block == 0) *entry = page;
+                } else {
+                    page = *entry;
+                }
+                slot = int64_t(page) * p.block + position % p.block;
+            }
+            p.slots[t] = slot;
+            p.positions[t] = int(position);
+        }
+        upto_ends += total;
+        upto_need += total_need;
+        __syncthreads();
+    }
+    for (int64_t t = max(t0, upto_ends) + tid; t < t1; t += 256) {  // tokens of no request
+        p.slots[t] = -1;
+        p.positions[t] = 0;
+    }
+    if (blockIdx.x == 0) {
+        int64_t total_granted, total_refused;
+        scan256(granted, lds4, total_granted);
+        scan256(refused, lds4, total_refused);
+        if (!tid) {
+            if (!p.requests) p.starts[0] = 0;
+            *p.used_out = int(used + total_granted);
+            *p.missing = int(total_refused);
+        }
+    }
+}
+
+// ---- writes --------------------------------------------------------------------------------------------------------
+struct CacheArgs {
+    const void* x[2];          // keys, values (token, head, channel)
+    void* y[2];                // reads: outputs (token, head, channel), contiguous
+    int64_t token_stride[2], head_stride[2];
+    int8_t* codes[2];
+    float* scales[2];
+    const int64_t* slots;
+    int* owner;
+    int64_t tokens, pages;
+    int heads, block, head_dim;
+};
+
+// owner[slot] = the token written there. Nothing clears it: an entry holds if it names a token of this call whose slot it is,
+// which an entry of another call only does where it happens to be right.
+__global__ void __launch_bounds__(256) kv_owner(CacheArgs p) {
+    const int64_t t = blockIdx.x * int64_t(256) + threadIdx.x;
+    if (t >= p.tokens) return;
+    const int64_t slot = p.slots[t];
+    if (slot >= 0 && slot < p.pages * p.block) p.owner[slot] = int(t);
+}
+
+// A finite value for the cache: NaN counts as zero, infinities as the largest finite number (a few steps below it: 127 times the
+// rounded scale has to stay finite), so that one bad token does not turn its page's other tokens into NaN.
+WQ8_DEVICE float cached_value(float v) {
+    constexpr float MOST = 0x1.fffff8p+127f;
+    return v != v ? 0.0f : fminf(fmaxf(v, -MOST), MOST);
+}
+
+// round(v / scale), inv = 1 / scale: v * inv with one correction by the remainder, so that the quotient is within an ulp and
+// codes differ from those of an exact division only where v lies within that of a tie. Scales below 2^-120, whose inverse may
+// overflow, divide.
+WQ8_DEVICE int code_of(float v, float scale, float inv) {
+    float q = v * inv;
+    q = scale < 0x1p-120f ? v / scale : __builtin_fmaf(__builtin_fmaf(-q, scale, v), inv, q);
+    return rne_int(__builtin_amdgcn_fmed3f(q, -127.0f, 127.0f));
+}
+
+WQ8_DEVICE float block_max(float v, float* lds4) {
+    v = wave_max(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds4[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return fmaxf(fmaxf(lds4[0], lds4[1]), fmaxf(lds4[2], lds4[3]));
+}
+
+// One page and head: rows[] names the token of each of its slots that is written, -1 for the others. The scale becomes the larger
+// of the held one (none when the page's first slot is written: the page begins anew) and the new tokens' amax / 127; tokens
+// that the page held are coded again where it grew.
+template <int DT> WQ8_DEVICE void write_page(const CacheArgs& p, int which, int64_t page, int head, const int* rows, float* lds4) {
+    using raw = typename Elem<DT>::raw;
+    const int per_row = p.head_dim >> 3, items = p.block * per_row;
+    const raw* x = static_cast<const raw*>(p.x[which]) + head * p.head_stride[which];
+    float amax = 0.0f;
+    for (int i = threadIdx.x; i < items; i += 256) {
+        const int r = i / per_row, t = rows[r];
+        if (t < 0) continue;
+        float v[8];
+        load8<DT>(x + t * p.token_stride[which] + 8 * (i - r * per_row), v, true);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, __builtin_fabsf(cached_value(v[j])));
+    }
+    amax = block_max(amax, lds4);
+    float* held = p.scales[which] + page * p.heads + head;
+    const float old = rows[0] >= 0 ? 0.0f : fmaxf(*held, 0.0f);
+    const float scale = fmaxf(old, div127(amax));
+    const float by = scale > 0.0f ? scale : 1.0f, inv = 1.0f / by, again = old / by;
+    int8_t* codes = p.codes[which] + (page * p.heads + head) * int64_t(p.block) * p.head_dim;
+    for (int i = threadIdx.x; i < items; i += 256) {
+        const int r = i / per_row, c = i - r * per_row, t = rows[r];
+        u32x2* at = reinterpret_cast<u32x2*>(codes + r * p.head_dim + 8 * c);
+        int q[8];
+        if (t >= 0) {
+            float v[8];
+            load8<DT>(x + t * p.token_stride[which] + 8 * c, v, true);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) q[j] = code_of(cached_value(v[j]), by, inv);
+        } else {
+            if (!(old < scale) || old == 0.0f) continue;
+            const u32x2 before = *at;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) q[j] = rne_int(float(int8_t(before[j >> 2] >> (8 * (j & 3)))) * again);
+        }
+        *at = u32x2{pack_s8x4(q[0], q[1], q[2], q[3]), pack_s8x4(q[4], q[5], q[6], q[7])};
+    }
+    __syncthreads();  // every thread has read the held scale
+    if (!threadIdx.x) *held = scale;
+}
+
+constexpr int KV_MAX_BLOCK = 128;
+// Up to this many tokens a workgroup reads every slot by itself to find its page's tokens, and the owner pass is left out.
+constexpr int KV_SCAN_TOKENS = 512;
+constexpr int KV_OWNED_TOKENS = 16;
+
+template <int DT>
+__global__ void __launch_bounds__(256) kv_write_scan(CacheArgs p) {
+    __shared__ int rows[KV_MAX_BLOCK];
+    __shared__ float lds4[4];
+    const int token = blockIdx.x, head = blockIdx.y, which = blockIdx.z;
+    const int64_t slot = p.slots[token];
+    if (slot < 0 || slot >= p.pages * p.block) return;
+    const int64_t page = slot / p.block;
+    const int at = int(slot - page * p.block);
+    for (int i = threadIdx.x; i < p.block; i += 256) rows[i] = -1;
+    __syncthreads();
+    for (int t = threadIdx.x; t < p.tokens; t += 256) {
+        const int64_t s = p.slots[t] - page * p.block;
+        if (s >= 0 && s < p.block) atomicMax(&rows[s], t);
+    }
+    __syncthreads();
+    // the page is its lowest slot's token's
+    if (rows[at] != token) return;
+    for (int i = 0; i < at; ++i)
+        if (rows[i] >= 0) return;
+    write_page<DT>(p, which, page, head, rows, lds4);
+}
+
+template <int DT>
+__global__ void __launch_bounds__(256) kv_write_owned(CacheArgs p) {
+    __shared__ int rows[KV_MAX_BLOCK];
+    __shared__ int lowest[KV_OWNED_TOKENS];
+    __shared__ float lds4[4];
+    const int head = blockIdx.y, which = blockIdx.z;
+    const auto writer = [&](int64_t slot) {
+        const int t = p.owner[slot];
+        return t >= 0 && t < p.tokens && p.slots[t] == slot ? t : -1;
+    };
+    if (threadIdx.x < KV_OWNED_TOKENS) {
+        const int64_t token = blockIdx.x * int64_t(KV_OWNED_TOKENS) + threadIdx.x;
+        int mine = 0;
+        if (token < p.tokens) {
+            const int64_t slot = p.slots[token];
+            if (slot >= 0 && slot < p.pages * p.block && writer(slot) == token) {
+                mine = 1;
+                for (int64_t s = slot - 1; s >= slot / p.block * p.block && mine; --s) mine = writer(s) < 0;
+            }
+        }
+        lowest[threadIdx.x] = mine;
+    }
+    __syncthreads();
+    for (int i = 0; i < KV_OWNED_TOKENS; ++i) {
+        if (!lowest[i]) continue;
+        const int64_t page = p.slots[blockIdx.x * int64_t(KV_OWNED_TOKENS) + i] / p.block;
+        for (int r = threadIdx.x; r < p.block; r += 256) rows[r] = writer(page * p.block + r);
+        __syncthreads();
+        write_page<DT>(p, which, page, head, rows, lds4);
+        __syncthreads();
+    }
+}
+
+template <int DT> static int launch_write(const CacheArgs& p, hipStream_t stream) {
+    if (p.tokens <= KV_SCAN_TOKENS) {
+        kv_write_scan<DT><<<dim3(unsigned(p.tokens), p.heads, 2), 256, 0, stream>>>(p);
+    } else {
+        kv_owner<<<unsigned((p.tokens + 255) / 256), 256, 0, stream>>>(p);
+        kv_write_owned<DT><<<dim3(unsigned((p.tokens + KV_OWNED_TOKENS - 1) / KV_OWNED_TOKENS), p.heads, 2), 256, 0, stream>>>(p);
+    }
+    return int(hipGetLastError());
+}
+
+// ---- reads ---------------------------------------------------------------------------------------------------------
+template <int DT>
+__global__ void __launch_bounds__(256) kv_read_rows(CacheArgs p) {
+    using raw = typename Elem<DT>::raw;
+    const int per_row = p.head_dim >> 3, which = blockIdx.y;
+    const int64_t i = blockIdx.x * int64_t(256) + threadIdx.x;
+    const int64_t row = i / per_row, token = row / p.heads;
+    if (token >= p.tokens) return;
+    const int head = int(row - token * p.heads), c = int(i - row * per_row);
+    const int64_t slot = p.slots[token];
+    float v[8] = {};
+    if (slot >= 0 && slot < p.pages * p.block) {
+        const int64_t page = slot / p.block, at = slot - page * p.block;
+        const float scale = p.scales[which][page * p.heads + head];
+        const u32x2 q = *reinterpret_cast<const u32x2*>(p.codes[which] + ((page * p.heads + head) * p.block + at) * p.head_dim + 8 * c);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = float(int8_t(q[j >> 2] >> (8 * (j & 3)))) * scale;
+    }
+    store8<DT>(static_cast<raw*>(p.y[which]) + row * p.head_dim + 8 * c, v);
+}
+
+static bool bad_cache(int64_t tokens, int64_t pages, int heads, int block, int head_dim) {
+    return tokens < 0 || tokens > 0x7fffffff || pages < 0 || heads < 1 || heads > 65535 || head_dim < 8 || head_dim % 8 || head_dim > 1024 ||
+           block < 1 || block > KV_MAX_BLOCK || pages > (int64_t(1) << 62) / block;
+}
+
+}  // namespace wq8
+
+using namespace wq8;
+
+WQ8_API int wq8_kv_plan(const void* past, const void* fresh, int32_t* tables, int64_t table_stride, const void* pages, int pages_count, const void* used,
+                        int requests, int width, int block, int64_t tokens, int64_t* slots, int32_t* positions, int32_t* starts, int32_t* lens,
+                        int32_t* used_out, int32_t* missing, hipStream_t stream) {
+    if (requests < 0 || width < 0 || block < 1 || tokens < 0 || tokens > 0x7fffffff || pages_count < 0) return -2;
+    const PlanArgs p = {static_cast<const int*>(past), static_cast<const int*>(fresh), static_cast<const int*>(pages), static_cast<const int*>(used),
+                        tables, table_stride, tokens, pages_count, requests, width, block, slots, positions, starts, lens, used_out, missing};
+    kv_plan_tokens<<<unsigned(std::max<int64_t>(1, (tokens + PLAN_TOKENS - 1) / PLAN_TOKENS)), 256, 0, stream>>>(p);
+    return int(hipGetLastError());
+}
+
+WQ8_API int wq8_kv_write(const void* k, const void* v, const long long* strides, const long long* slots, int64_t tokens, int8_t* k_codes, float* k_scales,
+                         int8_t* v_codes, float* v_scales, int64_t pages, int heads, int block, int head_dim, int dtype, int32_t* owner,
+                         hipStream_t stream) {
+    if (dtype < 0 || dtype > 2) return -1;
+    if (bad_cache(tokens, pages, heads, block, head_dim)) return -2;
+    if (!tokens || !pages) return 0;
+    const CacheArgs p = {{k, v}, {}, {strides[0], strides[2]}, {strides[1], strides[3]}, {k_codes, v_codes}, {k_scales, v_scales},
+                         reinterpret_cast<const int64_t*>(slots), owner, tokens, pages, heads, block, head_dim};
+    return dtype == DT_F16 ? launch_write<DT_F16>(p, stream) : dtype == DT_BF16 ? launch_write<DT_BF16>(p, stream) : launch_write<DT_F32>(p, stream);
+}
+
+WQ8_API int wq8_kv_read(const int8_t* k_codes, const float* k_scales, const int8_t* v_codes, const float* v_scales, const long long* slots, int64_t tokens,
+                        void* k, void* v, int64_t pages, int heads, int block, int head_dim, int dtype, hipStream_t stream) {
+    if (dtype < 0 || dtype > 2) return -1;
+    if (bad_cache(tokens, pages, heads, block, head_dim)) return -2;
+    if (!tokens) return 0;
+    const CacheArgs p = {{}, {k, v}, {}, {}, {const_cast<int8_t*>(k_codes), const_cast<int8_t*>(v_codes)},
+                         {const_cast<float*>(k_scales), const_cast<float*>(v_scales)}, reinterpret_cast<const int64_t*>(slots), nullptr, tokens, pages, heads,
+                         block, head_dim};
+    const int64_t blocks = (tokens * heads * (head_dim >> 3) + 255) / 256;
+    if (blocks > 0x7fffffff) return -2;
+    const dim3 grid(static_cast<unsigned>(blocks), 2);
+    if (dtype == DT_F16) kv_read_rows<DT_F16><<<grid, 256, 0, stream>>>(p);
+    else if (dtype == DT_BF16) kv_read_rows<DT_BF16><<<grid, 256, 0, stream>>>(p);
+    else kv_read_rows<DT_F32><<<grid, 256, 0, stream>>>(p);
+    return int(hipGetLastError());
+}

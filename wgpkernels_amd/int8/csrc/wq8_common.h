@@ -65,6 +65,19 @@ template <int DT> WQ8_DEVICE void load8(const typename Elem<DT>::raw* p, float* 
     }
 }
 
+// 8 FP32 values rounded once to DT and stored at a 16-byte aligned address.
+template <int DT> WQ8_DEVICE void store8(typename Elem<DT>::raw* p, const float* v) {
+    if constexpr (DT == DT_F32) {
+        reinterpret_cast<v4f*>(p)[0] = v4f{v[0], v[1], v[2], v[3]};
+        reinterpret_cast<v4f*>(p)[1] = v4f{v[4], v[5], v[6], v[7]};
+    } else {
+        u32x4 packed;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) packed[j] = uint32_t(Elem<DT>::from_f(v[2 * j])) | (uint32_t(Elem<DT>::from_f(v[2 * j + 1])) << 16);
+        *reinterpret_cast<u32x4*>(p) = packed;
+    }
+}
+
 // ---- exp / logistic of this build ---------------------------------------------------------------------------
 // exp_core(z) for z in [-87, 80]: t = z log2(e) + 1.5 2^23 in one FMA, so t holds n = rint(z log2 e) in its low
 // mantissa bits and t - 1.5 2^23 = n exactly; r = z - n ln2 with ln2 split in two (Cody & Waite, |r| <= 0.347);
