@@ -144,12 +144,13 @@ int wq8_kv_read(const int8_t* k_codes, const float* k_scales, const int8_t* v_co
 
 /* Attention of q (tokens, heads * group, head_dim), dtype 0-1, over the cache: request r has rows starts[r] to starts[r + 1] and the
  * first lens[r] tokens of its row of tables (int32; width entries, table_stride apart); strides (host): {token, head} of q, of out;
- * head_dim 64, 128 or 256; block 16, 32, 64 or 128; workspace: of the bytes that the query gives for `keys` = width * block (sizes[1] is 0). */
+ * head_dim 64, 128 or 256; block 16, 32, 64 or 128; workspace: of the bytes that the query
+ * gives (sizes[0]; sizes[1] is 0), 16-byte aligned. */
 int wq8_kv_attention(const void* q, void* out, const long long* strides, const int8_t* k_codes, const float* k_scales, const int8_t* v_codes,
                      const float* v_scales, const void* tables, int64_t table_stride, int width, const void* lens, const void* starts, int tokens,
                      int requests, int heads, int group, int head_dim, int block, int64_t pages, float scale, int causal, int window, int dtype, int sms,
                      void* workspace, wq8_stream_t stream);
-void wq8_kv_attention_workspace(int tokens, int requests, int heads, int group, int head_dim, int64_t keys, int sms, int64_t* sizes);
+void wq8_kv_attention_workspace(int tokens, int requests, int heads, int group, int head_dim, int sms, int64_t* sizes);
 
 /* Cold-cache timing: reads `bytes` of a library-owned buffer on `stream` (nonzero if it cannot be allocated);
  * release frees it. Replace K8:1997-2016; bound at I:77-78. */

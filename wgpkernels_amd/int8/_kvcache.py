@@ -184,7 +184,7 @@ def kv_attention(q, cache, tables, lens, starts, causal=True, window=0, scale=No
     _check_device(device, queries=q, tables=tables, lens=lens, starts=starts, outputs=out)
     lib, state = library(), _native.gpu(codes)
     group, columns = q_heads // heads, tables.shape[1]
-    lib.wq8_kv_attention_workspace(tokens, requests, heads, group, head_dim, columns * block, state.cus, _sizes)
+    lib.wq8_kv_attention_workspace(tokens, requests, heads, group, head_dim, state.cus, _sizes)
     workspace = torch.empty(_sizes[0], dtype=torch.uint8, device=q.device) if _sizes[0] else None
     sq, so = q.stride(), out.stride()
     lib.call("wq8_kv_attention", q.data_ptr(), out.data_ptr(), (ctypes.c_longlong * 4)(sq[0], sq[1], so[0], so[1]), codes.data_ptr(), cache.k_scales.data_ptr(),

@@ -43,7 +43,7 @@ SIGNATURES = {
     "wq8_kv_write": ("i", "pppp" "lpppp" "liiii" "pp"),
     "wq8_kv_read": ("i", "ppppp" "lpp" "liiii" "p"),
     "wq8_kv_attention": ("i", "ppp" "pppp" "plipp" "iiiiiil" "fiii" "ip" "p"),
-    "wq8_kv_attention_workspace": ("-", "iiiii" "li" "p"),
+    "wq8_kv_attention_workspace": ("-", "iiiiii" "p"),
     "wq8_l2_flush": ("i", "il" "p"),
     "wq8_l2_flush_release": ("-", ""),
 }
