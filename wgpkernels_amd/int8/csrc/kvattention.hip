@@ -11,15 +11,15 @@
 // - Queries are FP16; BF16 ones are first scaled by a power of two of their row's largest value, which keeps their 8 bits exact down to
 //   2^-32 of it.
 // - t_j = log2(e) scale ks q . k_j + log2(vs), ks and vs the scales of j's page; w_j = 2^(t_j - m) is the row's weight times its value
-//   scale, rounded once to FP16 for the second product; the sum of weights takes w_j / vs, in FP32, 16 keys (of one page) at a time.
-//   So weights are relative to the largest product of weight and scale, and one page of large values does not cost the others.
-// - m is the running maximum, left alone until a t_j passes it by more than 8 (2^8 is far from FP16's end), so that sums are
-//   rarely scaled again.
+//   scale, rounded once to FP16 for the second product; the sum of weights takes w_j / vs, in FP32 (a page of small values has weights
+//   that FP16 does not hold), 16 keys of one page at a time. So weights are relative to the largest product of weight and scale, and one page of large values does not cost the others.
+// - m follows the running maximum, and is left alone until a t_j would leave FP16's range, so that sums are rarely scaled again.
 // - A value scale is taken as at least 2^-40 of the largest seen before it (and 2^-100): sums of weights stay in range over pages of zeros.
 //
-// Work. A tile is ROWS rows (token, query head) of one request and key/value head; its keys are cut into `splits` parts where
-// tiles alone would not fill the GPU, and kv_attention_join adds the parts. Which item a workgroup takes is found on the GPU, from the
-// requests' lengths: nothing is read on the host.
+// Work. A tile is ROWS rows (token, query head) of one request and key/value head, over the keys that they see together. The tiles of
+// a launch stand in one line (request, head, tile), each as long as its keys, and the workgroups, as many as the GPU holds at once,
+// take equal lengths of it: whole tiles, and parts of the two at a share's ends, whose results kv_attention_join adds. So requests of any
+// lengths fill the GPU evenly; and nothing is read on the host, each workgroup finds its share from the lengths on the GPU.
 #include "wq8_common.h"
 #include "wq8_abi.h"
 #include <algorithm>
@@ -39,48 +39,60 @@ struct AttentionArgs {
     int64_t table_stride, pages;
     int width, tokens, requests, heads, group, block_log2, causal, window;
     int few_rows, many_rows;  // the rows of a request that this launch serves: more than few_rows, up to many_rows
-    int split_items;          // items wanted of a launch that may split keys; 0: whole keys
-    int max_items;
+    int shares;               // workgroups that take a share (a multiple of 8)
     float scale;
-    // workspace of a launch that may split keys: the number of tiles, per tile {first item, parts, first row, request} and its head, partial results
-    int* tile_count;
-    int4* tiles;
-    int* tile_heads;
+    // workspace: per share the split tile that begins in it, {parts, first row, rows, first token} and its head; two partial results a share
+    int4* split_tiles;
+    int* split_heads;
     float* slots;
 };
 
-// ---- which rows and keys -------------------------------------------------------------------------------------------
-struct Span { int rows, tiles, first_token, tokens; int64_t past, total; int span; };
+// ---- shares --------------------------------------------------------------------------------------------------------
+// A request's part of the line: tiles of length first + more * i, i = 0 to tiles - 1, for each head.
+struct Span {
+    int rows, tiles, first_token;
+    int64_t past, total, first, more;
+    WQ8_DEVICE int64_t upto(int64_t i) const { return first * i + more * (i * (i - 1) / 2); }
+};
+
+constexpr int TILE_KEYS_OVERHEAD = 128;  // what a tile costs besides its keys, in keys
 
 template <int ROWS> WQ8_DEVICE Span span_of(const AttentionArgs& p, int r) {
     Span s = {};
     if (r >= p.requests) return s;
     const int begin = min(max(p.starts[r], 0), p.tokens), end = min(max(p.starts[r + 1], begin), p.tokens);
-    const int64_t len = p.lens[r];
+    const int64_t len = p.lens[r], rows = int64_t(end - begin) * p.group;
+    if (rows <= p.few_rows || rows > p.many_rows) return s;
+    s.rows = int(rows);
+    s.tiles = (s.rows + ROWS - 1) / ROWS;
     s.first_token = begin;
-    s.tokens = end - begin;
-    s.past = len - s.tokens;
+    s.past = len - (end - begin);
     s.total = p.pages ? max(int64_t(0), min(len, int64_t(p.width) << p.block_log2)) : 0;
-    const int64_t rows = int64_t(s.tokens) * p.group;
-    if (rows > p.few_rows && rows <= p.many_rows) {
-        s.rows = int(rows);
-        s.tiles = (s.rows + ROWS - 1) / ROWS;
+    // lengths in keys * group: a causal tile's rows see ROWS / group keys more than those of the tile before
+    const int64_t seen = p.causal ? min(s.total, max(int64_t(0), s.past)) : s.total;
+    if (p.causal && !p.window) {
+        s.first = (seen + TILE_KEYS_OVERHEAD) * p.group + ROWS;
+        s.more = ROWS;
+    } else {
+        s.first = ((p.window ? min(s.total, int64_t(p.window)) : seen) + TILE_KEYS_OVERHEAD) * p.group + ROWS;
     }
-    const int64_t most = p.window ? min(s.total, int64_t(p.window) + (ROWS + p.group - 1) / p.group + 64) : s.total;
-    s.span = int(min(most, int64_t(0x7fffff00)));
     return s;
 }
 
-WQ8_DEVICE int scan256(int v, int* lds4, int& total) {
+WQ8_DEVICE int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+WQ8_DEVICE int64_t uniform(int64_t v) { return int64_t(uint64_t(uint32_t(uniform(int(v >> 32)))) << 32 | uint32_t(uniform(int(v)))); }
+
+// Over the first 256 threads.
+WQ8_DEVICE int64_t scan256(int64_t v, int64_t* lds4, int64_t& total) {
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(v, d);
+        const int64_t o = __shfl_up(v, d);
         if (int(threadIdx.x & 63) >= d) v += o;
     }
     __syncthreads();
-    if ((threadIdx.x & 63) == 63) lds4[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 63 && threadIdx.x < 256) lds4[threadIdx.x >> 6] = v;
     __syncthreads();
-    int before = 0;
+    int64_t before = 0;
     total = 0;
     for (int w = 0; w < 4; ++w) {
         if (w < int(threadIdx.x >> 6)) before += lds4[w];
@@ -89,81 +101,82 @@ WQ8_DEVICE int scan256(int v, int* lds4, int& total) {
     return v + before;
 }
 
-struct Item {
-    int live, request, row0, rows, first_token, head, split, splits, tile_index, item;
-    int64_t past, total;
-};
-WQ8_DEVICE int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-WQ8_DEVICE int64_t uniform(int64_t v) { return int64_t(uint64_t(uint32_t(uniform(int(v >> 32)))) << 32 | uint32_t(uniform(int(v)))); }
+// A workgroup's share [at, end) of the line, and the tile that stands at `at`.
+struct Item { int request, row0, rows, first_token, head; int64_t past, total, line_begin, line_end; };
+template <int ROWS> struct Share {
+    const AttentionArgs& p;
+    int64_t* lds4;
+    int64_t* ends;     // where each of 256 requests ends in the line
+    int64_t at, end, share, line;
+    int64_t base_at;
+    int base, index;
 
-// Item number -> request, head, tile, part of its keys; in this order, parts innermost. Consecutive workgroups go round the 8
-// XCDs: item numbers are dealt so that each XCD takes a contiguous range, whose tiles share keys and values in its L2.
-template <int ROWS> WQ8_DEVICE Item find_item(const AttentionArgs& p) {
-    __shared__ int lds4[4];
-    __shared__ Item found;
-    const int tid = threadIdx.x;
-    int chunk = 0x7fffff00;
-    if (p.split_items) {
-        float work = 0.0f;
-        for (int base = 0; base < p.requests; base += 256) {
-            const Span s = span_of<ROWS>(p, base + tid);
-            work += float(s.tiles) * float(s.span);
-        }
-        work = wave_sum(work);
-        __shared__ float sums[4];
-        if ((tid & 63) == 0) sums[tid >> 6] = work;
+    // 256 requests from `first` on: spans a thread each, their ends in LDS
+    WQ8_DEVICE int64_t strip(int first, int64_t before) {
+        base = first;
+        base_at = before;
+        const Span s = span_of<ROWS>(p, threadIdx.x < 256 ? first + int(threadIdx.x) : p.requests);
+        int64_t total;
+        const int64_t e = before + scan256(s.upto(s.tiles) * p.heads, lds4, total);
+        if (threadIdx.x < 256) ends[threadIdx.x] = e;
         __syncthreads();
-        work = ((sums[0] + sums[1]) + sums[2]) + sums[3];
-        // keys of a part: the work over the items wanted, at least 256
-        chunk = int(fminf(fmaxf(work * float(p.heads) / float(p.split_items), 256.0f), 2.0e9f)) + 63 & ~63;
+        return before + total;
     }
-    const auto count_of = [&](const Span& s, int& splits) {
-        splits = max(1, (s.span + chunk - 1) / chunk);
-        return s.tiles * p.heads * splits;
-    };
-    int all = 0, all_tiles = 0;
-    for (int base = 0; base < p.requests; base += 256) {
-        const Span s = span_of<ROWS>(p, base + tid);
-        int splits, total;
-        scan256(count_of(s, splits), lds4, total);
-        all += total;
-        if (p.split_items && !blockIdx.x) {
-            scan256(s.tiles * p.heads, lds4, total);
-            all_tiles += total;
+    // Consecutive workgroups go round the 8 XCDs: each XCD takes a contiguous length of the line, whose tiles share keys and
+    // values in its L2. A share is at least `least` keys.
+    WQ8_DEVICE Share(const AttentionArgs& args, int64_t* scan, int64_t* request_ends, int least) : p(args), lds4(scan), ends(request_ends) {
+        line = 0;
+        for (int r = 0; r < p.requests; r += 256) line = strip(r, line);
+        line = uniform(line);
+        share = max((line + p.shares - 1) / p.shares, int64_t(least) * p.group);
+        index = int(blockIdx.x & 7) * (p.shares >> 3) + int(blockIdx.x >> 3);
+        at = index * share;
+        end = min(line, at + share);
+    }
+    WQ8_DEVICE Item item() {
+        if (at < base_at || p.requests > 256) {
+            int64_t upto = 0;
+            for (int r = 0; r < p.requests; r += 256) {
+                __syncthreads();
+                upto = uniform(strip(r, upto));
+                if (at < upto) break;
+            }
         }
-    }
-    if (p.split_items && !blockIdx.x && !tid) *p.tile_count = all_tiles;
-    const int per = (all + 7) >> 3, item = int(blockIdx.x & 7) * per + int(blockIdx.x >> 3);
-    if (!tid) found.live = 0;
-    int before = 0, tiles_before = 0;
-    for (int base = 0; base < p.requests; base += 256) {
-        const Span s = span_of<ROWS>(p, base + tid);
-        int splits, total, total_tiles;
-        const int count = count_of(s, splits);
-        const int end = before + scan256(count, lds4, total);
-        const int tiles_end = tiles_before + scan256(s.tiles * p.heads, lds4, total_tiles);
-        if (item >= end - count && item < end && int(blockIdx.x >> 3) < per) {
-            const int at = item - (end - count), tile = at / splits;
-            found = {item < p.max_items, base + tid, tile % s.tiles * ROWS, s.rows, s.first_token, tile / s.tiles, at % splits, splits,
-                     tiles_end - s.tiles * p.heads + tile, item, s.past, s.total};
+        int a = 0, b = min(256, p.requests - base) - 1;  // the first request that ends past `at`
+        while (a < b) {
+            const int m = (a + b) >> 1;
+            if (uniform(ends[m]) > at) b = m; else a = m + 1;
         }
-        before += total;
-        tiles_before += total_tiles;
-        if (item < before) break;
+        const Span s = span_of<ROWS>(p, base + a);
+        const int64_t begin = a ? uniform(ends[a - 1]) : base_at, per_head = s.upto(s.tiles);
+        int64_t in = at - begin;
+        int head = min(int(double(in) / double(per_head)), p.heads - 1);
+        if (in < head * per_head) --head;
+        else if (in >= (head + 1) * per_head) ++head;
+        in -= head * per_head;
+        int tile;
+        if (s.more) {  // first i + more i (i - 1) / 2 <= in
+            const double h = double(s.first) - 0.5 * double(s.more);
+            tile = int((__builtin_sqrt(h * h + 2.0 * double(s.more) * double(in)) - h) / double(s.more));
+        } else {
+            tile = int(double(in) / double(s.first));
+        }
+        tile = min(max(tile, 0), s.tiles - 1);
+        while (tile > 0 && s.upto(tile) > in) --tile;
+        while (tile + 1 < s.tiles && s.upto(tile + 1) <= in) ++tile;
+        const int64_t head_at = begin + head * per_head;
+        return {uniform(base + a), uniform(tile * ROWS), uniform(s.rows), uniform(s.first_token), uniform(head), uniform(s.past), uniform(s.total),
+                uniform(head_at + s.upto(tile)), uniform(head_at + s.upto(tile + 1))};
     }
-    __syncthreads();
-    return {uniform(found.live), uniform(found.request), uniform(found.row0), uniform(found.rows), uniform(found.first_token), uniform(found.head),
-            uniform(found.split), uniform(found.splits), uniform(found.tile_index), uniform(found.item), uniform(found.past), uniform(found.total)};
-}
+    // Of `steps` steps of the item's keys, the ones before place x of the line: the same for the shares on both sides of x.
+    WQ8_DEVICE int step_of(const Item& it, int64_t x, int steps) const {
+        if (x <= it.line_begin) return 0;
+        if (x >= it.line_end) return steps;
+        return uniform(int(double(x - it.line_begin) * double(steps) / double(it.line_end - it.line_begin)));
+    }
+};
 
-// Where the parts of a tile are, for kv_attention_join: written by the tile's first part.
-WQ8_DEVICE void note_tile(const AttentionArgs& p, const Item& it) {
-    if (!p.split_items || threadIdx.x || it.split) return;
-    p.tiles[it.tile_index] = int4{it.item, it.splits, it.row0, it.request};
-    p.tile_heads[it.tile_index] = it.head;
-}
-
-// Keys that the rows of tokens [first, last] see together: [low, high); and this part of them.
+// Keys that the rows of tokens [first, last] see together: [low, high).
 struct Keys { int64_t low, high; };
 WQ8_DEVICE Keys keys_of(const AttentionArgs& p, const Item& it, int64_t first, int64_t last) {
     Keys k;
@@ -233,256 +246,279 @@ WQ8_DEVICE PageScales page_scales(float ks, float vs, float seen, bool live) {
 }
 
 constexpr float LOWEST = -0x1p+120f;  // the running maximum before any key: below every t, and -inf - LOWEST = -inf
-constexpr float LAG = 8.0f;
+// Weights are taken relative to 2^-HEAD of the largest, and to that until one passes it by 2^LAG (FP16 ends at 2^16): small weights keep
+// their bits down to 2^-21 of the largest.
+constexpr float HEAD = 7.0f, LAG = 15.0f;
 
 WQ8_DEVICE f16x8 weights8(const float* w) {
     f16x8 r;
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-        r[j] = static_cast<_Float16>(w[j]);
-        r[j + 1] = static_cast<_Float16>(w[j + 1]);
-    }
+    for (int j = 0; j < 8; ++j) r[j] = static_cast<_Float16>(w[j]);
     return r;
 }
 
 WQ8_DEVICE float finish(float acc, float mass) { return mass > 0.0f ? acc / mass : mass == 0.0f ? 0.0f : mass; }
 
 // A tile's partial result: rows x D sums, then rows pairs (maximum, sum of weights).
-template <int ROWS, int D> WQ8_DEVICE float* slot_of(const AttentionArgs& p, int item) { return p.slots + int64_t(item) * (ROWS * (D + 2)); }
+// A share has two: 2 i for a tile that began in an earlier share, 2 i + 1 for one that goes on in a later one.
+template <int ROWS, int D> WQ8_DEVICE float* slot_of(const AttentionArgs& p, int slot) { return p.slots + int64_t(slot) * (ROWS * (D + 2)); }
+
+// A tile that begins in this share and goes on in later ones, for kv_attention_join.
+template <int ROWS> WQ8_DEVICE void note_split(const AttentionArgs& p, const Share<ROWS>& share, const Item& it) {
+    if (threadIdx.x) return;
+    p.split_tiles[share.index] = int4{int((it.line_end - 1) / share.share) - share.index + 1, it.row0, it.rows, it.first_token};
+    p.split_heads[share.index] = it.head;
+}
 
 // ---- tiles of many rows --------------------------------------------------------------------------------------------
-// 128 rows, 32 a wave, over 64 keys at a time. S^T = K Q^T and O^T = V^T P^T on 32x32x16: a lane holds one row (lane % 32) and, of S^T,
-// the keys 8 (i / 4) + 4 (lane / 32) + i % 4. With the second product's keys in that order a lane's weights are its operand as they
-// are. The workgroup converts each 64 keys once, into LDS in the operands' order (1 KB a fragment, 16 bytes a lane,
-// swizzled so that the transposing writes spread over the banks), in two buffers: while one is used, the next keys' codes are on their way
-// in registers.
-constexpr int TILE_ROWS = 128, TILE_KEYS = 64;
+// 32 rows a wave, 64 keys a step. S^T = K Q^T and O^T = V^T P^T on 32x32x16: a lane holds one row (lane % 32) and, of S^T, the keys
+// 8 (i / 4) + 4 (lane / 32) + i % 4. With the second product's keys in that order a lane's weights are its operand as they are. The
+// workgroup converts each step's codes once, into LDS in the operands' order (1 KB a fragment, 16 bytes a lane, swizzled so that the
+// writes spread over the banks), in two buffers: while one is used, the next step's codes are on their way in registers. Wave w
+// converts the 16 keys (of one page: its place is scalar work) 16 (w % 4) of the step: with 8 waves the first four the values, the
+// others the keys; with 4 waves each does both. The second four waves convert before their products, the first four after them, so that of
+// a SIMD's two waves one mostly feeds the matrix cores while the other converts.
+constexpr int STEP_KEYS = 64;
 
-template <int DT, int D>
-__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_tiles(AttentionArgs p) {
-    constexpr int KF = D / 16, CH = D / 16, KC = TILE_KEYS * CH / 256, VD = D / 4, VG = 256 / VD, VC = VG < 8 ? 8 / VG : 1;
-    constexpr int SWZ = D == 64 ? 2 : 1;
+WQ8_DEVICE float max3(float a, float b, float c) {  // without the quieting moves of fmaxf
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+template <typename T> WQ8_DEVICE T scalar_load(const T* p) { return *(const __attribute__((address_space(4))) T*)(uint64_t)p; }
+WQ8_DEVICE int near32(int64_t v) { return int(min(max(v, int64_t(-(1 << 30))), int64_t(1 << 30))); }
+
+template <int DT, int D, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_tiles(AttentionArgs p) {
+    constexpr int ROWS = 32 * WAVES, KF = D / 16, KI = D / 64, VI = D == 256 ? 2 : 1, RAW = D == 256 ? 16 : 8, SWZ = 256 / D;
     __shared__ u32x4 k_lds[2][2 * KF * 64];
     __shared__ u32x4 v_lds[2][4 * (D / 32) * 64];
-    __shared__ PageScales scales[2][4];
-    const Item it = find_item<TILE_ROWS>(p);
-    if (!it.live) return;
-    note_tile(p, it);
-    const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, half = lane >> 5;
-
-    // this lane's row
-    const int row = it.row0 + 32 * wave + (lane & 31);
-    const bool live_row = row < it.rows;
-    const int token = min(row, it.rows - 1) / p.group, member = min(row, it.rows - 1) - token * p.group;
-    const uint16_t* q = static_cast<const uint16_t*>(p.q) + (it.first_token + token) * p.q_token + (it.head * p.group + member) * p.q_head;
-    f16x8 query[KF];
-    const float query_scale = load_query<DT, KF>(q + 8 * half, 16, live_row, query, [](uint32_t t) {
-        const LanePair o = swap32(__builtin_bit_cast(float, t));
-        return max(__builtin_bit_cast(uint32_t, o.a), __builtin_bit_cast(uint32_t, o.b));
-    }) * p.scale * 0x1.715476p+0f;
-
-    // keys: of the tile, of the part, of the wave, of the row
-    const int last_row = min(it.row0 + TILE_ROWS, it.rows) - 1;
-    Keys tile = keys_of(p, it, it.row0 / p.group, last_row / p.group);
-    tile.low &= ~int64_t(TILE_KEYS - 1);
-    const int64_t part = ((tile.high - tile.low + it.splits - 1) / it.splits + TILE_KEYS - 1) & ~int64_t(TILE_KEYS - 1);
-    const int64_t key0 = tile.low + it.split * part, key1 = min(tile.high, key0 + part);
-    const int steps = key1 > key0 ? int((key1 - key0 + TILE_KEYS - 1) / TILE_KEYS) : 0;
-    const int wave_first = it.row0 + 32 * wave, wave_last = min(wave_first + 31, it.rows - 1);
-    const bool live_wave = wave_first < it.rows;
-    const Keys own = keys_of(p, it, token, token);
-    const Keys first = keys_of(p, it, min(wave_first, it.rows - 1) / p.group, min(wave_first, it.rows - 1) / p.group);
-    const Keys last = keys_of(p, it, wave_last / p.group, wave_last / p.group);
-
-    // loads of a step: K chunks of 16 channels of a key, V dwords (4 channels) of the 8 keys of an operand
-    const int* table = p.tables + it.request * p.table_stride;
+    __shared__ v4f page_k[2], page_log_v[2], page_inv_v[2];
+    __shared__ int64_t scan[4], ends[256];
+    const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, half = lane >> 5, granule = wave & 3;
+    const bool does_v = WAVES == 4 || wave < 4, does_k = WAVES == 4 || wave >= 4;
+    Share<ROWS> share(p, scan, ends, 4 * STEP_KEYS);
+    if (!tid) p.split_tiles[share.index].x = 0;
+    // lane constants: places of the codes in memory and LDS, of the operands
+    const int v_half = D == 64 ? lane >> 4 : D == 128 ? lane >> 5 : 0, v_dw = D == 64 ? lane & 15 : D == 128 ? lane & 31 : lane;
+    const int v_at = 4 * v_half * D + 4 * v_dw;
+    const int v_entry = lane ^ (lane >> 3 & 3);
     const int block_mask = (1 << p.block_log2) - 1;
     const int64_t page_bytes = (int64_t(p.heads) << p.block_log2) * D;
-    const auto page_at = [&](int64_t key) -> int { return key < key1 ? table[key >> p.block_log2] : -1; };
-    int k_page[KC], v_page[VC], s_page;
-    u32x4 k_raw[KC];
-    uint32_t v_raw[VC][8];
-    float ks_raw, vs_raw;
-    const int k_key = tid / CH, k_chunk = tid % CH, v_dw = tid % VD, v_group = tid / VD;
-    const auto load_pages = [&](int step) {
-        const int64_t base = key0 + int64_t(step) * TILE_KEYS;
-#pragma unroll
-        for (int i = 0; i < KC; ++i) k_page[i] = page_at(base + k_key + i * (256 / CH));
-#pragma unroll
-        for (int i = 0; i < VC; ++i) v_page[i] = page_at(base + (v_group + i * VG) / 2 * 16);
-        s_page = page_at(base + (tid & 3) * 16);
-    };
-    bool s_live;
-    const auto load_codes = [&](int step) {
-        const int64_t base = key0 + int64_t(step) * TILE_KEYS;
-        const auto row_of = [&](int page, int64_t key) {
-            const int64_t at = page >= 0 && page < p.pages ? page : 0;
-            return at * page_bytes + (int64_t(it.head) << p.block_log2) * D + int(key & block_mask) * D;
+
+    for (; share.at < share.end; __syncthreads()) {
+        const Item it = share.item();
+        // this lane's row
+        const int row = it.row0 + 32 * wave + (lane & 31);
+        const bool live_row = row < it.rows;
+        const int token = min(row, it.rows - 1) / p.group, member = min(row, it.rows - 1) - token * p.group;
+        f16x8 query[KF];
+        const float query_scale = load_query<DT, KF>(static_cast<const uint16_t*>(p.q) + (it.first_token + token) * p.q_token +
+                                                         (it.head * p.group + member) * p.q_head + 8 * half, 16, live_row, query, [](uint32_t t) {
+            const LanePair o = swap32(__builtin_bit_cast(float, t));
+            return max(__builtin_bit_cast(uint32_t, o.a), __builtin_bit_cast(uint32_t, o.b));
+        }) * p.scale * 0x1.715476p+0f;
+
+        // keys: of the tile, of the part, and from the part's first on those of the wave and of the row
+        Keys tile = keys_of(p, it, it.row0 / p.group, (min(it.row0 + ROWS, it.rows) - 1) / p.group);
+        tile.low = min(tile.low, tile.high) & ~int64_t(STEP_KEYS - 1);
+        const int all_steps = int((tile.high - tile.low + STEP_KEYS - 1) / STEP_KEYS), step0 = share.step_of(it, share.at, all_steps);
+        const int steps = share.step_of(it, share.end, all_steps) - step0;
+        const int64_t key0 = tile.low + int64_t(step0) * STEP_KEYS, key1 = min(tile.high, key0 + int64_t(steps) * STEP_KEYS);
+        const bool began = share.at > it.line_begin, goes_on = share.end < it.line_end;
+        const int wave_first = it.row0 + 32 * wave, wave_last = min(wave_first + 31, it.rows - 1);
+        const Keys own = keys_of(p, it, token, token);
+        const Keys first = keys_of(p, it, min(wave_first, it.rows - 1) / p.group, min(wave_first, it.rows - 1) / p.group);
+        const Keys last = keys_of(p, it, wave_last / p.group, wave_last / p.group);
+        const int own_low = near32(own.low - key0) - 4 * half, own_high = near32(own.high - key0) - 4 * half;
+        const int some_low = near32(first.low - key0), some_high = wave_first < it.rows ? near32(last.high - key0) : -(1 << 30);
+        const int all_low = near32(last.low - key0), all_high = near32(first.high - key0);
+
+        // this wave's 16 keys of a step: their page, codes and scales
+        const int* table = p.tables + it.request * p.table_stride;
+        const int64_t head_bytes = (int64_t(it.head) << p.block_log2) * D;
+        const auto page_of = [&](int step) -> int {
+            const int64_t key = key0 + int64_t(step) * STEP_KEYS + 16 * granule;
+            return key < key1 ? scalar_load(table + (key >> p.block_log2)) : -1;
         };
+        uint32_t v_raw[RAW];
+        u32x4 k_raw[KI];
+        float ks = 0.0f, vs = 0.0f, seen = 0.0f;
+        bool live_page = false;
+        const auto load_codes = [&](int step, int page) {
+            live_page = page >= 0 && page < p.pages;
+            if (!live_page) page = 0;
+            const int64_t at = page * page_bytes + head_bytes + (int(key0 + int64_t(step) * STEP_KEYS + 16 * granule) & block_mask) * D;
+            if (does_v) {
 #pragma unroll
-        for (int i = 0; i < KC; ++i)
-            k_raw[i] = *reinterpret_cast<const u32x4*>(p.k_codes + row_of(k_page[i], base + k_key + i * (256 / CH)) + 16 * k_chunk);
+                for (int i = 0; i < VI; ++i)
+                    if (D > 64 || lane < 32)
 #pragma unroll
-        for (int i = 0; i < VC; ++i) {
-            const int g = v_group + i * VG;
-            if (VG > 8 && g >= 8) break;
-            // operand keys 16 (g / 2) + 4 (g % 2) + {0-3, 8-11}
-            const int8_t* at = p.v_codes + row_of(v_page[i], base + g / 2 * 16) + (g & 1) * 4 * D + 4 * v_dw;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v_raw[i][j] = *reinterpret_cast<const uint32_t*>(at + (j < 4 ? j : j + 4) * D);
-        }
-        s_live = s_page >= 0 && s_page < p.pages;
-        const int64_t at = int64_t(s_live ? s_page : 0) * p.heads + it.head;
-        ks_raw = p.k_scales[at];
-        vs_raw = p.v_scales[at];
-    };
-    float seen = 0.0f;
-    const auto store_codes = [&](int buffer) {
-#pragma unroll
-        for (int i = 0; i < KC; ++i) {
-            const int key = k_key + i * (256 / CH);
-            u32x4* at = k_lds[buffer] + ((key >> 5) * KF + k_chunk) * 64;
-            const u32x2 a = codes4(k_raw[i][0]), b = codes4(k_raw[i][1]), c = codes4(k_raw[i][2]), d = codes4(k_raw[i][3]);
-            const int entry = (key & 31) ^ (SWZ * k_chunk & 7);
-            at[entry] = u32x4{a[0], a[1], b[0], b[1]};
-            at[entry + 32] = u32x4{c[0], c[1], d[0], d[1]};
-        }
-#pragma unroll
-        for (int i = 0; i < VC; ++i) {
-            const int g = v_group + i * VG;
-            if (VG > 8 && g >= 8) break;
-            uint32_t pairs[4][4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) code_pairs(v_raw[i][2 * j], v_raw[i][2 * j + 1], pairs[j]);
-            u32x4* at = v_lds[buffer] + ((v_dw >> 3) * 4 + (g >> 1)) * 64;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int entry = 4 * (v_dw & 7) + c + 32 * (g & 1);
-                at[entry ^ (entry >> 3 & 3)] = u32x4{pairs[0][c], pairs[1][c], pairs[2][c], pairs[3][c]};
+                        for (int j = 0; j < 8; ++j)
+                            v_raw[8 * i + j] = *reinterpret_cast<const uint32_t*>(p.v_codes + at + (v_at + 4 * i * D + (j < 4 ? j : j + 4) * D));
+                ks = scalar_load(p.k_scales + int64_t(page) * p.heads + it.head);
+                vs = scalar_load(p.v_scales + int64_t(page) * p.heads + it.head);
             }
-        }
-        const float v = s_live ? vs_raw : 0.0f;
-        float top = fmaxf(v, lane_xor<1>(v));
-        top = fmaxf(top, lane_xor<2>(top));
-        seen = fmaxf(seen, top);
-        if (tid < 4) scales[buffer][tid] = page_scales(ks_raw, vs_raw, seen, s_live);
-    };
-
-    float top = LOWEST, mass = 0.0f;
-    v16f acc[D / 32];
+            if (does_k) {
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] = v16f{};
-    const int v_entry = lane ^ (lane >> 3 & 3);
-
-    if (steps) {
-        load_pages(0);
-        load_codes(0);
-        load_pages(1);
-        store_codes(0);
-        load_codes(1);
-        load_pages(2);
-        __syncthreads();
-    }
-    for (int step = 0; step < steps; ++step) {
-        const int buffer = step & 1;
-        const int64_t base = key0 + int64_t(step) * TILE_KEYS;
-        if (live_wave && base < last.high && base + TILE_KEYS > first.low) {
-            float t[2][16];
+                for (int i = 0; i < KI; ++i) k_raw[i] = *reinterpret_cast<const u32x4*>(p.k_codes + at + (16 * lane + 1024 * i));
+            }
+        };
+        const auto store_codes = [&](int buffer) {
+            if (does_v) {
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                v16f s = {};
+                for (int i = 0; i < VI; ++i) {
+                    uint32_t pairs[4][4];
 #pragma unroll
-                for (int f = 0; f < KF; ++f) {
-                    const f16x8 k = __builtin_bit_cast(f16x8, k_lds[buffer][(b * KF + f) * 64 + (lane ^ (SWZ * f & 7))]);
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, query[f], s, 0, 0, 0);
+                    for (int j = 0; j < 4; ++j) code_pairs(v_raw[8 * i + 2 * j], v_raw[8 * i + 2 * j + 1], pairs[j]);
+                    u32x4* at = v_lds[buffer] + ((v_dw >> 3) * 4 + granule) * 64;
+                    if (D > 64 || lane < 32)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const int entry = 4 * (v_dw & 7) + c + 32 * (v_half + i);
+                            at[entry ^ (entry >> 3 & 3) ^ (v_dw & 8)] = u32x4{pairs[0][c], pairs[1][c], pairs[2][c], pairs[3][c]};
+                        }
                 }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) t[b][i] = s[i];
+                seen = fmaxf(seen, live_page ? vs : 0.0f);
+                const PageScales s = page_scales(ks, vs, seen, live_page);
+                if (!lane) {
+                    reinterpret_cast<float*>(&page_k[buffer])[granule] = s.k;
+                    reinterpret_cast<float*>(&page_log_v[buffer])[granule] = s.log_v;
+                    reinterpret_cast<float*>(&page_inv_v[buffer])[granule] = s.inv_v;
+                }
             }
-            PageScales ps[4];
+            if (does_k) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) ps[g] = scales[buffer][g];
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const float k = ps[g].k * query_scale;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) t[g >> 1][(g & 1) * 8 + i] = __builtin_fmaf(t[g >> 1][(g & 1) * 8 + i], k, ps[g].log_v);
+                for (int i = 0; i < KI; ++i) {
+                    const int unit = lane + 64 * i, key = unit / KF, chunk = unit % KF;
+                    u32x4* at = k_lds[buffer] + ((granule >> 1) * KF + chunk) * 64;
+                    const u32x2 a = codes4(k_raw[i][0]), b = codes4(k_raw[i][1]), c = codes4(k_raw[i][2]), d = codes4(k_raw[i][3]);
+                    const int entry = (16 * (granule & 1) + key) ^ (SWZ * chunk & 15);
+                    at[entry] = u32x4{a[0], a[1], b[0], b[1]};
+                    at[entry + 32] = u32x4{c[0], c[1], d[0], d[1]};
+                }
             }
-            if (base + TILE_KEYS > first.high || base < last.low) {  // some row does not see every key of the step
-                const int high = int(min(own.high - base, int64_t(64))) - 4 * half, low = int(max(own.low - base, int64_t(-64))) - 4 * half;
+        };
+
+        float top = LOWEST, mass = 0.0f;
+        v16f acc[D / 32];
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+        for (int i = 0; i < D / 32; ++i) acc[i] = v16f{};
+
+        int page = page_of(0);
+        if (steps > 0) {
+            load_codes(0, page);
+            page = page_of(1);
+            store_codes(0);
+            load_codes(1, page);
+            page = page_of(2);
+            __syncthreads();
+        }
+        for (int step = 0; step < steps; ++step) {
+            const int buffer = step & 1, base = step * STEP_KEYS;
+            const auto next = [&] {
+                if (step + 1 < steps) {
+                    store_codes(buffer ^ 1);
+                    load_codes(step + 2, page);
+                    page = page_of(step + 3);
+                }
+            };
+            if (wave >= 4) next();
+            if (base < some_high && base + STEP_KEYS > some_low) {
+                v16f s[2];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int key = 32 * b + 8 * (i / 4) + i % 4;
-                        if (key >= high || key < low) t[b][i] = -__builtin_inff();
+                for (int b = 0; b < 2; ++b) {
+                    s[b] = v16f{};
+#pragma unroll
+                    for (int f = 0; f < KF; ++f) {
+                        const f16x8 k = __builtin_bit_cast(f16x8, k_lds[buffer][(b * KF + f) * 64 + (lane ^ (SWZ * f & 15))]);
+                        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, query[f], s[b], 0, 0, 0);
                     }
-            }
-            float high = t[0][0];
-#pragma unroll
-            for (int i = 1; i < 32; ++i) high = fmaxf(high, t[i >> 4][i & 15]);
-            if (__ballot(high > top + LAG)) {
-                const LanePair o = swap32(high);
-                const float next = fmaxf(top, fmaxf(o.a, o.b)), keep = __builtin_amdgcn_exp2f(top - next);
-                top = next;
-                mass *= keep;
-#pragma unroll
-                for (int i = 0; i < D / 32; ++i) acc[i] *= keep;
-            }
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                float w[8], sum = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    w[i] = __builtin_amdgcn_exp2f(t[g >> 1][(g & 1) * 8 + i] - top);
-                    sum += w[i];
                 }
-                mass = __builtin_fmaf(sum, ps[g].inv_v, mass);
-                const f16x8 weights = weights8(w);
+                // t = a s + b of the 16 keys of a page
+                v4f a = page_k[buffer] * query_scale, b = page_log_v[buffer];
+                const v4f inv_v = page_inv_v[buffer];
+                if (base + STEP_KEYS > all_high || base < all_low) {  // some row does not see every key of the step
+                    const int high = own_high - base, low = own_low - base;
 #pragma unroll
-                for (int c = 0; c < D / 32; ++c) {
-                    const f16x8 v = __builtin_bit_cast(f16x8, v_lds[buffer][(c * 4 + g) * 64 + v_entry]);
-                    acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, weights, acc[c], 0, 0, 0);
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int key = 32 * h + 8 * (i / 4) + i % 4, g = 2 * h + i / 8;
+                            s[h][i] = key >= high || key < low ? -__builtin_inff() : __builtin_fmaf(s[h][i], a[g], b[g]);
+                        }
+                    a = v4f{1.0f, 1.0f, 1.0f, 1.0f};
+                    b = v4f{};
+                }
+                float high = LOWEST;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const v16f& t = s[g >> 1];
+                    const int i = 8 * (g & 1);
+                    const float m = max3(max3(t[i], t[i + 1], t[i + 2]), max3(t[i + 3], t[i + 4], t[i + 5]), max3(t[i + 6], t[i + 7], t[i + 7]));
+                    high = fmaxf(high, __builtin_fmaf(m, a[g], b[g]));
+                }
+                if (__ballot(high > top + LAG)) {
+                    const LanePair o = swap32(high);
+                    const float next_top = fmaxf(top, fmaxf(o.a, o.b) - HEAD), keep = __builtin_amdgcn_exp2f(top - next_top);
+                    top = next_top;
+                    mass *= keep;
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) acc[i] *= keep;
+                }
+                b -= top;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    float w[8], sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 1][8 * (g & 1) + i], a[g], b[g]));
+                        sum += w[i];
+                    }
+                    const f16x8 weights = weights8(w);
+                    mass = __builtin_fmaf(sum, inv_v[g], mass);
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        const f16x8 v = __builtin_bit_cast(f16x8, v_lds[buffer][(c * 4 + g) * 64 + (v_entry ^ (8 * (c & 1)))]);
+                        acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, weights, acc[c], 0, 0, 0);
+                    }
                 }
             }
+            if (wave < 4) next();
+            __syncthreads();
         }
-        if (step + 1 < steps) {
-            store_codes(buffer ^ 1);
-            load_codes(step + 2);
-            load_pages(step + 3);
-        }
-        __syncthreads();
-    }
 
-    const LanePair both = swap32(mass);
-    mass = both.a + both.b;
-    if (it.splits > 1) {
-        float* slot = slot_of<TILE_ROWS, D>(p, it.item);
-        const int r = 32 * wave + (lane & 31);
-        if (live_row) {
+        const LanePair both = swap32(mass);
+        mass = both.a + both.b;
+        if (began || goes_on) {
+            float* slot = slot_of<ROWS, D>(p, 2 * share.index + !began);
+            const int r = 32 * wave + (lane & 31);
+            if (live_row) {
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<v4f*>(slot + r * D + 32 * c + 8 * i + 4 * half) = v4f{acc[c][4 * i], acc[c][4 * i + 1], acc[c][4 * i + 2], acc[c][4 * i + 3]};
+                if (!half) {
+                    slot[ROWS * D + 2 * r] = top;
+                    slot[ROWS * D + 2 * r + 1] = mass;
+                }
+            }
+            if (!began) note_split(p, share, it);
+        } else if (live_row) {
+            uint16_t* out = static_cast<uint16_t*>(p.out) + (it.first_token + token) * p.out_token + (it.head * p.group + member) * p.out_head;
 #pragma unroll
             for (int c = 0; c < D / 32; ++c)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<v4f*>(slot + r * D + 32 * c + 8 * i + 4 * half) = v4f{acc[c][4 * i], acc[c][4 * i + 1], acc[c][4 * i + 2], acc[c][4 * i + 3]};
-            if (!half) {
-                slot[TILE_ROWS * D + 2 * r] = top;
-                slot[TILE_ROWS * D + 2 * r + 1] = mass;
-            }
+                for (int i = 0; i < 4; ++i) {
+                    uint16_t o[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[j] = Elem<DT>::from_f(finish(acc[c][4 * i + j], mass));
+                    *reinterpret_cast<u32x2*>(out + 32 * c + 8 * i + 4 * half) = u32x2{o[0] | uint32_t(o[1]) << 16, o[2] | uint32_t(o[3]) << 16};
+                }
         }
-        return;
+        share.at = it.line_end;
     }
-    if (!live_row) return;
-    uint16_t* out = static_cast<uint16_t*>(p.out) + (it.first_token + token) * p.out_token + (it.head * p.group + member) * p.out_head;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint16_t o[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] = Elem<DT>::from_f(finish(acc[c][4 * i + j], mass));
-            *reinterpret_cast<u32x2*>(out + 32 * c + 8 * i + 4 * half) = u32x2{o[0] | uint32_t(o[1]) << 16, o[2] | uint32_t(o[3]) << 16};
-        }
 }
 
 // ---- tiles of few rows ---------------------------------------------------------------------------------------------
@@ -494,14 +530,16 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_tiles(Atte
 constexpr int FEW_ROWS = 16, FEW_KEYS = 32;
 
 template <int DT, int D>
-__global__ void __launch_bounds__(256, 2) kv_attention_few(AttentionArgs p) {
+__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(AttentionArgs p) {
     constexpr int KF = D / 32, KV = D / 64, VF = D / 16, VW = D / 64;  // fragments; 16-byte loads of K a lane; dwords of V a key
     __shared__ float sums[4][FEW_ROWS][D + 4];
     __shared__ float tops[4][FEW_ROWS], masses[4][FEW_ROWS];
-    const Item it = find_item<FEW_ROWS>(p);
-    if (!it.live) return;
-    note_tile(p, it);
+    __shared__ int64_t scan[4], ends[256];
     const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, quarter = lane >> 4;
+    Share<FEW_ROWS> share(p, scan, ends, 8 * FEW_KEYS);
+    if (!tid) p.split_tiles[share.index].x = 0;
+    for (; share.at < share.end; __syncthreads()) {
+    const Item it = share.item();
     const int row = it.row0 + (lane & 15);
     const bool live_row = row < it.rows;
     const int token = min(row, it.rows - 1) / p.group, member = min(row, it.rows - 1) - token * p.group;
@@ -517,9 +555,10 @@ __global__ void __launch_bounds__(256, 2) kv_attention_few(AttentionArgs p) {
     const int last_row = min(it.row0 + FEW_ROWS, it.rows) - 1;
     const int64_t first_token = it.row0 / p.group, last_token = last_row / p.group;
     Keys tile = keys_of(p, it, first_token, last_token);
-    tile.low &= ~int64_t(FEW_KEYS - 1);
-    const int64_t part = ((tile.high - tile.low + it.splits - 1) / it.splits + 4 * FEW_KEYS - 1) & ~int64_t(4 * FEW_KEYS - 1);
-    const int64_t key0 = tile.low + it.split * part, key1 = min(tile.high, key0 + part);
+    tile.low = min(tile.low, tile.high) & ~int64_t(FEW_KEYS - 1);
+    const int all_steps = int((tile.high - tile.low + FEW_KEYS - 1) / FEW_KEYS), step0 = share.step_of(it, share.at, all_steps);
+    const int64_t key0 = tile.low + int64_t(step0) * FEW_KEYS, key1 = min(tile.high, tile.low + int64_t(share.step_of(it, share.end, all_steps)) * FEW_KEYS);
+    const bool began = share.at > it.line_begin, goes_on = share.end < it.line_end;
     const Keys own = keys_of(p, it, token, token);
     const Keys first = keys_of(p, it, first_token, first_token), last = keys_of(p, it, last_token, last_token);
 
@@ -628,7 +667,7 @@ __global__ void __launch_bounds__(256, 2) kv_attention_few(AttentionArgs p) {
         if (__ballot(high > top + LAG)) {
             LanePair o = swap16(high);
             o = swap32(fmaxf(o.a, o.b));
-            const float next = fmaxf(top, fmaxf(o.a, o.b)), keep = __builtin_amdgcn_exp2f(top - next);
+            const float next = fmaxf(top, fmaxf(o.a, o.b) - HEAD), keep = __builtin_amdgcn_exp2f(top - next);
             top = next;
             mass *= keep;
 #pragma unroll
@@ -672,8 +711,8 @@ __global__ void __launch_bounds__(256, 2) kv_attention_few(AttentionArgs p) {
         for (int j = 0; j < D / 16; ++j) o[j] = __builtin_fmaf(sums[w][r][c0 + j], keep, o[j]);
     }
     const int out_row = it.row0 + r;
-    if (it.splits > 1) {
-        float* slot = slot_of<FEW_ROWS, D>(p, it.item);
+    if (began || goes_on) {
+        float* slot = slot_of<FEW_ROWS, D>(p, 2 * share.index + !began);
         if (out_row < it.rows) {
 #pragma unroll
             for (int j = 0; j < D / 16; j += 4) *reinterpret_cast<v4f*>(slot + r * D + c0 + j) = v4f{o[j], o[j + 1], o[j + 2], o[j + 3]};
@@ -682,9 +721,8 @@ __global__ void __launch_bounds__(256, 2) kv_attention_few(AttentionArgs p) {
                 slot[FEW_ROWS * D + 2 * r + 1] = total;
             }
         }
-        return;
-    }
-    if (out_row >= it.rows) return;
+        if (!began) note_split(p, share, it);
+    } else if (out_row < it.rows) {
     const int out_token = out_row / p.group, out_member = out_row - out_token * p.group;
     uint16_t* out = static_cast<uint16_t*>(p.out) + (it.first_token + out_token) * p.out_token + (it.head * p.group + out_member) * p.out_head + c0;
 #pragma unroll
@@ -694,38 +732,53 @@ __global__ void __launch_bounds__(256, 2) kv_attention_few(AttentionArgs p) {
         for (int i = 0; i < 4; ++i) e[i] = Elem<DT>::from_f(finish(o[j + i], total));
         *reinterpret_cast<u32x2*>(out + j) = u32x2{e[0] | uint32_t(e[1]) << 16, e[2] | uint32_t(e[3]) << 16};
     }
+    }
+    share.at = it.line_end;
+    }
 }
 
 // ---- parts joined --------------------------------------------------------------------------------------------------
-// Adds the parts of a tile in order. WAVES waves a row (few rows in many parts: each takes every WAVES-th part, their sums then added
-// in order), 4 / WAVES rows at a time.
-template <int DT, int ROWS, int D, int ROWS_WG>
+// Adds the parts of a split tile, in order: a workgroup ROWS_WG rows, 4 / WAVES at a time, with WAVES waves a row (each takes every
+// WAVES-th part of a row's channels; their sums are then added in order). A wave's lanes first take the maxima and sums of up to 64
+// parts at once, then walk the channels with the parts' weights.
+template <int DT, int ROWS, int D, int ROWS_WG, int WAVES>
 __global__ void __launch_bounds__(256) kv_attention_join(AttentionArgs p) {
-    constexpr int WAVES = ROWS_WG == 1 ? 4 : 1, C = D / 64;
-    __shared__ float sums[4][D], masses[4], tops[4];
-    if (int(blockIdx.x) >= *p.tile_count) return;
-    const int4 tile = p.tiles[blockIdx.x];
-    const Span s = span_of<ROWS>(p, tile.w);
+    constexpr int C = D / 64;
+    typedef float vc __attribute__((ext_vector_type(C)));
+    __shared__ vc sums[4][64];
+    __shared__ float masses[4], tops[4];
+    const int4 tile = p.split_tiles[blockIdx.x];
+    const int head = p.split_heads[blockIdx.x], parts = tile.x;
+    if (parts < 2) return;
     const int wave = uniform(int(threadIdx.x) >> 6), lane = threadIdx.x & 63;
-    if (tile.y <= 1) return;
-    for (int i = WAVES == 4 ? 0 : wave; i < ROWS_WG; i += WAVES == 4 ? 1 : 4) {
-        const int r = blockIdx.y * ROWS_WG + i, row = tile.z + r;
-        if (row >= s.rows) return;
-        const int part0 = WAVES == 4 ? wave : 0;
-        float top = LOWEST;
-        for (int part = part0; part < tile.y; part += WAVES) top = fmaxf(top, slot_of<ROWS, D>(p, tile.x + part)[ROWS * D + 2 * r]);
-        float mass = 0.0f, acc[C] = {};
-#pragma unroll 4
-        for (int part = part0; part < tile.y; part += WAVES) {
-            const float* slot = slot_of<ROWS, D>(p, tile.x + part);
-            const float keep = __builtin_amdgcn_exp2f(slot[ROWS * D + 2 * r] - top);
-            mass = __builtin_fmaf(slot[ROWS * D + 2 * r + 1], keep, mass);
+    const auto slot_at = [&](int part) { return slot_of<ROWS, D>(p, 2 * (int(blockIdx.x) + part) + !part); };
+    for (int i = WAVES == 4 ? 0 : wave; i < ROWS_WG; i += 4 / WAVES) {
+        const int r = blockIdx.y * ROWS_WG + i, row = tile.y + r;
+        if (row >= tile.z) return;
+        float top = LOWEST, mass = 0.0f;
+        vc acc = {};
+        for (int base = WAVES == 4 ? wave : 0; base < parts; base += 64 * WAVES) {
+            const int part = base + lane * WAVES, count = min(64, (parts - base + WAVES - 1) / WAVES);
+            const float* end = slot_at(min(part, parts - 1)) + ROWS * D + 2 * r;
+            const float part_top = part < parts ? end[0] : LOWEST, part_mass = part < parts ? end[1] : 0.0f;
+            float next = part_top;
 #pragma unroll
-            for (int c = 0; c < C; ++c) acc[c] = __builtin_fmaf(slot[r * D + C * lane + c], keep, acc[c]);
+            for (int d = 1; d < 64; d <<= 1) next = fmaxf(next, __shfl_xor(next, d));
+            next = fmaxf(next, top);
+            const float keep = __builtin_amdgcn_exp2f(top - next), weight = __builtin_amdgcn_exp2f(part_top - next);
+            top = next;
+            mass = __builtin_fmaf(mass, keep, wave_sum(part_mass * weight));
+            acc *= keep;
+#pragma unroll 8
+            for (int j = 0; j < count; ++j) {
+                const vc x = *reinterpret_cast<const vc*>(slot_at(base + j * WAVES) + r * D + C * lane);
+                const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), j));
+#pragma unroll
+                for (int c = 0; c < C; ++c) acc[c] = __builtin_fmaf(x[c], w, acc[c]);
+            }
         }
         if constexpr (WAVES == 4) {
-#pragma unroll
-            for (int c = 0; c < C; ++c) sums[wave][C * lane + c] = acc[c];
+            sums[wave][lane] = acc;
             if (!lane) {
                 masses[wave] = mass;
                 tops[wave] = top;
@@ -734,76 +787,67 @@ __global__ void __launch_bounds__(256) kv_attention_join(AttentionArgs p) {
             if (wave) return;
             top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             mass = 0.0f;
-#pragma unroll
-            for (int c = 0; c < C; ++c) acc[c] = 0.0f;
+            acc = vc{};
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 const float keep = __builtin_amdgcn_exp2f(tops[w] - top);
                 mass = __builtin_fmaf(masses[w], keep, mass);
 #pragma unroll
-                for (int c = 0; c < C; ++c) acc[c] = __builtin_fmaf(sums[w][C * lane + c], keep, acc[c]);
+                for (int c = 0; c < C; ++c) acc[c] = __builtin_fmaf(sums[w][lane][c], keep, acc[c]);
             }
         }
         const int token = row / p.group, member = row - token * p.group;
-        uint16_t* out = static_cast<uint16_t*>(p.out) + (s.first_token + token) * p.out_token +
-                        (p.tile_heads[blockIdx.x] * p.group + member) * p.out_head + C * lane;
+        uint16_t* out = static_cast<uint16_t*>(p.out) + (tile.w + token) * p.out_token + (head * p.group + member) * p.out_head + C * lane;
 #pragma unroll
         for (int c = 0; c < C; ++c) out[c] = Elem<DT>::from_f(finish(acc[c], mass));
     }
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------------
-// Which launches serve a call, and their workspaces: few: requests of up to `limit` rows on tiles of 16; many: the others on tiles of 128.
+// Which launches serve a call, and their workspaces: [0] requests of up to `limit` rows on tiles of 16, [1] the others on tiles of 32 rows
+// a wave.
 struct Launches {
-    bool few, many;
-    int limit;
-    int64_t tiles[2];       // most tiles (of a request and head) of each
-    int split_items[2];
-    int64_t items[2], bytes[2];
+    bool used[2];
+    int limit, shares[2], waves;
+    int64_t bytes[2];
 };
 
 static int64_t align256(int64_t v) { return (v + 255) & ~int64_t(255); }
 
-static Launches plan_launches(int64_t tokens, int64_t requests, int64_t heads, int64_t group, int head_dim, int sms) {
+static Launches plan_launches(int64_t tokens, int64_t requests, int64_t group, int head_dim, int sms) {
     Launches l = {};
-    const int64_t rows = tokens * group, live = std::min(tokens, requests);
+    const int64_t rows = tokens * group;
     // A request's rows are known on the GPU alone. On average up to 16 a request: all on the tiles of few rows (one launch)
     l.limit = 32;
-    l.many = requests == 1 ? rows > l.limit : rows > FEW_ROWS * requests;
-    l.few = !l.many || requests > 1;
-    if (!l.many) l.limit = 0x7fffffff;
-    const int64_t most[2] = {l.many ? live * ((l.limit + FEW_ROWS - 1) / FEW_ROWS) : rows / FEW_ROWS + live, rows / TILE_ROWS + live};
-    const int64_t wanted[2] = {8 * int64_t(sms), 2 * int64_t(sms)};
-    const int tile_rows[2] = {FEW_ROWS, TILE_ROWS};
+    l.used[1] = requests == 1 ? rows > l.limit : rows > FEW_ROWS * requests;
+    l.used[0] = !l.used[1] || requests > 1;
+    if (!l.used[1]) l.limit = 0x7fffffff;
+    l.waves = head_dim == 256 ? 4 : 8;
+    const int per_cu[2] = {2, 1}, tile_rows[2] = {FEW_ROWS, 32 * l.waves};
     for (int i = 0; i < 2; ++i) {
-        l.tiles[i] = most[i] * heads;
-        // parts of keys where tiles alone are too few for the GPU; tiles of few rows always, requests being of many lengths
-        l.split_items[i] = i == 0 || l.tiles[i] < wanted[i] ? int(wanted[i]) : 0;
-        l.items[i] = l.tiles[i] + (l.split_items[i] ? l.split_items[i] + 64 : 0);
-        if ((i ? l.many : l.few) && l.split_items[i])
-            l.bytes[i] = 256 + align256(l.tiles[i] * 20) + align256(l.items[i] * tile_rows[i] * (head_dim + 2) * 4);
+        l.shares[i] = (per_cu[i] * sms + 7) & ~7;
+        if (l.used[i]) l.bytes[i] = align256(int64_t(l.shares[i]) * 20) + align256(int64_t(l.shares[i]) * 2 * tile_rows[i] * (head_dim + 2) * 4);
     }
     return l;
 }
 
 template <int DT, int D> static int launch_attention(AttentionArgs p, const Launches& l, char* workspace, hipStream_t stream) {
     for (int i = 0; i < 2; ++i) {
-        if (!(i ? l.many : l.few)) continue;
+        if (!l.used[i]) continue;
         p.few_rows = i ? l.limit : 0;
         p.many_rows = i ? 0x7fffffff : l.limit;
-        p.split_items = l.split_items[i];
-        p.max_items = int(l.items[i]);
+        p.shares = l.shares[i];
         char* at = workspace + (i ? l.bytes[0] : 0);
-        p.tile_count = reinterpret_cast<int*>(at);
-        p.tiles = reinterpret_cast<int4*>(at + 256);
-        p.tile_heads = reinterpret_cast<int*>(p.tiles + l.tiles[i]);
-        p.slots = reinterpret_cast<float*>(at + 256 + align256(l.tiles[i] * 20));
-        const unsigned grid = unsigned((l.items[i] + 7) & ~int64_t(7));
-        if (i) kv_attention_tiles<DT, D><<<grid, 256, 0, stream>>>(p);
-        else kv_attention_few<DT, D><<<grid, 256, 0, stream>>>(p);
-        if (p.split_items) {
-            if (i) kv_attention_join<DT, TILE_ROWS, D, 16><<<dim3(unsigned(l.tiles[i]), TILE_ROWS / 16), 256, 0, stream>>>(p);
-            else kv_attention_join<DT, FEW_ROWS, D, 1><<<dim3(unsigned(l.tiles[i]), FEW_ROWS), 256, 0, stream>>>(p);
+        p.split_tiles = reinterpret_cast<int4*>(at);
+        p.split_heads = reinterpret_cast<int*>(p.split_tiles + p.shares);
+        p.slots = reinterpret_cast<float*>(at + align256(int64_t(p.shares) * 20));
+        if (i) {
+            constexpr int WAVES = D == 256 ? 4 : 8;
+            kv_attention_tiles<DT, D, WAVES><<<p.shares, 64 * WAVES, 0, stream>>>(p);
+            kv_attention_join<DT, 32 * WAVES, D, 16, 1><<<dim3(p.shares, 2 * WAVES), 256, 0, stream>>>(p);
+        } else {
+            kv_attention_few<DT, D><<<p.shares, 256, 0, stream>>>(p);
+            kv_attention_join<DT, FEW_ROWS, D, 1, 4><<<dim3(p.shares, FEW_ROWS), 256, 0, stream>>>(p);
         }
     }
     return int(hipGetLastError());
@@ -816,7 +860,7 @@ using namespace wq8;
 WQ8_API void wq8_kv_attention_workspace(int tokens, int requests, int heads, int group, int head_dim, int sms, int64_t* sizes) {
     sizes[0] = sizes[1] = 0;
     if (tokens < 1 || requests < 1 || heads < 1 || group < 1) return;
-    const Launches l = plan_launches(tokens, requests, heads, group, head_dim, sms);
+    const Launches l = plan_launches(tokens, requests, group, head_dim, sms);
     sizes[0] = l.bytes[0] + l.bytes[1];
 }
 
@@ -829,9 +873,8 @@ WQ8_API int wq8_kv_attention(const void* q, void* out, const long long* strides,
         (block != 16 && block != 32 && block != 64 && block != 128) || window < 0 || pages < 0 || pages > 0x7fffffff || width < 0 || sms < 1)
         return -2;
     if (!tokens || !requests) return 0;
-    // rows and items are counted in 32 bits
-    if (int64_t(tokens) * group > 0x7fffffff - TILE_ROWS || (int64_t(tokens) * group / FEW_ROWS + requests) * heads > (1 << 30)) return -2;
-    const Launches l = plan_launches(tokens, requests, heads, group, head_dim, sms);
+    if (int64_t(tokens) * group > 0x7fffffff - 256) return -2;  // rows are counted in 32 bits
+    const Launches l = plan_launches(tokens, requests, group, head_dim, sms);
     if ((l.bytes[0] + l.bytes[1] && !workspace) || reinterpret_cast<uintptr_t>(workspace) % 16) return -2;
     AttentionArgs p = {};
     p.q = q; p.out = out;
