@@ -425,15 +425,37 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
             };
             if (wave >= 4) next();
             if (base < some_high && base + STEP_KEYS > some_low) {
-                v16f s[2];
+                // Stages of four matrix instructions, whose operands the stage before has read: what is between two
+                // sched_barriers stays there
+                v16f s[2] = {};
+                f16x8 now[4], then[4];
+                const auto read_keys = [&](f16x8* to, int stage) {
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    s[b] = v16f{};
-#pragma unroll
-                    for (int f = 0; f < KF; ++f) {
-                        const f16x8 k = __builtin_bit_cast(f16x8, k_lds[buffer][(b * KF + f) * 64 + (lane ^ (SWZ * f & 15))]);
-                        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, query[f], s[b], 0, 0, 0);
+                    for (int i = 0; i < 4; ++i) {
+                        const int f = (4 * stage + i) % KF, h = (4 * stage + i) / KF;
+                        to[i] = __builtin_bit_cast(f16x8, k_lds[buffer][(h * KF + f) * 64 + (lane ^ (SWZ * f & 15))]);
                     }
+                };
+                const auto read_values = [&](f16x8* to, int stage) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int c = (4 * stage + i) % (D / 32), g = (4 * stage + i) / (D / 32);
+                        to[i] = __builtin_bit_cast(f16x8, v_lds[buffer][(c * 4 + g) * 64 + (v_entry ^ (8 * (c & 1)))]);
+                    }
+                };
+                read_keys(now, 0);
+#pragma unroll
+                for (int stage = 0; stage < KF / 2; ++stage) {
+                    if (stage + 1 < KF / 2) read_keys(then, stage + 1);
+                    else read_values(then, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int f = (4 * stage + i) % KF, h = (4 * stage + i) / KF;
+                        s[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now[i], query[f], s[h], 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) now[i] = then[i];
                 }
                 // t = a s + b of the 16 keys of a page
                 v4f a = page_k[buffer] * query_scale, b = page_log_v[buffer];
@@ -467,21 +489,38 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
                     for (int i = 0; i < D / 32; ++i) acc[i] *= keep;
                 }
                 b -= top;
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
+                const auto weights_of = [&](int g) {
                     float w[8], sum = 0.0f;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 1][8 * (g & 1) + i], a[g], b[g]));
                         sum += w[i];
                     }
-                    const f16x8 weights = weights8(w);
                     mass = __builtin_fmaf(sum, inv_v[g], mass);
+                    return weights8(w);
+                };
+                constexpr int PER = D / 128 ? D / 128 : 1, WIDE = 4 / (D / 32) ? 4 / (D / 32) : 1;  // stages a page, pages a stage
+                f16x8 weights[WIDE], next_weights[WIDE];
 #pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        const f16x8 v = __builtin_bit_cast(f16x8, v_lds[buffer][(c * 4 + g) * 64 + (v_entry ^ (8 * (c & 1)))]);
-                        acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, weights, acc[c], 0, 0, 0);
+                for (int i = 0; i < WIDE; ++i) weights[i] = weights_of(i);
+#pragma unroll
+                for (int stage = 0; stage < D / 32; ++stage) {
+                    if (stage + 1 < D / 32) read_values(then, stage + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    const bool turn = (stage + 1) % PER == 0 && stage + 1 < D / 32;  // the next stage takes other pages' weights
+                    if (turn)
+#pragma unroll
+                        for (int i = 0; i < WIDE; ++i) next_weights[i] = weights_of((stage + 1) / PER * WIDE + i);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int c = (4 * stage + i) % (D / 32), g = (4 * stage + i) / (D / 32);
+                        acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now[i], weights[g % WIDE], acc[c], 0, 0, 0);
                     }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) now[i] = then[i];
+                    if (turn)
+#pragma unroll
+                        for (int i = 0; i < WIDE; ++i) weights[i] = next_weights[i];
                 }
             }
             if (wave < 4) next();
