@@ -134,7 +134,7 @@ int wq8_kv_plan(const void* past, const void* fresh, int32_t* tables, int64_t ta
                 int32_t* missing, wq8_stream_t stream);
 
 /* Rows (tokens, heads, head_dim) of dtype 0-2 into the cache at slots; strides (host): {token, head} of k, of v, in elements; rows 16-byte
- * aligned; block up to 128, head_dim a multiple of 8 up to 1024; owner: pages * block int32 of scratch, never cleared. */
+ * aligned; block a power of two up to 128, head_dim a multiple of 8 up to 1024; owner: pages * block int32 of scratch, never cleared. */
 int wq8_kv_write(const void* k, const void* v, const long long* strides, const long long* slots, int64_t tokens, int8_t* k_codes, float* k_scales,
                  int8_t* v_codes, float* v_scales, int64_t pages, int heads, int block, int head_dim, int dtype, int32_t* owner, wq8_stream_t stream);
 

@@ -158,14 +158,17 @@ def test_values_that_are_not_finite(wq):
     cache = wq.KVCache(3, 2, 64, 16)
     k = torch.randn(4, 2, 64, device="cuda").bfloat16()
     wq.kv_write(cache, k, k, ints([16, 17, 32, 33], torch.int64))
-    good = wq.kv_read(cache, ints([16, 32, 33], torch.int64))
+    good, before = wq.kv_read(cache, ints([16, 32, 33], torch.int64)), cache.k_scales.clone()
     bad = k[:2].clone()
     bad[0, 0, 5], bad[1, 1, 3] = math.nan, -math.inf
     wq.kv_write(cache, bad, bad, ints([18, 34], torch.int64))
     assert all(torch.isfinite(t).all() for t in (cache.k_scales, cache.v_scales))
     again = wq.kv_read(cache, ints([16, 32, 33], torch.int64))
+    # where the new tokens' finite values made a scale grow, tokens were coded again: within half a step of what they were (and read in BF16)
+    grown = torch.where(cache.k_scales > before, step_of(cache.k_scales), 0.0)
     for a, b in zip(good, again):
-        assert (a[:1] - b[:1]).abs().max() <= 2 * cache.k_scales[1].max() and torch.equal(a[1:, 0], b[1:, 0])
+        off = (a.double() - b.double()).abs() - 2.0 ** -8 * (a.double().abs() + b.double().abs()) * (a != b)
+        assert (off[:1] <= grown[1][:, None]).all() and (off[1:, 0] <= grown[2, 0]).all()
     k, _ = wq.kv_read(cache, ints([18, 34], torch.int64), torch.float32)
     assert k[0, 0, 5] == 0 and abs(k[1, 1, 3].item() / -torch.finfo(torch.float32).max - 1) < 2 ** -20
 

@@ -129,8 +129,8 @@ struct CacheArgs {
     float* scales[2];
     const int64_t* slots;
     int* owner;
-    int64_t tokens, pages;
-    int heads, block, head_dim;
+    int64_t tokens, all_slots;
+    int heads, block_log2, head_dim, group;  // group: tokens a workgroup looks through (kv_write_owned)
 };
 
 // owner[slot] = the token written there. Nothing clears it: an entry holds if it names a token of this call whose slot it is,
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(256) kv_owner(CacheArgs p) {
     const int64_t t = blockIdx.x * int64_t(256) + threadIdx.x;
     if (t >= p.tokens) return;
     const int64_t slot = p.slots[t];
-    if (slot >= 0 && slot < p.pages * p.block) p.owner[slot] = int(t);
+    if (slot >= 0 && slot < p.all_slots) p.owner[slot] = int(t);
 }
 
 // A finite value for the cache: NaN counts as zero, infinities as the largest finite number (a few steps below it: 127 times the
@@ -166,45 +166,85 @@ WQ8_DEVICE float block_max(float v, float* lds4) {
     return fmaxf(fmaxf(lds4[0], lds4[1]), fmaxf(lds4[2], lds4[3]));
 }
 
+// 8 consecutive channels as they are in memory.
+template <int DT> struct Raw8 {
+    u32x4 v[DT == DT_F32 ? 2 : 1];
+    WQ8_DEVICE void load(const typename Elem<DT>::raw* p) {
+        v[0] = reinterpret_cast<const u32x4*>(p)[0];
+        if constexpr (DT == DT_F32) v[1] = reinterpret_cast<const u32x4*>(p)[1];
+    }
+    WQ8_DEVICE void zero() {
+        v[0] = u32x4{0, 0, 0, 0};
+        if constexpr (DT == DT_F32) v[1] = v[0];
+    }
+    WQ8_DEVICE float value(int j) const {
+        if constexpr (DT == DT_F32) return cached_value(__builtin_bit_cast(float, uint32_t(v[j >> 2][j & 3])));
+        else return cached_value(Elem<DT>::to_f(uint16_t(v[0][j >> 1] >> (16 * (j & 1)))));
+    }
+};
+
 // One page and head: rows[] names the token of each of its slots that is written, -1 for the others. The scale becomes the larger
 // of the held one (none when the page's first slot is written: the page begins anew) and the new tokens' amax / 127; tokens
-// that the page held are coded again where it grew.
-template <int DT> WQ8_DEVICE void write_page(const CacheArgs& p, int which, int64_t page, int head, const int* rows, float* lds4) {
+// that the page held are coded again where it grew. NI: vectors of 8 channels a thread, kept in registers between the maximum and the
+// codes (0: any number, read twice).
+template <int DT, int NI> WQ8_DEVICE void write_page(const CacheArgs& p, int which, int64_t page, int head, const int* rows, float* lds4) {
     using raw = typename Elem<DT>::raw;
-    const int per_row = p.head_dim >> 3, items = p.block * per_row;
+    const int block = 1 << p.block_log2, per_row = p.head_dim >> 3, items = block * per_row;
+    const int row_step = 256 / per_row, chunk_step = 256 - row_step * per_row;
+    const int row0 = int(threadIdx.x) / per_row, chunk0 = int(threadIdx.x) - row0 * per_row;
     const raw* x = static_cast<const raw*>(p.x[which]) + head * p.head_stride[which];
-    float amax = 0.0f;
-    for (int i = threadIdx.x; i < items; i += 256) {
-        const int r = i / per_row, t = rows[r];
-        if (t < 0) continue;
-        float v[8];
-        load8<DT>(x + t * p.token_stride[which] + 8 * (i - r * per_row), v, true);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, __builtin_fabsf(cached_value(v[j])));
-    }
-    amax = block_max(amax, lds4);
     float* held = p.scales[which] + page * p.heads + head;
-    const float old = rows[0] >= 0 ? 0.0f : fmaxf(*held, 0.0f);
+    const float was = *held;
+    Raw8<DT> kept[NI ? NI : 1];
+    float amax = 0.0f;
+    // the thread's vectors: (row, chunk) from (row0, chunk0) on, 256 vectors apart
+    const auto each = [&](auto body) {
+        int row = row0, chunk = chunk0;
+        const auto step = [&](int n) {
+            if (row < block) body(n, row, chunk);
+            row += row_step;
+            chunk += chunk_step;
+            if (chunk >= per_row) { chunk -= per_row; ++row; }
+        };
+        if constexpr (NI > 0) {
+#pragma unroll
+            for (int n = 0; n < NI; ++n) step(n);
+        } else {
+            for (int i = threadIdx.x; i < items; i += 256) step(0);
+        }
+    };
+    const auto largest = [&](const Raw8<DT>& v) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, __builtin_fabsf(v.value(j)));
+    };
+    each([&](int n, int row, int chunk) {
+        const int t = rows[row];
+        if (t >= 0) kept[n].load(x + t * p.token_stride[which] + 8 * chunk);
+        else kept[n].zero();
+        if constexpr (!NI) largest(kept[0]);
+    });
+    if constexpr (NI > 0) each([&](int n, int, int) { largest(kept[n]); });
+    amax = block_max(amax, lds4);
+    const float old = rows[0] >= 0 ? 0.0f : fmaxf(was, 0.0f);
     const float scale = fmaxf(old, div127(amax));
     const float by = scale > 0.0f ? scale : 1.0f, inv = 1.0f / by, again = old / by;
-    int8_t* codes = p.codes[which] + (page * p.heads + head) * int64_t(p.block) * p.head_dim;
-    for (int i = threadIdx.x; i < items; i += 256) {
-        const int r = i / per_row, c = i - r * per_row, t = rows[r];
-        u32x2* at = reinterpret_cast<u32x2*>(codes + r * p.head_dim + 8 * c);
+    int8_t* codes = p.codes[which] + ((page * p.heads + head) << p.block_log2) * p.head_dim;
+    each([&](int n, int row, int chunk) {
+        const int t = rows[row];
+        u32x2* at = reinterpret_cast<u32x2*>(codes + row * p.head_dim + 8 * chunk);
         int q[8];
         if (t >= 0) {
-            float v[8];
-            load8<DT>(x + t * p.token_stride[which] + 8 * c, v, true);
+            if constexpr (!NI) kept[0].load(x + t * p.token_stride[which] + 8 * chunk);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) q[j] = code_of(cached_value(v[j]), by, inv);
+            for (int j = 0; j < 8; ++j) q[j] = code_of(kept[n].value(j), by, inv);
         } else {
-            if (!(old < scale) || old == 0.0f) continue;
+            if (!(old < scale) || old == 0.0f) return;
             const u32x2 before = *at;
 #pragma unroll
             for (int j = 0; j < 8; ++j) q[j] = rne_int(float(int8_t(before[j >> 2] >> (8 * (j & 3)))) * again);
         }
         *at = u32x2{pack_s8x4(q[0], q[1], q[2], q[3]), pack_s8x4(q[4], q[5], q[6], q[7])};
-    }
+    });
     __syncthreads();  // every thread has read the held scale
     if (!threadIdx.x) *held = scale;
 }
@@ -212,98 +252,113 @@ template <int DT> WQ8_DEVICE void write_page(const CacheArgs& p, int which, int6
 constexpr int KV_MAX_BLOCK = 128;
 // Up to this many tokens a workgroup reads every slot by itself to find its page's tokens, and the owner pass is left out.
 constexpr int KV_SCAN_TOKENS = 512;
-constexpr int KV_OWNED_TOKENS = 16;
 
-template <int DT>
+template <int DT, int NI>
 __global__ void __launch_bounds__(256) kv_write_scan(CacheArgs p) {
     __shared__ int rows[KV_MAX_BLOCK];
     __shared__ float lds4[4];
-    const int token = blockIdx.x, head = blockIdx.y, which = blockIdx.z;
+    const int token = blockIdx.x, head = blockIdx.y, which = blockIdx.z, block = 1 << p.block_log2;
     const int64_t slot = p.slots[token];
-    if (slot < 0 || slot >= p.pages * p.block) return;
-    const int64_t page = slot / p.block;
-    const int at = int(slot - page * p.block);
-    for (int i = threadIdx.x; i < p.block; i += 256) rows[i] = -1;
+    if (slot < 0 || slot >= p.all_slots) return;
+    const int64_t page = slot >> p.block_log2, page_slot = page << p.block_log2;
+    const int at = int(slot - page_slot);
+    if (int(threadIdx.x) < block) rows[threadIdx.x] = -1;
     __syncthreads();
     for (int t = threadIdx.x; t < p.tokens; t += 256) {
-        const int64_t s = p.slots[t] - page * p.block;
-        if (s >= 0 && s < p.block) atomicMax(&rows[s], t);
+        const int64_t s = p.slots[t] - page_slot;
+        if (s >= 0 && s < block) atomicMax(&rows[s], t);
     }
     __syncthreads();
     // the page is its lowest slot's token's
     if (rows[at] != token) return;
     for (int i = 0; i < at; ++i)
         if (rows[i] >= 0) return;
-    write_page<DT>(p, which, page, head, rows, lds4);
+    write_page<DT, NI>(p, which, page, head, rows, lds4);
 }
 
-template <int DT>
+// Many tokens: a workgroup looks through p.group of them (64 at most) for those that have the lowest written slot of a page, and writes these
+// pages' codes of one head, keys and values.
+template <int DT, int NI>
 __global__ void __launch_bounds__(256) kv_write_owned(CacheArgs p) {
     __shared__ int rows[KV_MAX_BLOCK];
-    __shared__ int lowest[KV_OWNED_TOKENS];
+    __shared__ int64_t pages[64];
     __shared__ float lds4[4];
-    const int head = blockIdx.y, which = blockIdx.z;
+    const int head = blockIdx.y, block = 1 << p.block_log2;
     const auto writer = [&](int64_t slot) {
         const int t = p.owner[slot];
         return t >= 0 && t < p.tokens && p.slots[t] == slot ? t : -1;
     };
-    if (threadIdx.x < KV_OWNED_TOKENS) {
-        const int64_t token = blockIdx.x * int64_t(KV_OWNED_TOKENS) + threadIdx.x;
-        int mine = 0;
-        if (token < p.tokens) {
+    if (threadIdx.x < 64) {
+        const int64_t token = blockIdx.x * int64_t(p.group) + threadIdx.x;
+        int64_t page = -1;
+        if (int(threadIdx.x) < p.group && token < p.tokens) {
             const int64_t slot = p.slots[token];
-            if (slot >= 0 && slot < p.pages * p.block && writer(slot) == token) {
-                mine = 1;
-                for (int64_t s = slot - 1; s >= slot / p.block * p.block && mine; --s) mine = writer(s) < 0;
+            if (slot >= 0 && slot < p.all_slots) {
+                const int64_t begin = slot >> p.block_log2 << p.block_log2;
+                bool lowest = p.owner[slot] == token;
+                for (int64_t s = slot - 1; s >= begin && lowest; --s) lowest = writer(s) < 0;
+                if (lowest) page = slot >> p.block_log2;
             }
         }
-        lowest[threadIdx.x] = mine;
+        pages[threadIdx.x] = page;
     }
     __syncthreads();
-    for (int i = 0; i < KV_OWNED_TOKENS; ++i) {
-        if (!lowest[i]) continue;
-        const int64_t page = p.slots[blockIdx.x * int64_t(KV_OWNED_TOKENS) + i] / p.block;
-        for (int r = threadIdx.x; r < p.block; r += 256) rows[r] = writer(page * p.block + r);
+    for (int i = 0; i < p.group; ++i) {
+        const int64_t page = pages[i];
+        if (page < 0) continue;
+        if (int(threadIdx.x) < block) rows[threadIdx.x] = writer((page << p.block_log2) + threadIdx.x);
         __syncthreads();
-        write_page<DT>(p, which, page, head, rows, lds4);
+        for (int which = blockIdx.z; which < 2; which += gridDim.z) write_page<DT, NI>(p, which, page, head, rows, lds4);
         __syncthreads();
     }
 }
 
-template <int DT> static int launch_write(const CacheArgs& p, hipStream_t stream) {
+template <int DT, int NI> static int launch_pages(CacheArgs p, hipStream_t stream) {
     if (p.tokens <= KV_SCAN_TOKENS) {
-        kv_write_scan<DT><<<dim3(unsigned(p.tokens), p.heads, 2), 256, 0, stream>>>(p);
+        kv_write_scan<DT, NI><<<dim3(unsigned(p.tokens), p.heads, 2), 256, 0, stream>>>(p);
     } else {
+        // tokens a workgroup: fewer where workgroups are few (each token may have a page of its own); keys and values in one where they are many
+        p.group = 64;
+        while (p.group > 4 && p.tokens * p.heads * 2 < p.group * int64_t(4096)) p.group >>= 1;
+        const int64_t groups = (p.tokens + p.group - 1) / p.group;
         kv_owner<<<unsigned((p.tokens + 255) / 256), 256, 0, stream>>>(p);
-        kv_write_owned<DT><<<dim3(unsigned((p.tokens + KV_OWNED_TOKENS - 1) / KV_OWNED_TOKENS), p.heads, 2), 256, 0, stream>>>(p);
+        kv_write_owned<DT, NI><<<dim3(unsigned(groups), p.heads, groups * p.heads >= 4096 ? 1 : 2), 256, 0, stream>>>(p);
     }
     return int(hipGetLastError());
+}
+
+template <int DT> static int launch_write(const CacheArgs& p, hipStream_t stream) {
+    const int vectors = (p.head_dim << p.block_log2) + 2047 >> 11;
+    return vectors <= 1 ? launch_pages<DT, 1>(p, stream) : vectors <= 2 ? launch_pages<DT, 2>(p, stream) : vectors <= 4 ? launch_pages<DT, 4>(p, stream)
+         : vectors <= 8 ? launch_pages<DT, 8>(p, stream) : vectors <= 16 ? launch_pages<DT, 16>(p, stream) : launch_pages<DT, 0>(p, stream);
 }
 
 // ---- reads ---------------------------------------------------------------------------------------------------------
 template <int DT>
 __global__ void __launch_bounds__(256) kv_read_rows(CacheArgs p) {
     using raw = typename Elem<DT>::raw;
-    const int per_row = p.head_dim >> 3, which = blockIdx.y;
-    const int64_t i = blockIdx.x * int64_t(256) + threadIdx.x;
-    const int64_t row = i / per_row, token = row / p.heads;
+    const int per_row = p.head_dim >> 3, per_token = p.heads * per_row, which = blockIdx.y;
+    // vector blockIdx.x * 256 + threadIdx.x of (token, head, chunk): the wide division is the workgroup's alone
+    const int64_t token0 = blockIdx.x * int64_t(256) / per_token;
+    const unsigned in = unsigned(blockIdx.x * int64_t(256) - token0 * per_token) + threadIdx.x;
+    const int64_t token = token0 + in / unsigned(per_token);
     if (token >= p.tokens) return;
-    const int head = int(row - token * p.heads), c = int(i - row * per_row);
+    const unsigned rest = in % unsigned(per_token), head = rest / unsigned(per_row), c = rest % unsigned(per_row);
     const int64_t slot = p.slots[token];
     float v[8] = {};
-    if (slot >= 0 && slot < p.pages * p.block) {
-        const int64_t page = slot / p.block, at = slot - page * p.block;
-        const float scale = p.scales[which][page * p.heads + head];
-        const u32x2 q = *reinterpret_cast<const u32x2*>(p.codes[which] + ((page * p.heads + head) * p.block + at) * p.head_dim + 8 * c);
+    if (slot >= 0 && slot < p.all_slots) {
+        const int64_t row = (slot >> p.block_log2) * p.heads + head;
+        const float scale = p.scales[which][row];
+        const u32x2 q = *reinterpret_cast<const u32x2*>(p.codes[which] + ((row << p.block_log2) + (slot & ((1 << p.block_log2) - 1))) * p.head_dim + 8 * c);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = float(int8_t(q[j >> 2] >> (8 * (j & 3)))) * scale;
     }
-    store8<DT>(static_cast<raw*>(p.y[which]) + row * p.head_dim + 8 * c, v);
+    store8<DT>(static_cast<raw*>(p.y[which]) + (token * per_token + rest) * 8, v);
 }
 
 static bool bad_cache(int64_t tokens, int64_t pages, int heads, int block, int head_dim) {
     return tokens < 0 || tokens > 0x7fffffff || pages < 0 || heads < 1 || heads > 65535 || head_dim < 8 || head_dim % 8 || head_dim > 1024 ||
-           block < 1 || block > KV_MAX_BLOCK || pages > (int64_t(1) << 62) / block;
+           block < 1 || block > KV_MAX_BLOCK || (block & (block - 1)) || pages > 0x7fffffff;
 }
 
 }  // namespace wq8
@@ -327,7 +382,7 @@ WQ8_API int wq8_kv_write(const void* k, const void* v, const long long* strides,
     if (bad_cache(tokens, pages, heads, block, head_dim)) return -2;
     if (!tokens || !pages) return 0;
     const CacheArgs p = {{k, v}, {}, {strides[0], strides[2]}, {strides[1], strides[3]}, {k_codes, v_codes}, {k_scales, v_scales},
-                         reinterpret_cast<const int64_t*>(slots), owner, tokens, pages, heads, block, head_dim};
+                         reinterpret_cast<const int64_t*>(slots), owner, tokens, pages * block, heads, __builtin_ctz(block), head_dim, 0};
     return dtype == DT_F16 ? launch_write<DT_F16>(p, stream) : dtype == DT_BF16 ? launch_write<DT_BF16>(p, stream) : launch_write<DT_F32>(p, stream);
 }
 
@@ -337,8 +392,8 @@ WQ8_API int wq8_kv_read(const int8_t* k_codes, const float* k_scales, const int8
     if (bad_cache(tokens, pages, heads, block, head_dim)) return -2;
     if (!tokens) return 0;
     const CacheArgs p = {{}, {k, v}, {}, {}, {const_cast<int8_t*>(k_codes), const_cast<int8_t*>(v_codes)},
-                         {const_cast<float*>(k_scales), const_cast<float*>(v_scales)}, reinterpret_cast<const int64_t*>(slots), nullptr, tokens, pages, heads,
-                         block, head_dim};
+                         {const_cast<float*>(k_scales), const_cast<float*>(v_scales)}, reinterpret_cast<const int64_t*>(slots), nullptr, tokens, pages * block,
+                         heads, __builtin_ctz(block), head_dim, 0};
     const int64_t blocks = (tokens * heads * (head_dim >> 3) + 255) / 256;
     if (blocks > 0x7fffffff) return -2;
     const dim3 grid(static_cast<unsigned>(blocks), 2);
