@@ -16,7 +16,7 @@ from typing import NamedTuple
 import torch
 
 from . import DTYPES, _native, library
-from ._rotary import _check_device, _check_rows
+from ._rotary import Layouts, _check_places, _check_rows
 
 BLOCKS = (16, 32, 64, 128)
 ATTENTION_HEAD_DIMS = (64, 128, 256)
@@ -34,7 +34,7 @@ class KVPlan(NamedTuple):
 
 class KVCache:
     """An empty cache of `pages` pages of `block` tokens (16, 32, 64 or 128) on a GPU."""
-    __slots__ = ("k_codes", "k_scales", "v_codes", "v_scales", "owner")
+    __slots__ = ("k_codes", "k_scales", "v_codes", "v_scales", "owner", "layouts")
 
     def __init__(self, pages, heads, head_dim, block=64, device="cuda"):
         codes = lambda: torch.zeros(pages, heads, block, head_dim, dtype=torch.int8, device=device)
@@ -62,6 +62,7 @@ class KVCache:
         if any(t.device != k_codes.device for t in parts):
             raise ValueError("cache codes and scales must be on one device")
         self.k_codes, self.k_scales, self.v_codes, self.v_scales = parts
+        self.layouts = Layouts()
         # which token of a kv_write() call each slot takes: scratch of that call (entries are checked, never cleared)
         self.owner = torch.empty(k_codes.shape[0] * k_codes.shape[2], dtype=torch.int32, device=k_codes.device)
 
@@ -90,6 +91,27 @@ def kv_plan(past, new, tables, free, used, block, tokens):
     the table's width, `tokens` or the free pages left cannot hold gets no page, slots -1 and its old length, and so does
     every later one that needs a page where the free list ran out. Everything is int32 / int64 on the GPU; nothing is read
     on the host."""
+    key = (past.shape, past.dtype, past.stride(), new.shape, new.dtype, new.stride(), free.shape, free.dtype, free.stride(), tables.shape, tables.stride(),
+           tables.dtype, used.shape, used.dtype, block, tokens)
+    splits = _plan_layouts.get(key) or _plan_layouts.keep(key, _check_plan(past, new, tables, free, used, block, tokens))
+    _check_places(past.get_device(), (), (new, tables, free, used))
+    slots = past.new_empty(tokens, dtype=torch.int64)
+    held = past.new_empty(tokens + 2 * splits[2] + 3)
+    positions, starts, lens, used_out, missing = held.split(splits)
+    requests, at = splits[2], held.data_ptr()
+    starts_at = at + 4 * tokens
+    lens_at = starts_at + 4 * requests + 4
+    used_at = lens_at + 4 * requests
+    library().call("wq8_kv_plan", past.data_ptr(), new.data_ptr(), tables.data_ptr(), tables.stride(0), free.data_ptr(), free.shape[0], used.data_ptr(),
+                   requests, tables.shape[1], block, tokens, slots.data_ptr(), at, starts_at, lens_at, used_at, used_at + 4, _native.gpu(past).stream())
+    return KVPlan(slots, positions, starts, lens, used_out, missing)
+
+
+_plan_layouts = Layouts()
+
+
+def _check_plan(past, new, tables, free, used, block, tokens):
+    """Lengths of a plan's int32 results."""
     _check_ints(past, "past")
     _check_ints(new, "new")
     _check_ints(free, "free")
@@ -101,52 +123,50 @@ def kv_plan(past, new, tables, free, used, block, tokens):
         raise ValueError(f"past, new and tables must be of as many requests, not {requests}, {new.shape[0]} and {tables.shape[0]}")
     if block < 1 or not 0 <= tokens < 2 ** 31:
         raise ValueError("a block of at least one token and a token count are wanted")
-    _check_device(past.get_device(), new=new, tables=tables, free=free, used=used)
-    state = _native.gpu(past)
-    slots = torch.empty(tokens, dtype=torch.int64, device=past.device)
-    positions, starts, lens, used_out, missing = torch.empty(tokens + 2 * requests + 3, dtype=torch.int32, device=past.device).split(
-        [tokens, requests + 1, requests, 1, 1])
-    library().call("wq8_kv_plan", past.data_ptr(), new.data_ptr(), tables.data_ptr(), tables.stride(0), free.data_ptr(), free.shape[0], used.data_ptr(),
-                   requests, tables.shape[1], block, tokens, slots.data_ptr(), positions.data_ptr(), starts.data_ptr(), lens.data_ptr(),
-                   used_out.data_ptr(), missing.data_ptr(), state.stream())
-    return KVPlan(slots, positions, starts, lens, used_out, missing)
+    return [tokens, requests + 1, requests, 1, 1]
+
+
+def _check_write(cache, k, v, slots):
+    _check_rows(k, "keys")
+    _check_rows(v, "values")
+    _check_ints(slots, "slots", torch.int64)
+    if k.shape != v.shape or k.dtype != v.dtype or k.shape[1:] != (cache.heads, cache.head_dim) or slots.shape[0] != k.shape[0]:
+        raise ValueError(f"keys and values must be (tokens, {cache.heads}, {cache.head_dim}), of one type, with a slot each")
+    return (ctypes.c_longlong * 4)(k.stride(0), k.stride(1), v.stride(0), v.stride(1)), k.shape[0], DTYPES[k.dtype], (cache.pages, cache.heads, cache.block, cache.head_dim)
 
 
 def kv_write(cache, k, v, slots):
     """Keys and values (tokens, heads, head_dim), BF16, FP16 or FP32, into the cache at `slots` (int64; any order, each at most once;
     those outside the cache, as -1, are left out). A page's scale grows to its largest value, and tokens that it holds are then
     coded again; a write to its first slot begins it anew. NaN is held as 0 and infinities as the largest finite number."""
-    _check_rows(k, "keys")
-    _check_rows(v, "values")
-    _check_ints(slots, "slots", torch.int64)
+    key = (k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, slots.shape, slots.stride(), slots.dtype)
+    strides, tokens, dtype, shape = cache.layouts.get(key) or cache.layouts.keep(key, _check_write(cache, k, v, slots))
     codes = cache.k_codes
-    pages, heads, block, head_dim = codes.shape
-    if k.shape != v.shape or k.dtype != v.dtype or k.shape[1:] != (heads, head_dim) or slots.shape[0] != k.shape[0]:
-        raise ValueError(f"keys and values must be (tokens, {heads}, {head_dim}), of one type, with a slot each")
-    device = codes.get_device()
-    _check_device(device, keys=k, values=v, slots=slots)
-    sk, sv = k.stride(), v.stride()
-    library().call("wq8_kv_write", k.data_ptr(), v.data_ptr(), (ctypes.c_longlong * 4)(sk[0], sk[1], sv[0], sv[1]), slots.data_ptr(), k.shape[0],
-                   codes.data_ptr(), cache.k_scales.data_ptr(), cache.v_codes.data_ptr(), cache.v_scales.data_ptr(), pages, heads, block, head_dim,
-                   DTYPES[k.dtype], cache.owner.data_ptr(), _native.gpu(codes).stream())
+    k_at, v_at = _check_places(codes.get_device(), (k, v), (slots,))
+    library().call("wq8_kv_write", k_at, v_at, strides, slots.data_ptr(), tokens, codes.data_ptr(), cache.k_scales.data_ptr(), cache.v_codes.data_ptr(),
+                   cache.v_scales.data_ptr(), *shape, dtype, cache.owner.data_ptr(), _native.gpu(codes).stream())
 
 
 def kv_read(cache, slots, dtype=torch.bfloat16):
     """The keys and values at `slots` (int64; zeros outside the cache), rounded once to dtype: two (tokens, heads, head_dim) tensors."""
-    _check_ints(slots, "slots", torch.int64)
-    if dtype not in DTYPES:
-        raise ValueError(f"dtype must be FP16, BF16 or FP32, not {dtype}")
+    key = (slots.shape, slots.stride(), slots.dtype, dtype)
+    shape, like = cache.layouts.get(key) or cache.layouts.keep(key, _check_read(cache, slots, dtype))
     codes = cache.k_codes
-    pages, heads, block, head_dim = codes.shape
-    _check_device(codes.get_device(), slots=slots)
-    tokens = slots.shape[0]
-    k, v = (torch.empty(tokens, heads, head_dim, dtype=dtype, device=codes.device) for _ in range(2))
-    library().call("wq8_kv_read", codes.data_ptr(), cache.k_scales.data_ptr(), cache.v_codes.data_ptr(), cache.v_scales.data_ptr(), slots.data_ptr(), tokens,
-                   k.data_ptr(), v.data_ptr(), pages, heads, block, head_dim, DTYPES[dtype], _native.gpu(codes).stream())
+    _check_places(codes.get_device(), (), (slots,))
+    k = codes.new_empty(like, dtype=dtype)
+    v = torch.empty_like(k)
+    library().call("wq8_kv_read", codes.data_ptr(), cache.k_scales.data_ptr(), cache.v_codes.data_ptr(), cache.v_scales.data_ptr(), slots.data_ptr(), like[0],
+                   k.data_ptr(), v.data_ptr(), *shape, DTYPES[dtype], _native.gpu(codes).stream())
     return k, v
 
 
-_sizes = (ctypes.c_int64 * 2)()
+def _check_read(cache, slots, dtype):
+    _check_ints(slots, "slots", torch.int64)
+    if dtype not in DTYPES:
+        raise ValueError(f"dtype must be FP16, BF16 or FP32, not {dtype}")
+    return (cache.pages, cache.heads, cache.block, cache.head_dim), (slots.shape[0], cache.heads, cache.head_dim)
+
+
 
 
 def kv_attention(q, cache, tables, lens, starts, causal=True, window=0, scale=None, out=None):
@@ -158,37 +178,45 @@ def kv_attention(q, cache, tables, lens, starts, causal=True, window=0, scale=No
     position - window. scale: of the scores, 1 / sqrt(head_dim) by default. Rows that see nothing are zero; pages outside the cache are
     hidden; rows of no request are not written. Returns (tokens, query heads, head_dim) in q's dtype. Sums and the softmax's
     statistics are FP32, its weights FP16 relative to the largest."""
-    _check_rows(q, "queries")
-    _check_ints(lens, "lens")
-    _check_ints(starts, "starts")
-    _check_tables(tables)
-    codes = cache.k_codes
-    pages, heads, block, head_dim = codes.shape
-    tokens, q_heads, width = q.shape
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"queries must be FP16 or BF16, not {q.dtype}")
-    if width != head_dim or head_dim not in ATTENTION_HEAD_DIMS or not q_heads or q_heads % heads:
-        raise ValueError(f"queries must have heads of {head_dim} channels ({', '.join(map(str, ATTENTION_HEAD_DIMS))}), a multiple of the cache's {heads}")
-    requests = lens.shape[0]
-    if tables.shape[0] != requests or starts.shape[0] != requests + 1:
-        raise ValueError(f"tables and starts must be of {requests} requests")
-    if window < 0 or window >= 2 ** 31:
+    key = (q.shape, q.stride(), q.dtype, tables.shape, tables.stride(), tables.dtype, lens.shape, lens.stride(), lens.dtype, starts.shape, starts.stride(),
+           starts.dtype)
+    layout = cache.layouts.get(key) or cache.layouts.keep(key, _check_attention(q, cache, tables, lens, starts))
+    strides, table_stride, shape, default_scale, dtype, cus, workspace_bytes = layout
+    if not 0 <= window < 2 ** 31:
         raise ValueError("the window must not be negative")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _check_rows(out, "outputs")
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError("outputs do not match the queries")
-    device = codes.get_device()
-    _check_device(device, queries=q, tables=tables, lens=lens, starts=starts, outputs=out)
-    lib, state = library(), _native.gpu(codes)
-    group, columns = q_heads // heads, tables.shape[1]
-    lib.wq8_kv_attention_workspace(tokens, requests, heads, group, head_dim, state.cus, _sizes)
-    workspace = torch.empty(_sizes[0], dtype=torch.uint8, device=q.device) if _sizes[0] else None
-    sq, so = q.stride(), out.stride()
-    lib.call("wq8_kv_attention", q.data_ptr(), out.data_ptr(), (ctypes.c_longlong * 4)(sq[0], sq[1], so[0], so[1]), codes.data_ptr(), cache.k_scales.data_ptr(),
-             cache.v_codes.data_ptr(), cache.v_scales.data_ptr(), tables.data_ptr(), tables.stride(0), columns, lens.data_ptr(), starts.data_ptr(), tokens,
-             requests, heads, group, head_dim, block, pages, head_dim ** -0.5 if scale is None else scale, causal, window, DTYPES[q.dtype], state.cus,
-             _native.ptr(workspace), state.stream())
+        strides = type(strides)(strides[0], strides[1], out.stride(0), out.stride(1))
+    codes = cache.k_codes
+    q_at, out_at = _check_places(codes.get_device(), (q, out), (tables, lens, starts))
+    workspace = codes.new_empty(workspace_bytes) if workspace_bytes else None
+    library().call("wq8_kv_attention", q_at, out_at, strides, codes.data_ptr(), cache.k_scales.data_ptr(), cache.v_codes.data_ptr(), cache.v_scales.data_ptr(),
+                   tables.data_ptr(), table_stride, tables.shape[1], lens.data_ptr(), starts.data_ptr(), *shape, default_scale if scale is None else scale,
+                   causal, window, dtype, cus, _native.ptr(workspace), _native.gpu(codes).stream())
     return out
+
+
+def _check_attention(q, cache, tables, lens, starts):
+    _check_rows(q, "queries")
+    _check_ints(lens, "lens")
+    _check_ints(starts, "starts")
+    _check_tables(tables)
+    tokens, q_heads, width = q.shape
+    heads, head_dim, requests = cache.heads, cache.head_dim, lens.shape[0]
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"queries must be FP16 or BF16, not {q.dtype}")
+    if width != head_dim or head_dim not in ATTENTION_HEAD_DIMS or not q_heads or q_heads % heads:
+        raise ValueError(f"queries must have heads of {head_dim} channels ({', '.join(map(str, ATTENTION_HEAD_DIMS))}), a multiple of the cache's {heads}")
+    if tables.shape[0] != requests or starts.shape[0] != requests + 1:
+        raise ValueError(f"tables and starts must be of {requests} requests")
+    if not q.is_cuda:
+        raise ValueError("tensors must be on the GPU")
+    group, state = q_heads // heads, _native.gpu(q)
+    sizes = (ctypes.c_int64 * 2)()
+    library().wq8_kv_attention_workspace(tokens, requests, heads, group, head_dim, state.cus, sizes)
+    return ((ctypes.c_longlong * 4)(q.stride(0), q.stride(1), q_heads * head_dim, head_dim), tables.stride(0),
+            (tokens, requests, heads, group, head_dim, cache.block, cache.pages), head_dim ** -0.5, DTYPES[q.dtype], state.cus, sizes[0])

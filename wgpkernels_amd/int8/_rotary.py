@@ -18,12 +18,25 @@ STYLES = {"pairs": 0, "halves": 1}
 MAX_AXES, MAX_TENSORS = 3, 4
 
 
+class Layouts(dict):
+    """Shapes, strides and types that calls have been checked for, and what the kernels are told of them: a decode step's host time is its
+    checks (10 us of 19 in rotary()), and its shapes repeat."""
+    MOST = 4096
+
+    def keep(self, key, value):
+        if len(self) >= self.MOST:
+            self.clear()
+        self[key] = value
+        return value
+
+
 class RotaryPlan:
     """Which pairs turn, about which axis and how fast, on one GPU (rotary_plan()). Made once per model."""
-    __slots__ = ("sections", "style", "pairs", "turns", "axis")
+    __slots__ = ("sections", "style", "pairs", "turns", "axis", "layouts")
 
     def __init__(self, sections, style, turns, axis):
         self.sections, self.style, self.pairs, self.turns, self.axis = sections, style, sum(sections), turns, axis
+        self.layouts = Layouts()
 
 
 def rotary_plan(sections, ladder="axis", style="pairs", base=10000.0, frequencies=None, device="cuda"):
@@ -70,13 +83,42 @@ def _check_rows(x, name):
         raise ValueError(f"rows of {name} must be 16-byte aligned")
 
 
-def _check_device(device, **tensors):
-    """Every tensor on GPU `device` (an index; the kernels take raw pointers)."""
+def _check_places(device, aligned, others=()):
+    """Tensors on GPU `device` (an index; the kernels take raw pointers), the first ones 16-byte aligned; their addresses."""
     if device < 0:
         raise ValueError("tensors must be on the GPU")
-    for name, t in tensors.items():
+    pointers = [t.data_ptr() for t in aligned]
+    for t, p in zip(aligned, pointers):
+        if p & 15:
+            raise ValueError("rows must be 16-byte aligned")
         if t.get_device() != device:
-            raise ValueError(f"{name} must be on the same GPU as the other tensors")
+            raise ValueError("tensors must be on one GPU")
+    for t in others:
+        if t.get_device() != device:
+            raise ValueError("tensors must be on one GPU")
+    return pointers
+
+
+def _check_rotary(tensors, positions, plan):
+    """What the kernel is told of a call's inputs: tokens, head width, strides of positions, and per tensor heads and strides."""
+    if not 1 <= len(tensors) <= MAX_TENSORS:
+        raise ValueError(f"rotary takes 1 to {MAX_TENSORS} tensors")
+    first = tensors[0]
+    for x in tensors:
+        _check_rows(x, "rotary rows")
+        if x.dtype != first.dtype or x.shape[0] != first.shape[0] or x.shape[2] != first.shape[2]:
+            raise ValueError("rotary tensors must agree in type, tokens and head width")
+    tokens, _, head_dim = first.shape
+    axes = len(plan.sections)
+    if 2 * plan.pairs > head_dim:
+        raise ValueError(f"the plan turns {2 * plan.pairs} channels, the heads have {head_dim}")
+    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in ((tokens, axes), (tokens,) if axes == 1 else (tokens, axes)):
+        raise ValueError(f"rotary positions must be ({tokens}, {axes}) int32 or int64, not {tuple(positions.shape)} {positions.dtype}")
+    count = len(tensors)
+    # a new output is contiguous
+    strides = [v for x in tensors for v in (x.shape[1], x.stride(0), x.stride(1), x.shape[1] * head_dim, head_dim)]
+    return (ctypes.c_void_p * count, (ctypes.c_longlong * (5 * count))(*strides), positions.stride(0), positions.stride(1) if positions.dim() == 2 else 0,
+            positions.dtype == torch.int64, tokens, head_dim, DTYPES[first.dtype])
 
 
 def rotary(xs, positions, plan, inverse=False, out=None):
@@ -87,34 +129,21 @@ def rotary(xs, positions, plan, inverse=False, out=None):
     them in no other way."""
     many = not isinstance(xs, torch.Tensor)
     tensors = tuple(xs) if many else (xs,)
-    if not 1 <= len(tensors) <= MAX_TENSORS:
-        raise ValueError(f"rotary takes 1 to {MAX_TENSORS} tensors")
-    outs = tuple(torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in tensors) if out is None else (tuple(out) if many else (out,))
-    if len(outs) != len(tensors):
-        raise ValueError("rotary outputs do not match its inputs")
-    first = tensors[0]
-    shapes = []
-    for x, y in zip(tensors, outs):
-        _check_rows(x, "rotary rows")
-        if x.dtype != first.dtype or x.shape[0] != first.shape[0] or x.shape[2] != first.shape[2]:
-            raise ValueError("rotary tensors must agree in type, tokens and head width")
-        if out is not None:
+    key = (positions.shape, positions.stride(), positions.dtype, *[(x.shape, x.stride(), x.dtype) for x in tensors])
+    layout = plan.layouts.get(key) or plan.layouts.keep(key, _check_rotary(tensors, positions, plan))
+    pointers, strides, pos_token, pos_axis, wide, tokens, head_dim, dtype = layout
+    if out is None:
+        outs = tuple([torch.empty_like(x, memory_format=torch.contiguous_format) for x in tensors])
+    else:
+        outs = tuple(out) if many else (out,)
+        if len(outs) != len(tensors) or any(y.shape != x.shape or y.dtype != x.dtype for x, y in zip(tensors, outs)):
+            raise ValueError("rotary outputs do not match its inputs")
+        for y in outs:
             _check_rows(y, "rotary outputs")
-            if y.shape != x.shape or y.dtype != x.dtype:
-                raise ValueError("rotary outputs do not match its inputs")
-        sx, sy = x.stride(), y.stride()
-        shapes += (x.shape[1], sx[0], sx[1], sy[0], sy[1])
-    tokens, _, head_dim = first.shape
-    axes = len(plan.sections)
-    if 2 * plan.pairs > head_dim:
-        raise ValueError(f"the plan turns {2 * plan.pairs} channels, the heads have {head_dim}")
-    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in ((tokens, axes), (tokens,) if axes == 1 else (tokens, axes)):
-        raise ValueError(f"rotary positions must be ({tokens}, {axes}) int32 or int64, not {tuple(positions.shape)} {positions.dtype}")
-    _check_device(first.get_device(), positions=positions, plan=plan.turns, **{f"rows {i}": t for i, t in enumerate(tensors + outs)})
+        strides = type(strides)(*[v for x, y in zip(tensors, outs) for v in (x.shape[1], x.stride(0), x.stride(1), y.stride(0), y.stride(1))])
+    device = tensors[0].get_device()
+    places = _check_places(device, tensors + outs, (positions, plan.turns))
     count = len(tensors)
-    pointers = ctypes.c_void_p * count
-    library().call("wq8_rotary", pointers(*[x.data_ptr() for x in tensors]), pointers(*[y.data_ptr() for y in outs]), (ctypes.c_longlong * (5 * count))(*shapes),
-                   count, positions.data_ptr(), positions.stride(0), positions.stride(1) if positions.dim() == 2 else 0, positions.dtype == torch.int64,
-                   tokens, plan.turns.data_ptr(), plan.axis.data_ptr(), plan.pairs, head_dim, STYLES[plan.style], inverse, DTYPES[first.dtype],
-                   _native.gpu(first).stream())
+    library().call("wq8_rotary", pointers(*places[:count]), pointers(*places[count:]), strides, count, positions.data_ptr(), pos_token, pos_axis, wide, tokens,
+                   plan.turns.data_ptr(), plan.axis.data_ptr(), plan.pairs, head_dim, STYLES[plan.style], inverse, dtype, _native.gpu(tensors[0]).stream())
     return outs if many else outs[0]

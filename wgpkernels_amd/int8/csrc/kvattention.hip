@@ -42,7 +42,7 @@ struct AttentionArgs {
     int shares;               // workgroups that take a share (a multiple of 8)
     float scale;
     // workspace: per share the split tile that begins in it, {parts, first row, rows, first token} and its head; two partial results a share
-    int4* split_tiles;
+    v4i* split_tiles;
     int* split_heads;
     float* slots;
 };
@@ -57,11 +57,15 @@ struct Span {
 
 constexpr int TILE_KEYS_OVERHEAD = 128;  // what a tile costs besides its keys, in keys
 
-template <int ROWS> WQ8_DEVICE Span span_of(const AttentionArgs& p, int r) {
+template <typename T> WQ8_DEVICE T scalar_load(const T* p) { return *(const __attribute__((address_space(4))) T*)(uint64_t)p; }
+
+// UNIFORM: r is the same in every lane (scalar loads and arithmetic).
+template <int ROWS, bool UNIFORM> WQ8_DEVICE Span span_of(const AttentionArgs& p, int r) {
     Span s = {};
     if (r >= p.requests) return s;
-    const int begin = min(max(p.starts[r], 0), p.tokens), end = min(max(p.starts[r + 1], begin), p.tokens);
-    const int64_t len = p.lens[r], rows = int64_t(end - begin) * p.group;
+    const auto load = [](const int* at) { return UNIFORM ? scalar_load(at) : *at; };
+    const int begin = min(max(load(p.starts + r), 0), p.tokens), end = min(max(load(p.starts + r + 1), begin), p.tokens);
+    const int64_t len = load(p.lens + r), rows = int64_t(end - begin) * p.group;
     if (rows <= p.few_rows || rows > p.many_rows) return s;
     s.rows = int(rows);
     s.tiles = (s.rows + ROWS - 1) / ROWS;
@@ -115,7 +119,7 @@ template <int ROWS> struct Share {
     WQ8_DEVICE int64_t strip(int first, int64_t before) {
         base = first;
         base_at = before;
-        const Span s = span_of<ROWS>(p, threadIdx.x < 256 ? first + int(threadIdx.x) : p.requests);
+        const Span s = span_of<ROWS, false>(p, threadIdx.x < 256 ? first + int(threadIdx.x) : p.requests);
         int64_t total;
         const int64_t e = before + scan256(s.upto(s.tiles) * p.heads, lds4, total);
         if (threadIdx.x < 256) ends[threadIdx.x] = e;
@@ -125,16 +129,25 @@ template <int ROWS> struct Share {
     // Consecutive workgroups go round the 8 XCDs: each XCD takes a contiguous length of the line, whose tiles share keys and
     // values in its L2. A share is at least `least` keys.
     WQ8_DEVICE Share(const AttentionArgs& args, int64_t* scan, int64_t* request_ends, int least) : p(args), lds4(scan), ends(request_ends) {
-        line = 0;
-        for (int r = 0; r < p.requests; r += 256) line = strip(r, line);
-        line = uniform(line);
-        share = max((line + p.shares - 1) / p.shares, int64_t(least) * p.group);
+        if (p.requests == 1) {
+            const Span s = span_of<ROWS, true>(p, 0);
+            line = s.upto(s.tiles) * p.heads;
+            base = 0;
+            base_at = 0;
+        } else {
+            line = 0;
+            for (int r = 0; r < p.requests; r += 256) line = strip(r, line);
+            line = uniform(line);
+        }
+        int64_t even = int64_t(double(line) / double(p.shares));
+        while (even * p.shares < line) ++even;
+        share = uniform(max(even, int64_t(least) * p.group));
         index = int(blockIdx.x & 7) * (p.shares >> 3) + int(blockIdx.x >> 3);
         at = index * share;
         end = min(line, at + share);
     }
     WQ8_DEVICE Item item() {
-        if (at < base_at || p.requests > 256) {
+        if (p.requests > 256) {
             int64_t upto = 0;
             for (int r = 0; r < p.requests; r += 256) {
                 __syncthreads();
@@ -147,10 +160,10 @@ template <int ROWS> struct Share {
             const int m = (a + b) >> 1;
             if (uniform(ends[m]) > at) b = m; else a = m + 1;
         }
-        const Span s = span_of<ROWS>(p, base + a);
+        const Span s = span_of<ROWS, true>(p, uniform(base + a));
         const int64_t begin = a ? uniform(ends[a - 1]) : base_at, per_head = s.upto(s.tiles);
         int64_t in = at - begin;
-        int head = min(int(double(in) / double(per_head)), p.heads - 1);
+        int head = uniform(min(int(double(in) / double(per_head)), p.heads - 1));
         if (in < head * per_head) --head;
         else if (in >= (head + 1) * per_head) ++head;
         in -= head * per_head;
@@ -161,12 +174,18 @@ template <int ROWS> struct Share {
         } else {
             tile = int(double(in) / double(s.first));
         }
-        tile = min(max(tile, 0), s.tiles - 1);
+        tile = uniform(min(max(tile, 0), s.tiles - 1));
         while (tile > 0 && s.upto(tile) > in) --tile;
         while (tile + 1 < s.tiles && s.upto(tile + 1) <= in) ++tile;
         const int64_t head_at = begin + head * per_head;
         return {uniform(base + a), uniform(tile * ROWS), uniform(s.rows), uniform(s.first_token), uniform(head), uniform(s.past), uniform(s.total),
                 uniform(head_at + s.upto(tile)), uniform(head_at + s.upto(tile + 1))};
+    }
+    // Where this share's part of the item begins and ends in the line. A piece too short to be worth a part is left to the share on the other
+    // side of its boundary, which finds the same.
+    WQ8_DEVICE int64_t snapped(const Item& it, int64_t x) const {
+        const int64_t least = min(it.line_end - it.line_begin, share) >> 7;
+        return x - it.line_begin < least ? it.line_begin : it.line_end - x < least ? it.line_end : x;
     }
     // Of `steps` steps of the item's keys, the ones before place x of the line: the same for the shares on both sides of x.
     WQ8_DEVICE int step_of(const Item& it, int64_t x, int steps) const {
@@ -266,7 +285,11 @@ template <int ROWS, int D> WQ8_DEVICE float* slot_of(const AttentionArgs& p, int
 // A tile that begins in this share and goes on in later ones, for kv_attention_join.
 template <int ROWS> WQ8_DEVICE void note_split(const AttentionArgs& p, const Share<ROWS>& share, const Item& it) {
     if (threadIdx.x) return;
-    p.split_tiles[share.index] = int4{int((it.line_end - 1) / share.share) - share.index + 1, it.row0, it.rows, it.first_token};
+    int last = int(double(it.line_end - 1) / double(share.share));  // the share that its end is in
+    if (int64_t(last) * share.share > it.line_end - 1) --last;
+    else if (int64_t(last + 1) * share.share <= it.line_end - 1) ++last;
+    if (share.snapped(it, int64_t(last) * share.share) == it.line_end) --last;
+    p.split_tiles[share.index] = v4i{last - share.index + 1, it.row0, it.rows, it.first_token};
     p.split_heads[share.index] = it.head;
 }
 
@@ -278,27 +301,26 @@ template <int ROWS> WQ8_DEVICE void note_split(const AttentionArgs& p, const Sha
 // converts the 16 keys (of one page: its place is scalar work) 16 (w % 4) of the step: with 8 waves the first four the values, the
 // others the keys; with 4 waves each does both. The second four waves convert before their products, the first four after them, so that of
 // a SIMD's two waves one mostly feeds the matrix cores while the other converts.
-constexpr int STEP_KEYS = 64;
 
 WQ8_DEVICE float max3(float a, float b, float c) {  // without the quieting moves of fmaxf
     float r;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
     return r;
 }
-template <typename T> WQ8_DEVICE T scalar_load(const T* p) { return *(const __attribute__((address_space(4))) T*)(uint64_t)p; }
 WQ8_DEVICE int near32(int64_t v) { return int(min(max(v, int64_t(-(1 << 30))), int64_t(1 << 30))); }
 
 template <int DT, int D, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_tiles(AttentionArgs p) {
-    constexpr int ROWS = 32 * WAVES, KF = D / 16, KI = D / 64, VI = D == 256 ? 2 : 1, RAW = D == 256 ? 16 : 8, SWZ = 256 / D;
-    __shared__ u32x4 k_lds[2][2 * KF * 64];
-    __shared__ u32x4 v_lds[2][4 * (D / 32) * 64];
-    __shared__ v4f page_k[2], page_log_v[2], page_inv_v[2];
+    constexpr int ROWS = 32 * WAVES, KF = D / 16, KI = D / 64, VI = D == 256 ? 2 : 1, RAW = 8 * VI > 4 * KI ? 8 * VI : 4 * KI, SWZ = 256 / D;
+    constexpr int SUBS = D == 256 ? 1 : 2, STEP_KEYS = 64 * SUBS, K_SUB = 2 * KF * 64, V_SUB = 4 * (D / 32) * 64;
+    __shared__ u32x4 k_lds[2][SUBS * K_SUB];
+    __shared__ u32x4 v_lds[2][SUBS * V_SUB];
+    __shared__ v4f page_k[2][SUBS], page_log_v[2][SUBS], page_inv_v[2][SUBS];
     __shared__ int64_t scan[4], ends[256];
     const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, half = lane >> 5, granule = wave & 3;
     const bool does_v = WAVES == 4 || wave < 4, does_k = WAVES == 4 || wave >= 4;
-    Share<ROWS> share(p, scan, ends, 4 * STEP_KEYS);
-    if (!tid) p.split_tiles[share.index].x = 0;
+    Share<ROWS> share(p, scan, ends, 256);
+    if (!tid) p.split_tiles[share.index][0] = 0;
     // lane constants: places of the codes in memory and LDS, of the operands
     const int v_half = D == 64 ? lane >> 4 : D == 128 ? lane >> 5 : 0, v_dw = D == 64 ? lane & 15 : D == 128 ? lane & 31 : lane;
     const int v_at = 4 * v_half * D + 4 * v_dw;
@@ -308,6 +330,9 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
 
     for (; share.at < share.end; __syncthreads()) {
         const Item it = share.item();
+        const int64_t part0 = share.snapped(it, share.at), part1 = share.snapped(it, min(share.end, it.line_end));
+        share.at = it.line_end;
+        if (part0 >= part1) continue;
         // this lane's row
         const int row = it.row0 + 32 * wave + (lane & 31);
         const bool live_row = row < it.rows;
@@ -322,10 +347,10 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
         // keys: of the tile, of the part, and from the part's first on those of the wave and of the row
         Keys tile = keys_of(p, it, it.row0 / p.group, (min(it.row0 + ROWS, it.rows) - 1) / p.group);
         tile.low = min(tile.low, tile.high) & ~int64_t(STEP_KEYS - 1);
-        const int all_steps = int((tile.high - tile.low + STEP_KEYS - 1) / STEP_KEYS), step0 = share.step_of(it, share.at, all_steps);
-        const int steps = share.step_of(it, share.end, all_steps) - step0;
+        const int all_steps = int((tile.high - tile.low + STEP_KEYS - 1) / STEP_KEYS), step0 = share.step_of(it, part0, all_steps);
+        const int steps = share.step_of(it, part1, all_steps) - step0;
         const int64_t key0 = tile.low + int64_t(step0) * STEP_KEYS, key1 = min(tile.high, key0 + int64_t(steps) * STEP_KEYS);
-        const bool began = share.at > it.line_begin, goes_on = share.end < it.line_end;
+        const bool began = part0 > it.line_begin, goes_on = part1 < it.line_end;
         const int wave_first = it.row0 + 32 * wave, wave_last = min(wave_first + 31, it.rows - 1);
         const Keys own = keys_of(p, it, token, token);
         const Keys first = keys_of(p, it, min(wave_first, it.rows - 1) / p.group, min(wave_first, it.rows - 1) / p.group);
@@ -337,65 +362,87 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
         // this wave's 16 keys of a step: their page, codes and scales
         const int* table = p.tables + it.request * p.table_stride;
         const int64_t head_bytes = (int64_t(it.head) << p.block_log2) * D;
-        const auto page_of = [&](int step) -> int {
-            const int64_t key = key0 + int64_t(step) * STEP_KEYS + 16 * granule;
-            return key < key1 ? scalar_load(table + (key >> p.block_log2)) : -1;
-        };
-        uint32_t v_raw[RAW];
-        u32x4 k_raw[KI];
-        float ks = 0.0f, vs = 0.0f, seen = 0.0f;
-        bool live_page = false;
-        const auto load_codes = [&](int step, int page) {
-            live_page = page >= 0 && page < p.pages;
-            if (!live_page) page = 0;
-            const int64_t at = page * page_bytes + head_bytes + (int(key0 + int64_t(step) * STEP_KEYS + 16 * granule) & block_mask) * D;
-            if (does_v) {
+        struct Pages { int of[SUBS]; };
+        const auto pages_of = [&](int step) {
+            Pages r;
 #pragma unroll
-                for (int i = 0; i < VI; ++i)
-                    if (D > 64 || lane < 32)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            v_raw[8 * i + j] = *reinterpret_cast<const uint32_t*>(p.v_codes + at + (v_at + 4 * i * D + (j < 4 ? j : j + 4) * D));
-                ks = scalar_load(p.k_scales + int64_t(page) * p.heads + it.head);
-                vs = scalar_load(p.v_scales + int64_t(page) * p.heads + it.head);
+            for (int u = 0; u < SUBS; ++u) {
+                const int64_t key = key0 + int64_t(step) * STEP_KEYS + 64 * u + 16 * granule;
+                r.of[u] = key < key1 ? scalar_load(table + (key >> p.block_log2)) : -1;
             }
-            if (does_k) {
+            return r;
+        };
+        // codes on their way: with 8 waves a wave has keys or values, in the same registers
+        constexpr bool BOTH = WAVES == 4;
+        uint32_t v_raw[SUBS][RAW], own_k_raw[BOTH ? SUBS : 1][BOTH ? 4 * KI : 1];
+        const auto k_raw = [&](int u, int i) -> uint32_t& {
+            if constexpr (BOTH) return own_k_raw[u][i];
+            else return v_raw[u][i];
+        };
+        float ks[SUBS] = {}, vs[SUBS] = {}, seen = 0.0f;
+        bool live_page[SUBS] = {};
+        const auto load_codes = [&](int step, const Pages& pages) {
 #pragma unroll
-                for (int i = 0; i < KI; ++i) k_raw[i] = *reinterpret_cast<const u32x4*>(p.k_codes + at + (16 * lane + 1024 * i));
+            for (int u = 0; u < SUBS; ++u) {
+                int page = pages.of[u];
+                live_page[u] = page >= 0 && page < p.pages;
+                if (!live_page[u]) page = 0;
+                const int64_t at = page * page_bytes + head_bytes + (int(key0 + int64_t(step) * STEP_KEYS + 64 * u + 16 * granule) & block_mask) * D;
+                if (does_v) {
+#pragma unroll
+                    for (int i = 0; i < VI; ++i)
+                        if (D > 64 || lane < 32)
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                v_raw[u][8 * i + j] = *reinterpret_cast<const uint32_t*>(p.v_codes + at + (v_at + 4 * i * D + (j < 4 ? j : j + 4) * D));
+                    ks[u] = scalar_load(p.k_scales + int64_t(page) * p.heads + it.head);
+                    vs[u] = scalar_load(p.v_scales + int64_t(page) * p.heads + it.head);
+                }
+                if (does_k) {
+#pragma unroll
+                    for (int i = 0; i < KI; ++i) {
+                        const u32x4 raw = *reinterpret_cast<const u32x4*>(p.k_codes + at + (16 * lane + 1024 * i));
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) k_raw(u, 4 * i + j) = raw[j];
+                    }
+                }
             }
         };
         const auto store_codes = [&](int buffer) {
-            if (does_v) {
 #pragma unroll
-                for (int i = 0; i < VI; ++i) {
-                    uint32_t pairs[4][4];
+            for (int u = 0; u < SUBS; ++u) {
+                if (does_v) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) code_pairs(v_raw[8 * i + 2 * j], v_raw[8 * i + 2 * j + 1], pairs[j]);
-                    u32x4* at = v_lds[buffer] + ((v_dw >> 3) * 4 + granule) * 64;
-                    if (D > 64 || lane < 32)
+                    for (int i = 0; i < VI; ++i) {
+                        uint32_t pairs[4][4];
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const int entry = 4 * (v_dw & 7) + c + 32 * (v_half + i);
-                            at[entry ^ (entry >> 3 & 3) ^ (v_dw & 8)] = u32x4{pairs[0][c], pairs[1][c], pairs[2][c], pairs[3][c]};
-                        }
+                        for (int j = 0; j < 4; ++j) code_pairs(v_raw[u][8 * i + 2 * j], v_raw[u][8 * i + 2 * j + 1], pairs[j]);
+                        u32x4* at = v_lds[buffer] + u * V_SUB + ((v_dw >> 3) * 4 + granule) * 64;
+                        if (D > 64 || lane < 32)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                const int entry = 4 * (v_dw & 7) + c + 32 * (v_half + i);
+                                at[entry ^ (entry >> 3 & 3) ^ (v_dw & 8)] = u32x4{pairs[0][c], pairs[1][c], pairs[2][c], pairs[3][c]};
+                            }
+                    }
+                    seen = fmaxf(seen, live_page[u] ? vs[u] : 0.0f);
+                    const PageScales s = page_scales(ks[u], vs[u], seen, live_page[u]);
+                    if (!lane) {
+                        reinterpret_cast<float*>(&page_k[buffer][u])[granule] = s.k;
+                        reinterpret_cast<float*>(&page_log_v[buffer][u])[granule] = s.log_v;
+                        reinterpret_cast<float*>(&page_inv_v[buffer][u])[granule] = s.inv_v;
+                    }
                 }
-                seen = fmaxf(seen, live_page ? vs : 0.0f);
-                const PageScales s = page_scales(ks, vs, seen, live_page);
-                if (!lane) {
-                    reinterpret_cast<float*>(&page_k[buffer])[granule] = s.k;
-                    reinterpret_cast<float*>(&page_log_v[buffer])[granule] = s.log_v;
-                    reinterpret_cast<float*>(&page_inv_v[buffer])[granule] = s.inv_v;
-                }
-            }
-            if (does_k) {
+                if (does_k) {
 #pragma unroll
-                for (int i = 0; i < KI; ++i) {
-                    const int unit = lane + 64 * i, key = unit / KF, chunk = unit % KF;
-                    u32x4* at = k_lds[buffer] + ((granule >> 1) * KF + chunk) * 64;
-                    const u32x2 a = codes4(k_raw[i][0]), b = codes4(k_raw[i][1]), c = codes4(k_raw[i][2]), d = codes4(k_raw[i][3]);
-                    const int entry = (16 * (granule & 1) + key) ^ (SWZ * chunk & 15);
-                    at[entry] = u32x4{a[0], a[1], b[0], b[1]};
-                    at[entry + 32] = u32x4{c[0], c[1], d[0], d[1]};
+                    for (int i = 0; i < KI; ++i) {
+                        const int unit = lane + 64 * i, key = unit / KF, chunk = unit % KF;
+                        u32x4* at = k_lds[buffer] + u * K_SUB + ((granule >> 1) * KF + chunk) * 64;
+                        const u32x2 a = codes4(k_raw(u, 4 * i)), b = codes4(k_raw(u, 4 * i + 1)), c = codes4(k_raw(u, 4 * i + 2)), d = codes4(k_raw(u, 4 * i + 3));
+                        const int entry = (16 * (granule & 1) + key) ^ (SWZ * chunk & 15);
+                        at[entry] = u32x4{a[0], a[1], b[0], b[1]};
+                        at[entry + 32] = u32x4{c[0], c[1], d[0], d[1]};
+                    }
                 }
             }
         };
@@ -405,62 +452,61 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) acc[i] = v16f{};
 
-        int page = page_of(0);
+        Pages pages = pages_of(0);
         if (steps > 0) {
-            load_codes(0, page);
-            page = page_of(1);
+            load_codes(0, pages);
+            pages = pages_of(1);
             store_codes(0);
-            load_codes(1, page);
-            page = page_of(2);
+            load_codes(1, pages);
+            pages = pages_of(2);
             __syncthreads();
         }
         for (int step = 0; step < steps; ++step) {
-            const int buffer = step & 1, base = step * STEP_KEYS;
+            const int buffer = step & 1;
             const auto next = [&] {
                 if (step + 1 < steps) {
                     store_codes(buffer ^ 1);
-                    load_codes(step + 2, page);
-                    page = page_of(step + 3);
+                    load_codes(step + 2, pages);
+                    pages = pages_of(step + 3);
                 }
             };
             if (wave >= 4) next();
-            if (base < some_high && base + STEP_KEYS > some_low) {
-                // Stages of four matrix instructions, whose operands the stage before has read: what is between two
-                // sched_barriers stays there
+#pragma unroll 1
+            for (int u = 0; u < SUBS; ++u) {
+                const int base = step * STEP_KEYS + 64 * u;
+                if (base >= some_high || base + 64 <= some_low) continue;
+                // Stages of four matrix instructions, whose operands were read two stages before (an LDS read takes longer than four of
+                // them): what is between two sched_barriers stays there.
                 v16f s[2] = {};
-                f16x8 now[4], then[4];
-                const auto read_keys = [&](f16x8* to, int stage) {
+                constexpr int FIRST = KF / 2, STAGES = FIRST + D / 32;
+                f16x8 operands[3][4];
+                const auto read = [&](int stage) {
+                    if (stage >= STAGES) return;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int f = (4 * stage + i) % KF, h = (4 * stage + i) / KF;
-                        to[i] = __builtin_bit_cast(f16x8, k_lds[buffer][(h * KF + f) * 64 + (lane ^ (SWZ * f & 15))]);
+                        if (stage < FIRST) {
+                            const int f = 2 * stage + i / 2, h = i % 2;
+                            operands[stage % 3][i] = __builtin_bit_cast(f16x8, k_lds[buffer][u * K_SUB + (h * KF + f) * 64 + (lane ^ (SWZ * f & 15))]);
+                        } else {
+                            const int c = (4 * (stage - FIRST) + i) % (D / 32), g = (4 * (stage - FIRST) + i) / (D / 32);
+                            operands[stage % 3][i] = __builtin_bit_cast(f16x8, v_lds[buffer][u * V_SUB + (c * 4 + g) * 64 + (v_entry ^ (8 * (c & 1)))]);
+                        }
                     }
                 };
-                const auto read_values = [&](f16x8* to, int stage) {
+                read(0);
+                read(1);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int c = (4 * stage + i) % (D / 32), g = (4 * stage + i) / (D / 32);
-                        to[i] = __builtin_bit_cast(f16x8, v_lds[buffer][(c * 4 + g) * 64 + (v_entry ^ (8 * (c & 1)))]);
-                    }
-                };
-                read_keys(now, 0);
-#pragma unroll
-                for (int stage = 0; stage < KF / 2; ++stage) {
-                    if (stage + 1 < KF / 2) read_keys(then, stage + 1);
-                    else read_values(then, 0);
+                for (int stage = 0; stage < FIRST; ++stage) {
+                    read(stage + 2);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int f = (4 * stage + i) % KF, h = (4 * stage + i) / KF;
-                        s[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now[i], query[f], s[h], 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) now[i] = then[i];
+                    for (int i = 0; i < 4; ++i)
+                        s[i % 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(operands[stage % 3][i], query[2 * stage + i / 2], s[i % 2], 0, 0, 0);
                 }
                 // t = a s + b of the 16 keys of a page
-                v4f a = page_k[buffer] * query_scale, b = page_log_v[buffer];
-                const v4f inv_v = page_inv_v[buffer];
-                if (base + STEP_KEYS > all_high || base < all_low) {  // some row does not see every key of the step
+                v4f a = page_k[buffer][u] * query_scale, b = page_log_v[buffer][u];
+                const v4f inv_v = page_inv_v[buffer][u];
+                if (base + 64 > all_high || base < all_low) {  // some row does not see every key of the step
                     const int high = own_high - base, low = own_low - base;
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
@@ -504,20 +550,19 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
 #pragma unroll
                 for (int i = 0; i < WIDE; ++i) weights[i] = weights_of(i);
 #pragma unroll
-                for (int stage = 0; stage < D / 32; ++stage) {
-                    if (stage + 1 < D / 32) read_values(then, stage + 1);
+                for (int stage = FIRST; stage < STAGES; ++stage) {
+                    read(stage + 2);
                     __builtin_amdgcn_sched_barrier(0);
-                    const bool turn = (stage + 1) % PER == 0 && stage + 1 < D / 32;  // the next stage takes other pages' weights
+                    const int done = stage - FIRST + 1;
+                    const bool turn = done % PER == 0 && done < D / 32;  // the next stage takes other pages' weights
                     if (turn)
 #pragma unroll
-                        for (int i = 0; i < WIDE; ++i) next_weights[i] = weights_of((stage + 1) / PER * WIDE + i);
+                        for (int i = 0; i < WIDE; ++i) next_weights[i] = weights_of(done / PER * WIDE + i);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int c = (4 * stage + i) % (D / 32), g = (4 * stage + i) / (D / 32);
-                        acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now[i], weights[g % WIDE], acc[c], 0, 0, 0);
+                        const int c = (4 * (done - 1) + i) % (D / 32), g = (4 * (done - 1) + i) / (D / 32);
+                        acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(operands[stage % 3][i], weights[g % WIDE], acc[c], 0, 0, 0);
                     }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) now[i] = then[i];
                     if (turn)
 #pragma unroll
                         for (int i = 0; i < WIDE; ++i) weights[i] = next_weights[i];
@@ -556,7 +601,6 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
                     *reinterpret_cast<u32x2*>(out + 32 * c + 8 * i + 4 * half) = u32x2{o[0] | uint32_t(o[1]) << 16, o[2] | uint32_t(o[3]) << 16};
                 }
         }
-        share.at = it.line_end;
     }
 }
 
@@ -576,9 +620,12 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
     __shared__ int64_t scan[4], ends[256];
     const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, quarter = lane >> 4;
     Share<FEW_ROWS> share(p, scan, ends, 8 * FEW_KEYS);
-    if (!tid) p.split_tiles[share.index].x = 0;
+    if (!tid) p.split_tiles[share.index][0] = 0;
     for (; share.at < share.end; __syncthreads()) {
     const Item it = share.item();
+    const int64_t part0 = share.snapped(it, share.at), part1 = share.snapped(it, min(share.end, it.line_end));
+    share.at = it.line_end;
+    if (part0 >= part1) continue;
     const int row = it.row0 + (lane & 15);
     const bool live_row = row < it.rows;
     const int token = min(row, it.rows - 1) / p.group, member = min(row, it.rows - 1) - token * p.group;
@@ -595,9 +642,9 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
     const int64_t first_token = it.row0 / p.group, last_token = last_row / p.group;
     Keys tile = keys_of(p, it, first_token, last_token);
     tile.low = min(tile.low, tile.high) & ~int64_t(FEW_KEYS - 1);
-    const int all_steps = int((tile.high - tile.low + FEW_KEYS - 1) / FEW_KEYS), step0 = share.step_of(it, share.at, all_steps);
-    const int64_t key0 = tile.low + int64_t(step0) * FEW_KEYS, key1 = min(tile.high, tile.low + int64_t(share.step_of(it, share.end, all_steps)) * FEW_KEYS);
-    const bool began = share.at > it.line_begin, goes_on = share.end < it.line_end;
+    const int all_steps = int((tile.high - tile.low + FEW_KEYS - 1) / FEW_KEYS), step0 = share.step_of(it, part0, all_steps);
+    const int64_t key0 = tile.low + int64_t(step0) * FEW_KEYS, key1 = min(tile.high, tile.low + int64_t(share.step_of(it, part1, all_steps)) * FEW_KEYS);
+    const bool began = part0 > it.line_begin, goes_on = part1 < it.line_end;
     const Keys own = keys_of(p, it, token, token);
     const Keys first = keys_of(p, it, first_token, first_token), last = keys_of(p, it, last_token, last_token);
 
@@ -609,37 +656,54 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
 
     // granule i of the wave: keys wave_key0 + 128 (i / 2) + 16 (i % 2); a lane holds granule 64 n + lane
     int page = 0;
-    float ks = 0.0f, log_v = 0.0f, inv_v = 0.0f, seen = 0.0f;
+    bool live_page = false;
+    float ks = 0.0f, vs = 0.0f, log_v = 0.0f, inv_v = 0.0f, seen = 0.0f;
     const auto load_granules = [&](int step) {
         const int64_t key = wave_key0 + int64_t(4 * FEW_KEYS) * (step + (lane >> 1)) + 16 * (lane & 1);
         page = key < key1 ? table[key >> p.block_log2] : -1;
-        const bool live = page >= 0 && page < p.pages;
-        if (!live) page = 0;
+        live_page = page >= 0 && page < p.pages;
+        if (!live_page) page = 0;
         const int64_t at = int64_t(page) * p.heads + it.head;
-        const float vs = live ? p.v_scales[at] : 0.0f;
+        ks = p.k_scales[at];
+        vs = p.v_scales[at];
+    };
+    const auto use_granules = [&] {
+        if (!live_page) vs = 0.0f;
         seen = fmaxf(seen, wave_max(vs));
-        const PageScales s = page_scales(p.k_scales[at], vs, seen, live);
+        const PageScales s = page_scales(ks, vs, seen, live_page);
         ks = s.k;
         log_v = s.log_v;
         inv_v = s.inv_v;
     };
     const auto from_lane = [](float v, int from) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), from)); };
 
-    u32x4 k_raw[2][KV];
-    uint32_t v_raw[8][VW];
-    const auto load_codes = [&](int step) {
+    struct Raw {  // a step on its way: its codes, and its pages' scales
+        u32x4 k[2][KV];
+        uint32_t v[8][VW];
+        float scale[2], log_v[2], inv_v[2];
+    };
+    const auto take_scales = [&](Raw& raw, int step) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int from = 2 * (step & 31) + b;
+            raw.scale[b] = from_lane(ks, from);
+            raw.log_v[b] = from_lane(log_v, from);
+            raw.inv_v[b] = from_lane(inv_v, from);
+        }
+    };
+    const auto load_codes = [&](Raw& raw, int step) {
         const int64_t key = wave_key0 + int64_t(4 * FEW_KEYS) * step;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const int64_t at = __builtin_amdgcn_readlane(page, 2 * (step & 31) + b) * page_bytes + head_bytes + (int(key + 16 * b) & block_mask) * D;
             const int8_t* k = p.k_codes + at + (lane & 15) * D + D / 4 * quarter;
 #pragma unroll
-            for (int i = 0; i < KV; ++i) k_raw[b][i] = reinterpret_cast<const u32x4*>(k)[i];
+            for (int i = 0; i < KV; ++i) raw.k[b][i] = reinterpret_cast<const u32x4*>(k)[i];
             const int8_t* v = p.v_codes + at + 4 * quarter * D + D / 16 * (lane & 15);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < VW; ++j) v_raw[4 * b + i][j] = reinterpret_cast<const uint32_t*>(v + i * D)[j];
+                for (int j = 0; j < VW; ++j) raw.v[4 * b + i][j] = reinterpret_cast<const uint32_t*>(v + i * D)[j];
         }
     };
 
@@ -647,40 +711,32 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
     v4f acc[VF];
 #pragma unroll
     for (int i = 0; i < VF; ++i) acc[i] = v4f{};
-    if (steps) {
-        load_granules(0);
-        load_codes(0);
-    }
-    for (int step = 0; step < steps; ++step) {
+    const auto take_step = [&](Raw& raw, int step) {
         const int64_t key = wave_key0 + int64_t(4 * FEW_KEYS) * step;
-        // this step's operands out of the raw registers, then the next step's loads
+        // this step's operands out of the raw registers, then the loads of the step after the next
         f16x8 k[2][KF], v[VF];
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int f = 0; f < KF; ++f) {
-                const u32x2 a = codes4(k_raw[b][f >> 1][2 * (f & 1)]), c = codes4(k_raw[b][f >> 1][2 * (f & 1) + 1]);
+                const u32x2 a = codes4(raw.k[b][f >> 1][2 * (f & 1)]), c = codes4(raw.k[b][f >> 1][2 * (f & 1) + 1]);
                 k[b][f] = __builtin_bit_cast(f16x8, u32x4{a[0], a[1], c[0], c[1]});
             }
 #pragma unroll
         for (int j = 0; j < VW; ++j) {
             uint32_t pairs[4][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) code_pairs(v_raw[2 * i][j], v_raw[2 * i + 1][j], pairs[i]);
+            for (int i = 0; i < 4; ++i) code_pairs(raw.v[2 * i][j], raw.v[2 * i + 1][j], pairs[i]);
 #pragma unroll
             for (int c = 0; c < 4; ++c) v[4 * j + c] = __builtin_bit_cast(f16x8, u32x4{pairs[0][c], pairs[1][c], pairs[2][c], pairs[3][c]});
         }
-        float page_k[2], page_log_v[2], page_inv_v[2];
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const int from = 2 * (step & 31) + b;
-            page_k[b] = from_lane(ks, from);
-            page_log_v[b] = from_lane(log_v, from);
-            page_inv_v[b] = from_lane(inv_v, from);
-        }
-        if (step + 1 < steps) {
-            if (((step + 1) & 31) == 0) load_granules(step + 1);
-            load_codes(step + 1);
+        const float scale[2] = {raw.scale[0], raw.scale[1]}, page_log_v[2] = {raw.log_v[0], raw.log_v[1]}, page_inv_v[2] = {raw.inv_v[0], raw.inv_v[1]};
+        if (step + 2 < steps) {
+            const bool turn = ((step + 2) & 31) == 0;
+            if (turn) load_granules(step + 2);
+            load_codes(raw, step + 2);
+            if (turn) use_granules();
+            take_scales(raw, step + 2);
         }
         float t[8];
 #pragma unroll
@@ -688,7 +744,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
             v4f s = {};
 #pragma unroll
             for (int f = 0; f < KF; ++f) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[b][f], query[f], s, 0, 0, 0);
-            const float m = page_k[b] * query_scale;
+            const float m = scale[b] * query_scale;
 #pragma unroll
             for (int i = 0; i < 4; ++i) t[4 * b + i] = __builtin_fmaf(s[i], m, page_log_v[b]);
         }
@@ -726,6 +782,19 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
         const f16x8 weights = weights8(w);
 #pragma unroll
         for (int i = 0; i < VF; ++i) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[i], weights, acc[i], 0, 0, 0);
+    };
+    Raw even, odd;
+    if (steps) {
+        load_granules(0);
+        load_codes(even, 0);
+        if (steps > 1) load_codes(odd, 1);
+        use_granules();
+        take_scales(even, 0);
+        take_scales(odd, 1);
+    }
+    for (int step = 0; step < steps; step += 2) {
+        take_step(even, step);
+        if (step + 1 < steps) take_step(odd, step + 1);
     }
     mass = add_xor32(add_xor16(mass));
     // a lane's sums: channels D / 4 * quarter + D / 16 * i + j of its row, i = 0-3, j = fragment
@@ -772,73 +841,70 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
         *reinterpret_cast<u32x2*>(out + j) = u32x2{e[0] | uint32_t(e[1]) << 16, e[2] | uint32_t(e[3]) << 16};
     }
     }
-    share.at = it.line_end;
     }
 }
 
 // ---- parts joined --------------------------------------------------------------------------------------------------
-// Adds the parts of a split tile, in order: a workgroup ROWS_WG rows, 4 / WAVES at a time, with WAVES waves a row (each takes every
-// WAVES-th part of a row's channels; their sums are then added in order). A wave's lanes first take the maxima and sums of up to 64
-// parts at once, then walk the channels with the parts' weights.
-template <int DT, int ROWS, int D, int ROWS_WG, int WAVES>
+// Adds the parts of a split tile: D / 4 lanes a row, GROUPS of them that each take every GROUPS-th part, U parts' loads on their way at a time;
+// the groups' sums are added in an order of their own, the same every time.
+template <int DT, int ROWS, int D, int ROWS_WG, int GROUPS>
 __global__ void __launch_bounds__(256) kv_attention_join(AttentionArgs p) {
-    constexpr int C = D / 64;
-    typedef float vc __attribute__((ext_vector_type(C)));
-    __shared__ vc sums[4][64];
-    __shared__ float masses[4], tops[4];
-    const int4 tile = p.split_tiles[blockIdx.x];
-    const int head = p.split_heads[blockIdx.x], parts = tile.x;
+    constexpr int LANES = D / 4, AT_ONCE = 256 / (LANES * GROUPS), U = ROWS == FEW_ROWS ? 16 : 4;
+    const v4i tile = scalar_load(p.split_tiles + blockIdx.x);
+    const int head = scalar_load(p.split_heads + blockIdx.x), parts = tile[0];
     if (parts < 2) return;
-    const int wave = uniform(int(threadIdx.x) >> 6), lane = threadIdx.x & 63;
-    const auto slot_at = [&](int part) { return slot_of<ROWS, D>(p, 2 * (int(blockIdx.x) + part) + !part); };
-    for (int i = WAVES == 4 ? 0 : wave; i < ROWS_WG; i += 4 / WAVES) {
-        const int r = blockIdx.y * ROWS_WG + i, row = tile.y + r;
-        if (row >= tile.z) return;
+    const int c = 4 * (threadIdx.x % LANES), group = threadIdx.x / LANES % GROUPS;
+#pragma unroll 2
+    for (int i = threadIdx.x / (LANES * GROUPS); i < ROWS_WG; i += AT_ONCE) {
+        const int r = blockIdx.y * ROWS_WG + i, row = tile[1] + r;
+        if (r >= ROWS || row >= tile[2]) continue;
         float top = LOWEST, mass = 0.0f;
-        vc acc = {};
-        for (int base = WAVES == 4 ? wave : 0; base < parts; base += 64 * WAVES) {
-            const int part = base + lane * WAVES, count = min(64, (parts - base + WAVES - 1) / WAVES);
-            const float* end = slot_at(min(part, parts - 1)) + ROWS * D + 2 * r;
-            const float part_top = part < parts ? end[0] : LOWEST, part_mass = part < parts ? end[1] : 0.0f;
-            float next = part_top;
+        v4f acc = {};
+        for (int base = group; base < parts; base += GROUPS * U) {
+            v4f x[U];
+            float t[U], m[U];
 #pragma unroll
-            for (int d = 1; d < 64; d <<= 1) next = fmaxf(next, __shfl_xor(next, d));
-            next = fmaxf(next, top);
-            const float keep = __builtin_amdgcn_exp2f(top - next), weight = __builtin_amdgcn_exp2f(part_top - next);
+            for (int u = 0; u < U; ++u) {
+                const int part = min(base + u * GROUPS, parts - 1);
+                const float* slot = slot_of<ROWS, D>(p, 2 * (int(blockIdx.x) + part) + !part);
+                x[u] = *reinterpret_cast<const v4f*>(slot + r * D + c);
+                t[u] = slot[ROWS * D + 2 * r];
+                m[u] = slot[ROWS * D + 2 * r + 1];
+            }
+            float next = top;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (base + u * GROUPS >= parts) t[u] = -__builtin_inff();
+                next = fmaxf(next, t[u]);
+            }
+            const float keep = __builtin_amdgcn_exp2f(top - next);
             top = next;
-            mass = __builtin_fmaf(mass, keep, wave_sum(part_mass * weight));
+            mass *= keep;
             acc *= keep;
-#pragma unroll 8
-            for (int j = 0; j < count; ++j) {
-                const vc x = *reinterpret_cast<const vc*>(slot_at(base + j * WAVES) + r * D + C * lane);
-                const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), j));
 #pragma unroll
-                for (int c = 0; c < C; ++c) acc[c] = __builtin_fmaf(x[c], w, acc[c]);
+            for (int u = 0; u < U; ++u) {
+                const float w = __builtin_amdgcn_exp2f(t[u] - next);
+                mass = __builtin_fmaf(m[u], w, mass);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j] = __builtin_fmaf(x[u][j], w, acc[j]);
             }
         }
-        if constexpr (WAVES == 4) {
-            sums[wave][lane] = acc;
-            if (!lane) {
-                masses[wave] = mass;
-                tops[wave] = top;
-            }
-            __syncthreads();
-            if (wave) return;
-            top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-            mass = 0.0f;
-            acc = vc{};
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float keep = __builtin_amdgcn_exp2f(tops[w] - top);
-                mass = __builtin_fmaf(masses[w], keep, mass);
+        for (int d = LANES; d < LANES * GROUPS; d <<= 1) {
+            const float other = __shfl_xor(top, d), next = fmaxf(top, other);
+            const float keep = __builtin_amdgcn_exp2f(top - next), take = __builtin_amdgcn_exp2f(other - next);
+            mass = __builtin_fmaf(mass, keep, __shfl_xor(mass, d) * take);
 #pragma unroll
-                for (int c = 0; c < C; ++c) acc[c] = __builtin_fmaf(sums[w][lane][c], keep, acc[c]);
-            }
+            for (int j = 0; j < 4; ++j) acc[j] = __builtin_fmaf(acc[j], keep, __shfl_xor(acc[j], d) * take);
+            top = next;
         }
+        if (group) continue;
         const int token = row / p.group, member = row - token * p.group;
-        uint16_t* out = static_cast<uint16_t*>(p.out) + (tile.w + token) * p.out_token + (head * p.group + member) * p.out_head + C * lane;
+        uint16_t* out = static_cast<uint16_t*>(p.out) + (tile[3] + token) * p.out_token + (head * p.group + member) * p.out_head + c;
+        uint16_t o[4];
 #pragma unroll
-        for (int c = 0; c < C; ++c) out[c] = Elem<DT>::from_f(finish(acc[c], mass));
+        for (int j = 0; j < 4; ++j) o[j] = Elem<DT>::from_f(finish(acc[j], mass));
+        *reinterpret_cast<u32x2*>(out) = u32x2{o[0] | uint32_t(o[1]) << 16, o[2] | uint32_t(o[3]) << 16};
     }
 }
 
@@ -847,7 +913,7 @@ __global__ void __launch_bounds__(256) kv_attention_join(AttentionArgs p) {
 // a wave.
 struct Launches {
     bool used[2];
-    int limit, shares[2], waves;
+    int limit, shares[2], waves, few_rows;
     int64_t bytes[2];
 };
 
@@ -856,11 +922,14 @@ static int64_t align256(int64_t v) { return (v + 255) & ~int64_t(255); }
 static Launches plan_launches(int64_t tokens, int64_t requests, int64_t group, int head_dim, int sms) {
     Launches l = {};
     const int64_t rows = tokens * group;
-    // A request's rows are known on the GPU alone. On average up to 16 a request: all on the tiles of few rows (one launch)
+    // A request's rows are known on the GPU alone. On average up to 16 a request: all on the tiles of few rows; more than 64: all on
+    // the others (each launch is about 5 us, used or not); between, each request by its rows.
     l.limit = 32;
     l.used[1] = requests == 1 ? rows > l.limit : rows > FEW_ROWS * requests;
-    l.used[0] = !l.used[1] || requests > 1;
+    l.used[0] = !l.used[1] || (requests > 1 && rows <= 64 * requests);
     if (!l.used[1]) l.limit = 0x7fffffff;
+    if (!l.used[0]) l.limit = 0;
+    l.few_rows = int(std::min<int64_t>(rows, FEW_ROWS));
     l.waves = head_dim == 256 ? 4 : 8;
     const int per_cu[2] = {2, 1}, tile_rows[2] = {FEW_ROWS, 32 * l.waves};
     for (int i = 0; i < 2; ++i) {
@@ -877,16 +946,16 @@ template <int DT, int D> static int launch_attention(AttentionArgs p, const Laun
         p.many_rows = i ? 0x7fffffff : l.limit;
         p.shares = l.shares[i];
         char* at = workspace + (i ? l.bytes[0] : 0);
-        p.split_tiles = reinterpret_cast<int4*>(at);
+        p.split_tiles = reinterpret_cast<v4i*>(at);
         p.split_heads = reinterpret_cast<int*>(p.split_tiles + p.shares);
         p.slots = reinterpret_cast<float*>(at + align256(int64_t(p.shares) * 20));
         if (i) {
             constexpr int WAVES = D == 256 ? 4 : 8;
             kv_attention_tiles<DT, D, WAVES><<<p.shares, 64 * WAVES, 0, stream>>>(p);
-            kv_attention_join<DT, 32 * WAVES, D, 16, 1><<<dim3(p.shares, 2 * WAVES), 256, 0, stream>>>(p);
+            kv_attention_join<DT, 32 * WAVES, D, 32, 1><<<dim3(p.shares, WAVES), 256, 0, stream>>>(p);
         } else {
             kv_attention_few<DT, D><<<p.shares, 256, 0, stream>>>(p);
-            kv_attention_join<DT, FEW_ROWS, D, 1, 4><<<dim3(p.shares, FEW_ROWS), 256, 0, stream>>>(p);
+            kv_attention_join<DT, FEW_ROWS, D, 4, 256 / D><<<dim3(p.shares, (l.few_rows + 3) / 4), 256, 0, stream>>>(p);
         }
     }
     return int(hipGetLastError());
