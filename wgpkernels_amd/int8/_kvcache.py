@@ -97,7 +97,7 @@ def kv_plan(past, new, tables, free, used, block, tokens):
     _check_places(past.get_device(), (), (new, tables, free, used))
     slots = past.new_empty(tokens, dtype=torch.int64)
     held = past.new_empty(tokens + 2 * splits[2] + 3)
-    positions, starts, lens, used_out, missing = held.split(splits)
+    positions, starts, lens, used_out, missing = held.split_with_sizes(splits)
     requests, at = splits[2], held.data_ptr()
     starts_at = at + 4 * tokens
     lens_at = starts_at + 4 * requests + 4
@@ -213,6 +213,8 @@ def _check_attention(q, cache, tables, lens, starts):
         raise ValueError(f"queries must have heads of {head_dim} channels ({', '.join(map(str, ATTENTION_HEAD_DIMS))}), a multiple of the cache's {heads}")
     if tables.shape[0] != requests or starts.shape[0] != requests + 1:
         raise ValueError(f"tables and starts must be of {requests} requests")
+    if tables.shape[1] * cache.block > 2 ** 30:
+        raise ValueError("block tables reach 2^30 tokens a request at most")
     if not q.is_cuda:
         raise ValueError("tensors must be on the GPU")
     group, state = q_heads // heads, _native.gpu(q)

@@ -67,7 +67,8 @@ def rotary_plan(sections, ladder="axis", style="pairs", base=10000.0, frequencie
     turns = [round(math.fmod(f / (2 * math.pi), 1.0) * 2.0 ** 64) for f in frequencies]
     turns = [(t + 2 ** 63) % 2 ** 64 - 2 ** 63 for t in turns]
     axis = [a for a, n in enumerate(sections) for _ in range(n)]
-    return RotaryPlan(sections, style, torch.tensor(turns, dtype=torch.int64, device=device), torch.tensor(axis, dtype=torch.int32, device=device))
+    packed = torch.tensor(turns + axis, dtype=torch.int64).to(device)  # one copy
+    return RotaryPlan(sections, style, packed[:pairs], packed[pairs:].to(torch.int32))
 
 
 def _check_rows(x, name):

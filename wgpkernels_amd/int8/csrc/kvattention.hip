@@ -38,6 +38,7 @@ struct AttentionArgs {
     const int *tables, *lens, *starts;
     int64_t table_stride, pages;
     int width, tokens, requests, heads, group, block_log2, causal, window;
+    unsigned group_inverse;   // 2^32 / group, rounded down
     int few_rows, many_rows;  // the rows of a request that this launch serves: more than few_rows, up to many_rows
     int shares;               // workgroups that take a share (a multiple of 8)
     float scale;
@@ -50,8 +51,8 @@ struct AttentionArgs {
 // ---- shares --------------------------------------------------------------------------------------------------------
 // A request's part of the line: tiles of length first + more * i, i = 0 to tiles - 1, for each head.
 struct Span {
-    int rows, tiles, first_token;
-    int64_t past, total, first, more;
+    int rows, tiles, first_token, past, total;
+    int64_t first, more;
     WQ8_DEVICE int64_t upto(int64_t i) const { return first * i + more * (i * (i - 1) / 2); }
 };
 
@@ -65,23 +66,28 @@ template <int ROWS, bool UNIFORM> WQ8_DEVICE Span span_of(const AttentionArgs& p
     if (r >= p.requests) return s;
     const auto load = [](const int* at) { return UNIFORM ? scalar_load(at) : *at; };
     const int begin = min(max(load(p.starts + r), 0), p.tokens), end = min(max(load(p.starts + r + 1), begin), p.tokens);
-    const int64_t len = load(p.lens + r), rows = int64_t(end - begin) * p.group;
+    const int len = max(0, load(p.lens + r));
+    const int64_t rows = int64_t(end - begin) * p.group;
     if (rows <= p.few_rows || rows > p.many_rows) return s;
     s.rows = int(rows);
     s.tiles = (s.rows + ROWS - 1) / ROWS;
     s.first_token = begin;
-    s.past = len - (end - begin);
-    s.total = p.pages ? max(int64_t(0), min(len, int64_t(p.width) << p.block_log2)) : 0;
+    s.past = len - (end - begin);  // a length below zero counts as zero keys: positions stay in range
+    s.total = p.pages ? max(0, min(len, p.width << p.block_log2)) : 0;
     // lengths in keys * group: a causal tile's rows see ROWS / group keys more than those of the tile before
-    const int64_t seen = p.causal ? min(s.total, max(int64_t(0), s.past)) : s.total;
-    if (p.causal && !p.window) {
-        s.first = (seen + TILE_KEYS_OVERHEAD) * p.group + ROWS;
-        s.more = ROWS;
-    } else {
-        s.first = ((p.window ? min(s.total, int64_t(p.window)) : seen) + TILE_KEYS_OVERHEAD) * p.group + ROWS;
-    }
+    const bool grows = p.causal && !p.window;
+    const int seen = p.window ? min(s.total, p.window) : p.causal ? min(s.total, max(0, s.past)) : s.total;
+    s.first = int64_t(seen + TILE_KEYS_OVERHEAD) * p.group + ROWS;
+    s.more = grows ? ROWS : 0;
     return s;
 }
+
+WQ8_DEVICE int by_group(const AttentionArgs& p, int row) {  // row / group
+    const unsigned q = __umulhi(unsigned(row), p.group_inverse);
+    return int(unsigned(row) - q * unsigned(p.group) >= unsigned(p.group) ? q + 1 : q);
+}
+// a / b to about 2^-22 of itself; a starting point for counting, the same in every workgroup
+WQ8_DEVICE float ratio(int64_t a, int64_t b) { return float(a) * __builtin_amdgcn_rcpf(float(b)); }
 
 WQ8_DEVICE int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 WQ8_DEVICE int64_t uniform(int64_t v) { return int64_t(uint64_t(uint32_t(uniform(int(v >> 32)))) << 32 | uint32_t(uniform(int(v)))); }
@@ -106,7 +112,7 @@ WQ8_DEVICE int64_t scan256(int64_t v, int64_t* lds4, int64_t& total) {
 }
 
 // A workgroup's share [at, end) of the line, and the tile that stands at `at`.
-struct Item { int request, row0, rows, first_token, head; int64_t past, total, line_begin, line_end; };
+struct Item { int request, row0, rows, first_token, head, past, total; int64_t line_begin, line_end; };
 template <int ROWS> struct Share {
     const AttentionArgs& p;
     int64_t* lds4;
@@ -139,9 +145,8 @@ template <int ROWS> struct Share {
             for (int r = 0; r < p.requests; r += 256) line = strip(r, line);
             line = uniform(line);
         }
-        int64_t even = int64_t(double(line) / double(p.shares));
-        while (even * p.shares < line) ++even;
-        share = uniform(max(even, int64_t(least) * p.group));
+        // no less than line / shares
+        share = uniform(max(int64_t(float(line) * 0x1.00002p0f * __builtin_amdgcn_rcpf(float(p.shares))) + 1, int64_t(least) * p.group));
         index = int(blockIdx.x & 7) * (p.shares >> 3) + int(blockIdx.x >> 3);
         at = index * share;
         end = min(line, at + share);
@@ -163,16 +168,16 @@ template <int ROWS> struct Share {
         const Span s = span_of<ROWS, true>(p, uniform(base + a));
         const int64_t begin = a ? uniform(ends[a - 1]) : base_at, per_head = s.upto(s.tiles);
         int64_t in = at - begin;
-        int head = uniform(min(int(double(in) / double(per_head)), p.heads - 1));
-        if (in < head * per_head) --head;
-        else if (in >= (head + 1) * per_head) ++head;
+        int head = uniform(int(ratio(in, per_head)));
+        while (head > 0 && in < head * per_head) --head;
+        while (head + 1 < p.heads && in >= (head + 1) * per_head) ++head;
         in -= head * per_head;
         int tile;
         if (s.more) {  // first i + more i (i - 1) / 2 <= in
-            const double h = double(s.first) - 0.5 * double(s.more);
-            tile = int((__builtin_sqrt(h * h + 2.0 * double(s.more) * double(in)) - h) / double(s.more));
+            const float h = float(s.first) - 0.5f * float(s.more), m = float(s.more);
+            tile = int((__builtin_amdgcn_sqrtf(__builtin_fmaf(h, h, 2.0f * m * float(in))) - h) * __builtin_amdgcn_rcpf(m));
         } else {
-            tile = int(double(in) / double(s.first));
+            tile = int(ratio(in, s.first));
         }
         tile = uniform(min(max(tile, 0), s.tiles - 1));
         while (tile > 0 && s.upto(tile) > in) --tile;
@@ -191,17 +196,19 @@ template <int ROWS> struct Share {
     WQ8_DEVICE int step_of(const Item& it, int64_t x, int steps) const {
         if (x <= it.line_begin) return 0;
         if (x >= it.line_end) return steps;
-        return uniform(int(double(x - it.line_begin) * double(steps) / double(it.line_end - it.line_begin)));
+        return uniform(min(int(ratio(x - it.line_begin, it.line_end - it.line_begin) * float(steps)), steps));
     }
 };
 
 // Keys that the rows of tokens [first, last] see together: [low, high).
-struct Keys { int64_t low, high; };
-WQ8_DEVICE Keys keys_of(const AttentionArgs& p, const Item& it, int64_t first, int64_t last) {
+struct Keys { int low, high; };
+WQ8_DEVICE Keys keys_of(const AttentionArgs& p, const Item& it, int first, int last) {
     Keys k;
     k.high = p.causal ? min(it.total, it.past + last + 1) : it.total;
-    k.low = p.window ? max(int64_t(0), it.past + first - p.window + 1) : 0;
-    if (k.high < k.low) k.high = k.low;
+    const int at = it.past + first;
+    k.low = p.window && at >= p.window ? at - p.window + 1 : 0;
+    k.high = max(k.high, 0);
+    k.low = min(k.low, k.high);
     return k;
 }
 
@@ -285,9 +292,9 @@ template <int ROWS, int D> WQ8_DEVICE float* slot_of(const AttentionArgs& p, int
 // A tile that begins in this share and goes on in later ones, for kv_attention_join.
 template <int ROWS> WQ8_DEVICE void note_split(const AttentionArgs& p, const Share<ROWS>& share, const Item& it) {
     if (threadIdx.x) return;
-    int last = int(double(it.line_end - 1) / double(share.share));  // the share that its end is in
-    if (int64_t(last) * share.share > it.line_end - 1) --last;
-    else if (int64_t(last + 1) * share.share <= it.line_end - 1) ++last;
+    int last = int(ratio(it.line_end - 1, share.share));  // the share that its end is in
+    while (int64_t(last) * share.share > it.line_end - 1) --last;
+    while (int64_t(last + 1) * share.share <= it.line_end - 1) ++last;
     if (share.snapped(it, int64_t(last) * share.share) == it.line_end) --last;
     p.split_tiles[share.index] = v4i{last - share.index + 1, it.row0, it.rows, it.first_token};
     p.split_heads[share.index] = it.head;
@@ -307,7 +314,6 @@ WQ8_DEVICE float max3(float a, float b, float c) {  // without the quieting move
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
     return r;
 }
-WQ8_DEVICE int near32(int64_t v) { return int(min(max(v, int64_t(-(1 << 30))), int64_t(1 << 30))); }
 
 template <int DT, int D, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_tiles(AttentionArgs p) {
@@ -336,7 +342,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
         // this lane's row
         const int row = it.row0 + 32 * wave + (lane & 31);
         const bool live_row = row < it.rows;
-        const int token = min(row, it.rows - 1) / p.group, member = min(row, it.rows - 1) - token * p.group;
+        const int token = by_group(p, min(row, it.rows - 1)), member = min(row, it.rows - 1) - token * p.group;
         f16x8 query[KF];
         const float query_scale = load_query<DT, KF>(static_cast<const uint16_t*>(p.q) + (it.first_token + token) * p.q_token +
                                                          (it.head * p.group + member) * p.q_head + 8 * half, 16, live_row, query, [](uint32_t t) {
@@ -345,19 +351,19 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
         }) * p.scale * 0x1.715476p+0f;
 
         // keys: of the tile, of the part, and from the part's first on those of the wave and of the row
-        Keys tile = keys_of(p, it, it.row0 / p.group, (min(it.row0 + ROWS, it.rows) - 1) / p.group);
-        tile.low = min(tile.low, tile.high) & ~int64_t(STEP_KEYS - 1);
-        const int all_steps = int((tile.high - tile.low + STEP_KEYS - 1) / STEP_KEYS), step0 = share.step_of(it, part0, all_steps);
+        Keys tile = keys_of(p, it, by_group(p, it.row0), by_group(p, min(it.row0 + ROWS, it.rows) - 1));
+        tile.low &= ~(STEP_KEYS - 1);
+        const int all_steps = (tile.high - tile.low + STEP_KEYS - 1) / STEP_KEYS, step0 = share.step_of(it, part0, all_steps);
         const int steps = share.step_of(it, part1, all_steps) - step0;
-        const int64_t key0 = tile.low + int64_t(step0) * STEP_KEYS, key1 = min(tile.high, key0 + int64_t(steps) * STEP_KEYS);
+        const int key0 = tile.low + step0 * STEP_KEYS, key1 = min(tile.high, key0 + steps * STEP_KEYS);
         const bool began = part0 > it.line_begin, goes_on = part1 < it.line_end;
         const int wave_first = it.row0 + 32 * wave, wave_last = min(wave_first + 31, it.rows - 1);
         const Keys own = keys_of(p, it, token, token);
-        const Keys first = keys_of(p, it, min(wave_first, it.rows - 1) / p.group, min(wave_first, it.rows - 1) / p.group);
-        const Keys last = keys_of(p, it, wave_last / p.group, wave_last / p.group);
-        const int own_low = near32(own.low - key0) - 4 * half, own_high = near32(own.high - key0) - 4 * half;
-        const int some_low = near32(first.low - key0), some_high = wave_first < it.rows ? near32(last.high - key0) : -(1 << 30);
-        const int all_low = near32(last.low - key0), all_high = near32(first.high - key0);
+        const int first_at = by_group(p, min(wave_first, it.rows - 1)), last_at = by_group(p, wave_last);
+        const Keys first = keys_of(p, it, first_at, first_at), last = keys_of(p, it, last_at, last_at);
+        const int own_low = (own.low - key0) - 4 * half, own_high = (own.high - key0) - 4 * half;
+        const int some_low = (first.low - key0), some_high = wave_first < it.rows ? (last.high - key0) : -(1 << 30);
+        const int all_low = (last.low - key0), all_high = (first.high - key0);
 
         // this wave's 16 keys of a step: their page, codes and scales
         const int* table = p.tables + it.request * p.table_stride;
@@ -367,7 +373,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
             Pages r;
 #pragma unroll
             for (int u = 0; u < SUBS; ++u) {
-                const int64_t key = key0 + int64_t(step) * STEP_KEYS + 64 * u + 16 * granule;
+                const int key = key0 + step * STEP_KEYS + 64 * u + 16 * granule;
                 r.of[u] = key < key1 ? scalar_load(table + (key >> p.block_log2)) : -1;
             }
             return r;
@@ -387,7 +393,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
                 int page = pages.of[u];
                 live_page[u] = page >= 0 && page < p.pages;
                 if (!live_page[u]) page = 0;
-                const int64_t at = page * page_bytes + head_bytes + (int(key0 + int64_t(step) * STEP_KEYS + 64 * u + 16 * granule) & block_mask) * D;
+                const int64_t at = page * page_bytes + head_bytes + ((key0 + step * STEP_KEYS + 64 * u + 16 * granule) & block_mask) * D;
                 if (does_v) {
 #pragma unroll
                     for (int i = 0; i < VI; ++i)
@@ -615,7 +621,7 @@ constexpr int FEW_ROWS = 16, FEW_KEYS = 32;
 template <int DT, int D>
 __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(AttentionArgs p) {
     constexpr int KF = D / 32, KV = D / 64, VF = D / 16, VW = D / 64;  // fragments; 16-byte loads of K a lane; dwords of V a key
-    __shared__ float sums[4][FEW_ROWS][D + 4];
+    __shared__ __align__(16) float sums[4][FEW_ROWS][D + 4];
     __shared__ float tops[4][FEW_ROWS], masses[4][FEW_ROWS];
     __shared__ int64_t scan[4], ends[256];
     const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, quarter = lane >> 4;
@@ -628,7 +634,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
     if (part0 >= part1) continue;
     const int row = it.row0 + (lane & 15);
     const bool live_row = row < it.rows;
-    const int token = min(row, it.rows - 1) / p.group, member = min(row, it.rows - 1) - token * p.group;
+    const int token = by_group(p, min(row, it.rows - 1)), member = min(row, it.rows - 1) - token * p.group;
     const uint16_t* q = static_cast<const uint16_t*>(p.q) + (it.first_token + token) * p.q_token + (it.head * p.group + member) * p.q_head;
     f16x8 query[KF];
     const float query_scale = load_query<DT, KF>(q + D / 4 * quarter, 8, live_row, query, [](uint32_t t) {
@@ -639,11 +645,11 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
     }) * p.scale * 0x1.715476p+0f;
 
     const int last_row = min(it.row0 + FEW_ROWS, it.rows) - 1;
-    const int64_t first_token = it.row0 / p.group, last_token = last_row / p.group;
+    const int first_token = by_group(p, it.row0), last_token = by_group(p, last_row);
     Keys tile = keys_of(p, it, first_token, last_token);
-    tile.low = min(tile.low, tile.high) & ~int64_t(FEW_KEYS - 1);
-    const int all_steps = int((tile.high - tile.low + FEW_KEYS - 1) / FEW_KEYS), step0 = share.step_of(it, part0, all_steps);
-    const int64_t key0 = tile.low + int64_t(step0) * FEW_KEYS, key1 = min(tile.high, tile.low + int64_t(share.step_of(it, part1, all_steps)) * FEW_KEYS);
+    tile.low &= ~(FEW_KEYS - 1);
+    const int all_steps = (tile.high - tile.low + FEW_KEYS - 1) / FEW_KEYS, step0 = share.step_of(it, part0, all_steps);
+    const int key0 = tile.low + step0 * FEW_KEYS, key1 = min(tile.high, tile.low + share.step_of(it, part1, all_steps) * FEW_KEYS);
     const bool began = part0 > it.line_begin, goes_on = part1 < it.line_end;
     const Keys own = keys_of(p, it, token, token);
     const Keys first = keys_of(p, it, first_token, first_token), last = keys_of(p, it, last_token, last_token);
@@ -651,15 +657,15 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
     const int* table = p.tables + it.request * p.table_stride;
     const int block_mask = (1 << p.block_log2) - 1;
     const int64_t page_bytes = (int64_t(p.heads) << p.block_log2) * D, head_bytes = (int64_t(it.head) << p.block_log2) * D;
-    const int64_t wave_key0 = key0 + wave * FEW_KEYS;
-    const int steps = key1 > wave_key0 ? int((key1 - wave_key0 + 4 * FEW_KEYS - 1) / (4 * FEW_KEYS)) : 0;
+    const int wave_key0 = key0 + wave * FEW_KEYS;
+    const int steps = key1 > wave_key0 ? (key1 - wave_key0 + 4 * FEW_KEYS - 1) / (4 * FEW_KEYS) : 0;
 
     // granule i of the wave: keys wave_key0 + 128 (i / 2) + 16 (i % 2); a lane holds granule 64 n + lane
     int page = 0;
     bool live_page = false;
     float ks = 0.0f, vs = 0.0f, log_v = 0.0f, inv_v = 0.0f, seen = 0.0f;
     const auto load_granules = [&](int step) {
-        const int64_t key = wave_key0 + int64_t(4 * FEW_KEYS) * (step + (lane >> 1)) + 16 * (lane & 1);
+        const int key = wave_key0 + 4 * FEW_KEYS * (step + (lane >> 1)) + 16 * (lane & 1);
         page = key < key1 ? table[key >> p.block_log2] : -1;
         live_page = page >= 0 && page < p.pages;
         if (!live_page) page = 0;
@@ -692,10 +698,10 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
         }
     };
     const auto load_codes = [&](Raw& raw, int step) {
-        const int64_t key = wave_key0 + int64_t(4 * FEW_KEYS) * step;
+        const int key = wave_key0 + 4 * FEW_KEYS * step;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            const int64_t at = __builtin_amdgcn_readlane(page, 2 * (step & 31) + b) * page_bytes + head_bytes + (int(key + 16 * b) & block_mask) * D;
+            const int64_t at = __builtin_amdgcn_readlane(page, 2 * (step & 31) + b) * page_bytes + head_bytes + ((key + 16 * b) & block_mask) * D;
             const int8_t* k = p.k_codes + at + (lane & 15) * D + D / 4 * quarter;
 #pragma unroll
             for (int i = 0; i < KV; ++i) raw.k[b][i] = reinterpret_cast<const u32x4*>(k)[i];
@@ -712,7 +718,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
 #pragma unroll
     for (int i = 0; i < VF; ++i) acc[i] = v4f{};
     const auto take_step = [&](Raw& raw, int step) {
-        const int64_t key = wave_key0 + int64_t(4 * FEW_KEYS) * step;
+        const int key = wave_key0 + 4 * FEW_KEYS * step;
         // this step's operands out of the raw registers, then the loads of the step after the next
         f16x8 k[2][KF], v[VF];
 #pragma unroll
@@ -749,7 +755,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
             for (int i = 0; i < 4; ++i) t[4 * b + i] = __builtin_fmaf(s[i], m, page_log_v[b]);
         }
         if (key + FEW_KEYS > first.high || key + FEW_KEYS > key1 || key < last.low) {
-            const int high = int(min(min(own.high, key1) - key, int64_t(64))) - 4 * quarter, low = int(max(own.low - key, int64_t(-64))) - 4 * quarter;
+            const int high = min(own.high, key1) - key - 4 * quarter, low = own.low - key - 4 * quarter;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int at = 16 * (i >> 2) + (i & 3);
@@ -799,9 +805,10 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
     mass = add_xor32(add_xor16(mass));
     // a lane's sums: channels D / 4 * quarter + D / 16 * i + j of its row, i = 0-3, j = fragment
 #pragma unroll
-    for (int j = 0; j < VF; ++j)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sums[wave][lane & 15][D / 4 * quarter + VF * i + j] = acc[j][i];
+        for (int j = 0; j < VF; j += 4)
+            *reinterpret_cast<v4f*>(&sums[wave][lane & 15][D / 4 * quarter + VF * i + j]) = v4f{acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]};
     if (!quarter) {
         tops[wave][lane] = top;
         masses[wave][lane] = mass;
@@ -831,7 +838,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
         }
         if (!began) note_split(p, share, it);
     } else if (out_row < it.rows) {
-    const int out_token = out_row / p.group, out_member = out_row - out_token * p.group;
+    const int out_token = by_group(p, out_row), out_member = out_row - out_token * p.group;
     uint16_t* out = static_cast<uint16_t*>(p.out) + (it.first_token + out_token) * p.out_token + (it.head * p.group + out_member) * p.out_head + c0;
 #pragma unroll
     for (int j = 0; j < D / 16; j += 4) {
@@ -899,7 +906,7 @@ __global__ void __launch_bounds__(256) kv_attention_join(AttentionArgs p) {
             top = next;
         }
         if (group) continue;
-        const int token = row / p.group, member = row - token * p.group;
+        const int token = by_group(p, row), member = row - token * p.group;
         uint16_t* out = static_cast<uint16_t*>(p.out) + (tile[3] + token) * p.out_token + (head * p.group + member) * p.out_head + c;
         uint16_t o[4];
 #pragma unroll
@@ -919,7 +926,7 @@ struct Launches {
 
 static int64_t align256(int64_t v) { return (v + 255) & ~int64_t(255); }
 
-static Launches plan_launches(int64_t tokens, int64_t requests, int64_t group, int head_dim, int sms) {
+static Launches plan_launches(int64_t tokens, int64_t requests, int64_t heads, int64_t group, int head_dim, int sms) {
     Launches l = {};
     const int64_t rows = tokens * group;
     // A request's rows are known on the GPU alone. On average up to 16 a request: all on the tiles of few rows; more than 64: all on
@@ -931,7 +938,11 @@ static Launches plan_launches(int64_t tokens, int64_t requests, int64_t group, i
     if (!l.used[0]) l.limit = 0;
     l.few_rows = int(std::min<int64_t>(rows, FEW_ROWS));
     l.waves = head_dim == 256 ? 4 : 8;
-    const int per_cu[2] = {2, 1}, tile_rows[2] = {FEW_ROWS, 32 * l.waves};
+    // Two workgroups a CU on the tiles of few rows hide more of the time that a tile takes besides its keys; one where a tile would come apart into
+    // more than 32 parts (1 token over 32760 keys, 8 heads: 28.5 us on 32 parts a tile, 34.7 on 64, their joining 5.6 and 10.2; 64 requests
+    // of up to 8192: 122.6 on 256 workgroups, 119.5 on 512).
+    const int64_t few_tiles = (rows / FEW_ROWS + std::min(tokens, requests)) * heads;
+    const int per_cu[2] = {2 * sms <= 32 * few_tiles ? 2 : 1, 1}, tile_rows[2] = {FEW_ROWS, 32 * l.waves};
     for (int i = 0; i < 2; ++i) {
         l.shares[i] = (per_cu[i] * sms + 7) & ~7;
         if (l.used[i]) l.bytes[i] = align256(int64_t(l.shares[i]) * 20) + align256(int64_t(l.shares[i]) * 2 * tile_rows[i] * (head_dim + 2) * 4);
@@ -968,7 +979,7 @@ using namespace wq8;
 WQ8_API void wq8_kv_attention_workspace(int tokens, int requests, int heads, int group, int head_dim, int sms, int64_t* sizes) {
     sizes[0] = sizes[1] = 0;
     if (tokens < 1 || requests < 1 || heads < 1 || group < 1) return;
-    const Launches l = plan_launches(tokens, requests, group, head_dim, sms);
+    const Launches l = plan_launches(tokens, requests, heads, group, head_dim, sms);
     sizes[0] = l.bytes[0] + l.bytes[1];
 }
 
@@ -978,11 +989,11 @@ WQ8_API int wq8_kv_attention(const void* q, void* out, const long long* strides,
                              int sms, void* workspace, hipStream_t stream) {
     if (dtype != DT_F16 && dtype != DT_BF16) return -1;
     if (tokens < 0 || requests < 0 || heads < 1 || group < 1 || (head_dim != 64 && head_dim != 128 && head_dim != 256) ||
-        (block != 16 && block != 32 && block != 64 && block != 128) || window < 0 || pages < 0 || pages > 0x7fffffff || width < 0 || sms < 1)
+        (block != 16 && block != 32 && block != 64 && block != 128) || window < 0 || pages < 0 || pages > 0x7fffffff || width < 0 || sms < 1 || int64_t(width) * block > (1 << 30))
         return -2;
     if (!tokens || !requests) return 0;
     if (int64_t(tokens) * group > 0x7fffffff - 256) return -2;  // rows are counted in 32 bits
-    const Launches l = plan_launches(tokens, requests, group, head_dim, sms);
+    const Launches l = plan_launches(tokens, requests, heads, group, head_dim, sms);
     if ((l.bytes[0] + l.bytes[1] && !workspace) || reinterpret_cast<uintptr_t>(workspace) % 16) return -2;
     AttentionArgs p = {};
     p.q = q; p.out = out;
@@ -990,6 +1001,7 @@ WQ8_API int wq8_kv_attention(const void* q, void* out, const long long* strides,
     p.k_codes = k_codes; p.k_scales = k_scales; p.v_codes = v_codes; p.v_scales = v_scales;
     p.tables = static_cast<const int*>(tables); p.lens = static_cast<const int*>(lens); p.starts = static_cast<const int*>(starts);
     p.table_stride = table_stride; p.pages = pages; p.width = width; p.tokens = tokens; p.requests = requests; p.heads = heads; p.group = group;
+    p.group_inverse = unsigned((uint64_t(1) << 32) / unsigned(group) - (group == 1));
     p.block_log2 = __builtin_ctz(block); p.causal = causal; p.window = window; p.scale = scale;
     char* ws = static_cast<char*>(workspace);
     const auto run = [&](auto dt, auto d) { return launch_attention<decltype(dt)::value, decltype(d)::value>(p, l, ws, stream); };
