@@ -365,18 +365,24 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
         const int some_low = (first.low - key0), some_high = wave_first < it.rows ? (last.high - key0) : -(1 << 30);
         const int all_low = (last.low - key0), all_high = (first.high - key0);
 
-        // this wave's 16 keys of a step: their page, codes and scales
+        // This wave's 16 keys of every 64: their pages and scales come 64 at a time, one a lane (vector loads: scalar ones would be waited for
+        // with every LDS read).
         const int* table = p.tables + it.request * p.table_stride;
         const int64_t head_bytes = (int64_t(it.head) << p.block_log2) * D;
-        struct Pages { int of[SUBS]; };
-        const auto pages_of = [&](int step) {
-            Pages r;
-#pragma unroll
-            for (int u = 0; u < SUBS; ++u) {
-                const int key = key0 + step * STEP_KEYS + 64 * u + 16 * granule;
-                r.of[u] = key < key1 ? scalar_load(table + (key >> p.block_log2)) : -1;
+        int page = 0;
+        float seen = 0.0f;
+        PageScales lane_scales = {};
+        const auto load_pages = [&](int first) {  // of the 64 keys first, first + 1, ... of the part
+            const int key = key0 + 64 * (first + lane) + 16 * granule;
+            page = key < key1 ? table[key >> p.block_log2] : -1;
+            const bool live = page >= 0 && page < p.pages;
+            if (!live) page = 0;
+            if (does_v) {
+                const int64_t at = int64_t(page) * p.heads + it.head;
+                const float ks = p.k_scales[at], vs = live ? p.v_scales[at] : 0.0f;
+                seen = fmaxf(seen, wave_max(vs));
+                lane_scales = page_scales(ks, vs, seen, live);
             }
-            return r;
         };
         // codes on their way: with 8 waves a wave has keys or values, in the same registers
         constexpr bool BOTH = WAVES == 4;
@@ -385,15 +391,11 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
             if constexpr (BOTH) return own_k_raw[u][i];
             else return v_raw[u][i];
         };
-        float ks[SUBS] = {}, vs[SUBS] = {}, seen = 0.0f;
-        bool live_page[SUBS] = {};
-        const auto load_codes = [&](int step, const Pages& pages) {
+        const auto load_codes = [&](int step) {
 #pragma unroll
             for (int u = 0; u < SUBS; ++u) {
-                int page = pages.of[u];
-                live_page[u] = page >= 0 && page < p.pages;
-                if (!live_page[u]) page = 0;
-                const int64_t at = page * page_bytes + head_bytes + ((key0 + step * STEP_KEYS + 64 * u + 16 * granule) & block_mask) * D;
+                const int n = step * SUBS + u;
+                const int64_t at = __builtin_amdgcn_readlane(page, n & 63) * page_bytes + head_bytes + ((key0 + 64 * n + 16 * granule) & block_mask) * D;
                 if (does_v) {
 #pragma unroll
                     for (int i = 0; i < VI; ++i)
@@ -401,8 +403,6 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
 #pragma unroll
                             for (int j = 0; j < 8; ++j)
                                 v_raw[u][8 * i + j] = *reinterpret_cast<const uint32_t*>(p.v_codes + at + (v_at + 4 * i * D + (j < 4 ? j : j + 4) * D));
-                    ks[u] = scalar_load(p.k_scales + int64_t(page) * p.heads + it.head);
-                    vs[u] = scalar_load(p.v_scales + int64_t(page) * p.heads + it.head);
                 }
                 if (does_k) {
 #pragma unroll
@@ -414,7 +414,8 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
                 }
             }
         };
-        const auto store_codes = [&](int buffer) {
+        const auto store_codes = [&](int step) {
+            const int buffer = step & 1;
 #pragma unroll
             for (int u = 0; u < SUBS; ++u) {
                 if (does_v) {
@@ -431,12 +432,10 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
                                 at[entry ^ (entry >> 3 & 3) ^ (v_dw & 8)] = u32x4{pairs[0][c], pairs[1][c], pairs[2][c], pairs[3][c]};
                             }
                     }
-                    seen = fmaxf(seen, live_page[u] ? vs[u] : 0.0f);
-                    const PageScales s = page_scales(ks[u], vs[u], seen, live_page[u]);
-                    if (!lane) {
-                        reinterpret_cast<float*>(&page_k[buffer][u])[granule] = s.k;
-                        reinterpret_cast<float*>(&page_log_v[buffer][u])[granule] = s.log_v;
-                        reinterpret_cast<float*>(&page_inv_v[buffer][u])[granule] = s.inv_v;
+                    if (lane == ((step * SUBS + u) & 63)) {
+                        reinterpret_cast<float*>(&page_k[buffer][u])[granule] = lane_scales.k;
+                        reinterpret_cast<float*>(&page_log_v[buffer][u])[granule] = lane_scales.log_v;
+                        reinterpret_cast<float*>(&page_inv_v[buffer][u])[granule] = lane_scales.inv_v;
                     }
                 }
                 if (does_k) {
@@ -458,22 +457,20 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) acc[i] = v16f{};
 
-        Pages pages = pages_of(0);
         if (steps > 0) {
-            load_codes(0, pages);
-            pages = pages_of(1);
+            load_pages(0);
+            load_codes(0);
             store_codes(0);
-            load_codes(1, pages);
-            pages = pages_of(2);
+            if (steps > 1) load_codes(1);
             __syncthreads();
         }
         for (int step = 0; step < steps; ++step) {
             const int buffer = step & 1;
             const auto next = [&] {
                 if (step + 1 < steps) {
-                    store_codes(buffer ^ 1);
-                    load_codes(step + 2, pages);
-                    pages = pages_of(step + 3);
+                    store_codes(step + 1);
+                    if ((step + 2) * SUBS % 64 == 0) load_pages((step + 2) * SUBS);
+                    if (step + 2 < steps) load_codes(step + 2);
                 }
             };
             if (wave >= 4) next();
