@@ -16,7 +16,7 @@ from typing import NamedTuple
 import torch
 
 from . import DTYPES, _native, library
-from ._rotary import Layouts, _check_places, _check_rows
+from ._rotary import Layouts, _check_aligned, _check_devices, _check_rows
 
 BLOCKS = (16, 32, 64, 128)
 ATTENTION_HEAD_DIMS = (64, 128, 256)
@@ -92,9 +92,8 @@ def kv_plan(past, new, tables, free, used, block, tokens):
     every later one that needs a page where the free list ran out. Everything is int32 / int64 on the GPU; nothing is read
     on the host."""
     key = (past.shape, past.dtype, past.stride(), new.shape, new.dtype, new.stride(), free.shape, free.dtype, free.stride(), tables.shape, tables.stride(),
-           tables.dtype, used.shape, used.dtype, block, tokens)
+           tables.dtype, used.shape, used.dtype, block, tokens, past.get_device(), new.get_device(), free.get_device(), tables.get_device(), used.get_device())
     splits = _plan_layouts.get(key) or _plan_layouts.keep(key, _check_plan(past, new, tables, free, used, block, tokens))
-    _check_places(past.get_device(), (), (new, tables, free, used))
     slots = past.new_empty(tokens, dtype=torch.int64)
     held = past.new_empty(tokens + 2 * splits[2] + 3)
     positions, starts, lens, used_out, missing = held.split_with_sizes(splits)
@@ -123,6 +122,7 @@ def _check_plan(past, new, tables, free, used, block, tokens):
         raise ValueError(f"past, new and tables must be of as many requests, not {requests}, {new.shape[0]} and {tables.shape[0]}")
     if block < 1 or not 0 <= tokens < 2 ** 31:
         raise ValueError("a block of at least one token and a token count are wanted")
+    _check_devices(past, new, tables, free, used)
     return [tokens, requests + 1, requests, 1, 1]
 
 
@@ -132,6 +132,7 @@ def _check_write(cache, k, v, slots):
     _check_ints(slots, "slots", torch.int64)
     if k.shape != v.shape or k.dtype != v.dtype or k.shape[1:] != (cache.heads, cache.head_dim) or slots.shape[0] != k.shape[0]:
         raise ValueError(f"keys and values must be (tokens, {cache.heads}, {cache.head_dim}), of one type, with a slot each")
+    _check_devices(cache.k_codes, k, v, slots)
     return (ctypes.c_longlong * 4)(k.stride(0), k.stride(1), v.stride(0), v.stride(1)), k.shape[0], DTYPES[k.dtype], (cache.pages, cache.heads, cache.block, cache.head_dim)
 
 
@@ -139,20 +140,21 @@ def kv_write(cache, k, v, slots):
     """Keys and values (tokens, heads, head_dim), BF16, FP16 or FP32, into the cache at `slots` (int64; any order, each at most once;
     those outside the cache, as -1, are left out). A page's scale grows to its largest value, and tokens that it holds are then
     coded again; a write to its first slot begins it anew. NaN is held as 0 and infinities as the largest finite number."""
-    key = (k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, slots.shape, slots.stride(), slots.dtype)
+    key = (k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(), v.dtype, v.get_device(), slots.shape, slots.stride(), slots.dtype,
+           slots.get_device())
     strides, tokens, dtype, shape = cache.layouts.get(key) or cache.layouts.keep(key, _check_write(cache, k, v, slots))
     codes = cache.k_codes
-    k_at, v_at = _check_places(codes.get_device(), (k, v), (slots,))
+    k_at, v_at = k.data_ptr(), v.data_ptr()
+    _check_aligned((k_at, v_at))
     library().call("wq8_kv_write", k_at, v_at, strides, slots.data_ptr(), tokens, codes.data_ptr(), cache.k_scales.data_ptr(), cache.v_codes.data_ptr(),
                    cache.v_scales.data_ptr(), *shape, dtype, cache.owner.data_ptr(), _native.gpu(codes).stream())
 
 
 def kv_read(cache, slots, dtype=torch.bfloat16):
     """The keys and values at `slots` (int64; zeros outside the cache), rounded once to dtype: two (tokens, heads, head_dim) tensors."""
-    key = (slots.shape, slots.stride(), slots.dtype, dtype)
+    key = (slots.shape, slots.stride(), slots.dtype, slots.get_device(), dtype)
     shape, like = cache.layouts.get(key) or cache.layouts.keep(key, _check_read(cache, slots, dtype))
     codes = cache.k_codes
-    _check_places(codes.get_device(), (), (slots,))
     k = codes.new_empty(like, dtype=dtype)
     v = torch.empty_like(k)
     library().call("wq8_kv_read", codes.data_ptr(), cache.k_scales.data_ptr(), cache.v_codes.data_ptr(), cache.v_scales.data_ptr(), slots.data_ptr(), like[0],
@@ -164,6 +166,7 @@ def _check_read(cache, slots, dtype):
     _check_ints(slots, "slots", torch.int64)
     if dtype not in DTYPES:
         raise ValueError(f"dtype must be FP16, BF16 or FP32, not {dtype}")
+    _check_devices(cache.k_codes, slots)
     return (cache.pages, cache.heads, cache.block, cache.head_dim), (slots.shape[0], cache.heads, cache.head_dim)
 
 
@@ -178,8 +181,8 @@ def kv_attention(q, cache, tables, lens, starts, causal=True, window=0, scale=No
     position - window. scale: of the scores, 1 / sqrt(head_dim) by default. Rows that see nothing are zero; pages outside the cache are
     hidden; rows of no request are not written. Returns (tokens, query heads, head_dim) in q's dtype. Sums and the softmax's
     statistics are FP32, its weights FP16 relative to the largest."""
-    key = (q.shape, q.stride(), q.dtype, tables.shape, tables.stride(), tables.dtype, lens.shape, lens.stride(), lens.dtype, starts.shape, starts.stride(),
-           starts.dtype)
+    key = (q.shape, q.stride(), q.dtype, q.get_device(), tables.shape, tables.stride(), tables.dtype, tables.get_device(), lens.shape, lens.stride(), lens.dtype,
+           lens.get_device(), starts.shape, starts.stride(), starts.dtype, starts.get_device())
     layout = cache.layouts.get(key) or cache.layouts.keep(key, _check_attention(q, cache, tables, lens, starts))
     strides, table_stride, shape, default_scale, dtype, cus, workspace_bytes = layout
     if not 0 <= window < 2 ** 31:
@@ -190,9 +193,11 @@ def kv_attention(q, cache, tables, lens, starts, causal=True, window=0, scale=No
         _check_rows(out, "outputs")
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError("outputs do not match the queries")
+        _check_devices(q, out)
         strides = type(strides)(strides[0], strides[1], out.stride(0), out.stride(1))
     codes = cache.k_codes
-    q_at, out_at = _check_places(codes.get_device(), (q, out), (tables, lens, starts))
+    q_at, out_at = q.data_ptr(), out.data_ptr()
+    _check_aligned((q_at,))
     workspace = codes.new_empty(workspace_bytes) if workspace_bytes else None
     library().call("wq8_kv_attention", q_at, out_at, strides, codes.data_ptr(), cache.k_scales.data_ptr(), cache.v_codes.data_ptr(), cache.v_scales.data_ptr(),
                    tables.data_ptr(), table_stride, tables.shape[1], lens.data_ptr(), starts.data_ptr(), *shape, default_scale if scale is None else scale,
@@ -215,8 +220,7 @@ def _check_attention(q, cache, tables, lens, starts):
         raise ValueError(f"tables and starts must be of {requests} requests")
     if tables.shape[1] * cache.block > 2 ** 30:
         raise ValueError("block tables reach 2^30 tokens a request at most")
-    if not q.is_cuda:
-        raise ValueError("tensors must be on the GPU")
+    _check_devices(cache.k_codes, q, tables, lens, starts)
     group, state = q_heads // heads, _native.gpu(q)
     sizes = (ctypes.c_int64 * 2)()
     library().wq8_kv_attention_workspace(tokens, requests, heads, group, head_dim, state.cus, sizes)

@@ -84,20 +84,19 @@ def _check_rows(x, name):
         raise ValueError(f"rows of {name} must be 16-byte aligned")
 
 
-def _check_places(device, aligned, others=()):
-    """Tensors on GPU `device` (an index; the kernels take raw pointers), the first ones 16-byte aligned; their addresses."""
+def _check_devices(*tensors):
+    """Tensors on one GPU: the kernels take raw pointers."""
+    device = tensors[0].get_device()
     if device < 0:
         raise ValueError("tensors must be on the GPU")
-    pointers = [t.data_ptr() for t in aligned]
-    for t, p in zip(aligned, pointers):
+    if any(t.get_device() != device for t in tensors):
+        raise ValueError("tensors must be on one GPU")
+
+
+def _check_aligned(pointers):
+    for p in pointers:
         if p & 15:
             raise ValueError("rows must be 16-byte aligned")
-        if t.get_device() != device:
-            raise ValueError("tensors must be on one GPU")
-    for t in others:
-        if t.get_device() != device:
-            raise ValueError("tensors must be on one GPU")
-    return pointers
 
 
 def _check_rotary(tensors, positions, plan):
@@ -115,6 +114,7 @@ def _check_rotary(tensors, positions, plan):
         raise ValueError(f"the plan turns {2 * plan.pairs} channels, the heads have {head_dim}")
     if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in ((tokens, axes), (tokens,) if axes == 1 else (tokens, axes)):
         raise ValueError(f"rotary positions must be ({tokens}, {axes}) int32 or int64, not {tuple(positions.shape)} {positions.dtype}")
+    _check_devices(*tensors, positions, plan.turns)
     count = len(tensors)
     # a new output is contiguous
     strides = [v for x in tensors for v in (x.shape[1], x.stride(0), x.stride(1), x.shape[1] * head_dim, head_dim)]
@@ -130,7 +130,7 @@ def rotary(xs, positions, plan, inverse=False, out=None):
     them in no other way."""
     many = not isinstance(xs, torch.Tensor)
     tensors = tuple(xs) if many else (xs,)
-    key = (positions.shape, positions.stride(), positions.dtype, *[(x.shape, x.stride(), x.dtype) for x in tensors])
+    key = (positions.shape, positions.stride(), positions.dtype, positions.get_device(), *[(x.shape, x.stride(), x.dtype, x.get_device()) for x in tensors])
     layout = plan.layouts.get(key) or plan.layouts.keep(key, _check_rotary(tensors, positions, plan))
     pointers, strides, pos_token, pos_axis, wide, tokens, head_dim, dtype = layout
     if out is None:
@@ -141,10 +141,11 @@ def rotary(xs, positions, plan, inverse=False, out=None):
             raise ValueError("rotary outputs do not match its inputs")
         for y in outs:
             _check_rows(y, "rotary outputs")
+        _check_devices(positions, *outs)
         strides = type(strides)(*[v for x, y in zip(tensors, outs) for v in (x.shape[1], x.stride(0), x.stride(1), y.stride(0), y.stride(1))])
-    device = tensors[0].get_device()
-    places = _check_places(device, tensors + outs, (positions, plan.turns))
-    count = len(tensors)
-    library().call("wq8_rotary", pointers(*places[:count]), pointers(*places[count:]), strides, count, positions.data_ptr(), pos_token, pos_axis, wide, tokens,
-                   plan.turns.data_ptr(), plan.axis.data_ptr(), plan.pairs, head_dim, STYLES[plan.style], inverse, dtype, _native.gpu(tensors[0]).stream())
+    places, to = [x.data_ptr() for x in tensors], [y.data_ptr() for y in outs]
+    _check_aligned(places)
+    count = len(places)
+    library().call("wq8_rotary", pointers(*places), pointers(*to), strides, count, positions.data_ptr(), pos_token, pos_axis, wide, tokens, plan.turns.data_ptr(),
+                   plan.axis.data_ptr(), plan.pairs, head_dim, STYLES[plan.style], inverse, dtype, _native.gpu(positions).stream())
     return outs if many else outs[0]

@@ -5,6 +5,7 @@
 #include "wq8_common.h"
 #include "wq8_abi.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace wq8 {
 
@@ -277,13 +278,13 @@ __global__ void __launch_bounds__(256) kv_write_scan(CacheArgs p) {
 }
 
 // Many tokens: a workgroup looks through p.group of them (64 at most) for those that have the lowest written slot of a page, and writes these
-// pages' codes of one head, keys and values.
+// pages' codes.
 template <int DT, int NI>
 __global__ void __launch_bounds__(256) kv_write_owned(CacheArgs p) {
     __shared__ int rows[KV_MAX_BLOCK];
     __shared__ int64_t pages[64];
     __shared__ float lds4[4];
-    const int head = blockIdx.y, block = 1 << p.block_log2;
+    const int block = 1 << p.block_log2;
     const auto writer = [&](int64_t slot) {
         const int t = p.owner[slot];
         return t >= 0 && t < p.tokens && p.slots[t] == slot ? t : -1;
@@ -308,7 +309,8 @@ __global__ void __launch_bounds__(256) kv_write_owned(CacheArgs p) {
         if (page < 0) continue;
         if (int(threadIdx.x) < block) rows[threadIdx.x] = writer((page << p.block_log2) + threadIdx.x);
         __syncthreads();
-        for (int which = blockIdx.z; which < 2; which += gridDim.z) write_page<DT, NI>(p, which, page, head, rows, lds4);
+        // keys and values of every gridDim.y-th head
+        for (int part = blockIdx.y; part < 2 * p.heads; part += gridDim.y) write_page<DT, NI>(p, part & 1, page, part >> 1, rows, lds4);
         __syncthreads();
     }
 }
@@ -317,12 +319,14 @@ template <int DT, int NI> static int launch_pages(CacheArgs p, hipStream_t strea
     if (p.tokens <= KV_SCAN_TOKENS) {
         kv_write_scan<DT, NI><<<dim3(unsigned(p.tokens), p.heads, 2), 256, 0, stream>>>(p);
     } else {
-        // tokens a workgroup: fewer where workgroups are few (each token may have a page of its own); keys and values in one where they are many
+        // Tokens a workgroup: fewer where workgroups are few (each token may have a page of its own). Finding the pages costs a workgroup about
+        // as much as writing one, so it then writes several heads where there are enough workgroups.
         p.group = 64;
         while (p.group > 4 && p.tokens * p.heads * 2 < p.group * int64_t(4096)) p.group >>= 1;
         const int64_t groups = (p.tokens + p.group - 1) / p.group;
+        const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(2 * p.heads, 4096 / groups));
         kv_owner<<<unsigned((p.tokens + 255) / 256), 256, 0, stream>>>(p);
-        kv_write_owned<DT, NI><<<dim3(unsigned(groups), p.heads, groups * p.heads >= 4096 ? 1 : 2), 256, 0, stream>>>(p);
+        kv_write_owned<DT, NI><<<dim3(unsigned(groups), unsigned(parts)), 256, 0, stream>>>(p);
     }
     return int(hipGetLastError());
 }
@@ -334,26 +338,36 @@ template <int DT> static int launch_write(const CacheArgs& p, hipStream_t stream
 }
 
 // ---- reads ---------------------------------------------------------------------------------------------------------
-template <int DT>
+// READ_VECTORS of 8 channels a thread: four where there are many (a 32760-token latent of 12 heads, keys and values: 61.6 us against 73 with one).
+template <int DT, int READ_VECTORS>
 __global__ void __launch_bounds__(256) kv_read_rows(CacheArgs p) {
     using raw = typename Elem<DT>::raw;
     const int per_row = p.head_dim >> 3, per_token = p.heads * per_row, which = blockIdx.y;
-    // vector blockIdx.x * 256 + threadIdx.x of (token, head, chunk): the wide division is the workgroup's alone
-    const int64_t token0 = blockIdx.x * int64_t(256) / per_token;
-    const unsigned in = unsigned(blockIdx.x * int64_t(256) - token0 * per_token) + threadIdx.x;
-    const int64_t token = token0 + in / unsigned(per_token);
-    if (token >= p.tokens) return;
-    const unsigned rest = in % unsigned(per_token), head = rest / unsigned(per_row), c = rest % unsigned(per_row);
-    const int64_t slot = p.slots[token];
-    float v[8] = {};
-    if (slot >= 0 && slot < p.all_slots) {
-        const int64_t row = (slot >> p.block_log2) * p.heads + head;
-        const float scale = p.scales[which][row];
-        const u32x2 q = *reinterpret_cast<const u32x2*>(p.codes[which] + ((row << p.block_log2) + (slot & ((1 << p.block_log2) - 1))) * p.head_dim + 8 * c);
+    // vectors blockIdx.x * 256 * READ_VECTORS + 256 n + threadIdx.x of (token, head, chunk): the wide division is the workgroup's alone
+    const int64_t first = blockIdx.x * int64_t(256 * READ_VECTORS), token0 = first / per_token;
+    const unsigned in = unsigned(first - token0 * per_token) + threadIdx.x;
+    float v[READ_VECTORS][8];
+    int64_t to[READ_VECTORS];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = float(int8_t(q[j >> 2] >> (8 * (j & 3)))) * scale;
+    for (int n = 0; n < READ_VECTORS; ++n) {
+        const unsigned at = in + 256 * n, rest = at % unsigned(per_token), head = rest / unsigned(per_row), c = rest % unsigned(per_row);
+        const int64_t token = token0 + at / unsigned(per_token);
+        to[n] = token < p.tokens ? token * per_token + rest : -1;
+        const int64_t slot = token < p.tokens ? p.slots[token] : -1;
+        const bool live = slot >= 0 && slot < p.all_slots;
+        const int64_t row = live ? (slot >> p.block_log2) * p.heads + head : 0, in_page = live ? slot & ((1 << p.block_log2) - 1) : 0;
+        u32x2 q = {0, 0};
+        float scale = 0.0f;
+        if (live) {
+            scale = p.scales[which][row];
+            q = *reinterpret_cast<const u32x2*>(p.codes[which] + ((row << p.block_log2) + in_page) * p.head_dim + 8 * c);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[n][j] = float(int8_t(q[j >> 2] >> (8 * (j & 3)))) * scale;
     }
-    store8<DT>(static_cast<raw*>(p.y[which]) + (token * per_token + rest) * 8, v);
+#pragma unroll
+    for (int n = 0; n < READ_VECTORS; ++n)
+        if (to[n] >= 0) store8<DT>(static_cast<raw*>(p.y[which]) + to[n] * 8, v[n]);
 }
 
 static bool bad_cache(int64_t tokens, int64_t pages, int heads, int block, int head_dim) {
@@ -394,11 +408,18 @@ WQ8_API int wq8_kv_read(const int8_t* k_codes, const float* k_scales, const int8
     const CacheArgs p = {{}, {k, v}, {}, {}, {const_cast<int8_t*>(k_codes), const_cast<int8_t*>(v_codes)},
                          {const_cast<float*>(k_scales), const_cast<float*>(v_scales)}, reinterpret_cast<const int64_t*>(slots), nullptr, tokens, pages * block,
                          heads, __builtin_ctz(block), head_dim, 0};
-    const int64_t blocks = (tokens * heads * (head_dim >> 3) + 255) / 256;
+    const int64_t vectors = tokens * heads * (head_dim >> 3);
+    const int each = vectors >= 1 << 20 ? 4 : 1;
+    const int64_t blocks = (vectors + 256 * each - 1) / (256 * each);
     if (blocks > 0x7fffffff) return -2;
     const dim3 grid(static_cast<unsigned>(blocks), 2);
-    if (dtype == DT_F16) kv_read_rows<DT_F16><<<grid, 256, 0, stream>>>(p);
-    else if (dtype == DT_BF16) kv_read_rows<DT_BF16><<<grid, 256, 0, stream>>>(p);
-    else kv_read_rows<DT_F32><<<grid, 256, 0, stream>>>(p);
+    const auto run = [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        if (each == 4) kv_read_rows<DT, 4><<<grid, 256, 0, stream>>>(p);
+        else kv_read_rows<DT, 1><<<grid, 256, 0, stream>>>(p);
+    };
+    if (dtype == DT_F16) run(std::integral_constant<int, DT_F16>());
+    else if (dtype == DT_BF16) run(std::integral_constant<int, DT_BF16>());
+    else run(std::integral_constant<int, DT_F32>());
     return int(hipGetLastError());
 }
