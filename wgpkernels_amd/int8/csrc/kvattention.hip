@@ -120,6 +120,7 @@ template <int ROWS> struct Share {
     int64_t at, end, share, line;
     int64_t base_at;
     int base, index;
+    Span only;         // the one request of a call that has one
 
     // 256 requests from `first` on: spans a thread each, their ends in LDS
     WQ8_DEVICE int64_t strip(int first, int64_t before) {
@@ -136,8 +137,8 @@ template <int ROWS> struct Share {
     // values in its L2. A share is at least `least` keys.
     WQ8_DEVICE Share(const AttentionArgs& args, int64_t* scan, int64_t* request_ends, int least) : p(args), lds4(scan), ends(request_ends) {
         if (p.requests == 1) {
-            const Span s = span_of<ROWS, true>(p, 0);
-            line = s.upto(s.tiles) * p.heads;
+            only = span_of<ROWS, true>(p, 0);
+            line = only.upto(only.tiles) * p.heads;
             base = 0;
             base_at = 0;
         } else {
@@ -165,23 +166,25 @@ template <int ROWS> struct Share {
             const int m = (a + b) >> 1;
             if (uniform(ends[m]) > at) b = m; else a = m + 1;
         }
-        const Span s = span_of<ROWS, true>(p, uniform(base + a));
+        const Span s = p.requests == 1 ? only : span_of<ROWS, true>(p, uniform(base + a));
         const int64_t begin = a ? uniform(ends[a - 1]) : base_at, per_head = s.upto(s.tiles);
         int64_t in = at - begin;
         int head = uniform(int(ratio(in, per_head)));
         while (head > 0 && in < head * per_head) --head;
         while (head + 1 < p.heads && in >= (head + 1) * per_head) ++head;
         in -= head * per_head;
-        int tile;
-        if (s.more) {  // first i + more i (i - 1) / 2 <= in
-            const float h = float(s.first) - 0.5f * float(s.more), m = float(s.more);
-            tile = int((__builtin_amdgcn_sqrtf(__builtin_fmaf(h, h, 2.0f * m * float(in))) - h) * __builtin_amdgcn_rcpf(m));
-        } else {
-            tile = int(ratio(in, s.first));
+        int tile = 0;
+        if (s.tiles > 1) {
+            if (s.more) {  // first i + more i (i - 1) / 2 <= in
+                const float h = float(s.first) - 0.5f * float(s.more), m = float(s.more);
+                tile = int((__builtin_amdgcn_sqrtf(__builtin_fmaf(h, h, 2.0f * m * float(in))) - h) * __builtin_amdgcn_rcpf(m));
+            } else {
+                tile = int(ratio(in, s.first));
+            }
+            tile = uniform(min(max(tile, 0), s.tiles - 1));
+            while (tile > 0 && s.upto(tile) > in) --tile;
+            while (tile + 1 < s.tiles && s.upto(tile + 1) <= in) ++tile;
         }
-        tile = uniform(min(max(tile, 0), s.tiles - 1));
-        while (tile > 0 && s.upto(tile) > in) --tile;
-        while (tile + 1 < s.tiles && s.upto(tile + 1) <= in) ++tile;
         const int64_t head_at = begin + head * per_head;
         return {uniform(base + a), uniform(tile * ROWS), uniform(s.rows), uniform(s.first_token), uniform(head), uniform(s.past), uniform(s.total),
                 uniform(head_at + s.upto(tile)), uniform(head_at + s.upto(tile + 1))};
@@ -233,12 +236,13 @@ WQ8_DEVICE void code_pairs(uint32_t a, uint32_t b, uint32_t* out) {
 }
 
 // ---- queries -------------------------------------------------------------------------------------------------------
-// N vectors of 8 channels of a row in FP16; returns what a product with them is multiplied by. A lane holds part of a row: `most`
-// gives the largest of its magnitudes over the row's lanes.
-template <int DT, int N, typename Most> WQ8_DEVICE float load_query(const uint16_t* row, int stride, bool live, f16x8* out, Most most) {
-    u32x4 raw[N];
+// N vectors of 8 channels of a row: as they are in memory, and in FP16; the latter returns what a product with them is multiplied by. A
+// lane holds part of a row: `most` gives the largest of its magnitudes over the row's lanes.
+template <int N> WQ8_DEVICE void fetch_query(const uint16_t* row, int stride, bool live, u32x4* raw) {
 #pragma unroll
     for (int i = 0; i < N; ++i) raw[i] = live ? *reinterpret_cast<const u32x4*>(row + i * stride) : u32x4{0, 0, 0, 0};
+}
+template <int DT, int N, typename Most> WQ8_DEVICE float use_query(const u32x4* raw, f16x8* out, Most most) {
     if constexpr (DT == DT_F16) {
 #pragma unroll
         for (int i = 0; i < N; ++i) out[i] = __builtin_bit_cast(f16x8, raw[i]);
@@ -343,9 +347,11 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
         const int row = it.row0 + 32 * wave + (lane & 31);
         const bool live_row = row < it.rows;
         const int token = by_group(p, min(row, it.rows - 1)), member = min(row, it.rows - 1) - token * p.group;
+        u32x4 query_raw[KF];
+        fetch_query<KF>(static_cast<const uint16_t*>(p.q) + (it.first_token + token) * p.q_token + (it.head * p.group + member) * p.q_head + 8 * half, 16,
+                        live_row, query_raw);
         f16x8 query[KF];
-        const float query_scale = load_query<DT, KF>(static_cast<const uint16_t*>(p.q) + (it.first_token + token) * p.q_token +
-                                                         (it.head * p.group + member) * p.q_head + 8 * half, 16, live_row, query, [](uint32_t t) {
+        const float query_scale = use_query<DT, KF>(query_raw, query, [](uint32_t t) {
             const LanePair o = swap32(__builtin_bit_cast(float, t));
             return max(__builtin_bit_cast(uint32_t, o.a), __builtin_bit_cast(uint32_t, o.b));
         }) * p.scale * 0x1.715476p+0f;
@@ -633,13 +639,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
     const bool live_row = row < it.rows;
     const int token = by_group(p, min(row, it.rows - 1)), member = min(row, it.rows - 1) - token * p.group;
     const uint16_t* q = static_cast<const uint16_t*>(p.q) + (it.first_token + token) * p.q_token + (it.head * p.group + member) * p.q_head;
-    f16x8 query[KF];
-    const float query_scale = load_query<DT, KF>(q + D / 4 * quarter, 8, live_row, query, [](uint32_t t) {
-        LanePair o = swap16(__builtin_bit_cast(float, t));
-        t = max(__builtin_bit_cast(uint32_t, o.a), __builtin_bit_cast(uint32_t, o.b));
-        o = swap32(__builtin_bit_cast(float, t));
-        return max(__builtin_bit_cast(uint32_t, o.a), __builtin_bit_cast(uint32_t, o.b));
-    }) * p.scale * 0x1.715476p+0f;
+    u32x4 query_raw[KF];  // on their way while the first codes are asked for
+    fetch_query<KF>(q + D / 4 * quarter, 8, live_row, query_raw);
 
     const int last_row = min(it.row0 + FEW_ROWS, it.rows) - 1;
     const int first_token = by_group(p, it.row0), last_token = by_group(p, last_row);
@@ -714,6 +715,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
     v4f acc[VF];
 #pragma unroll
     for (int i = 0; i < VF; ++i) acc[i] = v4f{};
+    f16x8 query[KF];
+    float query_scale = 0.0f;
     const auto take_step = [&](Raw& raw, int step) {
         const int key = wave_key0 + 4 * FEW_KEYS * step;
         // this step's operands out of the raw registers, then the loads of the step after the next
@@ -791,6 +794,12 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
         load_granules(0);
         load_codes(even, 0);
         if (steps > 1) load_codes(odd, 1);
+        query_scale = use_query<DT, KF>(query_raw, query, [](uint32_t t) {
+            LanePair o = swap16(__builtin_bit_cast(float, t));
+            t = max(__builtin_bit_cast(uint32_t, o.a), __builtin_bit_cast(uint32_t, o.b));
+            o = swap32(__builtin_bit_cast(float, t));
+            return max(__builtin_bit_cast(uint32_t, o.a), __builtin_bit_cast(uint32_t, o.b));
+        }) * p.scale * 0x1.715476p+0f;
         use_granules();
         take_scales(even, 0);
         take_scales(odd, 1);
