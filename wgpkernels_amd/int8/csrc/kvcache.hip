@@ -411,7 +411,7 @@ WQ8_API int wq8_kv_read(const int8_t* k_codes, const float* k_scales, const int8
     const int64_t vectors = tokens * heads * (head_dim >> 3);
     const int each = vectors >= 1 << 20 ? 4 : 1;
     const int64_t blocks = (vectors + 256 * each - 1) / (256 * each);
-    if (blocks > 0x7fffffff) return -2;
+    if (blocks > MAX_BLOCKS_256) return -2;
     const dim3 grid(static_cast<unsigned>(blocks), 2);
     const auto run = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;

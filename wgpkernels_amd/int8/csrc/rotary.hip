@@ -124,6 +124,7 @@ template <int DT, int STYLE> static int launch_rotary(RotaryArgs& p, hipStream_t
     const int pp = DT != DT_F32 && STYLE == ROTARY_HALVES && fits(8) ? 8 : fits(4) ? 4 : 1;
     const int64_t threads = p.tokens * (p.head_dim / (2 * pp));
     const int64_t blocks = (threads + 255) / 256;
+    if (blocks > MAX_BLOCKS_256) return -2;
     // heads per thread: up to 24, while 2^17 threads remain (a 32760-token latent of 24 heads: 82 us with all of them in a thread, 86.5 with 8: the
     // angles are made once)
     p.heads_per_thread = int(std::min<int64_t>(24, std::max<int64_t>(1, threads * p.heads >> 17)));
@@ -158,7 +159,6 @@ WQ8_API int wq8_rotary(const void* const* xs, void* const* ys, const long long* 
     p.turns = reinterpret_cast<const uint64_t*>(turns); p.axis = static_cast<const int*>(axis);
     p.tokens = tokens; p.count = count; p.pairs = pairs; p.head_dim = head_dim; p.inverse = inverse;
     if (!tokens || !p.heads) return 0;
-    if (tokens > (int64_t(1) << 31) / (head_dim / 2) * 128) return -2;  // the grid's width
     if (style == ROTARY_PAIRS)
         return dtype == DT_F16 ? launch_rotary<DT_F16, ROTARY_PAIRS>(p, stream) : dtype == DT_BF16 ? launch_rotary<DT_BF16, ROTARY_PAIRS>(p, stream)
                                                                                : launch_rotary<DT_F32, ROTARY_PAIRS>(p, stream);
