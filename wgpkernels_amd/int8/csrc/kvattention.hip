@@ -56,7 +56,7 @@ struct Span {
     WQ8_DEVICE int64_t upto(int64_t i) const { return first * i + more * (i * (i - 1) / 2); }
 };
 
-constexpr int TILE_KEYS_OVERHEAD = 128;  // what a tile costs besides its keys, in keys
+constexpr int TILE_KEYS_OVERHEAD = 256;  // what a tile costs besides its keys, in keys
 
 template <typename T> WQ8_DEVICE T scalar_load(const T* p) { return *(const __attribute__((address_space(4))) T*)(uint64_t)p; }
 
@@ -120,7 +120,11 @@ template <int ROWS> struct Share {
     int64_t at, end, share, line;
     int64_t base_at;
     int base, index;
-    Span only;         // the one request of a call that has one
+    // where item() stands
+    Span span;
+    int64_t head_at;   // where the head's tiles begin
+    int request, head, tile;
+    bool found = false;
 
     // 256 requests from `first` on: spans a thread each, their ends in LDS
     WQ8_DEVICE int64_t strip(int first, int64_t before) {
@@ -137,8 +141,8 @@ template <int ROWS> struct Share {
     // values in its L2. A share is at least `least` keys.
     WQ8_DEVICE Share(const AttentionArgs& args, int64_t* scan, int64_t* request_ends, int least) : p(args), lds4(scan), ends(request_ends) {
         if (p.requests == 1) {
-            only = span_of<ROWS, true>(p, 0);
-            line = only.upto(only.tiles) * p.heads;
+            span = span_of<ROWS, true>(p, 0);
+            line = span.upto(span.tiles) * p.heads;
             base = 0;
             base_at = 0;
         } else {
@@ -152,42 +156,57 @@ template <int ROWS> struct Share {
         at = index * share;
         end = min(line, at + share);
     }
+    // The tile at `at`: looked up the first time, and where a request ends; else the next tile.
     WQ8_DEVICE Item item() {
-        if (p.requests > 256) {
-            int64_t upto = 0;
-            for (int r = 0; r < p.requests; r += 256) {
-                __syncthreads();
-                upto = uniform(strip(r, upto));
-                if (at < upto) break;
+        if (found && ++tile == span.tiles) {
+            tile = 0;
+            head_at += span.upto(span.tiles);
+            found = ++head < p.heads;
+        }
+        if (!found) look_up();
+        found = true;
+        return {request, tile * ROWS, span.rows, span.first_token, head, span.past, span.total, head_at + span.upto(tile), head_at + span.upto(tile + 1)};
+    }
+    WQ8_DEVICE void look_up() {
+        int a = 0;
+        int64_t begin = 0;
+        if (p.requests > 1) {
+            if (p.requests > 256) {
+                int64_t upto = 0;
+                for (int r = 0; r < p.requests; r += 256) {
+                    __syncthreads();
+                    upto = uniform(strip(r, upto));
+                    if (at < upto) break;
+                }
             }
+            int b = min(256, p.requests - base) - 1;  // the first request that ends past `at`
+            while (a < b) {
+                const int m = (a + b) >> 1;
+                if (uniform(ends[m]) > at) b = m; else a = m + 1;
+            }
+            begin = a ? uniform(ends[a - 1]) : base_at;
+            span = span_of<ROWS, true>(p, uniform(base + a));
         }
-        int a = 0, b = min(256, p.requests - base) - 1;  // the first request that ends past `at`
-        while (a < b) {
-            const int m = (a + b) >> 1;
-            if (uniform(ends[m]) > at) b = m; else a = m + 1;
-        }
-        const Span s = p.requests == 1 ? only : span_of<ROWS, true>(p, uniform(base + a));
-        const int64_t begin = a ? uniform(ends[a - 1]) : base_at, per_head = s.upto(s.tiles);
+        request = uniform(base + a);
+        const int64_t per_head = span.upto(span.tiles);
         int64_t in = at - begin;
-        int head = uniform(int(ratio(in, per_head)));
+        head = uniform(int(ratio(in, per_head)));
         while (head > 0 && in < head * per_head) --head;
         while (head + 1 < p.heads && in >= (head + 1) * per_head) ++head;
         in -= head * per_head;
-        int tile = 0;
-        if (s.tiles > 1) {
-            if (s.more) {  // first i + more i (i - 1) / 2 <= in
-                const float h = float(s.first) - 0.5f * float(s.more), m = float(s.more);
+        head_at = uniform(begin + head * per_head);
+        tile = 0;
+        if (span.tiles > 1) {
+            if (span.more) {  // first i + more i (i - 1) / 2 <= in
+                const float h = float(span.first) - 0.5f * float(span.more), m = float(span.more);
                 tile = int((__builtin_amdgcn_sqrtf(__builtin_fmaf(h, h, 2.0f * m * float(in))) - h) * __builtin_amdgcn_rcpf(m));
             } else {
-                tile = int(ratio(in, s.first));
+                tile = int(ratio(in, span.first));
             }
-            tile = uniform(min(max(tile, 0), s.tiles - 1));
-            while (tile > 0 && s.upto(tile) > in) --tile;
-            while (tile + 1 < s.tiles && s.upto(tile + 1) <= in) ++tile;
+            tile = uniform(min(max(tile, 0), span.tiles - 1));
+            while (tile > 0 && span.upto(tile) > in) --tile;
+            while (tile + 1 < span.tiles && span.upto(tile + 1) <= in) ++tile;
         }
-        const int64_t head_at = begin + head * per_head;
-        return {uniform(base + a), uniform(tile * ROWS), uniform(s.rows), uniform(s.first_token), uniform(head), uniform(s.past), uniform(s.total),
-                uniform(head_at + s.upto(tile)), uniform(head_at + s.upto(tile + 1))};
     }
     // Where this share's part of the item begins and ends in the line. A piece too short to be worth a part is left to the share on the other
     // side of its boundary, which finds the same.
