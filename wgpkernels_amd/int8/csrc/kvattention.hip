@@ -341,7 +341,7 @@ WQ8_DEVICE float max3(float a, float b, float c) {  // without the quieting move
 template <int DT, int D, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_tiles(AttentionArgs p) {
     constexpr int ROWS = 32 * WAVES, KF = D / 16, KI = D / 64, VI = D == 256 ? 2 : 1, RAW = 8 * VI > 4 * KI ? 8 * VI : 4 * KI, SWZ = 256 / D;
-    constexpr int SUBS = D == 256 ? 1 : 2, STEP_KEYS = 64 * SUBS, K_SUB = 2 * KF * 64, V_SUB = 4 * (D / 32) * 64;
+    constexpr int SUBS = D == 128 ? 2 : 1, STEP_KEYS = 64 * SUBS, K_SUB = 2 * KF * 64, V_SUB = 4 * (D / 32) * 64;
     __shared__ u32x4 k_lds[2][SUBS * K_SUB];
     __shared__ u32x4 v_lds[2][SUBS * V_SUB];
     __shared__ v4f page_k[2][SUBS], page_log_v[2][SUBS], page_inv_v[2][SUBS];
@@ -877,21 +877,22 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
 }
 
 // ---- parts joined --------------------------------------------------------------------------------------------------
-// Adds the parts of a split tile: D / 4 lanes a row, GROUPS of them that each take every GROUPS-th part, U parts' loads on their way at a time;
-// the groups' sums are added in an order of their own, the same every time.
-template <int DT, int ROWS, int D, int ROWS_WG, int GROUPS>
+// Adds the parts of a split tile: D / 4 lanes a row, GROUPS of them that each take every GROUPS-th part, with the loads of several parts on
+// their way at a time; the groups' sums are added in an order of their own, the same every time. A workgroup has as many rows as that
+// takes of 256 lanes (at 32 parts of 80 rows 63 us became 58 for the whole call with this many workgroups and 16 parts at a time; most
+// tiles come apart into two or three, for which four at a time are faster, 77 us against 82 for six prompts of up to 1000 tokens).
+template <int DT, int ROWS, int D, int GROUPS>
 __global__ void __launch_bounds__(256) kv_attention_join(AttentionArgs p) {
-    constexpr int LANES = D / 4, AT_ONCE = 256 / (LANES * GROUPS), U = ROWS == FEW_ROWS ? 16 : 4;
+    constexpr int LANES = D / 4, AT_ONCE = 256 / (LANES * GROUPS);
     const v4i tile = scalar_load(p.split_tiles + blockIdx.x);
     const int head = scalar_load(p.split_heads + blockIdx.x), parts = tile[0];
-    if (parts < 2) return;
     const int c = 4 * (threadIdx.x % LANES), group = threadIdx.x / LANES % GROUPS;
-#pragma unroll 2
-    for (int i = threadIdx.x / (LANES * GROUPS); i < ROWS_WG; i += AT_ONCE) {
-        const int r = blockIdx.y * ROWS_WG + i, row = tile[1] + r;
-        if (r >= ROWS || row >= tile[2]) continue;
-        float top = LOWEST, mass = 0.0f;
-        v4f acc = {};
+    const int r = blockIdx.y * AT_ONCE + threadIdx.x / (LANES * GROUPS), row = tile[1] + r;
+    if (parts < 2 || r >= ROWS || row >= tile[2]) return;  // whole waves
+    float top = LOWEST, mass = 0.0f;
+    v4f acc = {};
+    const auto add = [&](auto at_a_time) {
+        constexpr int U = decltype(at_a_time)::value;
         for (int base = group; base < parts; base += GROUPS * U) {
             v4f x[U];
             float t[U], m[U];
@@ -921,23 +922,25 @@ __global__ void __launch_bounds__(256) kv_attention_join(AttentionArgs p) {
                 for (int j = 0; j < 4; ++j) acc[j] = __builtin_fmaf(x[u][j], w, acc[j]);
             }
         }
+    };
+    if (parts <= 4) add(std::integral_constant<int, 4 / GROUPS ? 4 / GROUPS : 1>());
+    else add(std::integral_constant<int, 16>());
 #pragma unroll
-        for (int d = LANES; d < LANES * GROUPS; d <<= 1) {
-            const float other = __shfl_xor(top, d), next = fmaxf(top, other);
-            const float keep = __builtin_amdgcn_exp2f(top - next), take = __builtin_amdgcn_exp2f(other - next);
-            mass = __builtin_fmaf(mass, keep, __shfl_xor(mass, d) * take);
+    for (int d = LANES; d < LANES * GROUPS; d <<= 1) {
+        const float other = __shfl_xor(top, d), next = fmaxf(top, other);
+        const float keep = __builtin_amdgcn_exp2f(top - next), take = __builtin_amdgcn_exp2f(other - next);
+        mass = __builtin_fmaf(mass, keep, __shfl_xor(mass, d) * take);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[j] = __builtin_fmaf(acc[j], keep, __shfl_xor(acc[j], d) * take);
-            top = next;
-        }
-        if (group) continue;
-        const int token = by_group(p, row), member = row - token * p.group;
-        uint16_t* out = static_cast<uint16_t*>(p.out) + (tile[3] + token) * p.out_token + (head * p.group + member) * p.out_head + c;
-        uint16_t o[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = Elem<DT>::from_f(finish(acc[j], mass));
-        *reinterpret_cast<u32x2*>(out) = u32x2{o[0] | uint32_t(o[1]) << 16, o[2] | uint32_t(o[3]) << 16};
+        for (int j = 0; j < 4; ++j) acc[j] = __builtin_fmaf(acc[j], keep, __shfl_xor(acc[j], d) * take);
+        top = next;
     }
+    if (group) return;
+    const int token = by_group(p, row), member = row - token * p.group;
+    uint16_t* out = static_cast<uint16_t*>(p.out) + (tile[3] + token) * p.out_token + (head * p.group + member) * p.out_head + c;
+    uint16_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = Elem<DT>::from_f(finish(acc[j], mass));
+    *reinterpret_cast<u32x2*>(out) = u32x2{o[0] | uint32_t(o[1]) << 16, o[2] | uint32_t(o[3]) << 16};
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------------
@@ -988,10 +991,10 @@ template <int DT, int D> static int launch_attention(AttentionArgs p, const Laun
         if (i) {
             constexpr int WAVES = D == 256 ? 4 : 8;
             kv_attention_tiles<DT, D, WAVES><<<p.shares, 64 * WAVES, 0, stream>>>(p);
-            kv_attention_join<DT, 32 * WAVES, D, 32, 1><<<dim3(p.shares, WAVES), 256, 0, stream>>>(p);
+            kv_attention_join<DT, 32 * WAVES, D, 1><<<dim3(p.shares, 32 * WAVES * D / 1024), 256, 0, stream>>>(p);
         } else {
             kv_attention_few<DT, D><<<p.shares, 256, 0, stream>>>(p);
-            kv_attention_join<DT, FEW_ROWS, D, 4, 256 / D><<<dim3(p.shares, (l.few_rows + 3) / 4), 256, 0, stream>>>(p);
+            kv_attention_join<DT, FEW_ROWS, D, 256 / D><<<dim3(p.shares, (l.few_rows + 3) / 4), 256, 0, stream>>>(p);
         }
     }
     return int(hipGetLastError());
