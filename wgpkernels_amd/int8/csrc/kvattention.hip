@@ -12,7 +12,8 @@
 //   2^-32 of it.
 // - t_j = log2(e) scale ks q . k_j + log2(vs), ks and vs the scales of j's page; w_j = 2^(t_j - m) is the row's weight times its value
 //   scale, rounded once to FP16 for the second product; the sum of weights takes w_j / vs, in FP32 (a page of small values has weights
-//   that FP16 does not hold), 16 keys of one page at a time. So weights are relative to the largest product of weight and scale, and one page of large values does not cost the others.
+//   that FP16 does not hold), 16 keys of one page at a time. So weights are relative to the largest product of weight and scale, and one
+//   page of large values does not cost the others.
 // - m follows the running maximum, and is left alone until a t_j would leave FP16's range, so that sums are rarely scaled again.
 // - A value scale is taken as at least 2^-40 of the largest seen before it (and 2^-100): sums of weights stay in range over pages of zeros.
 //
@@ -56,7 +57,8 @@ struct Span {
     WQ8_DEVICE int64_t upto(int64_t i) const { return first * i + more * (i * (i - 1) / 2); }
 };
 
-constexpr int TILE_KEYS_OVERHEAD = 256;  // what a tile costs besides its keys, in keys
+// What a tile costs besides its keys, in keys (six prompts of up to 1000 tokens: 84 us at 128, 79 at 256, 80 at 512).
+constexpr int TILE_KEYS_OVERHEAD = 256;
 
 template <typename T> WQ8_DEVICE T scalar_load(const T* p) { return *(const __attribute__((address_space(4))) T*)(uint64_t)p; }
 
@@ -328,9 +330,17 @@ template <int ROWS> WQ8_DEVICE void note_split(const AttentionArgs& p, const Sha
 // 8 (i / 4) + 4 (lane / 32) + i % 4. With the second product's keys in that order a lane's weights are its operand as they are. The
 // workgroup converts each step's codes once, into LDS in the operands' order (1 KB a fragment, 16 bytes a lane, swizzled so that the
 // writes spread over the banks), in two buffers: while one is used, the next step's codes are on their way in registers. Wave w
-// converts the 16 keys (of one page: its place is scalar work) 16 (w % 4) of the step: with 8 waves the first four the values, the
-// others the keys; with 4 waves each does both. The second four waves convert before their products, the first four after them, so that of
-// a SIMD's two waves one mostly feeds the matrix cores while the other converts.
+// converts the 16 keys (of one page) 16 (w % 4) of every 64: with 8 waves the first four the values, the others the keys; with 4 waves
+// each does both. The second four waves convert before their products, the first four after them, so that of a SIMD's two waves one mostly feeds
+// the matrix cores while the other converts.
+//
+// What bounds it: the power limit, with the matrix cores busy 49% of 1.99 GHz (32760 rows over as many keys, 12 heads of 128: 6.2-6.5 ms,
+// 1010-1060 TFLOP/s, where a library product of 8192^3 reaches 1220-1270; a form before it was busy 45% of 2.12 GHz). A SIMD's vector work overlaps
+// its matrix work by half (4 products and 32 FMAs on two waves: 66 and 72 ns alone, 104 together; exponentials fully), and 64 keys of 32 rows
+// take 32 products, about 240 vector instructions and 32 exponentials. Tried and not faster: the first product of the next keys beside this
+// softmax (in whole steps, and in halves of 32 keys), the two waves of a SIMD a barrier apart, wave priorities, accumulators in AGPRs, two waves
+// for the rows of a tile that has at most half of them. Steps of 64 keys are equal but where the keys come from far (a frame of 1560 rows over 32760
+// keys: 4% slower). Heads of 64 have half the products for the same vector work: 64 keys of 32 rows take as long.
 
 WQ8_DEVICE float max3(float a, float b, float c) {  // without the quieting moves of fmaxf
     float r;
@@ -638,6 +648,9 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
 // order for keys and queries alike). Values: a lane loads D / 16 channels of the 8 keys that the weights' layout gives it,
 // 16 b + 4 (lane / 16) + i, and transposes them in registers. Pages and scales come 64 granules of 16 keys at a time, one a
 // lane. The waves' sums are joined in LDS.
+// What bounds it: HBM (64 requests of up to 8192 keys, 545 MB of codes: 110 us, 4.95 TB/s, a 1 GiB copy's rate); for one request the time
+// besides its keys (32760 keys, 8 heads: 20 us, of which the codes take 9 to 12; finding the share, the first loads and the join of the
+// waves are about 8).
 constexpr int FEW_ROWS = 16, FEW_KEYS = 32;
 
 template <int DT, int D>
