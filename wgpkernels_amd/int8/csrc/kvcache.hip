@@ -131,7 +131,7 @@ struct CacheArgs {
     const int64_t* slots;
     int* owner;
     int64_t tokens, all_slots;
-    int heads, block_log2, head_dim, group;  // group: tokens a workgroup looks through (kv_write_owned)
+    int heads, block_log2, head_dim, group, parts;  // group: tokens a workgroup looks through, parts: workgroups that share their pages (kv_write_owned)
 };
 
 // owner[slot] = the token written there. Nothing clears it: an entry holds if it names a token of this call whose slot it is,
@@ -150,22 +150,34 @@ WQ8_DEVICE float cached_value(float v) {
     return v != v ? 0.0f : fminf(fmaxf(v, -MOST), MOST);
 }
 
-// round(v / scale), inv = 1 / scale: v * inv with one correction by the remainder, so that the quotient is within an ulp and
-// codes differ from those of an exact division only where v lies within that of a tie. Scales below 2^-120, whose inverse may
-// overflow, divide.
-WQ8_DEVICE int code_of(float v, float scale, float inv) {
+// round(v / scale) in the low byte, inv = 1 / scale: v * inv with one correction by the remainder, so that the quotient is within an ulp
+// and codes differ from those of an exact division only where v lies within that of a tie. |v / scale| <= 127 (1 + 2^-24), which rounds to
+// 127. TINY: scales below 2^-120, whose inverse may overflow, divide.
+template <bool TINY> WQ8_DEVICE int code_of(float v, float scale, float inv) {
     float q = v * inv;
-    q = scale < 0x1p-120f ? v / scale : __builtin_fmaf(__builtin_fmaf(-q, scale, v), inv, q);
-    return rne_int(__builtin_amdgcn_fmed3f(q, -127.0f, 127.0f));
+    if constexpr (TINY) q = v / scale;
+    else q = __builtin_fmaf(__builtin_fmaf(-q, scale, v), inv, q);
+    return rne_low_byte(q);
 }
 
-WQ8_DEVICE float block_max(float v, float* lds4) {
-    v = wave_max(v);
+// The low bytes of four words, by three byte permutations.
+WQ8_DEVICE uint32_t pack_low_bytes(int a, int b, int c, int d) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(uint32_t(d), uint32_t(c), 0x0c0c0400u), __builtin_amdgcn_perm(uint32_t(b), uint32_t(a), 0x0c0c0400u), 0x05040100u);
+}
+
+// The largest of the workgroup's bit patterns of magnitudes (they order as unsigned numbers, NaN above infinity).
+WQ8_DEVICE uint32_t block_max_bits(uint32_t v, uint32_t* lds4) {
+    v = __builtin_bit_cast(uint32_t, row16_max(__builtin_bit_cast(float, v)));
+    const auto two = [](LanePair p) { return max(__builtin_bit_cast(uint32_t, p.a), __builtin_bit_cast(uint32_t, p.b)); };
+    v = two(swap16(__builtin_bit_cast(float, v)));
+    v = two(swap32(__builtin_bit_cast(float, v)));
     __syncthreads();
     if ((threadIdx.x & 63) == 0) lds4[threadIdx.x >> 6] = v;
     __syncthreads();
-    return fmaxf(fmaxf(lds4[0], lds4[1]), fmaxf(lds4[2], lds4[3]));
+    return max(max(lds4[0], lds4[1]), max(lds4[2], lds4[3]));
 }
+
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 // 8 consecutive channels as they are in memory.
 template <int DT> struct Raw8 {
@@ -178,9 +190,28 @@ template <int DT> struct Raw8 {
         v[0] = u32x4{0, 0, 0, 0};
         if constexpr (DT == DT_F32) v[1] = v[0];
     }
-    WQ8_DEVICE float value(int j) const {
-        if constexpr (DT == DT_F32) return cached_value(__builtin_bit_cast(float, uint32_t(v[j >> 2][j & 3])));
-        else return cached_value(Elem<DT>::to_f(uint16_t(v[0][j >> 1] >> (16 * (j & 1)))));
+    template <bool FINITE> WQ8_DEVICE float value(int j) const {
+        float f;
+        if constexpr (DT == DT_F32) f = __builtin_bit_cast(float, uint32_t(v[j >> 2][j & 3]));
+        else f = Elem<DT>::to_f(uint16_t(v[0][j >> 1] >> (16 * (j & 1))));
+        return FINITE ? f : cached_value(f);
+    }
+    // the largest magnitude's bits so far: two 16-bit patterns in a word, or one of 32
+    WQ8_DEVICE uint32_t larger(uint32_t top) const {
+        if constexpr (DT == DT_F32) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = max(top, uint32_t(v[j >> 2][j & 3]) & 0x7fffffffu);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top), __builtin_bit_cast(u16x2, uint32_t(v[0][j]) & 0x7fff7fffu)));
+        }
+        return top;
+    }
+    static constexpr uint32_t INFINITY_BITS = DT == DT_F32 ? 0x7f800000u : DT == DT_BF16 ? 0x7f80u : 0x7c00u;
+    static WQ8_DEVICE float number(uint32_t bits) {
+        if constexpr (DT == DT_F32) return __builtin_bit_cast(float, bits);
+        else return Elem<DT>::to_f(uint16_t(bits));
     }
 };
 
@@ -188,7 +219,7 @@ template <int DT> struct Raw8 {
 // of the held one (none when the page's first slot is written: the page begins anew) and the new tokens' amax / 127; tokens
 // that the page held are coded again where it grew. NI: vectors of 8 channels a thread, kept in registers between the maximum and the
 // codes (0: any number, read twice).
-template <int DT, int NI> WQ8_DEVICE void write_page(const CacheArgs& p, int which, int64_t page, int head, const int* rows, float* lds4) {
+template <int DT, int NI> WQ8_DEVICE void write_page(const CacheArgs& p, int which, int64_t page, int head, const int* rows, uint32_t* lds4) {
     using raw = typename Elem<DT>::raw;
     const int block = 1 << p.block_log2, per_row = p.head_dim >> 3, items = block * per_row;
     const int row_step = 256 / per_row, chunk_step = 256 - row_step * per_row;
@@ -197,7 +228,6 @@ template <int DT, int NI> WQ8_DEVICE void write_page(const CacheArgs& p, int whi
     float* held = p.scales[which] + page * p.heads + head;
     const float was = *held;
     Raw8<DT> kept[NI ? NI : 1];
-    float amax = 0.0f;
     // the thread's vectors: (row, chunk) from (row0, chunk0) on, 256 vectors apart
     const auto each = [&](auto body) {
         int row = row0, chunk = chunk0;
@@ -214,38 +244,56 @@ template <int DT, int NI> WQ8_DEVICE void write_page(const CacheArgs& p, int whi
             for (int i = threadIdx.x; i < items; i += 256) step(0);
         }
     };
-    const auto largest = [&](const Raw8<DT>& v) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, __builtin_fabsf(v.value(j)));
-    };
+    uint32_t top = 0;
     each([&](int n, int row, int chunk) {
         const int t = rows[row];
         if (t >= 0) kept[n].load(x + t * p.token_stride[which] + 8 * chunk);
         else kept[n].zero();
-        if constexpr (!NI) largest(kept[0]);
+        if constexpr (!NI) top = kept[0].larger(top);
     });
-    if constexpr (NI > 0) each([&](int n, int, int) { largest(kept[n]); });
-    amax = block_max(amax, lds4);
+    if constexpr (NI > 0) each([&](int n, int, int) { top = kept[n].larger(top); });
+    if constexpr (DT != DT_F32) top = max(top & 0xffffu, top >> 16);
+    top = uint32_t(__builtin_amdgcn_readfirstlane(int(block_max_bits(top, lds4))));
+    const bool finite = top < Raw8<DT>::INFINITY_BITS;
+    const float amax = finite ? Raw8<DT>::number(top) : 0.0f;
     const float old = rows[0] >= 0 ? 0.0f : fmaxf(was, 0.0f);
-    const float scale = fmaxf(old, div127(amax));
-    const float by = scale > 0.0f ? scale : 1.0f, inv = 1.0f / by, again = old / by;
     int8_t* codes = p.codes[which] + ((page * p.heads + head) << p.block_log2) * p.head_dim;
-    each([&](int n, int row, int chunk) {
-        const int t = rows[row];
-        u32x2* at = reinterpret_cast<u32x2*>(codes + row * p.head_dim + 8 * chunk);
-        int q[8];
-        if (t >= 0) {
+    const auto write = [&](auto plain, float amax) {
+        constexpr bool PLAIN = decltype(plain)::value;  // finite values, and a scale whose inverse is finite
+        const float scale = fmaxf(old, div127(amax));
+        const float by = scale > 0.0f ? scale : 1.0f, inv = 1.0f / by, again = old / by;
+        each([&](int n, int row, int chunk) {
+            const int t = rows[row];
+            u32x2* at = reinterpret_cast<u32x2*>(codes + row * p.head_dim + 8 * chunk);
+            int q[8];
+            if (t >= 0) {
+                if constexpr (!NI) kept[0].load(x + t * p.token_stride[which] + 8 * chunk);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) q[j] = code_of<!PLAIN>(kept[n].template value<PLAIN>(j), by, inv);
+            } else {
+                if (!(old < scale) || old == 0.0f) return;
+                const u32x2 before = *at;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) q[j] = rne_int(float(int8_t(before[j >> 2] >> (8 * (j & 3)))) * again);
+            }
+            *at = u32x2{pack_low_bytes(q[0], q[1], q[2], q[3]), pack_low_bytes(q[4], q[5], q[6], q[7])};
+        });
+        return scale;
+    };
+    float scale;
+    if (finite && fmaxf(old, div127(amax)) >= 0x1p-120f) {
+        scale = write(std::true_type(), amax);
+    } else {
+        float most = 0.0f;
+        each([&](int n, int row, int chunk) {
+            const int t = rows[row];
+            if (t < 0) return;
             if constexpr (!NI) kept[0].load(x + t * p.token_stride[which] + 8 * chunk);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) q[j] = code_of(kept[n].value(j), by, inv);
-        } else {
-            if (!(old < scale) || old == 0.0f) return;
-            const u32x2 before = *at;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) q[j] = rne_int(float(int8_t(before[j >> 2] >> (8 * (j & 3)))) * again);
-        }
-        *at = u32x2{pack_s8x4(q[0], q[1], q[2], q[3]), pack_s8x4(q[4], q[5], q[6], q[7])};
-    });
+            for (int j = 0; j < 8; ++j) most = fmaxf(most, __builtin_fabsf(kept[n].template value<false>(j)));
+        });
+        scale = write(std::false_type(), __builtin_bit_cast(float, block_max_bits(__builtin_bit_cast(uint32_t, most), lds4)));
+    }
     __syncthreads();  // every thread has read the held scale
     if (!threadIdx.x) *held = scale;
 }
@@ -257,7 +305,7 @@ constexpr int KV_SCAN_TOKENS = 512;
 template <int DT, int NI>
 __global__ void __launch_bounds__(256) kv_write_scan(CacheArgs p) {
     __shared__ int rows[KV_MAX_BLOCK];
-    __shared__ float lds4[4];
+    __shared__ uint32_t lds4[4];
     const int token = blockIdx.x, head = blockIdx.y, which = blockIdx.z, block = 1 << p.block_log2;
     const int64_t slot = p.slots[token];
     if (slot < 0 || slot >= p.all_slots) return;
@@ -283,14 +331,15 @@ template <int DT, int NI>
 __global__ void __launch_bounds__(256) kv_write_owned(CacheArgs p) {
     __shared__ int rows[KV_MAX_BLOCK];
     __shared__ int64_t pages[64];
-    __shared__ float lds4[4];
+    __shared__ uint32_t lds4[4];
     const int block = 1 << p.block_log2;
+    const unsigned looked = blockIdx.x / unsigned(p.parts), first_part = blockIdx.x - looked * unsigned(p.parts);
     const auto writer = [&](int64_t slot) {
         const int t = p.owner[slot];
         return t >= 0 && t < p.tokens && p.slots[t] == slot ? t : -1;
     };
     if (threadIdx.x < 64) {
-        const int64_t token = blockIdx.x * int64_t(p.group) + threadIdx.x;
+        const int64_t token = looked * int64_t(p.group) + threadIdx.x;
         int64_t page = -1;
         if (int(threadIdx.x) < p.group && token < p.tokens) {
             const int64_t slot = p.slots[token];
@@ -309,8 +358,7 @@ __global__ void __launch_bounds__(256) kv_write_owned(CacheArgs p) {
         if (page < 0) continue;
         if (int(threadIdx.x) < block) rows[threadIdx.x] = writer((page << p.block_log2) + threadIdx.x);
         __syncthreads();
-        // keys and values of every gridDim.y-th head
-        for (int part = blockIdx.y; part < 2 * p.heads; part += gridDim.y) write_page<DT, NI>(p, part & 1, page, part >> 1, rows, lds4);
+        for (int part = first_part; part < 2 * p.heads; part += p.parts) write_page<DT, NI>(p, part & 1, page, part >> 1, rows, lds4);
         __syncthreads();
     }
 }
@@ -324,9 +372,10 @@ template <int DT, int NI> static int launch_pages(CacheArgs p, hipStream_t strea
         p.group = 64;
         while (p.group > 4 && p.tokens * p.heads * 2 < p.group * int64_t(4096)) p.group >>= 1;
         const int64_t groups = (p.tokens + p.group - 1) / p.group;
-        const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(2 * p.heads, 4096 / groups));
+        p.parts = int(std::max<int64_t>(1, std::min<int64_t>(2 * p.heads, 3072 / groups)));
+        if (groups * p.parts > MAX_BLOCKS_256) return -2;
         kv_owner<<<unsigned((p.tokens + 255) / 256), 256, 0, stream>>>(p);
-        kv_write_owned<DT, NI><<<dim3(unsigned(groups), unsigned(parts)), 256, 0, stream>>>(p);
+        kv_write_owned<DT, NI><<<unsigned(groups * p.parts), 256, 0, stream>>>(p);
     }
     return int(hipGetLastError());
 }
@@ -396,7 +445,7 @@ WQ8_API int wq8_kv_write(const void* k, const void* v, const long long* strides,
     if (bad_cache(tokens, pages, heads, block, head_dim)) return -2;
     if (!tokens || !pages) return 0;
     const CacheArgs p = {{k, v}, {}, {strides[0], strides[2]}, {strides[1], strides[3]}, {k_codes, v_codes}, {k_scales, v_scales},
-                         reinterpret_cast<const int64_t*>(slots), owner, tokens, pages * block, heads, __builtin_ctz(block), head_dim, 0};
+                         reinterpret_cast<const int64_t*>(slots), owner, tokens, pages * block, heads, __builtin_ctz(block), head_dim, 0, 0};
     return dtype == DT_F16 ? launch_write<DT_F16>(p, stream) : dtype == DT_BF16 ? launch_write<DT_BF16>(p, stream) : launch_write<DT_F32>(p, stream);
 }
 
@@ -407,7 +456,7 @@ WQ8_API int wq8_kv_read(const int8_t* k_codes, const float* k_scales, const int8
     if (!tokens) return 0;
     const CacheArgs p = {{}, {k, v}, {}, {}, {const_cast<int8_t*>(k_codes), const_cast<int8_t*>(v_codes)},
                          {const_cast<float*>(k_scales), const_cast<float*>(v_scales)}, reinterpret_cast<const int64_t*>(slots), nullptr, tokens, pages * block,
-                         heads, __builtin_ctz(block), head_dim, 0};
+                         heads, __builtin_ctz(block), head_dim, 0, 0};
     const int64_t vectors = tokens * heads * (head_dim >> 3);
     const int each = vectors >= 1 << 20 ? 4 : 1;
     const int64_t blocks = (vectors + 256 * each - 1) / (256 * each);
