@@ -372,7 +372,7 @@ template <int DT, int NI> static int launch_pages(CacheArgs p, hipStream_t strea
         p.group = 64;
         while (p.group > 4 && p.tokens * p.heads * 2 < p.group * int64_t(4096)) p.group >>= 1;
         const int64_t groups = (p.tokens + p.group - 1) / p.group;
-        p.parts = int(std::max<int64_t>(1, std::min<int64_t>(2 * p.heads, 3072 / groups)));
+        p.parts = int(std::max<int64_t>(1, std::min<int64_t>(2 * p.heads, 4096 / groups)));
         if (groups * p.parts > MAX_BLOCKS_256) return -2;
         kv_owner<<<unsigned((p.tokens + 255) / 256), 256, 0, stream>>>(p);
         kv_write_owned<DT, NI><<<unsigned(groups * p.parts), 256, 0, stream>>>(p);
