@@ -190,6 +190,16 @@ def test_extreme_queries(wq, new):
     assert torch.equal(got, clean)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("new", [1, 50])
+def test_negative_scale(wq, dtype, new):
+    lens = [400]
+    cache, tables = make(wq, lens, 1, 64, 32, 13)
+    q = rows(new, 3, 64, dtype, 14)
+    got = wq.kv_attention(q, cache, tables, ints(lens), starts_of([new]), scale=-2.0)
+    check(got, q, cache, tables, lens, [new], scale=-2.0)
+
+
 def test_far_pages(wq):
     """Codes beyond 2^31 bytes from the cache's start."""
     pages = (2 ** 31 + 2 ** 29) // (2 * 128 * 128)

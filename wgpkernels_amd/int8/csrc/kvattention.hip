@@ -258,16 +258,21 @@ WQ8_DEVICE void code_pairs(uint32_t a, uint32_t b, uint32_t* out) {
 
 // ---- queries -------------------------------------------------------------------------------------------------------
 // N vectors of 8 channels of a row: as they are in memory, and in FP16; the latter returns what a product with them is multiplied by. A
-// lane holds part of a row: `most` gives the largest of its magnitudes over the row's lanes.
+// lane holds part of a row: `most` gives the largest of its magnitudes over the row's lanes. A negative scale's sign goes to the queries, as
+// the largest of scores is looked for before their product with the scale.
 template <int N> WQ8_DEVICE void fetch_query(const uint16_t* row, int stride, bool live, u32x4* raw) {
 #pragma unroll
     for (int i = 0; i < N; ++i) raw[i] = live ? *reinterpret_cast<const u32x4*>(row + i * stride) : u32x4{0, 0, 0, 0};
 }
-template <int DT, int N, typename Most> WQ8_DEVICE float use_query(const u32x4* raw, f16x8* out, Most most) {
+template <int DT, int N, typename Most> WQ8_DEVICE float use_query(u32x4* raw, f16x8* out, float scale, Most most) {
+    const uint32_t flip = scale < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int i = 0; i < N; ++i) raw[i] ^= u32x4{flip, flip, flip, flip};
+    const float by = __builtin_fabsf(scale) * 0x1.715476p+0f;  // log2(e)
     if constexpr (DT == DT_F16) {
 #pragma unroll
         for (int i = 0; i < N; ++i) out[i] = __builtin_bit_cast(f16x8, raw[i]);
-        return 1.0f;
+        return by;
     } else {
         uint32_t top = 0;  // magnitudes order as their bits do
 #pragma unroll
@@ -285,7 +290,7 @@ template <int DT, int N, typename Most> WQ8_DEVICE float use_query(const u32x4* 
                 out[i][2 * j] = static_cast<_Float16>(__builtin_bit_cast(float, raw[i][j] << 16) * up);
                 out[i][2 * j + 1] = static_cast<_Float16>(__builtin_bit_cast(float, raw[i][j] & 0xffff0000u) * up);
             }
-        return down;
+        return down * by;
     }
 }
 
@@ -380,10 +385,10 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
         fetch_query<KF>(static_cast<const uint16_t*>(p.q) + (it.first_token + token) * p.q_token + (it.head * p.group + member) * p.q_head + 8 * half, 16,
                         live_row, query_raw);
         f16x8 query[KF];
-        const float query_scale = use_query<DT, KF>(query_raw, query, [](uint32_t t) {
+        const float query_scale = use_query<DT, KF>(query_raw, query, p.scale, [](uint32_t t) {
             const LanePair o = swap32(__builtin_bit_cast(float, t));
             return max(__builtin_bit_cast(uint32_t, o.a), __builtin_bit_cast(uint32_t, o.b));
-        }) * p.scale * 0x1.715476p+0f;
+        });
 
         // keys: of the tile, of the part, and from the part's first on those of the wave and of the row
         Keys tile = keys_of(p, it, by_group(p, it.row0), by_group(p, min(it.row0 + ROWS, it.rows) - 1));
@@ -826,12 +831,12 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
         load_granules(0);
         load_codes(even, 0);
         if (steps > 1) load_codes(odd, 1);
-        query_scale = use_query<DT, KF>(query_raw, query, [](uint32_t t) {
+        query_scale = use_query<DT, KF>(query_raw, query, p.scale, [](uint32_t t) {
             LanePair o = swap16(__builtin_bit_cast(float, t));
             t = max(__builtin_bit_cast(uint32_t, o.a), __builtin_bit_cast(uint32_t, o.b));
             o = swap32(__builtin_bit_cast(float, t));
             return max(__builtin_bit_cast(uint32_t, o.a), __builtin_bit_cast(uint32_t, o.b));
-        }) * p.scale * 0x1.715476p+0f;
+        });
         use_granules();
         take_scales(even, 0);
         take_scales(odd, 1);
