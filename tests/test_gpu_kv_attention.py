@@ -200,6 +200,60 @@ def test_negative_scale(wq, dtype, new):
     check(got, q, cache, tables, lens, [new], scale=-2.0)
 
 
+@pytest.mark.parametrize("block", [16, 64])
+@pytest.mark.parametrize("requests,new,window", [(70, 5, 0), (70, 5, 20), (1, 300, 0), (1, 300, 40)])
+def test_large_values_that_a_row_does_not_see(wq, block, requests, new, window):
+    """A page whose values are 2^100 times the others': rows before it, and those whose window has passed it, do not see it, and a page of zeros
+    counts in all of them as any other. The requests share their pages."""
+    length, heads = 640 + new // 2, 8 if requests > 1 else 1
+    cache, tables = make(wq, [length], heads, 64, block, 15)
+    tables = tables.repeat(requests, 1)
+    zero = tables[0, 448 // block].long()
+    cache.v_scales[zero] = 0
+    cache.v_codes[zero] = 0
+    lens, news = [length] * requests, [new] * requests
+    q = rows(new * requests, 3 * heads, 64, torch.bfloat16, 16)
+    for large in (640 // block, (length - new) // block, (length - 1) // block):
+        kept = cache.v_scales.clone()
+        cache.v_scales[tables[0, large].long()] *= 2.0 ** 100
+        got = wq.kv_attention(q, cache, tables, ints(lens), starts_of(news), window=window)
+        check(got, q, cache, tables, lens, news, window=window)
+        cache.v_scales.copy_(kept)
+
+
+@pytest.mark.parametrize("block", [16, 64])
+@pytest.mark.parametrize("new", [1, 50])
+@pytest.mark.parametrize("large", [0, 1, 6, 9])
+def test_values_further_apart_than_a_float_reaches(wq, block, new, large):
+    """The small values' weights are in the sum, though 2^-128 of the largest product of weight and scale."""
+    lens = [640]
+    cache, tables = make(wq, lens, 2, 128, block, 17)
+    cache.v_scales *= 2.0 ** -8
+    cache.v_scales[tables[0, large].long()] *= 2.0 ** 120
+    cache.v_scales[tables[0, large].long()] *= 2.0 ** 8
+    q = rows(new, 4, 128, torch.bfloat16, 18)
+    got = wq.kv_attention(q, cache, tables, ints(lens), starts_of([new]))
+    check(got, q, cache, tables, lens, [new])
+
+
+def test_many_zero_values_before_others(wq):
+    """24000 keys whose values are zero and whose weights are 2^7.5 of the first 128 keys', then a page of values: their share of the weights."""
+    length, heads, requests = 24000, 8, 75
+    cache = wq.KVCache(length // 16, heads, 64, 16)
+    tables = torch.arange(length // 16, dtype=torch.int32, device="cuda").repeat(requests, 1)
+    cache.k_codes[8:] = 1
+    cache.k_scales.fill_(1.0)
+    cache.k_scales[-1] = 2.0
+    cache.v_codes[-1] = 100
+    cache.v_scales[-1] = 0.01
+    q = torch.ones(requests, heads, 64, dtype=torch.bfloat16, device="cuda")
+    got = wq.kv_attention(q, cache, tables, ints([length] * requests), torch.arange(requests + 1, dtype=torch.int32, device="cuda"), scale=7.5 * math.log(2) / 64)
+    most = 16 * 2.0 ** 15
+    want = most / (most + (length - 144) * 2.0 ** 7.5 + 128)
+    # half a step of the output and as much of the weights; the scale in FP32 times scores of 2^4: 2^-20
+    assert (got.double() - want).abs().max() <= want * (2.0 ** -9 + 2.0 ** -11 + 2.0 ** -20)
+
+
 def test_far_pages(wq):
     """Codes beyond 2^31 bytes from the cache's start."""
     pages = (2 ** 31 + 2 ** 29) // (2 * 128 * 128)

@@ -13,9 +13,10 @@
 // - t_j = log2(e) scale ks q . k_j + log2(vs), ks and vs the scales of j's page; w_j = 2^(t_j - m) is the row's weight times its value
 //   scale, rounded once to FP16 for the second product; the sum of weights takes w_j / vs, in FP32 (a page of small values has weights
 //   that FP16 does not hold), 16 keys of one page at a time. So weights are relative to the largest product of weight and scale, and one
-//   page of large values does not cost the others.
+//   page of large values does not cost the others. Where w_j may be below FP32's range and 2^(t_j - m) / vs is not, beside
+//   a page whose values are 2^40 times as large, the sum takes exponentials of its own.
 // - m follows the running maximum, and is left alone until a t_j would leave FP16's range, so that sums are rarely scaled again.
-// - A value scale is taken as at least 2^-40 of the largest seen before it (and 2^-100): sums of weights stay in range over pages of zeros.
+// - A value scale is taken as at least 2^-90: sums of weights, of up to 2^LAG 2^90 a key, stay in range over 2^22 keys of zeros.
 //
 // Work. A tile is ROWS rows (token, query head) of one request and key/value head, over the keys that they see together. The tiles of
 // a launch stand in one line (request, head, tile), each as long as its keys, and the workgroups, as many as the GPU holds at once,
@@ -294,12 +295,20 @@ template <int DT, int N, typename Most> WQ8_DEVICE float use_query(u32x4* raw, f
     }
 }
 
-// A page's scales as the weights take them. `seen`: the largest value scale so far.
+// A page's scales as the weights take them.
 struct PageScales { float k, log_v, inv_v; };
-WQ8_DEVICE PageScales page_scales(float ks, float vs, float seen, bool live) {
-    const float v = fmaxf(fmaxf(vs, seen * 0x1p-40f), 0x1p-100f);
+constexpr float LEAST_V = 0x1p-90f, FAR = 0x1p-40f;  // values this much smaller than others are far from them
+WQ8_DEVICE PageScales page_scales(float ks, float vs, bool live) {
+    const float v = fmaxf(vs, LEAST_V);
     return {live ? ks : 0.0f, live ? __builtin_amdgcn_logf(v) : -__builtin_inff(), 1.0f / v};
 }
+
+// Sums go from one maximum to a larger one by 2^down: in two steps, as a sum of weights may stay in range where 2^down does not.
+struct Keep {
+    float half;
+    WQ8_DEVICE explicit Keep(float down) : half(__builtin_amdgcn_exp2f(0.5f * down)) {}
+    template <typename T> WQ8_DEVICE T operator()(T v) const { return v * half * half; }
+};
 
 constexpr float LOWEST = -0x1p+120f;  // the running maximum before any key: below every t, and -inf - LOWEST = -inf
 // Weights are taken relative to 2^-HEAD of the largest, and to that until one passes it by 2^LAG (FP16 ends at 2^16): small weights keep
@@ -360,6 +369,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
     __shared__ u32x4 k_lds[2][SUBS * K_SUB];
     __shared__ u32x4 v_lds[2][SUBS * V_SUB];
     __shared__ v4f page_k[2][SUBS], page_log_v[2][SUBS], page_inv_v[2][SUBS];
+    __shared__ float page_far[2][SUBS];
     __shared__ int64_t scan[4], ends[256];
     const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, half = lane >> 5, granule = wave & 3;
     const bool does_v = WAVES == 4 || wave < 4, does_k = WAVES == 4 || wave >= 4;
@@ -410,7 +420,8 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
         const int* table = p.tables + it.request * p.table_stride;
         const int64_t head_bytes = (int64_t(it.head) << p.block_log2) * D;
         int page = 0;
-        float seen = 0.0f;
+        float seen = 0.0f;  // the largest value scale so far
+        bool far = false;   // these 64 keys have a page far from it
         PageScales lane_scales = {};
         const auto load_pages = [&](int first) {  // of the 64 keys first, first + 1, ... of the part
             const int key = key0 + 64 * (first + lane) + 16 * granule;
@@ -419,9 +430,26 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
             if (!live) page = 0;
             if (does_v) {
                 const int64_t at = int64_t(page) * p.heads + it.head;
-                const float ks = p.k_scales[at], vs = live ? p.v_scales[at] : 0.0f;
-                seen = fmaxf(seen, wave_max(vs));
-                lane_scales = page_scales(ks, vs, seen, live);
+                const float ks = p.k_scales[at], vs = p.v_scales[at];
+                float least = live ? vs : __builtin_inff(), most = live ? vs : 0.0f;
+                if (p.block_log2 < 6) {  // the other waves' pages of the 64 keys too
+                    int other[4];
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int at = key - 16 * granule + 16 * g;
+                        other[g] = at < key1 ? table[at >> p.block_log2] : -1;
+                    }
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const bool there = other[g] >= 0 && other[g] < p.pages;
+                        const float v = p.v_scales[int64_t(there ? other[g] : 0) * p.heads + it.head];
+                        least = fminf(least, there ? v : __builtin_inff());
+                        most = fmaxf(most, there ? v : 0.0f);
+                    }
+                }
+                seen = fmaxf(seen, wave_max(most));
+                far = fmaxf(least, LEAST_V) < seen * FAR;
+                lane_scales = page_scales(ks, vs, live);
             }
         };
         // codes on their way: with 8 waves a wave has keys or values, in the same registers
@@ -476,6 +504,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
                         reinterpret_cast<float*>(&page_k[buffer][u])[granule] = lane_scales.k;
                         reinterpret_cast<float*>(&page_log_v[buffer][u])[granule] = lane_scales.log_v;
                         reinterpret_cast<float*>(&page_inv_v[buffer][u])[granule] = lane_scales.inv_v;
+                        if (!granule) page_far[buffer][u] = far ? __builtin_inff() : LOWEST;
                     }
                 }
                 if (does_k) {
@@ -548,7 +577,8 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
                 }
                 // t = a s + b of the 16 keys of a page
                 v4f a = page_k[buffer][u] * query_scale, b = page_log_v[buffer][u];
-                const v4f inv_v = page_inv_v[buffer][u];
+                v4f inv_v = page_inv_v[buffer][u];
+                const float some_far = page_far[buffer][u];
                 if (base + 64 > all_high || base < all_low) {  // some row does not see every key of the step
                     const int high = own_high - base, low = own_low - base;
 #pragma unroll
@@ -569,13 +599,23 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
                     const float m = max3(max3(t[i], t[i + 1], t[i + 2]), max3(t[i + 3], t[i + 4], t[i + 5]), max3(t[i + 6], t[i + 7], t[i + 7]));
                     high = fmaxf(high, __builtin_fmaf(m, a[g], b[g]));
                 }
-                if (__ballot(high > top + LAG)) {
+                if (__ballot(fmaxf(high, some_far) > top + LAG)) {
                     const LanePair o = swap32(high);
-                    const float next_top = fmaxf(top, fmaxf(o.a, o.b) - HEAD), keep = __builtin_amdgcn_exp2f(top - next_top);
+                    const float next_top = fmaxf(top, fmaxf(o.a, o.b) - HEAD);
+                    const Keep keep(top - next_top);
                     top = next_top;
-                    mass *= keep;
+                    mass = keep(mass);
 #pragma unroll
-                    for (int i = 0; i < D / 32; ++i) acc[i] *= keep;
+                    for (int i = 0; i < D / 32; ++i) acc[i] = keep(acc[i]);
+                    if (some_far > 0.0f) {
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            const float up = b[g] - top + __builtin_amdgcn_logf(inv_v[g]);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) mass += __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 1][8 * (g & 1) + i], a[g], up));
+                        }
+                        inv_v = v4f{};
+                    }
                 }
                 b -= top;
                 const auto weights_of = [&](int g) {
@@ -699,6 +739,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
     int page = 0;
     bool live_page = false;
     float ks = 0.0f, vs = 0.0f, log_v = 0.0f, inv_v = 0.0f, seen = 0.0f;
+    int far = 0;
     const auto load_granules = [&](int step) {
         const int key = wave_key0 + 4 * FEW_KEYS * (step + (lane >> 1)) + 16 * (lane & 1);
         page = key < key1 ? table[key >> p.block_log2] : -1;
@@ -709,9 +750,10 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
         vs = p.v_scales[at];
     };
     const auto use_granules = [&] {
-        if (!live_page) vs = 0.0f;
-        seen = fmaxf(seen, wave_max(vs));
-        const PageScales s = page_scales(ks, vs, seen, live_page);
+        seen = fmaxf(seen, wave_max(live_page ? vs : 0.0f));
+        far = live_page && fmaxf(vs, LEAST_V) < seen * FAR;
+        far |= __shfl_xor(far, 1);  // of the step's two granules
+        const PageScales s = page_scales(ks, vs, live_page);
         ks = s.k;
         log_v = s.log_v;
         inv_v = s.inv_v;
@@ -722,8 +764,10 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
         u32x4 k[2][KV];
         uint32_t v[8][VW];
         float scale[2], log_v[2], inv_v[2];
+        int far;
     };
     const auto take_scales = [&](Raw& raw, int step) {
+        raw.far = __builtin_amdgcn_readlane(far, 2 * (step & 31));
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const int from = 2 * (step & 31) + b;
@@ -773,7 +817,9 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
 #pragma unroll
             for (int c = 0; c < 4; ++c) v[4 * j + c] = __builtin_bit_cast(f16x8, u32x4{pairs[0][c], pairs[1][c], pairs[2][c], pairs[3][c]});
         }
-        const float scale[2] = {raw.scale[0], raw.scale[1]}, page_log_v[2] = {raw.log_v[0], raw.log_v[1]}, page_inv_v[2] = {raw.inv_v[0], raw.inv_v[1]};
+        const float scale[2] = {raw.scale[0], raw.scale[1]}, page_log_v[2] = {raw.log_v[0], raw.log_v[1]};
+        float page_inv_v[2] = {raw.inv_v[0], raw.inv_v[1]};
+        const int some_far = raw.far;
         if (step + 2 < steps) {
             const bool turn = ((step + 2) & 31) == 0;
             if (turn) load_granules(step + 2);
@@ -802,14 +848,24 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
         float high = t[0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) high = fmaxf(high, t[i]);
-        if (__ballot(high > top + LAG)) {
+        if (__ballot(high > top + LAG) || some_far) {
             LanePair o = swap16(high);
             o = swap32(fmaxf(o.a, o.b));
-            const float next = fmaxf(top, fmaxf(o.a, o.b) - HEAD), keep = __builtin_amdgcn_exp2f(top - next);
+            const float next = fmaxf(top, fmaxf(o.a, o.b) - HEAD);
+            const Keep keep(top - next);
             top = next;
-            mass *= keep;
+            mass = keep(mass);
 #pragma unroll
-            for (int i = 0; i < VF; ++i) acc[i] *= keep;
+            for (int i = 0; i < VF; ++i) acc[i] = keep(acc[i]);
+            if (some_far) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const float up = __builtin_amdgcn_logf(page_inv_v[b]) - top;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mass += __builtin_amdgcn_exp2f(t[4 * b + i] + up);
+                    page_inv_v[b] = 0.0f;
+                }
+            }
         }
         float w[8];
 #pragma unroll
@@ -863,10 +919,10 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
     float total = 0.0f, o[D / 16] = {};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-        const float keep = __builtin_amdgcn_exp2f(tops[w][r] - most);
-        total = __builtin_fmaf(masses[w][r], keep, total);
+        const Keep keep(tops[w][r] - most);
+        total += keep(masses[w][r]);
 #pragma unroll
-        for (int j = 0; j < D / 16; ++j) o[j] = __builtin_fmaf(sums[w][r][c0 + j], keep, o[j]);
+        for (int j = 0; j < D / 16; ++j) o[j] = __builtin_fmaf(sums[w][r][c0 + j], keep(1.0f), o[j]);
     }
     const int out_row = it.row0 + r;
     if (began || goes_on) {
@@ -928,16 +984,16 @@ __global__ void __launch_bounds__(256) kv_attention_join(AttentionArgs p) {
                 if (base + u * GROUPS >= parts) t[u] = -__builtin_inff();
                 next = fmaxf(next, t[u]);
             }
-            const float keep = __builtin_amdgcn_exp2f(top - next);
+            const Keep keep(top - next);
             top = next;
-            mass *= keep;
-            acc *= keep;
+            mass = keep(mass);
+            acc = keep(acc);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float w = __builtin_amdgcn_exp2f(t[u] - next);
-                mass = __builtin_fmaf(m[u], w, mass);
+                const Keep part(t[u] - next);
+                mass += part(m[u]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[j] = __builtin_fmaf(x[u][j], w, acc[j]);
+                for (int j = 0; j < 4; ++j) acc[j] = __builtin_fmaf(x[u][j], part(1.0f), acc[j]);
             }
         }
     };
@@ -946,10 +1002,10 @@ __global__ void __launch_bounds__(256) kv_attention_join(AttentionArgs p) {
 #pragma unroll
     for (int d = LANES; d < LANES * GROUPS; d <<= 1) {
         const float other = __shfl_xor(top, d), next = fmaxf(top, other);
-        const float keep = __builtin_amdgcn_exp2f(top - next), take = __builtin_amdgcn_exp2f(other - next);
-        mass = __builtin_fmaf(mass, keep, __shfl_xor(mass, d) * take);
+        const Keep keep(top - next), take(other - next);
+        mass = keep(mass) + take(__shfl_xor(mass, d));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j] = __builtin_fmaf(acc[j], keep, __shfl_xor(acc[j], d) * take);
+        for (int j = 0; j < 4; ++j) acc[j] = __builtin_fmaf(acc[j], keep(1.0f), __shfl_xor(acc[j], d) * take(1.0f));
         top = next;
     }
     if (group) return;
