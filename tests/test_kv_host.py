@@ -104,6 +104,11 @@ def test_cache_refuses_shapes(shape):
         wq.KVCache(shape[0], shape[1], shape[3], shape[2], device="cpu")
 
 
+def test_cache_refuses_no_heads():
+    with pytest.raises(ValueError, match="head"):
+        cache(heads=0)
+
+
 def test_cache_refuses_parts():
     good = cache()
     k, ks, v, vs = good.k_codes, good.k_scales, good.v_codes, good.v_scales

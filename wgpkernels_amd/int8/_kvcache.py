@@ -52,6 +52,8 @@ class KVCache:
     def _take(self, k_codes, k_scales, v_codes, v_scales):
         if k_codes.dim() != 4 or k_codes.shape != v_codes.shape or k_codes.shape[2] not in BLOCKS or k_codes.shape[3] % 8 or not 8 <= k_codes.shape[3] <= 1024:
             raise ValueError(f"cache codes must be (pages, heads, {' / '.join(map(str, BLOCKS))} tokens, a multiple of 8 channels), the same for keys and values")
+        if not k_codes.shape[1]:
+            raise ValueError("a cache needs heads")
         if k_codes.dtype != torch.int8 or v_codes.dtype != torch.int8 or k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32:
             raise ValueError("cache codes must be INT8, their scales FP32")
         if k_scales.shape != k_codes.shape[:2] or v_scales.shape != k_codes.shape[:2]:
