@@ -72,6 +72,17 @@ def test_plan(wq, requests, most_past, most_new, block, room):
         assert (wide[:, width:] == -7).all()
 
 
+def test_plan_at_the_last_positions(wq):
+    """Positions end at 2^31 - 1: a request that would pass them finds no room."""
+    last = 2 ** 31 - 1
+    tables = torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    past, new = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([last - 3, last - 2], [3, 3]))
+    plan = wq.kv_plan(past, new, tables, torch.arange(4, device="cuda").int(), torch.zeros(1, dtype=torch.int32, device="cuda"), 2 ** 30, 6)
+    assert plan.lens.tolist() == [last, last - 2] and plan.missing.tolist() == [1]
+    assert plan.positions[:3].tolist() == [last - 3, last - 2, last - 1] and plan.slots[:3].tolist() == [2 ** 30 - 4, 2 ** 30 - 3, 2 ** 30 - 2]
+    assert plan.slots[3:].tolist() == [-1] * 3
+
+
 def test_plan_of_nothing(wq):
     none = torch.empty(0, dtype=torch.int32, device="cuda")
     plan = wq.kv_plan(none, none, none.reshape(0, 4), none, ints([2]), 16, 3)

@@ -90,7 +90,7 @@ def kv_plan(past, new, tables, free, used, block, tokens):
 
     past, new: (R,) int32 (negative counts as 0). tables: (R, width) int32, completed in place with the pages that the new tokens
     begin: free[used], free[used + 1], ... in the order of requests and tokens. free: (F,) int32; used: (1,) int32. A request that
-    the table's width, `tokens` or the free pages left cannot hold gets no page, slots -1 and its old length, and so does
+    the table's width, `tokens`, 31-bit positions or the free pages left cannot hold gets no page, slots -1 and its old length, and so does
     every later one that needs a page where the free list ran out. Everything is int32 / int64 on the GPU; nothing is read
     on the host."""
     key = (past.shape, past.dtype, past.stride(), new.shape, new.dtype, new.stride(), free.shape, free.dtype, free.stride(), tables.shape, tables.stride(),
@@ -122,8 +122,8 @@ def _check_plan(past, new, tables, free, used, block, tokens):
     requests = past.shape[0]
     if new.shape[0] != requests or tables.shape[0] != requests:
         raise ValueError(f"past, new and tables must be of as many requests, not {requests}, {new.shape[0]} and {tables.shape[0]}")
-    if block < 1 or not 0 <= tokens < 2 ** 31:
-        raise ValueError("a block of at least one token and a token count are wanted")
+    if not 1 <= block <= 2 ** 30 or not 0 <= tokens < 2 ** 31:
+        raise ValueError("a block of 1 to 2^30 tokens and a token count are wanted")
     _check_devices(past, new, tables, free, used)
     return [tokens, requests + 1, requests, 1, 1]
 
@@ -141,7 +141,8 @@ def _check_write(cache, k, v, slots):
 def kv_write(cache, k, v, slots):
     """Keys and values (tokens, heads, head_dim), BF16, FP16 or FP32, into the cache at `slots` (int64; any order, each at most once;
     those outside the cache, as -1, are left out). A page's scale grows to its largest value, and tokens that it holds are then
-    coded again; a write to its first slot begins it anew. NaN is held as 0 and infinities as the largest finite number."""
+    coded again; a write to its first slot begins it anew. NaN is held as 0 and infinities as the largest finite number (beside
+    which the other tokens of the page come to 0)."""
     key = (k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(), v.dtype, v.get_device(), slots.shape, slots.stride(), slots.dtype,
            slots.get_device())
     strides, tokens, dtype, shape = cache.layouts.get(key) or cache.layouts.keep(key, _check_write(cache, k, v, slots))

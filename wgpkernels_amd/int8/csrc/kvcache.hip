@@ -38,7 +38,7 @@ WQ8_DEVICE int64_t scan256(int64_t v, int64_t* lds4, int64_t& total) {
 }
 
 // Pages in order of the free list: requests in order, each taking ceil((past + new) / block) - ceil(past / block). A request
-// that the tokens, its table's width or the free pages cannot hold takes none; nor then does any later one that needs pages.
+// that the tokens, its table's width, 31-bit positions or the free pages cannot hold takes none; nor then does any later one that needs pages.
 // Every workgroup walks the requests, 256 at a time, and serves PLAN_TOKENS tokens: the walk is a few hundred
 // nanoseconds, less than a launch of its own. A page's first token writes its table entry.
 constexpr int PLAN_TOKENS = 1024;
@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(256) kv_plan_tokens(PlanArgs p) {
         const int64_t have = (past + p.block - 1) / p.block, want = (past + fresh + p.block - 1) / p.block;
         int64_t total;
         const int64_t end = upto_ends + scan256(fresh, lds4, total);
-        const bool fits = live && want <= p.width && end <= p.tokens;
+        const bool fits = live && want <= p.width && end <= p.tokens && past + fresh <= 0x7fffffff;
         const int64_t need = fits ? want - have : 0;
         int64_t total_need;
         const int64_t upto = upto_need + scan256(need, lds4, total_need);
