@@ -348,12 +348,13 @@ template <int ROWS> WQ8_DEVICE void note_split(const AttentionArgs& p, const Sha
 // each does both. The second four waves convert before their products, the first four after them, so that of a SIMD's two waves one mostly feeds
 // the matrix cores while the other converts.
 //
-// What bounds it: the power limit, with the matrix cores busy 49% of 1.99 GHz (32760 rows over as many keys, 12 heads of 128: 6.2-6.5 ms,
-// 1010-1060 TFLOP/s, where a library product of 8192^3 reaches 1220-1270; a form before it was busy 45% of 2.12 GHz). A SIMD's vector work overlaps
+// What bounds it: the power limit, with the matrix cores busy 49% of 1.99 GHz (32760 rows over as many keys, 12 heads of 128: 6.4-6.5 ms,
+// 1010-1030 TFLOP/s, where a library product of 8192^3 reaches 1220-1270; a form before it was busy 45% of 2.12 GHz). A SIMD's vector work overlaps
 // its matrix work by half (4 products and 32 FMAs on two waves: 66 and 72 ns alone, 104 together; exponentials fully), and 64 keys of 32 rows
 // take 32 products, about 240 vector instructions and 32 exponentials. Tried and not faster: the first product of the next keys beside this
 // softmax (in whole steps, and in halves of 32 keys), the two waves of a SIMD a barrier apart, wave priorities, accumulators in AGPRs, two waves
-// for the rows of a tile that has at most half of them. Steps of 64 keys are equal but where the keys come from far (a frame of 1560 rows over 32760
+// for the rows of a tile that has at most half of them; slower: 64 rows a wave with one wave a SIMD (24%), codes converted between the first
+// product's instructions (5-9%). Steps of 64 keys are equal but where the keys come from far (a frame of 1560 rows over 32760
 // keys: 4% slower). Heads of 64 have half the products for the same vector work: 64 keys of 32 rows take as long.
 
 WQ8_DEVICE float max3(float a, float b, float c) {  // without the quieting moves of fmaxf
