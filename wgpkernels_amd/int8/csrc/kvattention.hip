@@ -60,6 +60,9 @@ struct Span {
 
 // What a tile costs besides its keys, in keys (six prompts of up to 1000 tokens: 84 us at 128, 79 at 256, 80 at 512).
 constexpr int TILE_KEYS_OVERHEAD = 256;
+// The line's units a key: shares are whole units, so that the ends of many drift from the tiles' by up to one each (one token over 8192 keys, 8
+// heads: 17.5 us at 1, 14.9 at 16).
+constexpr int UNITS = 16;
 
 template <typename T> WQ8_DEVICE T scalar_load(const T* p) { return *(const __attribute__((address_space(4))) T*)(uint64_t)p; }
 
@@ -77,11 +80,11 @@ template <int ROWS, bool UNIFORM> WQ8_DEVICE Span span_of(const AttentionArgs& p
     s.first_token = begin;
     s.past = len - (end - begin);  // a length below zero counts as zero keys: positions stay in range
     s.total = p.pages ? max(0, min(len, p.width << p.block_log2)) : 0;
-    // lengths in keys * group: a causal tile's rows see ROWS / group keys more than those of the tile before
+    // lengths in keys * group * UNITS: a causal tile's rows see ROWS / group keys more than those of the tile before
     const bool grows = p.causal && !p.window;
     const int seen = p.window ? min(s.total, p.window) : p.causal ? min(s.total, max(0, s.past)) : s.total;
-    s.first = int64_t(seen + TILE_KEYS_OVERHEAD) * p.group + ROWS;
-    s.more = grows ? ROWS : 0;
+    s.first = (int64_t(seen + TILE_KEYS_OVERHEAD) * p.group + ROWS) * UNITS;
+    s.more = grows ? ROWS * UNITS : 0;
     return s;
 }
 
@@ -154,7 +157,7 @@ template <int ROWS> struct Share {
             line = uniform(line);
         }
         // no less than line / shares
-        share = uniform(max(int64_t(float(line) * 0x1.00002p0f * __builtin_amdgcn_rcpf(float(p.shares))) + 1, int64_t(least) * p.group));
+        share = uniform(max(int64_t(float(line) * 0x1.00002p0f * __builtin_amdgcn_rcpf(float(p.shares))) + 1, int64_t(least) * p.group * UNITS));
         index = int(blockIdx.x & 7) * (p.shares >> 3) + int(blockIdx.x >> 3);
         at = index * share;
         end = min(line, at + share);
@@ -215,7 +218,7 @@ template <int ROWS> struct Share {
     // the tile and the share, is left to the share on the other side of its boundary, which finds the same (six prompts of up to 1000
     // tokens: 84 us with 1 / 128 of the tile and the share, 81 with this).
     WQ8_DEVICE int64_t snapped(const Item& it, int64_t x) const {
-        const int64_t least = min(min(it.line_end - it.line_begin, share) >> 4, int64_t(TILE_KEYS_OVERHEAD) * p.group);
+        const int64_t least = min(min(it.line_end - it.line_begin, share) >> 4, int64_t(TILE_KEYS_OVERHEAD) * p.group * UNITS);
         return x - it.line_begin < least ? it.line_begin : it.line_end - x < least ? it.line_end : x;
     }
     // Of `steps` steps of the item's keys, the ones before place x of the line: the same for the shares on both sides of x.
