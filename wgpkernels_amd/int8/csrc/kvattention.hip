@@ -103,6 +103,9 @@ WQ8_DEVICE int by_group(const AttentionArgs& p, int row) {  // row / group
 // a / b to about 2^-22 of itself; a starting point for counting, the same in every workgroup
 WQ8_DEVICE float ratio(int64_t a, int64_t b) { return float(a) * __builtin_amdgcn_rcpf(float(b)); }
 
+// a / b, no less but by rounding up
+WQ8_DEVICE int64_t no_less(int64_t a, int b) { return int64_t(float(a) * 0x1.00002p0f * __builtin_amdgcn_rcpf(float(b))) + 1; }
+
 WQ8_DEVICE int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 WQ8_DEVICE int64_t uniform(int64_t v) { return int64_t(uint64_t(uint32_t(uniform(int(v >> 32)))) << 32 | uint32_t(uniform(int(v)))); }
 
@@ -165,7 +168,14 @@ template <int ROWS> struct Share {
             line = uniform(line);
         }
         // no less than line / shares
-        share = uniform(max(int64_t(float(line) * 0x1.00002p0f * __builtin_amdgcn_rcpf(float(p.shares))) + 1, int64_t(least) * p.group * UNITS));
+        const int64_t shortest = int64_t(least) * p.group * UNITS;
+        share = uniform(max(no_less(line, p.shares), shortest));
+        // One request: as many parts as that gives a tile (but for rounding), of equal length, so that no workgroup has parts of two (1 token over
+        // 1000 keys: 16.4 us without, 13.3 with).
+        if (p.requests == 1 && span.tiles == 1) {
+            const int parts = min(int(ratio(span.first, share) + 0x1p-4f), int(unsigned(p.shares) / unsigned(p.heads)));
+            if (parts > 0) share = uniform(no_less(span.first, parts));
+        }
         index = int(blockIdx.x & 7) * (p.shares >> 3) + int(blockIdx.x >> 3);
         at = index * share;
         end = min(line, at + share);
