@@ -31,6 +31,8 @@ namespace wq8 {
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
+constexpr int FEW_ROWS = 16;  // rows of a tile of kv_attention_few
+
 struct AttentionArgs {
     const void* q;
     void* out;
@@ -181,30 +183,28 @@ template <int ROWS> struct Share {
             const int parts = min(int(ratio(span.first, share) + 0x1p-4f), int(unsigned(p.shares) / unsigned(p.heads)));
             if (parts > 0) share = uniform(no_less(span.first, parts));
         }
-        // Few tiles: none shares a workgroup with another's part, as beginning a tile takes about as long as a share. Of four lengths of
-        // a share, between those that suffice without and with a part more for each tile, the shortest that does. (16 requests of up to 2048
-        // keys, 8 heads: 23.5 us without, 20.9 with; 8 of up to 5000: 24.9 and 22.8; 3 of up to 30000, 4 heads: 30.3 and 27.5.)
-        if (ROWS == 16 && p.requests > 1 && p.requests <= 256 && p.requests * p.heads <= p.shares >> 1 && p.shares < 1 << 14) {
+        // Few tiles of few rows, one a head: none shares a workgroup with another's part, as beginning a tile takes about as long as a share. Of three lengths
+        // of a share, between those that suffice without and with a part more for each tile, the shortest that does. (16 requests of up to 2048
+        // keys, 8 heads: 23.5 us without, 20.9 with; 8 of up to 5000: 24.9 and 22.8; 3 of up to 30000, 4 heads: 30.3 and 27.5; 32 of up to 3000, 8
+        // heads: 31.5 and 29. Tiles of many rows: 5-8% faster for 20 to 60 rows a request, 5-9% slower for 80 to 128, and so not done.)
+        if (ROWS == FEW_ROWS && p.requests > 1 && p.requests <= 256 && p.requests * p.heads <= p.shares >> 1 && p.shares < 1 << 14) {
             const int tiles = p.requests * p.heads;
-            int64_t lengths[4], counts = 0, total;
+            int64_t lengths[3], counts = int64_t(mine_tiles > 1) << 48, total;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                lengths[i] = uniform(max(no_less(line, p.shares - tiles * i / 3), shortest));
-                const int parts = mine_tiles ? parts_of(mine, lengths[i]) + (mine_tiles > 1) : 0;
-                counts += int64_t(parts * p.heads) << (16 * i);  // at most twice the shares in all
+            for (int i = 0; i < 3; ++i) {
+                lengths[i] = uniform(max(no_less(line, p.shares - tiles * i / 2), shortest));
+                if (mine_tiles == 1) counts += int64_t(parts_of(mine, lengths[i]) * p.heads) << (16 * i);  // at most twice the shares in all
             }
             scan256(counts, lds4, total);
             total = uniform(total);
-            int which = 3;
-#pragma unroll
-            for (int i = 2; i >= 0; --i) which = int(total >> (16 * i) & 0xffff) <= p.shares ? i : which;
-            share = which == 0 ? lengths[0] : which == 1 ? lengths[1] : which == 2 ? lengths[2] : lengths[3];
-            rounded = true;
-            const int64_t length = mine_tiles == 1 ? parts_of(mine, share) * share : mine;
-            const int64_t e = scan256(length * p.heads, lds4, line);
-            line = uniform(line);
-            if (threadIdx.x < 256) ends[threadIdx.x] = e;
-            __syncthreads();
+            if (!(total >> 48)) {
+                rounded = true;
+                share = int(total & 0xffff) <= p.shares ? lengths[0] : int(total >> 16 & 0xffff) <= p.shares ? lengths[1] : lengths[2];
+                const int64_t e = scan256(mine_tiles ? parts_of(mine, share) * share * p.heads : 0, lds4, line);
+                line = uniform(line);
+                if (threadIdx.x < 256) ends[threadIdx.x] = e;
+                __syncthreads();
+            }
         }
         index = int(blockIdx.x & 7) * (p.shares >> 3) + int(blockIdx.x >> 3);
         at = index * share;
@@ -241,7 +241,7 @@ template <int ROWS> struct Share {
             }
             begin = a ? uniform(ends[a - 1]) : base_at;
             span = span_of<ROWS, true>(p, uniform(base + a));
-            if (rounded && span.tiles == 1) span.first = uniform(parts_of(span.first, share)) * share;
+            if (rounded) span.first = uniform(parts_of(span.first, share)) * share;
         }
         request = uniform(base + a);
         const int64_t per_head = span.upto(span.tiles);
@@ -752,7 +752,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
 // What bounds it: HBM (64 requests of up to 8192 keys, 545 MB of codes: 110 us, 4.95 TB/s, a 1 GiB copy's rate); for one request the time
 // besides its keys (32760 keys, 8 heads: 20 us, of which the codes take 9 to 12; finding the share, the first loads and the join of the
 // waves are about 8).
-constexpr int FEW_ROWS = 16, FEW_KEYS = 32;
+constexpr int FEW_KEYS = 32;
 
 template <int DT, int D>
 __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(AttentionArgs p) {
