@@ -402,8 +402,8 @@ template <int ROWS> WQ8_DEVICE void note_split(const AttentionArgs& p, const Sha
 // each does both. The second four waves convert before their products, the first four after them, so that of a SIMD's two waves one mostly feeds
 // the matrix cores while the other converts.
 //
-// What bounds it: the power limit, with the matrix cores busy 49% of 1.99 GHz (32760 rows over as many keys, 12 heads of 128: 6.4-6.5 ms,
-// 1010-1030 TFLOP/s, where a library product of 8192^3 reaches 1220-1270; a form before it was busy 45% of 2.12 GHz). A SIMD's vector work overlaps
+// What bounds it: the power limit, with the matrix cores busy 49% of 1.99 GHz (32760 rows over as many keys, 12 heads of 128: 6.4-6.7 ms,
+// 980-1030 TFLOP/s, where a library product of 8192^3 reaches 1220-1270; a form before it was busy 45% of 2.12 GHz). A SIMD's vector work overlaps
 // its matrix work by half (4 products and 32 FMAs on two waves: 66 and 72 ns alone, 104 together; exponentials fully), and 64 keys of 32 rows
 // take 32 products, about 240 vector instructions and 32 exponentials. Tried and not faster: the first product of the next keys beside this
 // softmax (in whole steps, and in halves of 32 keys), the two waves of a SIMD a barrier apart, wave priorities, accumulators in AGPRs, two waves
@@ -750,7 +750,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
 // 16 b + 4 (lane / 16) + i, and transposes them in registers. Pages and scales come 64 granules of 16 keys at a time, one a
 // lane. The waves' sums are joined in LDS.
 // What bounds it: HBM (64 requests of up to 8192 keys, 545 MB of codes: 110 us, 4.95 TB/s, a 1 GiB copy's rate); for one request the time
-// besides its keys (32760 keys, 8 heads: 20 us, of which the codes take 9 to 12; finding the share, the first loads and the join of the
+// besides its keys (32760 keys, 8 heads: 17.4 us, of which the codes take 9 to 10; finding the share, the first loads and the join of the
 // waves are about 8).
 constexpr int FEW_KEYS = 32;
 
@@ -1098,11 +1098,11 @@ static Launches plan_launches(int64_t tokens, int64_t requests, int64_t heads, i
     if (!l.used[0]) l.limit = 0;
     l.few_rows = int(std::min<int64_t>(rows, FEW_ROWS));
     l.waves = head_dim == 256 ? 4 : 8;
-    // Two workgroups a CU on the tiles of few rows hide more of the time that a tile takes besides its keys; one where a tile would come apart into
-    // more than 32 parts (1 token over 32760 keys, 8 heads: 28.5 us on 32 parts a tile, 34.7 on 64, their joining 5.6 and 10.2; 64 requests
-    // of up to 8192: 122.6 on 256 workgroups, 119.5 on 512).
+    // Two workgroups a CU on the tiles of few rows hide more of the time that a tile takes besides its keys, where there are as many tiles as CUs (64
+    // requests of up to 8192 keys, 8 heads: 119.5 us against 122.6); with fewer they are twice the parts to begin and to join (1 token over
+    // 32760 keys, 8 heads: 28 us against 22; 16 requests of up to 2048: 21.1 and 19.1; but 8 of up to 30000: 58.4 and 60.2).
     const int64_t few_tiles = (rows / FEW_ROWS + std::min(tokens, requests)) * heads;
-    const int per_cu[2] = {2 * sms <= 32 * few_tiles ? 2 : 1, 1}, tile_rows[2] = {FEW_ROWS, 32 * l.waves};
+    const int per_cu[2] = {few_tiles >= sms ? 2 : 1, 1}, tile_rows[2] = {FEW_ROWS, 32 * l.waves};
     for (int i = 0; i < 2; ++i) {
         l.shares[i] = (per_cu[i] * sms + 7) & ~7;
         if (l.used[i]) l.bytes[i] = align256(int64_t(l.shares[i]) * 20) + align256(int64_t(l.shares[i]) * 2 * tile_rows[i] * (head_dim + 2) * 4);
