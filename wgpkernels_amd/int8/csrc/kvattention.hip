@@ -185,8 +185,8 @@ template <int ROWS> struct Share {
         }
         // Few tiles of few rows, one a head: none shares a workgroup with another's part, as beginning a tile takes about as long as a share. Of three lengths
         // of a share, between those that suffice without and with a part more for each tile, the shortest that does. (16 requests of up to 2048
-        // keys, 8 heads: 23.5 us without, 20.9 with; 8 of up to 5000: 24.9 and 22.8; 3 of up to 30000, 4 heads: 30.3 and 27.5; 32 of up to 3000, 8
-        // heads: 31.5 and 29. Tiles of many rows: 5-8% faster for 20 to 60 rows a request, 5-9% slower for 80 to 128, and so not done.)
+        // keys, 8 heads: 22 us without, 19 with; 8 of up to 5000: 24.2 and 21.6; 3 of up to 30000, 4 heads: 27.6 and 24.6; 32 of up to 3000, 8
+        // heads: 32.4 and 29.1; four equal ones: 19.2 both. Tiles of many rows: 5-8% faster for 20 to 60 rows a request, 5-9% slower for 80 to 128, and so not done.)
         if (ROWS == FEW_ROWS && p.requests > 1 && p.requests <= 256 && p.requests * p.heads <= p.shares >> 1 && p.shares < 1 << 14) {
             const int tiles = p.requests * p.heads;
             int64_t lengths[3], counts = int64_t(mine_tiles > 1) << 48, total;
