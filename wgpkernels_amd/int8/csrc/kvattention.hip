@@ -52,14 +52,6 @@ struct AttentionArgs {
     float* slots;
 };
 
-// The arguments' cache lines, asked for together: the compiler loads them where they are used, and each line's first load is waited for.
-WQ8_DEVICE void touch_arguments() {
-    const auto at = (const __attribute__((address_space(4))) uint32_t*)__builtin_amdgcn_kernarg_segment_ptr();
-    constexpr int LINES = (sizeof(AttentionArgs) + 63) / 64;
-    static_assert(LINES <= 4);
-    asm volatile("" ::"s"(at[0]), "s"(at[16]), "s"(at[32]), "s"(at[LINES > 3 ? 48 : 32]));
-}
-
 // ---- shares --------------------------------------------------------------------------------------------------------
 // A request's part of the line: tiles of length first + more * i, i = 0 to tiles - 1, for each head.
 struct Span {
@@ -428,7 +420,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) kv_attention_til
     __shared__ int64_t scan[4], ends[256];
     const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, half = lane >> 5, granule = wave & 3;
     const bool does_v = WAVES == 4 || wave < 4, does_k = WAVES == 4 || wave >= 4;
-    touch_arguments();
+    touch_arguments<AttentionArgs>();
     Share<ROWS> share(p, scan, ends, 256);
     if (!tid) p.split_tiles[share.index][0] = 0;
     // lane constants: places of the codes in memory and LDS, of the operands
@@ -761,7 +753,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
     __shared__ float tops[4][FEW_ROWS], masses[4][FEW_ROWS];
     __shared__ int64_t scan[4], ends[256];
     const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, quarter = lane >> 4;
-    touch_arguments();
+    touch_arguments<AttentionArgs>();
     Share<FEW_ROWS> share(p, scan, ends, 8 * FEW_KEYS);
     if (!tid) p.split_tiles[share.index][0] = 0;
     for (; share.at < share.end; __syncthreads()) {
@@ -1015,7 +1007,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_few(Attent
 template <int DT, int ROWS, int D, int GROUPS>
 __global__ void __launch_bounds__(256) kv_attention_join(AttentionArgs p) {
     constexpr int LANES = D / 4, AT_ONCE = 256 / (LANES * GROUPS);
-    touch_arguments();
+    touch_arguments<AttentionArgs>();
     const v4i tile = scalar_load(p.split_tiles + blockIdx.x);
     const int head = scalar_load(p.split_heads + blockIdx.x), parts = tile[0];
     const int c = 4 * (threadIdx.x % LANES), group = threadIdx.x / LANES % GROUPS;

@@ -300,4 +300,14 @@ WQ8_DEVICE uint32_t pack_s8x4(int a, int b, int c, int d) {
     return (uint32_t(a) & 0xffu) | ((uint32_t(b) & 0xffu) << 8) | ((uint32_t(c) & 0xffu) << 16) | (uint32_t(d) << 24);
 }
 
+// The cache lines of a kernel's only argument, asked for together: the compiler loads its members where they are used, and each line's first
+// load is waited for there.
+template <typename Args> WQ8_DEVICE void touch_arguments() {
+    const auto at = (const __attribute__((address_space(4))) uint32_t*)__builtin_amdgcn_kernarg_segment_ptr();
+    constexpr int LAST = (sizeof(Args) - 4) / 64;
+    static_assert(LAST < 6);
+    asm volatile("" ::"s"(at[0]), "s"(at[16 * (LAST < 1 ? LAST : 1)]), "s"(at[16 * (LAST < 2 ? LAST : 2)]), "s"(at[16 * (LAST < 3 ? LAST : 3)]),
+                 "s"(at[16 * (LAST < 4 ? LAST : 4)]), "s"(at[16 * LAST]));
+}
+
 }  // namespace wq8
