@@ -286,6 +286,16 @@ def test_many_requests(wq, requests, most, new):
     check(got, q, cache, tables, lens, news)
 
 
+@pytest.mark.parametrize("lens,new", [([2500, 17, 900, 1, 0, 1700, 333, 64], [1] * 4 + [0] + [1] * 3), ([700] * 9, [1] * 9), ([40, 3000, 9], [1, 12, 1]),
+                                      ([5000, 4999], [3, 2]), ([250] * 20 + [4000], [1] * 21)], ids=["ragged", "equal", "several tiles", "two", "one long"])
+def test_few_tiles_over_many_workgroups(wq, lens, new):
+    """Tiles that come apart into whole shares, and those that do not: no keys twice, none left out."""
+    cache, tables = make(wq, lens, 2, 64, 32, len(lens))
+    q = rows(sum(new), 2 * 3, 64, torch.float16, 23)
+    got = wq.kv_attention(q, cache, tables, ints(lens), starts_of(new))
+    check(got, q, cache, tables, lens, new)
+
+
 def test_same_bits_again_and_on_a_side_stream(wq):
     """Nothing depends on the order in which workgroups end."""
     lens, new = [3000, 40, 1700], [1, 30, 1]
