@@ -121,3 +121,31 @@ def test_graph_and_side_stream(wq):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("style", ["pairs", "halves"])
+def test_far_positions_in_64_bits(wq, dtype, style):
+    """Positions up to 2^44: the angle, from integers, is off by |p| 2^-65 turns, 2^-18.3 at most, of |a| + |b|."""
+    from fractions import Fraction
+    frequencies = [1.0, 0.7071, 0.3, 10000.0 ** -0.3, 1e-5, 123.456]
+    plan = wq.rotary_plan((2, 4), style=style, frequencies=frequencies)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    positions = torch.randint(-(2 ** 44), 2 ** 44, (37, 2), generator=g, device="cuda")
+    x = torch.randn(37, 3, 16, generator=g, device="cuda").to(dtype)
+    # 2 pi to 80 digits
+    two_pi = Fraction("6.2831853071795864769252867665590057683943387987502116419498891846156328125724180")
+    turn = lambda p, f: (p * Fraction(f) / two_pi) % 1
+    axis = [0] * 2 + [1] * 4
+    angle = torch.tensor([[2 * math.pi * float(turn(row[a], f)) for a, f in zip(axis, frequencies)] for row in positions.tolist()], dtype=torch.float64)
+    for inverse in (False, True):
+        got = wq.rotary(x, positions, plan, inverse=inverse).cpu().double()
+        want, size = x.cpu().double(), torch.zeros(37, 3, 16, dtype=torch.float64)
+        a, b = (slice(0, 12, 2), slice(1, 12, 2)) if style == "pairs" else (slice(0, 6), slice(6, 12))
+        u, v, cos, sin = want[..., a].clone(), want[..., b].clone(), angle.cos()[:, None], (-angle.sin() if inverse else angle.sin())[:, None]
+        want[..., a], want[..., b] = u * cos - v * sin, u * sin + v * cos
+        size[..., a] = size[..., b] = u.abs() + v.abs()
+        far = 2 * math.pi * 2.0 ** -65 * positions.abs().max().item()
+        info = torch.finfo(dtype)
+        bound = info.eps / 2 * want.abs().clamp(min=info.smallest_normal) + (2.0 ** -22 + far) * size
+        assert ((got - want).abs() <= bound).all()

@@ -181,3 +181,27 @@ def test_c_entries_refuse():
     assert attend(dtype=2) == -1
     assert attend(head_dim=80) == attend(block=24) == attend(heads=0) == attend(group=0) == attend(window=-1) == attend(tokens=-1) == -2
     assert attend(tokens=0) == attend(requests=0) == 0
+
+
+@pytest.mark.parametrize("options", [{"base": 500000.0}, {"base": 500000.0, "ladder": "joint"}, {"base": 1e-300},
+                                     {"frequencies": [1.0, -0.3, 2 * math.pi * 3, 1e300, 5e-324, 0.0, 1e-9, 123456.789, 2.0 ** 1000]}])
+def test_plan_turns_at_far_positions(options):
+    """A pair's turns are the nearest fraction of 2^64 to its FP64 frequency over 2 pi, so that the angle of position p is off by
+    |p| 2^-65 turns and no more; against 2 pi from another series, in as many digits as 2^1024 and 2^62 leave."""
+    from decimal import Decimal, localcontext
+    from fractions import Fraction
+    plan = wq.rotary_plan((4, 5), device="cpu", **options)
+    steps = [i / 9 for i in range(9)] if options.get("ladder") == "joint" else [i / 4 for i in range(4)] + [i / 5 for i in range(5)]
+    frequencies = options.get("frequencies") or [options["base"] ** -s for s in steps]
+    with localcontext() as c:
+        c.prec = 420
+        held, t, n, na, d, da, pi = 0, Decimal(3), 1, 0, 0, 24, Decimal(3)  # pi = 6 arcsin(1 / 2)
+        while held != pi:
+            held, n, na, d, da = pi, n + na, na + 8, d + da, da + 32
+            t = t * n / d
+            pi += t
+        two_pi = 2 * Fraction(pi)
+    for f, turns in zip(frequencies, plan.turns.tolist()):
+        for position in (1, -1, 4097, 2 ** 31 - 1, -(2 ** 40) + 3, 2 ** 50 + 1, -(2 ** 62) + 5):
+            off = (Fraction(position * turns, 2 ** 64) - position * Fraction(f) / two_pi) % 1
+            assert min(off, 1 - off) <= abs(position) * Fraction(1, 2 ** 65), (f, position)

@@ -30,6 +30,29 @@ class Layouts(dict):
         return value
 
 
+def _arctan_inverse(x, bits):
+    """arctan(1 / x) in parts of 2^-bits, by its series."""
+    power = total = (1 << bits) // x
+    n = 1
+    while power:
+        power, n = -power // (x * x), n + 2
+        total += power // n
+    return total
+
+
+# 2 pi in parts of 2^-1280 (Machin's formula): a frequency of up to 2^1024 leaves more than the 64 bits of a turn that are kept
+_TWO_PI_BITS = 1280
+_TWO_PI = 2 * (16 * _arctan_inverse(5, _TWO_PI_BITS) - 4 * _arctan_inverse(239, _TWO_PI_BITS))
+
+
+def _turn(frequency):
+    """frequency / 2 pi modulo one, as the nearest fraction of 2^64 in two's complement: a position times it wraps at whole turns."""
+    a, b = frequency.as_integer_ratio()
+    whole = b * _TWO_PI
+    turns = ((a << _TWO_PI_BITS + 65) + whole) // (2 * whole)
+    return (turns + 2 ** 63) % 2 ** 64 - 2 ** 63
+
+
 class RotaryPlan:
     """Which pairs turn, about which axis and how fast, on one GPU (rotary_plan()). Made once per model."""
     __slots__ = ("sections", "style", "pairs", "turns", "axis", "layouts")
@@ -43,7 +66,8 @@ def rotary_plan(sections, ladder="axis", style="pairs", base=10000.0, frequencie
     """A plan of sum(sections) rotated pairs a head, sections[a] of them on axis a, in that order.
 
     ladder 'axis': pair i of a section of n turns by base ** (-i / n) a position, each axis with a ladder of its own; 'joint':
-    pair i of all n by base ** (-i / n), one ladder cut into the sections. frequencies (one a pair) replaces both.
+    pair i of all n by base ** (-i / n), one ladder cut into the sections. frequencies (one a pair) replaces both. Frequencies are FP64
+    numbers: one of a ladder is within about 2^-53 of itself.
     style 'pairs': pair i is channels 2 i and 2 i + 1; 'halves': channels i and i + sum(sections). Channels past the
     rotated ones pass through."""
     sections = tuple(int(s) for s in sections)
@@ -63,9 +87,7 @@ def rotary_plan(sections, ladder="axis", style="pairs", base=10000.0, frequencie
             raise ValueError("the rotary base must be positive and finite")
         steps = [i / n for n in sections for i in range(n)] if ladder == "axis" else [i / pairs for i in range(pairs)]
         frequencies = [float(base) ** -s for s in steps]
-    # turns a position, modulo one, as a fraction of 2^64 in two's complement: a position times it wraps at whole turns
-    turns = [round(math.fmod(f / (2 * math.pi), 1.0) * 2.0 ** 64) for f in frequencies]
-    turns = [(t + 2 ** 63) % 2 ** 64 - 2 ** 63 for t in turns]
+    turns = [_turn(f) for f in frequencies]
     axis = [a for a, n in enumerate(sections) for _ in range(n)]
     packed = torch.tensor(turns + axis, dtype=torch.int64).to(device)  # one copy
     return RotaryPlan(sections, style, packed[:pairs], packed[pairs:].to(torch.int32))
@@ -125,9 +147,9 @@ def _check_rotary(tensors, positions, plan):
 def rotary(xs, positions, plan, inverse=False, out=None):
     """Rows (tokens, heads, head_dim) of BF16, FP16 or FP32 turned by their positions: a tensor, or a tuple of up to four of one
     type, token count and head width (queries and keys; views of a packed projection). positions: (tokens, axes) int32 or
-    int64, or (tokens,) with one axis; any value. inverse turns back. Angles are exact at far positions: they are reduced to
-    parts of a turn as 64-bit integers. out: tensors of the same shapes, which may be the inputs themselves and overlap
-    them in no other way."""
+    int64, or (tokens,) with one axis. inverse turns back. Angles are reduced to parts of a turn as 64-bit integers: that of position
+    p is within |p| 2^-65 turns of p times the pair's FP64 frequency. out: tensors of the same shapes, which may be the inputs themselves
+    and overlap them in no other way."""
     many = not isinstance(xs, torch.Tensor)
     tensors = tuple(xs) if many else (xs,)
     key = (positions.shape, positions.stride(), positions.dtype, positions.get_device(), *[(x.shape, x.stride(), x.dtype, x.get_device()) for x in tensors])

@@ -2,8 +2,8 @@
 //
 // Pair i of a head turns by the angle 2 pi p u_i, p the token's position on the pair's axis, u_i = frequency_i / 2 pi turns:
 //     (a, b) -> (a cos - b sin, a sin + b cos); the inverse (and the gradient) turns the other way.
-// u_i comes as a 64-bit fixed-point fraction, so p u_i modulo one turn is one wrapping integer product: exact to
-// |p| 2^-65 turns for any position, where a product in FP32 has lost the angle at p = 10^5 and one in FP64 costs a
+// u_i comes as a 64-bit fixed-point fraction, the nearest to frequency_i / 2 pi, so p u_i modulo one turn is one wrapping integer
+// product: within |p| 2^-65 turns, where a product in FP32 has lost the angle at p = 10^5 and one in FP64 costs a
 // reduction. The top 32 bits give the quadrant and the rest of the turn, |r| <= 1/8, for two short polynomials.
 #include "wq8_common.h"
 #include "wq8_abi.h"
@@ -23,8 +23,8 @@ struct RotaryArgs {
     int count, heads, pairs, head_dim, wide, inverse, heads_per_thread;
 };
 
-// sin and cos of 2 pi phase / 2^32. Polynomials in r^2 fitted for least maximum error on |r| <= 1/8 turn (3e-9 and 5e-11
-// with the coefficients in FP32).
+// sin and cos of 2 pi phase / 2^32. Polynomials in r^2 fitted for least maximum error on |r| <= 1/8 turn: with the coefficients in FP32
+// off by 2.4e-8 (the rounding of 2 pi, half a step of FP32 of the sine) and 6.7e-9, evaluated in FP32 by 8.6e-8 and 5.8e-8.
 WQ8_DEVICE void turn_sincos(uint32_t phase, float& s, float& c) {
     const uint32_t quadrant = (phase + 0x20000000u) >> 30;
     const float r = float(int32_t(phase - (quadrant << 30))) * 0x1p-32f, z = r * r;
