@@ -119,3 +119,18 @@ def test_window_without_causality(wq, lens, new, window):
     for workgroups in (8, 64, 256):
         got = attention_on(wq, workgroups, q, cache, tables, ints(lens), starts_of(new), False, window)
         check(got, q, cache, tables, lens, new, False, window)
+
+
+def test_overlapping_outputs_are_refused(wq):
+    """Before any launch: rows that several workgroups would write at once."""
+    lens, new = [70, 20], [3, 2]
+    cache, tables = make(wq, lens, 2, 64, 32, 61)
+    q = rows(5, 4, 64, torch.bfloat16, 62)
+    for out in (q[:1].clone().expand(5, 4, 64), q[:, :1].clone().expand(5, 4, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            wq.kv_attention(q, cache, tables, ints(lens), starts_of(new), out=out)
+        with pytest.raises(ValueError, match="overlap"):
+            wq.rotary(q, torch.arange(5, device="cuda"), wq.rotary_plan((4,)), out=out)
+    out = torch.empty(4, 5, 64, dtype=torch.bfloat16, device="cuda").transpose(0, 1)  # heads first
+    assert wq.kv_attention(q, cache, tables, ints(lens), starts_of(new), out=out) is out
+    assert torch.equal(out, wq.kv_attention(q, cache, tables, ints(lens), starts_of(new)))

@@ -205,3 +205,19 @@ def test_plan_turns_at_far_positions(options):
         for position in (1, -1, 4097, 2 ** 31 - 1, -(2 ** 40) + 3, 2 ** 50 + 1, -(2 ** 62) + 5):
             off = (Fraction(position * turns, 2 ** 64) - position * Fraction(f) / two_pi) % 1
             assert min(off, 1 - off) <= abs(position) * Fraction(1, 2 ** 65), (f, position)
+
+
+def test_written_rows_do_not_overlap():
+    """Rows that several workgroups would write at once: block tables completed in place, outputs given by the caller."""
+    from wgpkernels_amd.int8._rotary import _check_written
+    past, new, free, used = ints(3, 4), ints(1, 1), ints(1, 2, 3), ints(0)
+    one = torch.zeros(5, dtype=torch.int32)
+    for tables in (one.expand(2, 5), torch.zeros(8, dtype=torch.int32).as_strided((2, 5), (3, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            wq.kv_plan(past, new, tables, free, used, 16, 2)
+    good = torch.zeros(6, 4, 8)
+    for rows_ in (good, good[:, 1:3], good.transpose(0, 1), good[::2, ::3], good[:1].expand(1, 4, 8), good[:0], torch.zeros(6, 1, 8), torch.zeros(1, 8).expand(0, 4, 8)):
+        _check_written(rows_, "outputs")
+    for rows_ in (good[:1].expand(6, 4, 8), good[:, :1].expand(6, 4, 8), good.as_strided((6, 4, 8), (24, 8, 1)), good.as_strided((6, 4, 8), (32, 4, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            _check_written(rows_, "outputs")

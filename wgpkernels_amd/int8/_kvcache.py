@@ -16,7 +16,7 @@ from typing import NamedTuple
 import torch
 
 from . import DTYPES, _native, library
-from ._rotary import Layouts, _check_aligned, _check_devices, _check_rows
+from ._rotary import Layouts, _check_aligned, _check_devices, _check_rows, _check_written
 
 BLOCKS = (16, 32, 64, 128)
 ATTENTION_HEAD_DIMS = (64, 128, 256)
@@ -122,6 +122,8 @@ def _check_plan(past, new, tables, free, used, block, tokens):
     requests = past.shape[0]
     if new.shape[0] != requests or tables.shape[0] != requests:
         raise ValueError(f"past, new and tables must be of as many requests, not {requests}, {new.shape[0]} and {tables.shape[0]}")
+    if requests > 1 and tables.stride(0) < tables.shape[1]:
+        raise ValueError("rows of block tables must not overlap: they are completed in place")
     if not 1 <= block <= 2 ** 30 or not 0 <= tokens < 2 ** 31:
         raise ValueError("a block of 1 to 2^30 tokens and a token count are wanted")
     _check_devices(past, new, tables, free, used)
@@ -194,6 +196,7 @@ def kv_attention(q, cache, tables, lens, starts, causal=True, window=0, scale=No
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _check_rows(out, "outputs")
+        _check_written(out, "outputs")
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError("outputs do not match the queries")
         _check_devices(q, out)

@@ -106,6 +106,17 @@ def _check_rows(x, name):
         raise ValueError(f"rows of {name} must be 16-byte aligned")
 
 
+def _check_written(x, name):
+    """Rows with places of their own, as different workgroups write them."""
+    if x.stride(0) >= x.shape[1] * x.stride(1) and x.stride(1) >= x.shape[2]:
+        return
+    span = 1
+    for stride, size in sorted((stride, size) for stride, size in zip(x.stride(), x.shape) if size > 1):
+        if stride < span and x.numel():
+            raise ValueError(f"rows of {name} must not overlap")
+        span += stride * (size - 1)
+
+
 def _check_devices(*tensors):
     """Tensors on one GPU: the kernels take raw pointers."""
     device = tensors[0].get_device()
@@ -148,8 +159,8 @@ def rotary(xs, positions, plan, inverse=False, out=None):
     """Rows (tokens, heads, head_dim) of BF16, FP16 or FP32 turned by their positions: a tensor, or a tuple of up to four of one
     type, token count and head width (queries and keys; views of a packed projection). positions: (tokens, axes) int32 or
     int64, or (tokens,) with one axis. inverse turns back. Angles are reduced to parts of a turn as 64-bit integers: that of position
-    p is within |p| 2^-65 turns of p times the pair's FP64 frequency. out: tensors of the same shapes, which may be the inputs themselves
-    and overlap them in no other way."""
+    p is within |p| 2^-65 turns of p times the pair's FP64 frequency. out: tensors of the same shapes whose rows do not overlap, which
+    may be the inputs themselves and share memory with them in no other way."""
     many = not isinstance(xs, torch.Tensor)
     tensors = tuple(xs) if many else (xs,)
     key = (positions.shape, positions.stride(), positions.dtype, positions.get_device(), *[(x.shape, x.stride(), x.dtype, x.get_device()) for x in tensors])
@@ -163,6 +174,7 @@ def rotary(xs, positions, plan, inverse=False, out=None):
             raise ValueError("rotary outputs do not match its inputs")
         for y in outs:
             _check_rows(y, "rotary outputs")
+            _check_written(y, "rotary outputs")
         _check_devices(positions, *outs)
         strides = type(strides)(*[v for x, y in zip(tensors, outs) for v in (x.shape[1], x.stride(0), x.stride(1), y.stride(0), y.stride(1))])
     places, to = [x.data_ptr() for x in tensors], [y.data_ptr() for y in outs]
