@@ -200,3 +200,28 @@ def test_no_tokens(wq):
     slots = torch.empty(0, dtype=torch.int64, device="cuda")
     wq.kv_write(cache, none, none, slots)
     assert wq.kv_read(cache, slots)[0].shape == (0, 1, 64) and not cache.k_codes.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("pages", [7, 70])
+def test_codes_are_the_rounded_quotients(wq, dtype, pages):
+    """16-bit values over their page's scale: the code is round(value / scale) in 64 bits, also of half the page's maximum, which is 63.5
+    but for the rounding of the scale. Whole pages, and pages that go on under the scale of what they hold."""
+    heads, d, block = 3, 64, 16
+    g = torch.Generator(device="cuda").manual_seed(pages)
+    x = torch.randn(pages, block, heads, d, generator=g, device="cuda").to(dtype)
+    top = x.abs().amax((1, 3))
+    x[:, 2, :, 9], x[:, 3, :, 1], x[:, 12, :, 30], x[:, 13, :, 31] = top, top / 2, top / 2, -top / 2
+    x = x.reshape(pages * block, heads, d)
+    slots = torch.arange(pages * block, device="cuda")
+    cache = wq.KVCache(pages, heads, d, block)
+    wq.kv_write(cache, x, x.neg(), slots)
+    quotient = x.double() / cache.k_scales.double().repeat_interleave(block, 0)[..., None]
+    assert (quotient.abs() - 63.5).abs().amin() < 2.0 ** -17 and torch.unique(torch.round(quotient).abs()).numel() > 100
+    codes = lambda c: c.transpose(1, 2).reshape(pages * block, heads, d).double()
+    assert torch.equal(codes(cache.k_codes), torch.round(quotient)) and torch.equal(codes(cache.v_codes), torch.round(-quotient))
+    parts = wq.KVCache(pages, heads, d, block)
+    first = slots % block < 8
+    for some in (first, ~first):
+        wq.kv_write(parts, x[some], x[some].neg(), slots[some])
+    assert torch.equal(parts.k_scales, cache.k_scales) and torch.equal(parts.k_codes, cache.k_codes) and torch.equal(parts.v_codes, cache.v_codes)
