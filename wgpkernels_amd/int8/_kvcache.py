@@ -180,12 +180,14 @@ def _check_read(cache, slots, dtype):
 def kv_attention(q, cache, tables, lens, starts, causal=True, window=0, scale=None, out=None):
     """Attention of the step's queries over the cache: q (tokens, query heads, head_dim) BF16 or FP16, head_dim 64, 128 or 256, each key/value
     head serving query heads / heads of them, in order. Request r owns rows starts[r] to starts[r + 1] (int32, not
-    decreasing) and sees the first lens[r] (int32) tokens of its row of `tables`, its own rows being the last of them.
+    decreasing) and sees the first lens[r] (int32) tokens of its row of `tables`, its own rows being the last of them. out: a tensor of
+    q's shape and type whose rows do not overlap, nor share memory with q.
 
     causal: a row sees the tokens up to itself, otherwise all of its request's; window > 0: of those, the ones after
     position - window. scale: of the scores, 1 / sqrt(head_dim) by default. Rows that see nothing are zero; pages outside the cache are
-    hidden; rows of no request are not written. Returns (tokens, query heads, head_dim) in q's dtype. Sums and the softmax's
-    statistics are FP32, its weights FP16 relative to the largest."""
+    hidden; rows of no request are not written (uninitialised in a new output). Returns (tokens, query heads, head_dim) in q's dtype. Sums and
+    the softmax's statistics are FP32, its weights FP16 relative to the largest; value scales below 2^-90 count as that (off by
+    less than 2^-83). Not recorded for autograd."""
     key = (q.shape, q.stride(), q.dtype, q.get_device(), tables.shape, tables.stride(), tables.dtype, tables.get_device(), lens.shape, lens.stride(), lens.dtype,
            lens.get_device(), starts.shape, starts.stride(), starts.dtype, starts.get_device())
     layout = cache.layouts.get(key) or cache.layouts.keep(key, _check_attention(q, cache, tables, lens, starts))

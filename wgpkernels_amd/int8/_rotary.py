@@ -160,7 +160,8 @@ def rotary(xs, positions, plan, inverse=False, out=None):
     type, token count and head width (queries and keys; views of a packed projection). positions: (tokens, axes) int32 or
     int64, or (tokens,) with one axis. inverse turns back. Angles are reduced to parts of a turn as 64-bit integers: that of position
     p is within |p| 2^-65 turns of p times the pair's FP64 frequency. out: tensors of the same shapes whose rows do not overlap, which
-    may be the inputs themselves and share memory with them in no other way."""
+    may be the inputs themselves and share memory with them in no other way. Not recorded for autograd: the caller's backward is this
+    function with inverse turned over."""
     many = not isinstance(xs, torch.Tensor)
     tensors = tuple(xs) if many else (xs,)
     key = (positions.shape, positions.stride(), positions.dtype, positions.get_device(), *[(x.shape, x.stride(), x.dtype, x.get_device()) for x in tensors])

@@ -16,12 +16,14 @@
 //   page of large values does not cost the others. Where w_j may be below FP32's range and 2^(t_j - m) / vs is not, beside
 //   a page whose values are 2^40 times as large, the sum takes exponentials of its own.
 // - m follows the running maximum, and is left alone until a t_j would leave FP16's range, so that sums are rarely scaled again.
-// - A value scale is taken as at least 2^-90: sums of weights, of up to 2^LAG 2^90 a key, stay in range over 2^22 keys of zeros.
+// - A value scale is taken as at least 2^-90: sums of weights, of up to 2^LAG 2^90 a key, stay in range over 2^22 keys of zeros. Pages of smaller
+//   scales that are not zero count as that large: off by less than 2^-83.
 //
 // Work. A tile is ROWS rows (token, query head) of one request and key/value head, over the keys that they see together. The tiles of
-// a launch stand in one line (request, head, tile), each as long as its keys, and the workgroups, as many as the GPU holds at once,
-// take equal lengths of it: whole tiles, and parts of the two at a share's ends, whose results kv_attention_join adds. So requests of any
-// lengths fill the GPU evenly; and nothing is read on the host, each workgroup finds its share from the lengths on the GPU.
+// a launch stand in one line (request, head, tile), each as long as its keys (a window without causality apart, see span_of), and the
+// workgroups, as many as the GPU holds at once, take equal lengths of it: whole tiles, and parts of the two at a share's ends, whose results
+// kv_attention_join adds. So requests of any lengths fill the GPU evenly; and nothing is read on the host, each workgroup finds its share
+// from the lengths on the GPU.
 #include "wq8_common.h"
 #include "wq8_abi.h"
 #include <algorithm>
@@ -83,6 +85,8 @@ template <int ROWS, bool UNIFORM> WQ8_DEVICE Span span_of(const AttentionArgs& p
     s.past = len - (end - begin);  // a length below zero counts as zero keys: positions stay in range
     s.total = p.pages ? max(0, min(len, p.width << p.block_log2)) : 0;
     // lengths in keys * group * UNITS: a causal tile's rows see ROWS / group keys more than those of the tile before
+    // With a window every tile counts as the window's keys. Without causality a tile sees to the request's end as well, and the shares of a request's
+    // first tiles take longest (32760 rows over themselves, 8 heads of 128, a window of 1000: 3990 us, 4120 without the window; causal: 210).
     const bool grows = p.causal && !p.window;
     const int seen = p.window ? min(s.total, p.window) : p.causal ? min(s.total, max(0, s.past)) : s.total;
     s.first = (int64_t(seen + TILE_KEYS_OVERHEAD) * p.group + ROWS) * UNITS;
@@ -394,8 +398,8 @@ template <int ROWS> WQ8_DEVICE void note_split(const AttentionArgs& p, const Sha
 // each does both. The second four waves convert before their products, the first four after them, so that of a SIMD's two waves one mostly feeds
 // the matrix cores while the other converts.
 //
-// What bounds it: the power limit, with the matrix cores busy 49% of 1.99 GHz (32760 rows over as many keys, 12 heads of 128: 6.4-6.7 ms,
-// 980-1030 TFLOP/s, where a library product of 8192^3 reaches 1220-1270; a form before it was busy 45% of 2.12 GHz). A SIMD's vector work overlaps
+// What bounds it: the power limit, with the matrix cores busy 49% of 1.99 GHz (32760 rows over as many keys, 12 heads of 128: 6.2-6.7 ms,
+// 980-1060 TFLOP/s, where a library product of 8192^3 reaches 1220-1270; a form before it was busy 45% of 2.12 GHz). A SIMD's vector work overlaps
 // its matrix work by half (4 products and 32 FMAs on two waves: 66 and 72 ns alone, 104 together; exponentials fully), and 64 keys of 32 rows
 // take 32 products, about 240 vector instructions and 32 exponentials. Tried and not faster: the first product of the next keys beside this
 // softmax (in whole steps, and in halves of 32 keys), the two waves of a SIMD a barrier apart, wave priorities, accumulators in AGPRs, two waves
@@ -1082,7 +1086,10 @@ static Launches plan_launches(int64_t tokens, int64_t requests, int64_t heads, i
     Launches l = {};
     const int64_t rows = tokens * group;
     // A request's rows are known on the GPU alone. On average up to 16 a request: all on the tiles of few rows; more than 64: all on
-    // the others (each launch is about 5 us, used or not); between, each request by its rows.
+    // the others (each launch is about 5 us, used or not); between, each request by its rows. The average is right for requests alike; beside a
+    // prompt, single tokens take a tile of 256 rows each: 63 of them over up to 8192 keys (8 heads of 128, group 8) 132 us, a prompt of 4096
+    // tokens 349, all in one call 674; with one of 1000 tokens 126, 65 and 386. 255 single tokens over up to 4096 keys (group 1) 222, a prompt
+    // of 3000 83, both on the tiles of few rows 278.
     l.limit = 32;
     l.used[1] = requests == 1 ? rows > l.limit : rows > FEW_ROWS * requests;
     l.used[0] = !l.used[1] || (requests > 1 && rows <= 64 * requests);
