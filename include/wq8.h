@@ -56,6 +56,17 @@ int wq8_transform_rows(const void* x, void* out, int m, int k, int64_t ldx, int 
 /* ConvRot rotation only (group 16, 64, 256), rounded once. Replaces K8:1871; bound at I:87. */
 int wq8_rotate_groups(const void* x, void* out, int m, int k, int64_t ldx, int dtype, int group, wq8_stream_t stream);
 
+/* The sum of two rows on its way into a linear, no counterpart in the reference: sum = residual + rscale * x (rscale: k values or null)
+ * in FP32, held in dtype 0-1; then RMS-normalised, rotated and prepared as the calls above prepare the sum: path 0 block codes (out,
+ * scale (m, ceil(k/128))), 1 row codes (out, lo optional, scale (m)), 2 rows of dtype (out). Rows ldx, ldr, lds elements apart, 16-byte
+ * aligned, as are rscale and act_weight; k % 8 == 0. sum may be x or residual in its place. */
+int wq8_add_prepare(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* rscale, void* sum, int64_t lds, int path, void* out,
+                    int8_t* lo, float* scale, int m, int k, int dtype, int group, const void* act_weight, float eps, wq8_stream_t stream);
+
+/* What codes stand for: out (m, k) of dtype 0-2 = q * scale, or (q + lo / 254) * scale with lo; scale per row, with blocks per row and
+ * 128-element block. k % 8 == 0, q and lo 8-byte aligned. No reference counterpart. */
+int wq8_prepared_values(const int8_t* q, const int8_t* lo, const float* scale, void* out, int m, int k, int blocks, int dtype, wq8_stream_t stream);
+
 /* Y (m, n) = epilogue(A (m, k) int8 [, A_lo], B (n, k) int8); variant ids keep the reference's modes: 0, 2, 6 row;
  * 1, 7 exact (a_lo required); 10, 11 block (sa (m, ceil(k/128))); 12, 13 block with weight scales sb (n, ceil(k/128));
  * 14 exact with such weight scales. Ids with no counterpart in the reference: 15 the short block tile with 10's biased

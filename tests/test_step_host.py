@@ -1,0 +1,63 @@
+"""add_prepare(), without a GPU: what it refuses, before anything is launched."""
+import pytest
+import torch
+
+from wgpkernels_amd import int8 as wq
+
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def rows(m=4, k=256, dtype=BF16):
+    return torch.zeros(m, k, dtype=dtype)
+
+
+ADDED = {
+    "dimensions": lambda: (rows()[0], rows()[0], {}),
+    "type": lambda: (rows(dtype=torch.float32), rows(dtype=torch.float32), {}),
+    "mixed types": lambda: (rows(), rows(dtype=FP16), {}),
+    "double": lambda: (rows(dtype=torch.float64), rows(dtype=torch.float64), {}),
+    "shapes": lambda: (rows(), rows(5), {}),
+    "broadcast": lambda: (rows(), rows(1), {}),
+    "width": lambda: (rows(k=252), rows(k=252), {}),
+    "no channels": lambda: (rows(k=0), rows(k=0), {}),
+    "columns": lambda: (torch.zeros(256, 4, dtype=BF16).t(), rows(), {}),
+    "pitch": lambda: (rows(k=260)[:, :256], rows(), {}),
+    "path": lambda: (rows(), rows(), {"path": "fast"}),
+    "group": lambda: (rows(), rows(), {"group": 32}),
+    "group width": lambda: (rows(k=264), rows(k=264), {"group": 16}),
+    "scale shape": lambda: (rows(), rows(), {"residual_scale": torch.zeros(128, dtype=BF16)}),
+    "scale type": lambda: (rows(), rows(), {"residual_scale": torch.zeros(256)}),
+    "weight shape": lambda: (rows(), rows(), {"act_weight": torch.zeros(1, 256, dtype=BF16)}),
+    "weight stride": lambda: (rows(), rows(), {"act_weight": torch.zeros(512, dtype=BF16)[::2]}),
+    "cpu": lambda: (rows(), rows(), {}),
+}
+
+
+@pytest.mark.parametrize("change", list(ADDED))
+def test_add_prepare_refuses(change):
+    x, residual, options = ADDED[change]()
+    with pytest.raises(ValueError):
+        wq.add_prepare(x, residual, **options)
+
+
+def test_sums_over_their_inputs():
+    from wgpkernels_amd.int8._added import _check_sum, _rows_meet
+    held = torch.zeros(8, 768, dtype=BF16)
+    x, residual, out = held.split(256, 1)
+    assert not _rows_meet(out, x) and not _rows_meet(x, out) and _rows_meet(x, x)
+    assert _rows_meet(held[:, 8:264], x) and _rows_meet(held[2:4, :256], held[3:5, :256]) and not _rows_meet(held[:2, :256], held[2:4, :256])
+    flat = torch.zeros(2048, dtype=BF16)
+    assert _rows_meet(flat[:496].view(2, 248), flat[8:504].view(2, 248)) and not _rows_meet(flat[:496].view(2, 248), flat[496:992].view(2, 248))
+    assert _rows_meet(flat[:496].view(2, 248), flat[:1024].view(2, 512)[:, :248]) and not _rows_meet(held[:2, 512:], held[2:4, :256])
+    for bad in (held[:, 8:264], held[1:5, :256], rows(5), rows(dtype=FP16), rows(1).expand(4, 256), torch.zeros(4, 260, dtype=BF16)[:, :256]):
+        a, b = (held[:, :256], rows(8)) if bad.shape[0] == 8 else (held[:4, :256], rows())
+        with pytest.raises(ValueError):
+            _check_sum(bad, a, b)
+
+
+def test_prepared_values_refuse():
+    codes = torch.zeros(4, 256, dtype=torch.int8)
+    for p in (wq.Prepared("block", codes, None, torch.zeros(4), BF16), wq.Prepared("row", codes, None, torch.zeros(5), BF16),
+              wq.Prepared("row", codes[:, :250], None, torch.zeros(4), BF16), wq.Prepared("row", codes[:, :128], None, torch.zeros(4), BF16)):
+        with pytest.raises(ValueError):
+            p.values()

@@ -395,6 +395,10 @@ class Prepared:
         return Prepared(self.path, self.x[start:stop], None if self.lo is None else self.lo[start:stop],
                         None if self.scale is None else self.scale[start:stop], self.dtype)
 
+    def values(self):
+        """The (M, K) values that the codes stand for, rounded once to the activations' type (prepared_values())."""
+        return prepared_values(self)
+
 
 def prepare(x, group=0, path="block", act=None, act_weight=None, eps=0.0):
     """op(x) prepared once for `path` (see choose_path()); x 2-D BF16/FP16 with 16-byte aligned rows, act_weight in
@@ -616,5 +620,6 @@ def linear(x, weight, scale, bias=None, group=0, precise=False, mode=None, act=N
 
 
 from ._rotary import RotaryPlan, rotary, rotary_plan  # noqa: E402,F401
+from ._added import add_prepare, prepared_values  # noqa: E402,F401
 from ._kvcache import KVCache, KVPlan, kv_attention, kv_plan, kv_read, kv_write  # noqa: E402,F401
 from ._selftest import reference_linear as _reference, reference_rotation as _reference_rotation, selftest  # noqa: E402,F401

@@ -28,6 +28,8 @@ SIGNATURES = {
     "wq8_quantize_blocks_at": ("i", "pppiilii" "ipfp" "pqq" "p"),
     "wq8_transform_rows": ("i", "ppiilii" "ipfp"),
     "wq8_rotate_groups": ("i", "ppiilii" "p"),
+    "wq8_add_prepare": ("i", "plplppl" "ippp" "iiiipf" "p"),
+    "wq8_prepared_values": ("i", "pppp" "iiii" "p"),
     "wq8_gemm": ("i", "ppppppppp" "iiiiiii" "ppp"),
     "wq8_gemm_workspace": ("-", "iiiiii" "p"),
     "wq8_gemm_select": ("i", "iiiii"),
@@ -49,7 +51,7 @@ SIGNATURES = {
 }
 # entry points an older or foreign build may lack: bound when present (segments_supported() reports the first)
 OPTIONAL = {"wq8_gemm_segments", "wq8_gemm_noalloc", "wq8_quantize_at", "wq8_quantize_blocks_at", "wq8_gemm_at", "wq8_gemv_line_act",
-            "wq8_rotary", "wq8_kv_plan", "wq8_kv_write", "wq8_kv_read", "wq8_kv_attention", "wq8_kv_attention_workspace"}
+            "wq8_add_prepare", "wq8_prepared_values", "wq8_rotary", "wq8_kv_plan", "wq8_kv_write", "wq8_kv_read", "wq8_kv_attention", "wq8_kv_attention_workspace"}
 # the test library's entry points (include/wq8_test.h; libwgp_int8_test.so, not part of the product library)
 TEST_SIGNATURES = {
     "wq8_debug_block_sums": ("i", "ppp" "iii" "i" "p"),

@@ -25,7 +25,34 @@ struct PrepArgs {
     int64_t ldx;
     int k, group, act;
     float eps;
+    // add_prepare: rows of residual + rscale x, held in `sum` (rscale: k values or null)
+    const void* residual; const void* rscale; void* sum;
+    int64_t ldr, lds;
 };
+
+// 8 values of residual + rscale x at `col`: FP32 in one rounding, then held in the 16-bit type, whose values are what is normalised (a later
+// prepare() of the stored sum gives the same bits).
+template <int DT> WQ8_DEVICE void load_added(const PrepArgs& p, int64_t r, int col, float* v, bool valid) {
+    using raw = typename Elem<DT>::raw;
+    float x[8], scale[8];
+    load8<DT>(static_cast<const raw*>(p.x) + r * p.ldx + col, x, valid);
+    load8<DT>(static_cast<const raw*>(p.residual) + r * p.ldr + col, v, valid);
+    if (p.rscale) load8<DT>(static_cast<const raw*>(p.rscale) + col, scale, valid);
+    u32x4 packed;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint32_t both = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int e = 2 * j + h;
+            const raw held = Elem<DT>::from_f(p.rscale ? __builtin_fmaf(scale[e], x[e], v[e]) : v[e] + x[e]);
+            v[e] = Elem<DT>::to_f(held);
+            both |= uint32_t(held) << (16 * h);
+        }
+        packed[j] = both;
+    }
+    if (valid) *reinterpret_cast<u32x4*>(static_cast<raw*>(p.sum) + r * p.lds + col) = packed;
+}
 
 // Sum over the 4 waves of a workgroup in the fixed order ((w0 + w1) + w2) + w3.
 WQ8_DEVICE float block_sum4(float wave_value, float* lds4) {
@@ -102,16 +129,17 @@ constexpr int prep_waves(int dt, int mode, int cpw) {
     return dt == DT_F16 && mode != PREP_ROWS ? (mode == PREP_BLOCKS && cpw == 6 ? 4 : 1) : cpw <= 4 ? 8 : cpw <= 7 ? 5 : 4;
 }
 
-template <int DT, int MODE, int CPW>
+template <int DT, int MODE, int CPW, bool ADD = false>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(prep_waves(DT, MODE, CPW)))) prep_rows(PrepArgs p) {
     using raw = typename Elem<DT>::raw;
     __shared__ float lds4[4];
     const int tid = threadIdx.x;
-    const int k = p.k, chunks = k >> 3, act = p.act, group = p.group;
-    const long long shift = p.counter ? p.first + __ldg(p.counter) * p.step : 0;
-    const raw* row = static_cast<const raw*>(p.x) + (int64_t(blockIdx.x) + shift) * p.ldx;
-    const raw* aw = static_cast<const raw*>(p.act_weight);
+    const int k = p.k, chunks = k >> 3, act = ADD ? int(ACT_RMS) : p.act, group = p.group;
+    const long long shift = !ADD && p.counter ? p.first + __ldg(p.counter) * p.step : 0;
     const int64_t r = blockIdx.x;
+    // passes over a long row read the sums that its first pass stored, each thread its own
+    const raw* row = ADD ? static_cast<const raw*>(p.sum) + r * p.lds : static_cast<const raw*>(p.x) + (int64_t(blockIdx.x) + shift) * p.ldx;
+    const raw* aw = static_cast<const raw*>(p.act_weight);
     const int iters = CPW ? CPW : (chunks + 255) >> 8;
 
     // RMSNorm: sum of squares in the fixed tree (per thread: chunks in order, fmaf per element; wave butterfly;
@@ -122,7 +150,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(prep_w
 #pragma unroll
         for (int i = 0; i < (CPW ? CPW : 1); ++i) {
             const int c = tid + 256 * i;
-            load_act<DT>(row, k, 8 * c, cache[i], c < chunks, act == ACT_RMS ? ACT_NONE : act);
+            if constexpr (ADD) load_added<DT>(p, r, 8 * c, cache[i], c < chunks);
+            else load_act<DT>(row, k, 8 * c, cache[i], c < chunks, act == ACT_RMS ? ACT_NONE : act);
         }
     }
     if (act == ACT_RMS) {
@@ -133,6 +162,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(prep_w
             if (CPW) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = cache[CPW ? i : 0][j];
+            } else if constexpr (ADD) {
+                load_added<DT>(p, r, 8 * c, v, c < chunks);
             } else {
                 load8<DT>(row + 8 * c, v, c < chunks);
             }
@@ -235,23 +266,24 @@ __global__ void __launch_bounds__(256) prep_parts(PrepArgs p, int parts) {
     else store_transformed<DT>(p, r, k, c, chunks, v);
 }
 
-// Row codes (and hi / lo) with G x 256 threads a row, ceil(chunks / (256 G)) chunks a thread: few rows then have G times
+// Row codes (and hi / lo; with ADD the other preparations too) with G x 256 threads a row, ceil(chunks / (256 G)) chunks a thread: few rows then have G times
 // the waves at work on each. Thread 256 q + s takes chunks s + 256 (q + G j); RMSNorm's sum of squares keeps prep_rows's
 // tree, its 256 chains handed from one group of 256 threads to the next through LDS.
-template <int DT, int G, int CPT>
+template <int DT, int G, int CPT, int MODE = PREP_ROWS, bool ADD = false>
 __global__ void __launch_bounds__(256 * G) prep_wide(PrepArgs p) {
     using raw = typename Elem<DT>::raw;
     __shared__ float lds[4 * G], chain[256];
     const int tid = threadIdx.x, slot = tid & 255, q = tid >> 8;
-    const int k = p.k, chunks = k >> 3, act = p.act;
+    const int k = p.k, chunks = k >> 3, act = ADD ? int(ACT_RMS) : p.act;
     const int64_t r = blockIdx.x;
-    const long long shift = p.counter ? p.first + __ldg(p.counter) * p.step : 0;
+    const long long shift = !ADD && p.counter ? p.first + __ldg(p.counter) * p.step : 0;
     const raw* row = static_cast<const raw*>(p.x) + (r + shift) * p.ldx;
     float v[CPT][8];
 #pragma unroll
     for (int j = 0; j < CPT; ++j) {
         const int c = slot + 256 * (q + G * j);
-        load_act<DT>(row, k, 8 * c, v[j], c < chunks, act == ACT_RMS ? ACT_NONE : act);
+        if constexpr (ADD) load_added<DT>(p, r, 8 * c, v[j], c < chunks);
+        else load_act<DT>(row, k, 8 * c, v[j], c < chunks, act == ACT_RMS ? ACT_NONE : act);
     }
     if (act == ACT_RMS) {
         if (q == 0) chain[slot] = 0.0f;
@@ -279,6 +311,17 @@ __global__ void __launch_bounds__(256 * G) prep_wide(PrepArgs p) {
             const int c = slot + 256 * (q + G * j);
             apply_rms<DT>(v[j], inv_rms, static_cast<const raw*>(p.act_weight), 8 * c, c < chunks);
         }
+    }
+    if constexpr (MODE != PREP_ROWS) {
+#pragma unroll
+        for (int j = 0; j < CPT; ++j) {
+            const int c = slot + 256 * (q + G * j);
+            if ((c & ~63) >= chunks) break;  // a wave whose chunks all lie past the row
+            rotate_chunk(v[j], p.group);
+            if constexpr (MODE == PREP_BLOCKS) store_block_codes<DT>(p, r, k, c, chunks, v[j]);
+            else store_transformed<DT>(p, r, k, c, chunks, v[j]);
+        }
+        return;
     }
     float amax = 0.0f;
 #pragma unroll
@@ -344,6 +387,46 @@ static int launch_prep(const PrepArgs& p, int m, hipStream_t stream) {
     return int(hipGetLastError());
 }
 
+// The sum of two rows, normalised and prepared. Every thread reads its own chunks before it stores their sum, so that the sum may be
+// written over either input; prep_parts, whose parts all read the whole row, is left out.
+template <int DT, int MODE>
+static int launch_added(const PrepArgs& p, int m, hipStream_t stream) {
+    const int chunks = p.k / 8, parts = (chunks + 255) / 256;
+    if (parts > 1 && parts <= 8 && m <= 256) {
+        if (parts == 2) prep_wide<DT, 2, 1, MODE, true><<<m, 512, 0, stream>>>(p);
+        else if (parts == 3) prep_wide<DT, 3, 1, MODE, true><<<m, 768, 0, stream>>>(p);
+        else if (parts == 4) prep_wide<DT, 4, 1, MODE, true><<<m, 1024, 0, stream>>>(p);
+        else prep_wide<DT, 4, 2, MODE, true><<<m, 1024, 0, stream>>>(p);
+    } else if (parts <= 1) prep_rows<DT, MODE, 1, true><<<m, 256, 0, stream>>>(p);
+    else if (parts == 2) prep_rows<DT, MODE, 2, true><<<m, 256, 0, stream>>>(p);
+    else if (parts == 3) prep_rows<DT, MODE, 3, true><<<m, 256, 0, stream>>>(p);
+    else if (parts == 4) prep_rows<DT, MODE, 4, true><<<m, 256, 0, stream>>>(p);
+    else if (parts <= 6) prep_rows<DT, MODE, 6, true><<<m, 256, 0, stream>>>(p);
+    else if (parts <= 8) prep_rows<DT, MODE, 8, true><<<m, 256, 0, stream>>>(p);
+    else prep_rows<DT, MODE, 0, true><<<m, 256, 0, stream>>>(p);
+    return int(hipGetLastError());
+}
+
+// What prepared codes stand for, 8 a thread: code * scale, (hi + lo / 254) * scale, rounded once to the output's type. `per` is the scales of a
+// row (1, or one a 128-element block).
+template <int DT>
+__global__ void __launch_bounds__(256) prepared_values(const int8_t* q, const int8_t* lo, const float* scale, void* out, int64_t chunks, int row_chunks, int per) {
+    const int64_t c = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (c >= chunks) return;
+    const int64_t r = c / row_chunks;
+    const float s = per == 1 ? scale[r] : scale[r * per + (int(c - r * row_chunks) >> 4)];
+    const u32x2 hi = reinterpret_cast<const u32x2*>(q)[c];
+    const u32x2 rest = lo ? reinterpret_cast<const u32x2*>(lo)[c] : u32x2{0, 0};
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int shift = 24 - 8 * (j & 3);
+        const float code = float(int(hi[j >> 2] << shift) >> 24), part = float(int(rest[j >> 2] << shift) >> 24);
+        v[j] = (lo ? __builtin_fmaf(part, 1.0f / 254.0f, code) : code) * s;
+    }
+    store8<DT>(static_cast<typename Elem<DT>::raw*>(out) + 8 * c, v);
+}
+
 template <int MODE>
 static int dispatch_prep(const PrepArgs& p, int m, int dtype, hipStream_t stream) {
     if (dtype == DT_F16) return launch_prep<DT_F16, MODE>(p, m, stream);
@@ -373,7 +456,7 @@ WQ8_API int wq8_quantize(const void* x, int8_t* hi, int8_t* lo, float* scale, in
     if (!m) return 0;
     if (int rc = check_prep(m, k, dtype, group, act)) return rc;
     PrepArgs p{x, hi, lo, scale, nullptr, nullptr, act_weight, g_prep_offset.counter, g_prep_offset.first, g_prep_offset.step,
-               ldx, k, group, act, eps};
+               ldx, k, group, act, eps, nullptr, nullptr, nullptr, 0, 0};
     return dispatch_prep<PREP_ROWS>(p, m, dtype, stream);
 }
 
@@ -385,7 +468,7 @@ WQ8_API int wq8_quantize_blocks(const void* x, int8_t* q, float* scale, int m, i
     // contract: this library fills it with the rows' 1 / RMS
     if (act == ACT_RMS && k > 16384 && !inv_rms) return -2;
     PrepArgs p{x, q, nullptr, scale, nullptr, inv_rms, act_weight, g_prep_offset.counter, g_prep_offset.first, g_prep_offset.step,
-               ldx, k, group, act, eps};
+               ldx, k, group, act, eps, nullptr, nullptr, nullptr, 0, 0};
     return dispatch_prep<PREP_BLOCKS>(p, m, dtype, stream);
 }
 
@@ -411,7 +494,7 @@ WQ8_API int wq8_transform_rows(const void* x, void* out, int m, int k, int64_t l
     if (!m) return 0;
     if (dtype != DT_F16 && dtype != DT_BF16) return -1;
     if (int rc = check_prep(m, k, dtype, group, act)) return rc;
-    PrepArgs p{x, nullptr, nullptr, nullptr, out, nullptr, act_weight, nullptr, 0, 0, ldx, k, group, act, eps};
+    PrepArgs p{x, nullptr, nullptr, nullptr, out, nullptr, act_weight, nullptr, 0, 0, ldx, k, group, act, eps, nullptr, nullptr, nullptr, 0, 0};
     return dispatch_prep<PREP_TRANSFORM>(p, m, dtype, stream);
 }
 
@@ -420,6 +503,37 @@ WQ8_API int wq8_rotate_groups(const void* x, void* out, int m, int k, int64_t ld
     if (dtype != DT_F16 && dtype != DT_BF16) return -1;
     if (group != 16 && group != 64 && group != 256) return -1;
     if (k <= 0 || k % group) return -2;
-    PrepArgs p{x, nullptr, nullptr, nullptr, out, nullptr, nullptr, nullptr, 0, 0, ldx, k, group, ACT_NONE, 0.0f};
+    PrepArgs p{x, nullptr, nullptr, nullptr, out, nullptr, nullptr, nullptr, 0, 0, ldx, k, group, ACT_NONE, 0.0f, nullptr, nullptr, nullptr, 0, 0};
     return dispatch_prep<PREP_TRANSFORM>(p, m, dtype, stream);
+}
+
+WQ8_API int wq8_add_prepare(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* rscale, void* sum, int64_t lds, int path, void* out,
+                            int8_t* lo, float* scale, int m, int k, int dtype, int group, const void* act_weight, float eps, hipStream_t stream) {
+    if (!m) return 0;
+    if (dtype != DT_F16 && dtype != DT_BF16) return -1;
+    if (path < PREP_BLOCKS || path > PREP_TRANSFORM) return -1;
+    if (int rc = check_prep(m, k, dtype, group, ACT_RMS)) return rc;
+    int8_t* q = path == PREP_TRANSFORM ? nullptr : static_cast<int8_t*>(out);
+    PrepArgs p{x, q, path == PREP_ROWS ? lo : nullptr, scale, path == PREP_TRANSFORM ? out : nullptr, nullptr, act_weight, nullptr, 0, 0,
+               ldx, k, group, ACT_RMS, eps, residual, rscale, sum, ldr, lds};
+    if (dtype == DT_F16)
+        return path == PREP_BLOCKS ? launch_added<DT_F16, PREP_BLOCKS>(p, m, stream)
+               : path == PREP_ROWS ? launch_added<DT_F16, PREP_ROWS>(p, m, stream)
+                                   : launch_added<DT_F16, PREP_TRANSFORM>(p, m, stream);
+    return path == PREP_BLOCKS ? launch_added<DT_BF16, PREP_BLOCKS>(p, m, stream)
+           : path == PREP_ROWS ? launch_added<DT_BF16, PREP_ROWS>(p, m, stream)
+                               : launch_added<DT_BF16, PREP_TRANSFORM>(p, m, stream);
+}
+
+WQ8_API int wq8_prepared_values(const int8_t* q, const int8_t* lo, const float* scale, void* out, int m, int k, int blocks, int dtype, hipStream_t stream) {
+    if (!m) return 0;
+    if (dtype < 0 || dtype > 2) return -1;
+    if (m < 0 || k <= 0 || k % 8) return -2;
+    const int64_t chunks = int64_t(m) * (k / 8), groups = (chunks + 255) / 256;
+    if (groups > MAX_BLOCKS_256) return -2;
+    const int per = blocks ? (k + 127) / 128 : 1;
+    if (dtype == DT_F16) prepared_values<DT_F16><<<int(groups), 256, 0, stream>>>(q, lo, scale, out, chunks, k / 8, per);
+    else if (dtype == DT_BF16) prepared_values<DT_BF16><<<int(groups), 256, 0, stream>>>(q, lo, scale, out, chunks, k / 8, per);
+    else prepared_values<DT_F32><<<int(groups), 256, 0, stream>>>(q, lo, scale, out, chunks, k / 8, per);
+    return int(hipGetLastError());
 }
