@@ -163,6 +163,22 @@ int wq8_kv_attention(const void* q, void* out, const long long* strides, const i
                      void* workspace, wq8_stream_t stream);
 void wq8_kv_attention_workspace(int tokens, int requests, int heads, int group, int head_dim, int sms, int64_t* sizes);
 
+/* A mixture-of-experts layer, no counterpart in the reference. route: x (tokens, k) of dtype 0-2, rows ldx elements apart, router (experts, k)
+ * of router_dtype 0-2, both 16-byte aligned, k % 8 == 0; scores of the FP64 products by softmax (score 0) or the logistic function (1);
+ * ids (tokens, top): the largest of score + bias (f32, or null), ties by the lowest index, in order; weights: their scores, with normalise over
+ * their sum, times factor. experts <= 1024, top <= 64; logits: tokens * experts FP64 of scratch. */
+int wq8_route(const void* x, int64_t ldx, int dtype, const void* router, int router_dtype, const float* bias, int tokens, int experts, int k, int top,
+              int score, int normalise, float factor, void* logits, int32_t* ids, float* weights, wq8_stream_t stream);
+
+/* out (tokens, k) = residual + rscale * sum over a token's choices of weights * down(silu(gate) up): gate_up (experts, 2 hidden, k) int8 with
+ * scales (experts, 2 hidden), gate rows first, down (experts, k, hidden) with scales (experts, k); x, residual, rscale (k values) and out of
+ * dtype 0-1 (residual and rscale may be null; out may be residual or x in its place), rows 16-byte aligned. ids (tokens, top) int32, at most 4096 in all; those
+ * outside the experts are left out. k and hidden multiples of 16. workspace: sizes[0] bytes, 256-byte aligned. */
+int wq8_experts(const void* x, int64_t ldx, int dtype, const void* ids, const float* weights, const int8_t* gate_up, const float* gate_up_scale,
+                const int8_t* down, const float* down_scale, const void* residual, int64_t ldr, const void* rscale, void* out, int64_t ldo, int tokens,
+                int top, int experts, int k, int hidden, void* workspace, wq8_stream_t stream);
+void wq8_experts_workspace(int tokens, int top, int k, int hidden, int64_t* sizes);
+
 /* Cold-cache timing: reads `bytes` of a library-owned buffer on `stream` (nonzero if it cannot be allocated);
  * release frees it. Replace K8:1997-2016; bound at I:77-78. */
 int wq8_l2_flush(int device, int64_t bytes, wq8_stream_t stream);

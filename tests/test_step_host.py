@@ -1,4 +1,4 @@
-"""add_prepare(), without a GPU: what it refuses, before anything is launched."""
+"""The operators around the linears of a decode step (add_prepare, route, experts), without a GPU: what they refuse, before anything is launched."""
 import pytest
 import torch
 
@@ -61,3 +61,72 @@ def test_prepared_values_refuse():
               wq.Prepared("row", codes[:, :250], None, torch.zeros(4), BF16), wq.Prepared("row", codes[:, :128], None, torch.zeros(4), BF16)):
         with pytest.raises(ValueError):
             p.values()
+
+
+def layer(count=4, k=64, hidden=32):
+    return {"gate_up": torch.zeros(count, 2 * hidden, k, dtype=torch.int8), "gate_up_scale": torch.zeros(count, 2 * hidden),
+            "down": torch.zeros(count, k, hidden, dtype=torch.int8), "down_scale": torch.zeros(count, k)}
+
+
+def routes(tokens=3, top=2):
+    return torch.zeros(tokens, top, dtype=torch.int32), torch.zeros(tokens, top)
+
+
+EXPERTS = {
+    "type": {"x": rows(3, 64, torch.float32)},
+    "width": {"x": rows(3, 80)},
+    "pitch": {"x": rows(3, 68)[:, :64]},
+    "columns": {"x": torch.zeros(64, 3, dtype=BF16).t()},
+    "tokens": {"x": rows(4, 64)},
+    "ids type": {"routes": (torch.zeros(3, 2, dtype=torch.int64), torch.zeros(3, 2))},
+    "weights type": {"routes": (torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, 2, dtype=BF16))},
+    "weights shape": {"routes": (torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, 1))},
+    "ids strides": {"routes": (torch.zeros(2, 3, dtype=torch.int32).t(), torch.zeros(3, 2))},
+    "no choices": {"routes": routes(3, 0)},
+    "many choices": {"x": rows(2049, 64), "routes": routes(2049, 2)},
+    "gate_up type": {"gate_up": torch.zeros(4, 64, 64)},
+    "gate_up strides": {"gate_up": torch.zeros(4, 64, 128, dtype=torch.int8)[..., :64]},
+    "hidden": {"gate_up": torch.zeros(4, 48, 64, dtype=torch.int8), "gate_up_scale": torch.zeros(4, 48)},
+    "channels": {"x": rows(3, 72), **layer(k=72)},
+    "down shape": {"down": torch.zeros(4, 64, 16, dtype=torch.int8)},
+    "down experts": {"down": torch.zeros(3, 64, 32, dtype=torch.int8), "down_scale": torch.zeros(3, 64)},
+    "scales": {"down_scale": torch.zeros(4, 32)},
+    "scale type": {"gate_up_scale": torch.zeros(4, 64, dtype=BF16)},
+    "group scales": {"down_scale": torch.zeros(4, 64, 1)},
+    "residual": {"residual": rows(3, 64, FP16)},
+    "residual shape": {"residual": rows(1, 64)},
+    "residual_scale alone": {"residual_scale": torch.zeros(64, dtype=BF16)},
+    "residual_scale": {"residual": rows(3, 64), "residual_scale": torch.zeros(64)},
+    "cpu": {},
+}
+
+
+@pytest.mark.parametrize("change", list(EXPERTS))
+def test_experts_refuse(change):
+    with pytest.raises(ValueError):
+        wq.experts(**{"x": rows(3, 64), "routes": routes(), **layer(), **EXPERTS[change]})
+
+
+ROUTE = {
+    "type": {"x": rows(3, 64, torch.float64)},
+    "width": {"x": rows(3, 72)},
+    "pitch": {"x": rows(3, 68)[:, :64]},
+    "router type": {"router": torch.zeros(8, 64, dtype=torch.float64)},
+    "router strides": {"router": torch.zeros(64, 8).t()},
+    "channels": {"x": rows(3, 60), "router": torch.zeros(8, 60)},
+    "no experts": {"router": torch.zeros(0, 64)},
+    "many experts": {"router": torch.zeros(1025, 64)},
+    "no choice": {"top": 0},
+    "more than there are": {"top": 9},
+    "many choices": {"top": 65, "router": torch.zeros(100, 64)},
+    "score": {"score": "linear"},
+    "bias type": {"bias": torch.zeros(8, dtype=BF16)},
+    "bias shape": {"bias": torch.zeros(8, 1)},
+    "cpu": {},
+}
+
+
+@pytest.mark.parametrize("change", list(ROUTE))
+def test_route_refuses(change):
+    with pytest.raises(ValueError):
+        wq.route(**{"x": rows(3, 64), "router": torch.zeros(8, 64), "top": 2, **ROUTE[change]})
