@@ -1,0 +1,192 @@
+"""sample() on the GPU against its definition on the CPU, weights as whole numbers of 2^-44 of the heaviest and sums as integers: the tokens are
+whole numbers and have to be equal. (An exponential whose last bit differs moves a weight by one such part, and the token only where a draw
+or top-p's border falls between: with these seeds it does not. Sums of FP64 weights would not do: half of 750 pairs is exactly a border.)"""
+import math
+from fractions import Fraction
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def defined(logits, draws, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One row after another, from the definition."""
+    found = []
+    for row in range(len(logits)):
+        of = lambda option: option[row].item() if isinstance(option, torch.Tensor) else torch.tensor(option).item()
+        t, k, p, m = of(temperature), int(of(top_k)), of(top_p), of(min_p)
+        l = logits[row].cpu().double()
+        l = torch.where(l.isnan(), -math.inf, l)
+        top = l.max()
+        if top == -math.inf:
+            found.append(-1)
+            continue
+        order = torch.sort(l, descending=True, stable=True).indices
+        if not t > 0:
+            found.append(order[0].item())
+            continue
+        weight = torch.where(l == top, 1.0, torch.exp(torch.where(l == top, 0.0, l - top) / t)) if top != math.inf else (l == top).double()
+        share = weight
+        weight = torch.round(weight * 2.0 ** 44).long()
+        ordered = weight[order]
+        kept = torch.ones(len(l), dtype=torch.bool)
+        if 0 < k < len(l):
+            kept[k:] = False
+        if p < 1:
+            mass = torch.cumsum(ordered * kept, 0)
+            before = torch.cat([torch.zeros(1, dtype=torch.int64), mass[:-1]])
+            kept &= before < math.ceil(Fraction(p) * mass[-1].item())
+            kept[0] = True
+        kept &= share[order] >= min(m, 1.0)
+        left = torch.zeros_like(weight)
+        left[order] = ordered * kept
+        upto = torch.cumsum(left, 0)
+        u = draws[row].item()
+        u = min(max(u, 0.0), 1 - 2.0 ** -24) if u == u else 0.0
+        found.append((upto > math.floor(Fraction(u) * upto[-1].item())).int().argmax().item())
+    return torch.tensor(found)
+
+
+def logits_of(rows, vocabulary, dtype, seed, spread=2.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    l = torch.randn(rows, vocabulary, generator=g, device="cuda") * spread
+    likely = max(1, min(200, vocabulary // 4))
+    at = torch.randint(0, vocabulary, (rows, likely), generator=g, device="cuda")
+    l.scatter_add_(1, at, -torch.log(torch.rand(rows, likely, generator=g, device="cuda").clamp_(min=1e-6)) * 2)
+    return l.to(dtype), torch.rand(rows, generator=g, device="cuda"), g
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("rows,vocabulary", [(1, 1), (3, 2), (5, 7), (4, 255), (7, 2048), (3, 2049), (40, 1000), (1, 50001), (9, 33333), (2, 131072), (1100, 300), (2, 262144)])
+@pytest.mark.parametrize("options", [{}, {"temperature": 0.6, "top_k": 40}, {"top_p": 0.9}, {"temperature": 1.7, "top_k": 30, "top_p": 0.8}, {"min_p": 0.1},
+                                     {"top_k": 1}, {"temperature": 0.0}, {"temperature": 3.0, "top_p": 0.999, "min_p": 0.001}, {"top_k": 500, "top_p": 0.3}])
+def test_tokens(wq, dtype, rows, vocabulary, options):
+    print(f"sample {rows} {vocabulary} {dtype} {options}", flush=True)
+    logits, draws, _ = logits_of(rows, vocabulary, dtype, seed=rows + vocabulary)
+    tokens = wq.sample(logits, draws, **options)
+    assert tokens.dtype == torch.int64
+    assert torch.equal(tokens.cpu(), defined(logits, draws, **options))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("vocabulary", [777, 20011])
+def test_every_row_its_own_options(wq, dtype, vocabulary):
+    rows = 96
+    logits, draws, g = logits_of(rows, vocabulary, dtype, seed=5)
+    pick = lambda values, kind: torch.tensor(values, dtype=kind, device="cuda")[torch.randint(0, len(values), (rows,), generator=g, device="cuda")]
+    options = {"temperature": pick([0.0, -1.0, 0.3, 1.0, 2.0, 1e-30, 1e30, math.nan], FP32), "top_k": pick([0, -5, 1, 2, 50, 10 ** 6, vocabulary - 1], torch.int32),
+               "top_p": pick([1.0, 2.0, 0.9, 0.5, 0.0, -1.0, 1e-30], FP32), "min_p": pick([0.0, 0.2, 1.0, 5.0, -1.0], FP32)}
+    assert torch.equal(wq.sample(logits, draws, **options).cpu(), defined(logits, draws, **options))
+
+
+@pytest.mark.parametrize("vocabulary", [5, 3000, 40000, 131072])
+@pytest.mark.parametrize("options", [{}, {"top_k": 2}, {"top_k": 2500}, {"top_p": 0.5}, {"top_k": 20000, "top_p": 0.7}, {"top_p": 0.5, "min_p": 1.0}])
+def test_equal_logits(wq, vocabulary, options):
+    """All alike, and two values only: ties by the lowest index, more of them than the list of keys holds."""
+    print(f"equal {vocabulary} {options}", flush=True)
+    draws = torch.tensor([0.0, 0.25, 0.5, 1 - 2.0 ** -24], device="cuda")
+    logits = torch.full((4, vocabulary), -3.5, device="cuda")
+    assert torch.equal(wq.sample(logits, draws, **options).cpu(), defined(logits, draws, **options))
+    logits[:, ::2] += 0.5
+    logits = logits.to(BF16)
+    assert torch.equal(wq.sample(logits, draws, **options).cpu(), defined(logits, draws, **options))
+
+
+def test_many_near_logits(wq):
+    """A flat FP32 row: tens of thousands of different keys in the bins of the cuts."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    logits = torch.rand(3, 100000, generator=g, device="cuda") * 1e-3
+    draws = torch.rand(3, generator=g, device="cuda")
+    for options in ({"top_k": 30001}, {"top_p": 0.31}, {"top_k": 60000, "top_p": 0.77}, {"top_k": 5}):
+        assert torch.equal(wq.sample(logits, draws, **options).cpu(), defined(logits, draws, **options)), options
+
+
+@pytest.mark.parametrize("options", [{}, {"top_k": 3}, {"top_p": 0.6}, {"temperature": 0.0}, {"min_p": 0.5}])
+def test_masks_infinities_and_nan(wq, options):
+    logits, draws, _ = logits_of(9, 5000, FP32, seed=8)
+    inf, nan = math.inf, math.nan
+    logits[0] = -inf
+    logits[1] = nan
+    logits[2] = -inf
+    logits[2, 4321] = -1e30          # a mask that leaves one token, far below the others of its kind
+    logits[3, 7:] = -inf
+    logits[4, ::3] = nan
+    logits[5, 100], logits[5, 200] = inf, inf
+    logits[6] = torch.finfo(FP32).min
+    logits[6, 17] = 0
+    logits[7, 1:] = torch.finfo(FP32).min  # the type's lowest value as a mask
+    logits[8] = torch.finfo(FP32).min
+    tokens = wq.sample(logits, draws, **options).cpu()
+    assert torch.equal(tokens, defined(logits, draws, **options))
+    assert tokens[:3].tolist() == [-1, -1, 4321] and tokens[3] < 7 and tokens[4] % 3 and tokens[5] in (100, 200) and tokens[6] == 17 and tokens[7] == 0
+
+
+def test_zeros_of_both_signs_are_alike(wq):
+    logits = torch.tensor([[-0.0, 0.0, -0.0, 0.0]], device="cuda")
+    for k in (1, 2, 3):
+        draws = torch.tensor([1 - 2.0 ** -24], device="cuda")
+        assert wq.sample(logits, draws, top_k=k).item() == k - 1
+    assert wq.sample(logits, draws, temperature=0.0).item() == 0
+
+
+def test_draws_at_the_ends_and_outside(wq):
+    logits, _, _ = logits_of(6, 300, FP32, seed=3)
+    logits[:, 0] = logits[:, 299] = 3.0
+    draws = torch.tensor([0.0, 1 - 2.0 ** -24, 1.0, 7.0, -1.0, math.nan], device="cuda")
+    assert wq.sample(logits, draws).tolist() == [0, 299, 299, 299, 0, 0]
+
+
+def test_rows_apart_and_unaligned(wq):
+    for dtype in (BF16, FP32):
+        held, draws, _ = logits_of(5, 7001, dtype, seed=6)
+        for first, last in ((1, 7000), (3, 4099), (5, 6)):
+            view = held[:, first:last]
+            for options in ({"top_k": 20, "top_p": 0.9}, {}):
+                assert torch.equal(wq.sample(view, draws, **options).cpu(), defined(view, draws, **options))
+        one = held[2, 1:].expand(4, 7000)  # the same row for several draws
+        assert torch.equal(wq.sample(one, draws[:4].contiguous(), top_p=0.9).cpu(), defined(one, draws[:4], top_p=0.9))
+
+
+def test_shares_follow_the_weights(wq):
+    """Draws spread evenly over [0, 1): every token as often as its share says, but for one at each border."""
+    logits = torch.log(torch.tensor([0.1, 0.4, 0.05, 0.25, 0.2], device="cuda"))
+    n = 4096
+    draws = (torch.arange(n, device="cuda").float() + 0.5) / n
+    tokens = wq.sample(logits.expand(n, 5).contiguous(), draws)
+    assert (tokens.bincount(minlength=5).cpu() - n * torch.softmax(logits.cpu(), 0)).abs().max() <= 1
+    tokens = wq.sample(logits.expand(n, 5).contiguous(), draws, top_k=3)
+    want = torch.tensor([0, 0.4, 0, 0.25, 0.2]) / 0.85 * n
+    assert (tokens.bincount(minlength=5).cpu() - want).abs().max() <= 1
+
+
+def test_no_rows(wq):
+    assert wq.sample(torch.empty(0, 10, device="cuda"), torch.empty(0, device="cuda")).shape == (0,)
+
+
+def test_captured_and_on_two_streams(wq):
+    logits, draws, g = logits_of(4, 30000, BF16, seed=9)
+    options = {"temperature": torch.full((4,), 0.8, device="cuda"), "top_k": 40, "top_p": 0.95}
+    wq.sample(logits, draws, **options)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tokens = wq.sample(logits, draws, **options)
+    for seed in range(4):
+        a, b, _ = logits_of(4, 30000, BF16, seed=20 + seed)
+        logits.copy_(a), draws.copy_(b)
+        options["temperature"].fill_(0.5 + 0.2 * seed)
+        graph.replay()
+        assert torch.equal(tokens.cpu(), defined(a, b, **options))
+        assert torch.equal(tokens, wq.sample(logits, draws, **options))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    inputs = [logits_of(64, 20000, FP32, seed=30 + i) for i in range(2)]
+    torch.cuda.synchronize()
+    found = []
+    for stream, (l, u, _) in zip(streams, inputs):
+        with torch.cuda.stream(stream):
+            found.append(wq.sample(l, u, top_k=50, top_p=0.9))
+    torch.cuda.synchronize()
+    for tokens, (l, u, _) in zip(found, inputs):
+        assert torch.equal(tokens.cpu(), defined(l, u, top_k=50, top_p=0.9))

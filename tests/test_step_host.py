@@ -1,4 +1,4 @@
-"""The operators around the linears of a decode step (add_prepare, route, experts), without a GPU: what they refuse, before anything is launched."""
+"""The operators around the linears of a decode step (add_prepare, route, experts, sample), without a GPU: what they refuse, before anything is launched."""
 import pytest
 import torch
 
@@ -130,3 +130,28 @@ ROUTE = {
 def test_route_refuses(change):
     with pytest.raises(ValueError):
         wq.route(**{"x": rows(3, 64), "router": torch.zeros(8, 64), "top": 2, **ROUTE[change]})
+
+
+SAMPLE = {
+    "dimensions": {"logits": torch.zeros(5)},
+    "type": {"logits": torch.zeros(3, 5, dtype=torch.float64)},
+    "columns": {"logits": torch.zeros(5, 3).t()},
+    "no vocabulary": {"logits": torch.zeros(3, 0)},
+    "wide": {"logits": torch.zeros(3, 1).expand(3, 2 ** 24 + 1)},
+    "many rows": {"logits": torch.zeros(1, 5).expand(2 ** 17 + 1, 5), "draws": torch.zeros(2 ** 17 + 1)},
+    "draws shape": {"draws": torch.zeros(3, 1)},
+    "draws type": {"draws": torch.zeros(3, dtype=torch.float64)},
+    "draws strides": {"draws": torch.zeros(6)[::2]},
+    "temperature type": {"temperature": torch.ones(3, dtype=BF16)},
+    "temperature shape": {"temperature": torch.ones(1)},
+    "top_k type": {"top_k": torch.ones(3)},
+    "top_p strides": {"top_p": torch.ones(6)[::2]},
+    "min_p shape": {"min_p": torch.ones(4)},
+    "cpu": {},
+}
+
+
+@pytest.mark.parametrize("change", list(SAMPLE))
+def test_sample_refuses(change):
+    with pytest.raises(ValueError):
+        wq.sample(**{"logits": torch.zeros(3, 5), "draws": torch.zeros(3), **SAMPLE[change]})

@@ -29,7 +29,7 @@ DEFAULT_ARCH = "gfx950"
 LIBRARIES = {"int8": ["int8/csrc/quantize.hip", "int8/csrc/gemm.hip", "int8/csrc/gemm_bf16.hip", "int8/csrc/gemm_f16.hip",
                       "int8/csrc/gemm_mid_bf16.hip", "int8/csrc/gemm_mid_f16.hip",
                       "int8/csrc/fewtoken.hip", "int8/csrc/rotary.hip", "int8/csrc/kvcache.hip", "int8/csrc/kvattention.hip",
-                      "int8/csrc/experts.hip", "int8/csrc/abi.hip"],
+                      "int8/csrc/experts.hip", "int8/csrc/sample.hip", "int8/csrc/abi.hip"],
              "int8_test": ["int8/csrc/test_entry.hip"]}
 HIP_FLAGS = [
     "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden",

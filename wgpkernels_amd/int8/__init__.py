@@ -620,6 +620,7 @@ def linear(x, weight, scale, bias=None, group=0, precise=False, mode=None, act=N
 
 
 from ._rotary import RotaryPlan, rotary, rotary_plan  # noqa: E402,F401
+from ._sample import sample  # noqa: E402,F401
 from ._added import add_prepare, prepared_values  # noqa: E402,F401
 from ._experts import Routes, experts, route  # noqa: E402,F401
 from ._kvcache import KVCache, KVPlan, kv_attention, kv_plan, kv_read, kv_write  # noqa: E402,F401

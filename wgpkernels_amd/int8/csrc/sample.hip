@@ -1,0 +1,520 @@
+// A token of every row of logits by given random numbers, with temperature, top-k, top-p and min-p, on gfx950. No reference counterpart.
+//
+// A token's weight is exp((logit - largest) / temperature) in FP64, held as a whole number of 2^-44 (2^-shift): sums of weights are then the same
+// in whatever order they are taken, so a row may be spread over workgroups and added up by atomics, and the token drawn is that of the
+// 64-bit definition but for borders within 2^-44 of each other. Tokens stand in the order of (logit, lowest index first), a 64-bit key:
+// top-k and top-p each keep the keys down to a last one, `cut`.
+//
+// Four launches, a row over up to 64 workgroups in the first three: the largest logit; a histogram (counts and weights) over (largest - logit) /
+// temperature; the keys of the histogram's bins in which the cuts lie, and the weights of what certainly stays; then a workgroup a row
+// finds the cut among those keys digit by digit, and the token whose running weight, in vocabulary order, passes draw * (weight kept).
+#include "wq8_common.h"
+#include "wq8_abi.h"
+
+namespace wq8 {
+
+constexpr int SAMPLE_BINS = 1024, SAMPLE_SPLITS = 64, SAMPLE_LIST = 2048, SAMPLE_PIECE = 2048;
+constexpr float BINS_PER_UNIT = 32.0f;  // the last bin begins at 31.97: weights below 2^-46, held as 0
+
+struct SampleRow {  // a row's workspace
+    uint64_t largest[SAMPLE_SPLITS];
+    uint64_t kept[SAMPLE_SPLITS];
+    uint64_t mass[SAMPLE_BINS];
+    uint32_t count[SAMPLE_BINS];
+    uint64_t list[SAMPLE_LIST];
+    uint32_t listed, unused;
+};
+
+struct SampleArgs {
+    const void* logits;
+    int64_t ld;
+    const float* draws;
+    const float* temperature;  // per row, or null: the value below
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    SampleRow* rows;
+    int64_t* tokens;
+    float temperature0, top_p0, min_p0;
+    int top_k0;
+    int vocabulary, split, splits, shift;
+};
+
+// The order of a logit: larger numbers for larger logits, 0 for NaN; both zeros alike.
+WQ8_DEVICE uint32_t logit_order(float l) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, l + 0.0f);
+    return l != l ? 0u : b >> 31 ? ~b : b | 0x80000000u;
+}
+WQ8_DEVICE float order_logit(uint32_t o) { return __builtin_bit_cast(float, o >> 31 ? o & 0x7fffffffu : ~o); }
+WQ8_DEVICE uint64_t token_key(float l, int index) { return uint64_t(logit_order(l)) << 32 | (0xffffffffu - uint32_t(index)); }
+WQ8_DEVICE int key_index(uint64_t key) { return int(0xffffffffu - uint32_t(key)); }
+
+// What a row is sampled by.
+struct Row {
+    float top;         // its largest logit
+    uint64_t first;    // the key of that
+    double inverse;    // of the temperature
+    float bins;        // bins a unit of logit
+    double scale, min_p;
+    float top_p;
+    int top_k;
+    bool greedy, nothing, by_p, by_k;
+
+    WQ8_DEVICE double weight(float l) const {
+        if (l == top) return 1.0;
+        const double z = (double(l) - double(top)) * inverse;
+        return z <= 0.0 ? exp(z) : 0.0;  // NaN: 0
+    }
+    WQ8_DEVICE uint64_t units(double w) const { return uint64_t(__builtin_rint(w * scale)); }
+    WQ8_DEVICE int bin(float l) const {
+        if (l == top) return 0;
+        const float b = (top - l) * bins;
+        return b < float(SAMPLE_BINS - 1) ? int(b) : SAMPLE_BINS - 1;
+    }
+};
+
+WQ8_DEVICE uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
+template <typename T> WQ8_DEVICE T wave_total(T v) {
+#pragma unroll
+    for (int step = 32; step; step >>= 1) v += __shfl_xor(v, step);
+    return v;
+}
+
+WQ8_DEVICE Row read_row(const SampleArgs& p, const SampleRow& state, int row) {
+    Row r;
+    const int lane = threadIdx.x & 63;
+    uint64_t best = lane < p.splits ? state.largest[lane] : 0;
+#pragma unroll
+    for (int step = 32; step; step >>= 1) best = max64(best, __shfl_xor(best, step));
+    r.first = best;
+    r.top = order_logit(uint32_t(best >> 32));
+    const float t = p.temperature ? p.temperature[row] : p.temperature0;
+    r.greedy = !(t > 0.0f);
+    r.nothing = uint32_t(best >> 32) <= logit_order(-__builtin_inff());
+    r.inverse = 1.0 / double(t);
+    r.bins = fminf(float(r.inverse) * BINS_PER_UNIT, 0x1.fffffep127f);  // (an infinity would part equal logits from others beside them)
+    r.scale = double(uint64_t(1) << p.shift);
+    r.min_p = fmin(double(p.min_p ? p.min_p[row] : p.min_p0), 1.0);
+    r.top_p = p.top_p ? p.top_p[row] : p.top_p0;
+    r.top_k = p.top_k ? p.top_k[row] : p.top_k0;
+    r.by_p = r.top_p < 1.0f;
+    r.by_k = r.top_k > 0 && r.top_k < p.vocabulary;
+    return r;
+}
+
+// f(logit, index) for the row's values from begin to end, 8 neighbouring ones a thread at a time. Rows may begin at any value: the loads of 16 bytes
+// are as unaligned as the row is.
+template <int DT, typename F> WQ8_DEVICE void each_logit(const SampleArgs& p, int row, int begin, int end, const F& f) {
+    using raw = typename Elem<DT>::raw;
+    const raw* values = static_cast<const raw*>(p.logits) + row * p.ld;
+    for (int i = begin + 8 * int(threadIdx.x); i < end; i += 8 * 256) {
+        raw v[8];
+        if (i + 8 <= end) __builtin_memcpy(v, values + i, sizeof(v));
+        else
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = values[min(i + j, end - 1)];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (i + j < end) f(Elem<DT>::to_f(v[j]), i + j);
+    }
+}
+
+// ---- 1: the largest logit of every part of a row -----------------------------------------------------------------------------
+template <int DT> __global__ void __launch_bounds__(256) sample_largest(SampleArgs p) {
+    __shared__ uint64_t best4[4];
+    const int row = blockIdx.x / p.splits, s = blockIdx.x % p.splits;
+    SampleRow& state = p.rows[row];
+    for (int b = s * 256 + threadIdx.x; b < SAMPLE_BINS; b += 256 * p.splits) state.mass[b] = 0, state.count[b] = 0;
+    if (!s && !threadIdx.x) state.listed = 0;
+    uint64_t best = 0;
+    each_logit<DT>(p, row, s * p.split, min(p.vocabulary, (s + 1) * p.split), [&](float l, int i) { best = max64(best, token_key(l, i)); });
+#pragma unroll
+    for (int step = 32; step; step >>= 1) best = max64(best, __shfl_xor(best, step));
+    if (!(threadIdx.x & 63)) best4[threadIdx.x >> 6] = best;
+    __syncthreads();
+    if (!threadIdx.x) state.largest[s] = max64(max64(best4[0], best4[1]), max64(best4[2], best4[3]));
+}
+
+// ---- 2: counts and weights over (largest - logit) / temperature ------------------------------------------------------------------
+template <int DT> __global__ void __launch_bounds__(256) sample_bins(SampleArgs p) {
+    __shared__ unsigned long long mass[SAMPLE_BINS];
+    __shared__ uint32_t count[SAMPLE_BINS];
+    const int row = blockIdx.x / p.splits, s = blockIdx.x % p.splits;
+    SampleRow& state = p.rows[row];
+    const Row r = read_row(p, state, row);
+    if (r.greedy || r.nothing || !(r.by_k || r.by_p)) return;
+    for (int b = threadIdx.x; b < SAMPLE_BINS; b += 256) mass[b] = 0, count[b] = 0;
+    __syncthreads();
+    each_logit<DT>(p, row, s * p.split, min(p.vocabulary, (s + 1) * p.split), [&](float l, int) {
+        if (l != l) return;
+        const int b = r.bin(l);
+        atomicAdd(&count[b], 1u);
+        if (b < SAMPLE_BINS - 1) atomicAdd(&mass[b], (unsigned long long)r.units(r.weight(l)));
+    });
+    __syncthreads();
+    for (int b = threadIdx.x; b < SAMPLE_BINS; b += 256) {
+        if (!count[b]) continue;
+        atomicAdd(&state.count[b], count[b]);
+        if (mass[b]) atomicAdd(reinterpret_cast<unsigned long long*>(&state.mass[b]), mass[b]);
+    }
+}
+
+// ---- the bins in which a row's cuts lie --------------------------------------------------------------------------------------
+// ceil(f * total) and floor(f * total) for 0 <= f < 1, exactly
+WQ8_DEVICE uint64_t share_of(float f, uint64_t total, bool up) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, f);
+    const uint32_t exponent = b >> 23 & 255;
+    const uint64_t mantissa = exponent ? (b & 0x7fffff) | 0x800000 : b & 0x7fffff;
+    const int shift = 150 - int(exponent ? exponent : 1);  // f = mantissa / 2^shift, shift >= 24
+    const uint64_t high = __umul64hi(mantissa, total), low = mantissa * total;
+    if (shift >= 128) return up && (high | low) ? 1 : 0;
+    const uint64_t whole = shift >= 64 ? high >> (shift - 64) : shift ? high << (64 - shift) | low >> shift : low;
+    const bool rest = shift >= 64 ? (low | (shift > 64 ? high << (128 - shift) : 0)) != 0 : (low << (64 - shift)) != 0;
+    return whole + (up && rest ? 1 : 0);
+}
+// The weight that top-p wants: a key stays while the weight before it is less. At least 1, so that the first one stays.
+WQ8_DEVICE uint64_t wanted_mass(float top_p, uint64_t total) {
+    const uint64_t m = top_p > 0.0f ? share_of(top_p, total, true) : 0;
+    return m ? m : 1;
+}
+
+struct Cut {
+    int k_bin;                      // the bin of top-k's last key, or SAMPLE_BINS: every weight is among the k
+    uint32_t k_left;                // how many of that bin's keys stay
+    uint64_t k_before;              // the weight before it
+    int low, high;                  // the bins of top-p's last key (low > high: no top-p)
+    uint64_t low_before;            // the weight before them
+    int certain;                    // bins below it stay whole
+    WQ8_DEVICE bool listed(int bin) const { return bin == k_bin || (bin >= low && bin <= high); }
+};
+
+// Exclusive sums over the workgroup's 256 threads, and their total.
+template <typename T> WQ8_DEVICE T scan256(T v, T* waves, T& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    T upto = v;
+#pragma unroll
+    for (int step = 1; step < 64; step <<= 1) {
+        const T below = __shfl_up(upto, step);
+        if (lane >= step) upto += below;
+    }
+    __syncthreads();
+    if (lane == 63) waves[wave] = upto;
+    __syncthreads();
+    T before = upto - v;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (w < wave) before += waves[w];
+        total += waves[w];
+    }
+    return before;
+}
+
+struct CutScratch {
+    uint64_t waves64[4];
+    uint32_t waves32[4];
+    uint64_t k_before, k_mass, low_before;
+    uint32_t k_left;
+    int k_bin, low, high;
+};
+
+WQ8_DEVICE Cut find_cut(const Row& r, const SampleRow& state, CutScratch& sc) {
+    constexpr int EACH = SAMPLE_BINS / 256;
+    uint64_t mass[EACH], masses = 0, total;
+    uint32_t count[EACH], counts = 0, all;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        mass[i] = state.mass[EACH * threadIdx.x + i];
+        count[i] = state.count[EACH * threadIdx.x + i];
+        masses += mass[i];
+        counts += count[i];
+    }
+    if (!threadIdx.x) sc.k_bin = SAMPLE_BINS, sc.low = 1, sc.high = 0, sc.low_before = 0;
+    const uint64_t mass_before = scan256(masses, sc.waves64, total);
+    const uint32_t count_before = scan256(counts, sc.waves32, all);
+    Cut c;
+    if (r.by_k) {
+        uint32_t n = count_before;
+        uint64_t m = mass_before;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            // (the last bin's weights are 0: a k that reaches it leaves nothing out)
+            if (n < uint32_t(r.top_k) && n + count[i] >= uint32_t(r.top_k) && EACH * int(threadIdx.x) + i < SAMPLE_BINS - 1) {
+                sc.k_bin = EACH * threadIdx.x + i;
+                sc.k_left = r.top_k - n;
+                sc.k_before = m;
+                sc.k_mass = mass[i];
+            }
+            n += count[i];
+            m += mass[i];
+        }
+        __syncthreads();
+    }
+    c.k_bin = sc.k_bin;
+    c.k_left = sc.k_left;
+    c.k_before = sc.k_before;
+    if (r.by_p) {
+        // the k's weight is known up to its bin: top-p's last key lies between those of the least and the most that it can be
+        const bool some = c.k_bin < SAMPLE_BINS;
+        const uint64_t least = wanted_mass(r.top_p, some ? c.k_before : total), most = wanted_mass(r.top_p, some ? c.k_before + sc.k_mass : total);
+        uint64_t m = mass_before;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            if (m < least && m + mass[i] >= least) {
+                sc.low = EACH * threadIdx.x + i;
+                sc.low_before = m;
+            }
+            if (m < most && m + mass[i] >= most) sc.high = EACH * threadIdx.x + i;
+            m += mass[i];
+        }
+        __syncthreads();
+    }
+    c.low = sc.low;
+    c.high = sc.high;
+    c.low_before = sc.low_before;
+    c.certain = r.by_p ? c.low : c.k_bin;
+    __syncthreads();
+    return c;
+}
+
+// ---- 3: the keys of those bins, and the weights that certainly stay ------------------------------------------------------------
+template <int DT> __global__ void __launch_bounds__(256) sample_list(SampleArgs p) {
+    __shared__ CutScratch scratch;
+    __shared__ uint64_t sums[4];
+    const int row = blockIdx.x / p.splits, s = blockIdx.x % p.splits;
+    SampleRow& state = p.rows[row];
+    const Row r = read_row(p, state, row);
+    if (r.greedy || r.nothing) return;
+    const bool cutting = r.by_k || r.by_p;
+    Cut c{};
+    if (cutting) c = find_cut(r, state, scratch);
+    uint64_t sum = 0;
+    each_logit<DT>(p, row, s * p.split, min(p.vocabulary, (s + 1) * p.split), [&](float l, int i) {
+        if (l != l) return;
+        if (cutting) {
+            const int b = r.bin(l);
+            if (c.listed(b)) {
+                const uint32_t at = atomicAdd(&state.listed, 1u);
+                if (at < uint32_t(SAMPLE_LIST)) state.list[at] = token_key(l, i);
+            }
+            if (b >= c.certain) return;
+        }
+        const double w = r.weight(l);
+        if (w >= r.min_p) sum += r.units(w);
+    });
+    sum = wave_total(sum);
+    if (!(threadIdx.x & 63)) sums[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    if (!threadIdx.x) state.kept[s] = sums[0] + sums[1] + sums[2] + sums[3];
+}
+
+// ---- 4: the cut among the listed keys, and the token ---------------------------------------------------------------------------
+struct PickScratch {
+    CutScratch cut;
+    uint64_t list[SAMPLE_LIST], units[SAMPLE_LIST];
+    unsigned long long mass[256];
+    uint32_t count[256];
+    unsigned long long kept[SAMPLE_SPLITS];
+    unsigned long long lowest, highest, found, need, before;
+    uint32_t in_digit;
+    int digit;
+    uint64_t waves64[4];
+    uint32_t waves32[4];
+};
+
+// The key at which the running count (by_count) or weight of `each`'s keys, from the largest on, reaches `need` (at least 1, at most their sum): digits of 8
+// bits from the first in which they differ, counts and weights of each digit's values. `above`: the weight of the larger keys.
+template <typename Each> WQ8_DEVICE uint64_t select_key(PickScratch& sc, const Each& each, bool by_count, uint64_t need, uint64_t& above) {
+    const int tid = threadIdx.x;
+    if (!tid) sc.lowest = ~0ull, sc.highest = 0;
+    __syncthreads();
+    uint64_t low = ~uint64_t(0), high = 0;
+    each([&](uint64_t key, uint64_t) {
+        low = key < low ? key : low;
+        high = max64(high, key);
+    });
+    if (low <= high) {
+        atomicMin(&sc.lowest, (unsigned long long)low);
+        atomicMax(&sc.highest, (unsigned long long)high);
+    }
+    __syncthreads();
+    const uint64_t differ = sc.lowest ^ sc.highest;
+    uint64_t key = sc.highest;
+    above = 0;
+    int width = differ ? 64 - __builtin_clzll(differ) : 0;  // the bits above are settled
+    while (width) {
+        const int shift = max(0, width - 8);
+        const uint64_t settled = width < 64 ? key >> width : 0;
+        sc.mass[tid] = 0;
+        sc.count[tid] = 0;
+        __syncthreads();
+        each([&](uint64_t k, uint64_t units) {
+            if ((width < 64 ? k >> width : 0) != settled) return;
+            const int d = int(k >> shift) & ((1 << (width - shift)) - 1);
+            atomicAdd(&sc.count[d], 1u);
+            atomicAdd(&sc.mass[d], (unsigned long long)units);
+        });
+        __syncthreads();
+        const int d = 255 - tid;
+        const uint32_t n = sc.count[d];
+        const uint64_t m = sc.mass[d];
+        uint32_t counts;
+        uint64_t masses;
+        const uint64_t n_before = scan256(n, sc.waves32, counts), m_before = scan256(m, sc.waves64, masses);
+        const uint64_t before = by_count ? n_before : m_before, here = by_count ? n : m;
+        if (before < need && before + here >= need) {
+            sc.digit = d;
+            sc.in_digit = n;
+            sc.need = need - before;
+            sc.before = m_before;
+        }
+        __syncthreads();
+        need = sc.need;
+        above += sc.before;
+        key = (settled << (width - shift) | uint64_t(sc.digit)) << shift;
+        if (sc.in_digit == 1 && shift) {  // one key left: find it
+            each([&](uint64_t k, uint64_t) {
+                if (k >> shift == key >> shift) sc.found = k;
+            });
+            __syncthreads();
+            key = sc.found;
+            break;
+        }
+        __syncthreads();
+        width = shift;
+    }
+    __syncthreads();
+    return key;
+}
+
+template <int DT> __global__ void __launch_bounds__(256) sample_pick(SampleArgs p) {
+    __shared__ PickScratch sc;
+    const int row = blockIdx.x, tid = threadIdx.x;
+    SampleRow& state = p.rows[row];
+    const Row r = read_row(p, state, row);
+    if (r.greedy || r.nothing) {
+        if (!tid) p.tokens[row] = r.nothing ? -1 : key_index(r.first);
+        return;
+    }
+    if (tid < p.splits) sc.kept[tid] = state.kept[tid];
+    uint64_t cut = 0;  // keys from it on stay
+    if (r.by_k || r.by_p) {
+        const Cut c = find_cut(r, state, sc.cut);
+        const uint32_t listed = state.listed;
+        const bool whole = listed <= uint32_t(SAMPLE_LIST);
+        if (whole)
+            for (int i = tid; i < int(listed); i += 256) {
+                const uint64_t key = state.list[i];
+                sc.list[i] = key;
+                sc.units[i] = r.units(r.weight(order_logit(uint32_t(key >> 32))));
+            }
+        __syncthreads();
+        // the listed keys of some of the bins; where they are too many for the list (logits that are alike), the row is read again instead
+        auto each = [&](int from, int to, const auto& f) {
+            if (whole) {
+                for (int i = tid; i < int(listed); i += 256) {
+                    const int b = r.bin(order_logit(uint32_t(sc.list[i] >> 32)));
+                    if (b >= from && b <= to) f(sc.list[i], sc.units[i]);
+                }
+            } else {
+                each_logit<DT>(p, row, 0, p.vocabulary, [&](float l, int i) {
+                    if (l != l) return;
+                    const int b = r.bin(l);
+                    if (b >= from && b <= to) f(token_key(l, i), r.units(r.weight(l)));
+                });
+            }
+        };
+        uint64_t total = 0, above;
+        if (c.k_bin < SAMPLE_BINS) {
+            cut = select_key(sc, [&](const auto& f) { each(c.k_bin, c.k_bin, f); }, true, c.k_left, above);
+            total = c.k_before + above + r.units(r.weight(order_logit(uint32_t(cut >> 32))));
+        } else if (r.by_p) {
+            uint64_t mass = 0;
+            for (int b = tid; b < SAMPLE_BINS; b += 256) mass += state.mass[b];
+            scan256(mass, sc.waves64, total);
+        }
+        if (r.by_p) cut = select_key(sc, [&](const auto& f) { each(c.low, c.high, f); }, false, wanted_mass(r.top_p, total) - c.low_before, above);
+        if (cut) {
+            const int from = c.certain, to = r.by_p ? c.high : c.k_bin;
+            each(from, to, [&](uint64_t key, uint64_t units) {
+                if (key >= cut && r.weight(order_logit(uint32_t(key >> 32))) >= r.min_p) atomicAdd(&sc.kept[key_index(key) / p.split], (unsigned long long)units);
+            });
+        }
+    }
+    __syncthreads();
+    // the part of the row in which the running weight passes the drawn one
+    uint64_t total = 0;
+    for (int s = 0; s < p.splits; ++s) total += sc.kept[s];
+    const float u = p.draws[row];
+    uint64_t target = u > 0.0f ? u < 1.0f ? share_of(u, total, false) : total - 1 : 0;
+    if (target >= total) target = total - 1;
+    int s = 0;
+    while (s < p.splits - 1 && target >= sc.kept[s]) target -= sc.kept[s++];
+    // in it, 8 neighbouring tokens a thread at a time
+    using raw = typename Elem<DT>::raw;
+    const raw* values = static_cast<const raw*>(p.logits) + row * p.ld;
+    const int end = min(p.vocabulary, (s + 1) * p.split);
+    for (int begin = s * p.split; begin < end; begin += 8 * 256) {
+        uint64_t units[8], mine = 0, piece;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int i = begin + 8 * tid + j;
+            const float l = Elem<DT>::to_f(values[min(i, end - 1)]);
+            const double w = i < end && l == l && token_key(l, i) >= cut ? r.weight(l) : 0.0;
+            units[j] = w >= r.min_p ? r.units(w) : 0;
+            mine += units[j];
+        }
+        uint64_t before = scan256(mine, sc.waves64, piece);
+        if (before <= target && target < before + mine) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (before <= target && target < before + units[j]) p.tokens[row] = begin + 8 * tid + j;
+                before += units[j];
+            }
+        }
+        if (target < piece) break;
+        target -= piece;
+    }
+}
+
+}  // namespace wq8
+
+using namespace wq8;
+
+template <int DT> static int launch_sample(const SampleArgs& p, int rows, hipStream_t stream) {
+    sample_largest<DT><<<rows * p.splits, 256, 0, stream>>>(p);
+    if (const int rc = int(hipGetLastError())) return rc;
+    sample_bins<DT><<<rows * p.splits, 256, 0, stream>>>(p);
+    if (const int rc = int(hipGetLastError())) return rc;
+    sample_list<DT><<<rows * p.splits, 256, 0, stream>>>(p);
+    if (const int rc = int(hipGetLastError())) return rc;
+    sample_pick<DT><<<rows, 256, 0, stream>>>(p);
+    return int(hipGetLastError());
+}
+
+WQ8_API int wq8_sample(const void* logits, int64_t ld, int dtype, const float* draws, const float* temperature, float temperature0, const void* top_k, int top_k0,
+                       const float* top_p, float top_p0, const float* min_p, float min_p0, int rows, int vocabulary, int64_t* tokens, void* workspace,
+                       hipStream_t stream) {
+    if (!rows) return 0;
+    if (dtype < 0 || dtype > 2) return -1;
+    if (rows < 0 || rows > (1 << 17) || vocabulary < 1 || vocabulary > (1 << 24)) return -2;
+    // parts of at least 2048 tokens, a thousand workgroups or so
+    const int pieces = (vocabulary + SAMPLE_PIECE - 1) / SAMPLE_PIECE;
+    int splits = (1023 + rows) / rows;
+    splits = splits < SAMPLE_SPLITS ? splits : SAMPLE_SPLITS;
+    splits = splits < pieces ? splits : pieces;
+    const int split = (pieces + splits - 1) / splits * SAMPLE_PIECE;
+    splits = (vocabulary + split - 1) / split;
+    int bits = 0;
+    while ((1 << bits) < vocabulary) ++bits;
+    const SampleArgs p{logits, ld, draws, temperature, static_cast<const int32_t*>(top_k), top_p, min_p, static_cast<SampleRow*>(workspace), tokens,
+                       temperature0, top_p0, min_p0, top_k0, vocabulary, split, splits, bits <= 18 ? 44 : 62 - bits};
+    if (dtype == DT_F16) return launch_sample<DT_F16>(p, rows, stream);
+    if (dtype == DT_BF16) return launch_sample<DT_BF16>(p, rows, stream);
+    return launch_sample<DT_F32>(p, rows, stream);
+}
+
+WQ8_API void wq8_sample_workspace(int rows, int64_t* sizes) {
+    sizes[0] = int64_t(rows) * int64_t(sizeof(SampleRow));
+    sizes[1] = 0;
+}
