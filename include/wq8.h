@@ -166,9 +166,12 @@ void wq8_kv_attention_workspace(int tokens, int requests, int heads, int group, 
 /* A mixture-of-experts layer, no counterpart in the reference. route: x (tokens, k) of dtype 0-2, rows ldx elements apart, router (experts, k)
  * of router_dtype 0-2, both 16-byte aligned, k % 8 == 0; scores of the FP64 products by softmax (score 0) or the logistic function (1);
  * ids (tokens, top): the largest of score + bias (f32, or null), ties by the lowest index, in order; weights: their scores, with normalise over
- * their sum, times factor. experts <= 1024, top <= 64; logits: tokens * experts FP64 of scratch. */
+ * their sum, times factor. experts <= 1024, top <= 64; logits: scratch of the bytes that the
+ * query gives (sizes[0]), 16-byte aligned. */
 int wq8_route(const void* x, int64_t ldx, int dtype, const void* router, int router_dtype, const float* bias, int tokens, int experts, int k, int top,
               int score, int normalise, float factor, void* logits, int32_t* ids, float* weights, wq8_stream_t stream);
+
+void wq8_route_workspace(int tokens, int experts, int k, int64_t* sizes);
 
 /* out (tokens, k) = residual + rscale * sum over a token's choices of weights * down(silu(gate) up): gate_up (experts, 2 hidden, k) int8 with
  * scales (experts, 2 hidden), gate rows first, down (experts, k, hidden) with scales (experts, k); x, residual, rscale (k values) and out of

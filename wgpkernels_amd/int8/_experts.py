@@ -45,7 +45,8 @@ def _check_route(x, router, top, score, bias):
     if x.shape[0] > 65535 * 16:
         raise ValueError("a route is of 2^20 - 16 tokens at most")
     _check_devices(*[t for t in (x, router, bias) if t is not None])
-    return x.shape[0], count, k, _row_pitch(x), DTYPES[x.dtype], DTYPES[router.dtype]
+    library().wq8_route_workspace(x.shape[0], count, k, _sizes)
+    return x.shape[0], count, k, _row_pitch(x), DTYPES[x.dtype], DTYPES[router.dtype], _sizes[0]
 
 
 def route(x, router, top, score="softmax", bias=None, normalise=True, factor=1.0):
@@ -56,13 +57,13 @@ def route(x, router, top, score="softmax", bias=None, normalise=True, factor=1.0
     chosen, ties by the lowest index, NaN last, and listed in that order. weights: the chosen scores, with normalise over their sum, times factor."""
     key = (x.shape, x.stride(), x.dtype, x.get_device(), router.shape, router.stride(), router.dtype, router.get_device(), top, score,
            None if bias is None else (bias.shape, bias.stride(), bias.dtype, bias.get_device()))
-    tokens, count, k, ldx, dtype, router_dtype = _route_layouts.get(key) or _route_layouts.keep(key, _check_route(x, router, top, score, bias))
+    tokens, count, k, ldx, dtype, router_dtype, workspace_bytes = _route_layouts.get(key) or _route_layouts.keep(key, _check_route(x, router, top, score, bias))
     x_at, router_at = x.data_ptr(), router.data_ptr()
     if (x_at | router_at) & 15:
         raise ValueError("rows of activations and router must be 16-byte aligned")
     ids = x.new_empty((tokens, top), dtype=torch.int32)
     weights = x.new_empty((tokens, top), dtype=torch.float32)
-    logits = x.new_empty(tokens * count, dtype=torch.float64)
+    logits = x.new_empty(workspace_bytes, dtype=torch.uint8)
     library().call("wq8_route", x_at, ldx, dtype, router_at, router_dtype, _native.ptr(bias), tokens, count, k, top, SCORES[score], normalise, factor,
                    logits.data_ptr(), ids.data_ptr(), weights.data_ptr(), _native.gpu(x).stream())
     return Routes(ids, weights)

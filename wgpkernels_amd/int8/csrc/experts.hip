@@ -19,34 +19,45 @@ struct RouteArgs {
     int32_t* ids;
     float* weights;
     int64_t ldx;
-    int tokens, experts, k, top, score, normalise;
+    int tokens, experts, k, top, score, normalise, parts, part;  // parts of `part` values of k
     float factor;
 };
 
-// 8 consecutive values as FP64; zeros when !valid.
-template <int DT> WQ8_DEVICE void load8d(const void* base, int64_t at, bool valid, double* v) {
-    float f[8];
-    load8<DT>(static_cast<const typename Elem<DT>::raw*>(base) + at, f, valid);
+// 8 consecutive values as they are in memory, one of them as FP64; zeros when !valid.
+template <int DT> struct Eight {
+    u32x4 held[DT == DT_F32 ? 2 : 1];
+    WQ8_DEVICE void load(const void* base, int64_t at, bool valid) {
+        const u32x4* from = reinterpret_cast<const u32x4*>(static_cast<const typename Elem<DT>::raw*>(base) + at);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = double(f[j]);
-}
+        for (int i = 0; i < (DT == DT_F32 ? 2 : 1); ++i) held[i] = valid ? from[i] : u32x4{0, 0, 0, 0};
+    }
+    WQ8_DEVICE double value(int j) const {
+        const uint32_t word = DT == DT_F32 ? held[j >> 2][j & 3] : held[0][j >> 1];  // (a bit cast takes a vector's element only by way of a number)
+        if constexpr (DT == DT_F32) return double(__builtin_bit_cast(float, word));
+        else return double(Elem<DT>::to_f(uint16_t(word >> (16 * (j & 1)))));
+    }
+};
 
-// Logits of 16 tokens x 16 experts in FP64 (the choice between near experts is a whole number: in FP32 one in some 10^4 tokens would go by the
-// order of the sum). 16 waves share K, 32 values of every row a step; their sums are added in order.
-constexpr int ROUTE_WAVES = 16;
+// Logits of 16 tokens x 16 experts over a part of K, in FP64 (the choice between near experts is a whole number: in FP32 one in some 10^4 tokens
+// would go by the order of the sum). 8 waves take 32 values of every row in turn; their sums are added in order, the parts by route_choose. Matrix
+// instructions of FP64 set the time (64 cycles for 4 values): parts short enough to fill the CUs.
+constexpr int ROUTE_WAVES = 8, ROUTE_STEP = 32 * ROUTE_WAVES;
 template <int XT, int RT>
 __global__ void __launch_bounds__(64 * ROUTE_WAVES) route_logits(RouteArgs p) {
     __shared__ double sums[ROUTE_WAVES][4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int expert = blockIdx.x * 16 + (lane & 15), token = blockIdx.y * 16 + (lane & 15);
+    // (the wave's number in a scalar: matrix instructions do not heed the lanes' mask, so no branch around them may go by one)
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int expert = blockIdx.x * 16 + (lane & 15), token = blockIdx.y * 16 + (lane & 15), end = min(p.k, int(blockIdx.z + 1) * p.part);
     const bool has_expert = expert < p.experts, has_token = token < p.tokens;
     v4d acc = {0, 0, 0, 0};
-    for (int k = 8 * (lane >> 4) + 32 * wave; k - 8 * (lane >> 4) < p.k; k += 32 * ROUTE_WAVES) {
-        double a[8], b[8];
-        load8d<XT>(p.x, token * p.ldx + k, has_token && k < p.k, a);
-        load8d<RT>(p.router, int64_t(expert) * p.k + k, has_expert && k < p.k, b);
+    for (int begin = blockIdx.z * p.part + 32 * wave; begin < end; begin += ROUTE_STEP) {
+        const int k = begin + 8 * (lane >> 4);
+        Eight<XT> a;
+        Eight<RT> b;
+        a.load(p.x, token * p.ldx + k, has_token && k < p.k);
+        b.load(p.router, int64_t(expert) * p.k + k, has_expert && k < p.k);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(a[j], b[j], acc, 0, 0, 0);
+        for (int j = 0; j < 8; ++j) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(a.value(j), b.value(j), acc, 0, 0, 0);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) sums[wave][i][lane] = acc[i];
@@ -58,7 +69,7 @@ __global__ void __launch_bounds__(64 * ROUTE_WAVES) route_logits(RouteArgs p) {
     for (int w = 0; w < ROUTE_WAVES; ++w) total += sums[w][i][lane];
     // element i of lane l is token 4 i + l / 16, expert l % 16
     const int t = blockIdx.y * 16 + 4 * i + (lane >> 4);
-    if (has_expert && t < p.tokens) p.logits[int64_t(t) * p.experts + expert] = total;
+    if (has_expert && t < p.tokens) p.logits[(int64_t(blockIdx.z) * p.tokens + t) * p.experts + expert] = total;
 }
 
 // A double's order as an unsigned number above 1; 1 for NaN.
@@ -66,18 +77,35 @@ WQ8_DEVICE uint64_t order_of(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
     return v != v ? 1 : b >> 63 ? ~b : b | (uint64_t(1) << 63);
 }
-WQ8_DEVICE uint64_t wave_max64(uint64_t v) {
-#pragma unroll
-    for (int step = 32; step; step >>= 1) {
-        const uint64_t other = __shfl_xor(v, step);
-        v = other > v ? other : v;
-    }
+// f(v, the value of another lane) until every lane has all 64: across the lanes of a row of 16 by DPP, then rows and halves by exchanges
+template <int CTRL> WQ8_DEVICE uint64_t dpp64(uint64_t v) {
+    return uint64_t(dpp_u<CTRL>(uint32_t(v >> 32))) << 32 | dpp_u<CTRL>(uint32_t(v));
+}
+template <typename F> WQ8_DEVICE uint64_t over_wave(uint64_t v, const F& f) {
+    v = f(v, dpp64<0xB1>(v));   // quad_perm [1,0,3,2]
+    v = f(v, dpp64<0x4E>(v));   // quad_perm [2,3,0,1]
+    v = f(v, dpp64<0x141>(v));  // row_half_mirror
+    v = f(v, dpp64<0x140>(v));  // row_mirror
+    auto exchange = [&](auto swap) {
+        const auto low = swap(uint32_t(v)), high = swap(uint32_t(v >> 32));
+        v = f(uint64_t(uint32_t(high[0])) << 32 | uint32_t(low[0]), uint64_t(uint32_t(high[1])) << 32 | uint32_t(low[1]));
+    };
+    exchange([](uint32_t u) { return __builtin_amdgcn_permlane16_swap(u, u, false, false); });
+    exchange([](uint32_t u) { return __builtin_amdgcn_permlane32_swap(u, u, false, false); });
     return v;
 }
+WQ8_DEVICE uint64_t wave_max64(uint64_t v) {
+    return over_wave(v, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+}
 WQ8_DEVICE double wave_sum64(double v) {
-#pragma unroll
-    for (int step = 32; step; step >>= 1) v += __shfl_xor(v, step);
-    return v;
+    return __builtin_bit_cast(double, over_wave(__builtin_bit_cast(uint64_t, v), [](uint64_t a, uint64_t b) {
+        return __builtin_bit_cast(uint64_t, __builtin_bit_cast(double, a) + __builtin_bit_cast(double, b));
+    }));
+}
+WQ8_DEVICE double lane_value(double v, int lane) {  // lane the same for all
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, uint64_t(uint32_t(__builtin_amdgcn_readlane(int(b >> 32), lane))) << 32 |
+                                          uint32_t(__builtin_amdgcn_readlane(int(uint32_t(b)), lane)));
 }
 
 // Scores, choice and weights of a token a wave; a lane holds NE neighbouring experts.
@@ -93,11 +121,29 @@ __global__ void __launch_bounds__(256) route_choose(RouteArgs p) {
     for (int i = 0; i < NE; ++i) {
         const int e = lane * NE + i;
         score[i] = e < p.experts ? logits[e] : -__builtin_inf();
+    }
+    constexpr int TOGETHER = NE <= 4 ? 8 : 2;  // parts whose loads are asked for at once
+    for (int first = 1; first < p.parts; first += TOGETHER) {
+        double more[TOGETHER][NE];
+#pragma unroll
+        for (int s = 0; s < TOGETHER; ++s)
+#pragma unroll
+            for (int i = 0; i < NE; ++i)
+                more[s][i] = logits[int64_t(min(first + s, p.parts - 1)) * p.tokens * p.experts + min(lane * NE + i, p.experts - 1)];
+#pragma unroll
+        for (int s = 0; s < TOGETHER; ++s)
+#pragma unroll
+            for (int i = 0; i < NE; ++i)
+                if (first + s < p.parts) score[i] += more[s][i];
+    }
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
         top = __builtin_fmax(top, score[i]);
     }
     if (p.score == 0) {
-#pragma unroll
-        for (int step = 32; step; step >>= 1) top = __builtin_fmax(top, __shfl_xor(top, step));
+        top = __builtin_bit_cast(double, over_wave(__builtin_bit_cast(uint64_t, top), [](uint64_t a, uint64_t b) {
+            return __builtin_bit_cast(uint64_t, __builtin_fmax(__builtin_bit_cast(double, a), __builtin_bit_cast(double, b)));
+        }));
         double sum = 0.0;
 #pragma unroll
         for (int i = 0; i < NE; ++i) {
@@ -123,7 +169,7 @@ __global__ void __launch_bounds__(256) route_choose(RouteArgs p) {
 #pragma unroll
         for (int i = 0; i < NE; ++i) best = wanted[i] > best ? wanted[i] : best;
         const uint64_t most = wave_max64(best);
-        const int from = __builtin_ctzll(__ballot(best == most));  // neighbouring experts a lane: the lowest lane has the lowest index
+        const int from = __builtin_amdgcn_readfirstlane(__builtin_ctzll(__ballot(best == most)));  // neighbouring experts a lane: the lowest lane has the lowest index
         double value = 0.0;
         int e = 0;
         if (lane == from) {
@@ -137,8 +183,8 @@ __global__ void __launch_bounds__(256) route_choose(RouteArgs p) {
                     wanted[i] = 0;
                 }
         }
-        value = __shfl(value, from);
-        e = __shfl(e, from);
+        value = lane_value(value, from);
+        e = __builtin_amdgcn_readlane(e, from);
         total += value;
         if (lane == j) {
             mine = value;
@@ -169,7 +215,7 @@ struct ExpertsArgs {
     int64_t ldx, ldr, ldo;
     int tokens, top, experts, k, hidden;
 };
-constexpr int MOST_PAIRS = 4096;
+constexpr int MOST_PAIRS = 4096, MOST_ONE = 64;  // choices of a call; of a token whose second product is experts_down_one
 
 template <int DT> struct ExpertOp;
 template <> struct ExpertOp<DT_BF16> {
@@ -197,20 +243,42 @@ template <int DT> WQ8_DEVICE typename ExpertOp<DT>::frag codes8(uint32_t lo, uin
 // one of an expert serves all of them; else it is an expert.
 WQ8_DEVICE bool slot_is_choice(const ExpertsArgs& p) { return p.tokens * p.top <= p.experts; }
 WQ8_DEVICE int slot_expert(const ExpertsArgs& p, int slot) { return slot_is_choice(p) ? p.ids[slot] : slot; }
-// Their number (0: another slot has them), and those from `first` on, up to MOST_LISTED, in LDS; every wave counts, the first one writes.
+// Their number (0: another slot has them), and those from `first` on, up to MOST_LISTED, in LDS; every wave counts, the first one writes. A lane
+// looks at 4 neighbouring choices at a time.
 constexpr int MOST_LISTED = 64;
 WQ8_DEVICE int find_choices(const ExpertsArgs& p, int slot, int expert, int first, uint16_t* list) {
     const int pairs = p.tokens * p.top, lane = threadIdx.x & 63;
     const bool by_choice = slot_is_choice(p);
+    const uint64_t lower = (uint64_t(1) << lane) - 1;
     int count = 0;
-    for (int base = 0; base < pairs; base += 64) {
-        const bool mine = base + lane < pairs && p.ids[base + lane] == expert;
-        const uint64_t mask = __ballot(mine);
-        if (!mask) continue;
-        if (by_choice && !count && base + __builtin_ctzll(mask) != slot) return 0;
-        const int at = count + __popcll(mask & ((uint64_t(1) << lane) - 1)) - first;
-        if (threadIdx.x < 64 && mine && at >= 0 && at < MOST_LISTED) list[at] = uint16_t(base + lane);
-        count += __popcll(mask);
+    for (int base = 0; base < pairs; base += 256) {
+        const int at = base + 4 * lane;
+        int id[4];
+        if (at + 4 <= pairs) __builtin_memcpy(id, p.ids + at, 16);
+        else
+#pragma unroll
+            for (int j = 0; j < 4; ++j) id[j] = at + j < pairs ? p.ids[at + j] : -1;  // (no expert is -1)
+        uint64_t mask[4];
+        int before = 0, here = 0, earliest = 1 << 30;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            mask[j] = __ballot(id[j] == expert);
+            before += __popcll(mask[j] & lower);
+            here += __popcll(mask[j]);
+            if (mask[j]) earliest = min(earliest, 4 * __builtin_ctzll(mask[j]) + j);
+        }
+        if (!here) continue;
+        if (by_choice && !count && base + earliest != slot) return 0;
+        if (threadIdx.x < 64) {
+            int place = count + before - first;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (id[j] == expert) {
+                    if (place >= 0 && place < MOST_LISTED) list[place] = uint16_t(at + j);
+                    ++place;
+                }
+        }
+        count += here;
     }
     return count;
 }
@@ -221,11 +289,11 @@ WQ8_DEVICE int find_choices(const ExpertsArgs& p, int slot, int expert, int firs
 // 16 rows meet different banks.
 constexpr int RING = 19 * 1024;  // a wave's: two workgroups a CU
 constexpr uint32_t OUT_OF_RANGE = 0x80000000u;
-template <int DT, int SLICE, int CAP, int PLANES, typename Source, typename Store>
-WQ8_DEVICE void ring_rows(sgpr4 rw, int row0, int row1, int rows, int width, sgpr4 rx, uint32_t plane_bytes, int count, uint8_t* rings, const Source& source,
-                          const Store& store) {
+template <int DT, int SLICE, int CAP, int PLANES, typename Source, typename Done>
+WQ8_DEVICE void ring_rows(sgpr4 rw, int row0, int row1, int width, sgpr4 rx, uint32_t plane_bytes, int count, uint8_t* rings, const Source& source,
+                          const Done& done) {
     constexpr int W_BYTES = 32 * SLICE, X_BYTES = CAP * PLANES * SLICE * 2, STAGE = W_BYTES + X_BYTES, STAGES = RING / STAGE < 8 ? RING / STAGE : 8;
-    constexpr int W_COPIES = W_BYTES / 1024, X_COPIES = X_BYTES / 1024, COPIES = W_COPIES + X_COPIES, MT = (CAP + 15) / 16;
+    constexpr int W_COPIES = W_BYTES / 1024, X_COPIES = X_BYTES / 1024, COPIES = W_COPIES + X_COPIES;
     constexpr int W_CHUNKS = SLICE / 16, X_CHUNKS = SLICE / 8;  // of a row in a stage
     static_assert(STAGES >= 2 && X_BYTES % 1024 == 0 && (STAGES - 1) * COPIES < 64, "a ring of stages of whole copies");
     using frag = typename ExpertOp<DT>::frag;
@@ -239,7 +307,7 @@ WQ8_DEVICE void ring_rows(sgpr4 rw, int row0, int row1, int rows, int width, sgp
     for (int j = 0; j < W_COPIES; ++j) {
         const int r = j * (64 / W_CHUNKS) + lane / W_CHUNKS, chunk = lane % W_CHUNKS ^ w_turn(r);
         w_k[j] = 16 * chunk;
-        w_from[j] = uint32_t(min(r < 16 ? row0 + r : row1 + r - 16, rows - 1)) * uint32_t(width) + 16u * chunk;
+        w_from[j] = uint32_t(r < 16 ? row0 + r : row1 + r - 16) * uint32_t(width) + 16u * chunk;  // rows past the matrix read zeros
     }
 #pragma unroll
     for (int j = 0; j < X_COPIES; ++j) {
@@ -254,9 +322,7 @@ WQ8_DEVICE void ring_rows(sgpr4 rw, int row0, int row1, int rows, int width, sgp
 #pragma unroll
         for (int j = 0; j < X_COPIES; ++j) bdma16(rx, k0 + x_k[j] < width ? x_from[j] + 2u * uint32_t(k0) : OUT_OF_RANGE, stage + W_BYTES + 1024 * j);
     };
-    v4f a0[MT], a1[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) a0[m] = a1[m] = v4f{0, 0, 0, 0};
+    v4f a0 = {0, 0, 0, 0}, a1 = {0, 0, 0, 0};
     const int slices = (width + SLICE - 1) / SLICE, mine = (slices - wave + 3) / 4;
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) issue(i, ring + i * STAGE);
@@ -280,140 +346,47 @@ WQ8_DEVICE void ring_rows(sgpr4 rw, int row0, int row1, int rows, int width, sgp
             for (int e = 0; e < 2; ++e) {
                 const frag f0 = codes8<DT>(c0[2 * e], c0[2 * e + 1]), f1 = codes8<DT>(c1[2 * e], c1[2 * e + 1]);
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int q = 0; q < PLANES; ++q) {
-                        const int t = q * CAP + (CAP < 16 ? r16 & (CAP - 1) : 16 * m + r16);
-                        const frag x = *reinterpret_cast<const frag*>(xs + t * 2 * SLICE + 16 * ((8 * h + 2 * sub + e) ^ x_turn(t)));
-                        a0[m] = ExpertOp<DT>::run(f0, x, a0[m]);
-                        a1[m] = ExpertOp<DT>::run(f1, x, a1[m]);
-                    }
+                for (int q = 0; q < PLANES; ++q) {
+                    const int t = q * CAP + (r16 & (CAP - 1));
+                    const frag x = *reinterpret_cast<const frag*>(xs + t * 2 * SLICE + 16 * ((8 * h + 2 * sub + e) ^ x_turn(t)));
+                    a0 = ExpertOp<DT>::run(f0, x, a0);
+                    a1 = ExpertOp<DT>::run(f1, x, a1);
+                }
             }
         }
     }
     wait_vmcnt<0>();
-    float (&red)[4][8][64] = *reinterpret_cast<float (*)[4][8][64]>(rings);
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            red[wave][i][lane] = a0[m][i];
-            red[wave][4 + i][lane] = a1[m][i];
-        }
-        __syncthreads();
-        // element i of lane l is row 4 (l / 16) + i, token l % 16
-        const int r = threadIdx.x & 15, t = threadIdx.x >> 4, l = 16 * (r >> 2) + t, i = r & 3;
-        if (t < CAP && 16 * m + t < count)
-            store(16 * m + t, r, ((red[0][i][l] + red[1][i][l]) + red[2][i][l]) + red[3][i][l],
-                  ((red[0][4 + i][l] + red[1][4 + i][l]) + red[2][4 + i][l]) + red[3][4 + i][l]);
-    }
+    __syncthreads();
+    v4f* red = reinterpret_cast<v4f*>(rings) + lane;  // of waves 1 to 3, two tiles each
+    if (wave) red[(wave - 1) * 128] = a0, red[(wave - 1) * 128 + 64] = a1;
+    __syncthreads();
+    if (!wave) done(((a0 + red[0]) + red[128]) + red[256], ((a1 + red[64]) + red[192]) + red[320]);
 }
 
-// The same tiles, every wave with tiles of its own over the whole width: `blocks` of them one after another, `step` rows apart, without a pause in the copies
-// between them. A workgroup of tiles this small would mostly begin and end. done(block, row's values of both tiles): element i is row
-// 4 (lane / 16) + i, token lane % 16.
-template <int DT, int SLICE, int CAP, int PLANES, typename Source, typename Done>
-WQ8_DEVICE void ring_blocks(sgpr4 rw, int row0, int row1, int step, int blocks, int width, sgpr4 rx, uint32_t plane_bytes, int count, uint8_t* rings,
-                            const Source& source, const Done& done) {
-    constexpr int W_BYTES = 32 * SLICE, X_BYTES = CAP * PLANES * SLICE * 2, STAGE = W_BYTES + X_BYTES, STAGES = RING / STAGE < 8 ? RING / STAGE : 8;
-    constexpr int W_COPIES = W_BYTES / 1024, X_COPIES = X_BYTES / 1024, COPIES = W_COPIES + X_COPIES;
-    constexpr int W_CHUNKS = SLICE / 16, X_CHUNKS = SLICE / 8;
-    static_assert(STAGES >= 3 && X_BYTES % 1024 == 0 && (STAGES - 1) * COPIES < 64 && CAP <= 16, "a ring of stages of whole copies");
+// More tokens: 128 rows a workgroup, two runs of 64 of which each wave has a tile of 16, and the tokens' slices in LDS once for all of them.
+// done(m, values of both tiles): element i is row 16 wave + 4 (lane / 16) + i of each run, token 16 m + lane % 16.
+template <int DT, int SLICE, int MT, int PLANES, typename Source, typename Done>
+WQ8_DEVICE void shared_rows(sgpr4 rw, int row0, int row1, int width, sgpr4 rx, uint32_t plane_bytes, int count, uint8_t* ring, const Source& source,
+                            const Done& done) {
+    constexpr int CAP = 16 * MT, W_BYTES = 128 * SLICE, X_BYTES = CAP * PLANES * SLICE * 2, STAGE = W_BYTES + X_BYTES;
+    constexpr int W_CHUNKS = SLICE / 16, X_CHUNKS = SLICE / 8, W_COPIES = W_BYTES / 4096, X_ALL = X_BYTES / 1024, X_COPIES = (X_ALL + 3) / 4;
+    constexpr int STAGES = 4 * RING / STAGE < 8 ? 4 * RING / STAGE : 8, COPIES = W_COPIES + X_COPIES;
+    static_assert(STAGES >= 3 && (STAGES - 1) * COPIES < 64, "a ring of stages");
     using frag = typename ExpertOp<DT>::frag;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, sub = lane >> 4;
-    uint8_t* ring = rings + wave * RING;
     auto w_turn = [](int r) { return SLICE == 128 ? r >> 1 & 7 : r >> 2 & 3; };
     auto x_turn = [](int q) { return SLICE == 128 ? q & 15 : q >> 1 & 7; };
     uint32_t w_from[W_COPIES], x_from[X_COPIES];
     int w_k[W_COPIES], x_k[X_COPIES];
 #pragma unroll
     for (int j = 0; j < W_COPIES; ++j) {
-        const int r = j * (64 / W_CHUNKS) + lane / W_CHUNKS, chunk = lane % W_CHUNKS ^ w_turn(r);
+        const int r = (wave + 4 * j) * (64 / W_CHUNKS) + lane / W_CHUNKS, chunk = lane % W_CHUNKS ^ w_turn(r);
         w_k[j] = 16 * chunk;
-        w_from[j] = uint32_t(r < 16 ? row0 + r : row1 + r - 16) * uint32_t(width) + 16u * chunk;  // rows past the matrix read zeros
+        w_from[j] = uint32_t(r < 64 ? row0 + r : row1 + r - 64) * uint32_t(width) + 16u * chunk;  // rows past the matrix read zeros
     }
 #pragma unroll
     for (int j = 0; j < X_COPIES; ++j) {
-        const int q = j * (64 / X_CHUNKS) + lane / X_CHUNKS, chunk = lane % X_CHUNKS ^ x_turn(q);
-        x_k[j] = 8 * chunk;
-        x_from[j] = source(min(q % CAP, count - 1)) + (PLANES > 1 && q >= CAP ? plane_bytes : 0u) + 16u * chunk;
-    }
-    int next_k = 0, to_issue = blocks;
-    uint32_t next_rows = 0;
-    auto issue = [&](uint8_t* stage) {
-        const int end = to_issue > 0 ? width : 0;
-#pragma unroll
-        for (int j = 0; j < W_COPIES; ++j) bdma16_nt(rw, next_k + w_k[j] < end ? w_from[j] + next_rows + uint32_t(next_k) : OUT_OF_RANGE, stage + 1024 * j);
-#pragma unroll
-        for (int j = 0; j < X_COPIES; ++j) bdma16(rx, next_k + x_k[j] < end ? x_from[j] + 2u * uint32_t(next_k) : OUT_OF_RANGE, stage + W_BYTES + 1024 * j);
-        next_k += SLICE;
-        if (next_k >= width) {
-            next_k = 0;
-            next_rows += uint32_t(step) * uint32_t(width);
-            --to_issue;
-        }
-    };
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) issue(ring + i * STAGE);
-    int at = 0, free = STAGES - 1;
-    for (int block = 0; block < blocks; ++block) {
-        v4f a0 = {0, 0, 0, 0}, a1 = {0, 0, 0, 0};
-        for (int k = 0; k < width; k += SLICE) {
-            wait_vmcnt<(STAGES - 2) * COPIES>();
-            wait_lgkm0();
-            asm volatile("" ::: "memory");
-            issue(ring + free * STAGE);
-            const uint8_t* ws = ring + at * STAGE;
-            const uint8_t* xs = ws + W_BYTES;
-            free = at;
-            at = at + 1 == STAGES ? 0 : at + 1;
-#pragma unroll
-            for (int h = 0; h < SLICE / 64; ++h) {
-                const int chunk = (4 * h + sub) ^ w_turn(r16);
-                const u32x4 c0 = *reinterpret_cast<const u32x4*>(ws + r16 * SLICE + 16 * chunk);
-                const u32x4 c1 = *reinterpret_cast<const u32x4*>(ws + (16 + r16) * SLICE + 16 * chunk);
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const frag f0 = codes8<DT>(c0[2 * e], c0[2 * e + 1]), f1 = codes8<DT>(c1[2 * e], c1[2 * e + 1]);
-#pragma unroll
-                    for (int q = 0; q < PLANES; ++q) {
-                        const int t = q * CAP + (r16 & (CAP - 1));
-                        const frag x = *reinterpret_cast<const frag*>(xs + t * 2 * SLICE + 16 * ((8 * h + 2 * sub + e) ^ x_turn(t)));
-                        a0 = ExpertOp<DT>::run(f0, x, a0);
-                        a1 = ExpertOp<DT>::run(f1, x, a1);
-                    }
-                }
-            }
-        }
-        done(block, a0, a1);
-    }
-    wait_vmcnt<0>();
-}
-
-// More tokens: 64 rows a workgroup (tile c of each of two runs of 32 rows, c = 0 and 1, for waves c and c + 2, which take alternate halves of a
-// slice), and the tokens' slices in LDS once for all of them. done(m, c, both tiles' values) of waves 0 and 1: element i is row 16 c + 4 (lane / 16) + i of each
-// run, token 16 m + lane % 16.
-template <int DT, int MT, int PLANES, typename Source, typename Done>
-WQ8_DEVICE void shared_rows(sgpr4 rw, int row0, int row1, int width, sgpr4 rx, uint32_t plane_bytes, int count, uint8_t* ring, const Source& source,
-                            const Done& done) {
-    constexpr int SLICE = 128, CAP = 16 * MT, W_BYTES = 64 * SLICE, X_BYTES = CAP * PLANES * SLICE * 2, STAGE = W_BYTES + X_BYTES;
-    constexpr int STAGES = 4 * RING / STAGE < 8 ? 4 * RING / STAGE : 8, W_COPIES = W_BYTES / 4096, X_COPIES = X_BYTES / 4096, COPIES = W_COPIES + X_COPIES;
-    static_assert(STAGES >= 3 && (STAGES - 1) * COPIES < 64, "a ring of stages");
-    using frag = typename ExpertOp<DT>::frag;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, sub = lane >> 4;
-    const int c = wave & 1, half = wave >> 1;
-    uint32_t w_from[W_COPIES], x_from[X_COPIES];
-    int w_k[W_COPIES], x_k[X_COPIES];
-#pragma unroll
-    for (int j = 0; j < W_COPIES; ++j) {
-        const int r = (wave + 4 * j) * 8 + lane / 8, chunk = lane % 8 ^ (r >> 1 & 7);  // LDS row r: run r / 32, row r % 32 of it
-        w_k[j] = 16 * chunk;
-        w_from[j] = uint32_t(r < 32 ? row0 + r : row1 + r - 32) * uint32_t(width) + 16u * chunk;
-    }
-#pragma unroll
-    for (int j = 0; j < X_COPIES; ++j) {
-        const int q = (wave + 4 * j) * 4 + lane / 16, chunk = lane % 16 ^ (q & 15);
+        const int q = (wave + 4 * j) % X_ALL * (64 / X_CHUNKS) + lane / X_CHUNKS, chunk = lane % X_CHUNKS ^ x_turn(q);  // (of two copies, two waves bring each)
         x_k[j] = 8 * chunk;
         x_from[j] = source(min(q % CAP, count - 1)) + (PLANES > 1 && q >= CAP ? plane_bytes : 0u) + 16u * chunk;
     }
@@ -423,7 +396,7 @@ WQ8_DEVICE void shared_rows(sgpr4 rw, int row0, int row1, int width, sgpr4 rx, u
             bdma16_nt(rw, k0 + w_k[j] < width ? w_from[j] + uint32_t(k0) : OUT_OF_RANGE, stage + 1024 * (wave + 4 * j));
 #pragma unroll
         for (int j = 0; j < X_COPIES; ++j)
-            bdma16(rx, k0 + x_k[j] < width ? x_from[j] + 2u * uint32_t(k0) : OUT_OF_RANGE, stage + W_BYTES + 1024 * (wave + 4 * j));
+            bdma16(rx, k0 + x_k[j] < width ? x_from[j] + 2u * uint32_t(k0) : OUT_OF_RANGE, stage + W_BYTES + 1024 * ((wave + 4 * j) % X_ALL));
     };
     v4f a0[MT], a1[MT];
 #pragma unroll
@@ -431,6 +404,7 @@ WQ8_DEVICE void shared_rows(sgpr4 rw, int row0, int row1, int width, sgpr4 rx, u
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) issue(i * SLICE, ring + i * STAGE);
     int at = 0, free = STAGES - 1;
+    const int r = 16 * wave + r16;
     for (int k = 0; k < width; k += SLICE) {
         wait_vmcnt<(STAGES - 2) * COPIES>();  // this wave's copies of the slice have landed
         wait_lgkm0();                         // and its reads of the last one are done
@@ -441,37 +415,28 @@ WQ8_DEVICE void shared_rows(sgpr4 rw, int row0, int row1, int width, sgpr4 rx, u
         const uint8_t* xs = ws + W_BYTES;
         free = at;
         at = at + 1 == STAGES ? 0 : at + 1;
-        const int r = 16 * c + r16, chunk = (4 * half + sub) ^ (r >> 1 & 7);
-        const u32x4 c0 = *reinterpret_cast<const u32x4*>(ws + r * SLICE + 16 * chunk);
-        const u32x4 c1 = *reinterpret_cast<const u32x4*>(ws + (32 + r) * SLICE + 16 * chunk);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const frag f0 = codes8<DT>(c0[2 * e], c0[2 * e + 1]), f1 = codes8<DT>(c1[2 * e], c1[2 * e + 1]);
+        for (int h = 0; h < SLICE / 64; ++h) {
+            const int w_at = r * SLICE + 16 * ((4 * h + sub) ^ w_turn(r));
+            const u32x4 c0 = *reinterpret_cast<const u32x4*>(ws + w_at), c1 = *reinterpret_cast<const u32x4*>(ws + 64 * SLICE + w_at);
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+            for (int e = 0; e < 2; ++e) {
+                const frag f0 = codes8<DT>(c0[2 * e], c0[2 * e + 1]), f1 = codes8<DT>(c1[2 * e], c1[2 * e + 1]);
 #pragma unroll
-                for (int q = 0; q < PLANES; ++q) {
-                    const int t = q * CAP + 16 * m + r16;
-                    const frag x = *reinterpret_cast<const frag*>(xs + t * 2 * SLICE + 16 * ((8 * half + 2 * sub + e) ^ r16));
-                    a0[m] = ExpertOp<DT>::run(f0, x, a0[m]);
-                    a1[m] = ExpertOp<DT>::run(f1, x, a1[m]);
-                }
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int q = 0; q < PLANES; ++q) {
+                        const int t = q * CAP + 16 * m + r16;
+                        const frag x = *reinterpret_cast<const frag*>(xs + t * 2 * SLICE + 16 * ((8 * h + 2 * sub + e) ^ x_turn(r16)));
+                        a0[m] = ExpertOp<DT>::run(f0, x, a0[m]);
+                        a1[m] = ExpertOp<DT>::run(f1, x, a1[m]);
+                    }
+            }
         }
     }
     wait_vmcnt<0>();
-    __syncthreads();
-    // the second waves hand their sums over
-    v4f* red = reinterpret_cast<v4f*>(ring) + c * MT * 2 * 64 + lane;
-    if (half)
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            red[m * 128] = a0[m];
-            red[m * 128 + 64] = a1[m];
-        }
-    __syncthreads();
-    if (half) return;
-#pragma unroll
-    for (int m = 0; m < MT; ++m) done(m, c, a0[m] + red[m * 128], a1[m] + red[m * 128 + 64]);
+    for (int m = 0; m < MT; ++m) done(m, a0[m], a1[m]);
 }
 
 // Hidden values are held as the sum of two BF16: FP16 would overflow where FP32 does not, and one rounding to 16 bits would add as much again to
@@ -482,139 +447,111 @@ WQ8_DEVICE void split_hidden(float h, uint32_t& hi, uint32_t& lo) {
     lo = __builtin_isfinite(back) ? Elem<DT_BF16>::from_f(h - back) : 0u;
 }
 
-constexpr int MOST_BLOCKS = 4;  // tiles a wave, one after another
+// 4 neighbouring scales, from `rows` on zeros (a multiple of 4)
+WQ8_DEVICE v4f scales4(const float* scale, int at, int rows) {
+    v4f v = {0, 0, 0, 0};
+    if (at < rows) __builtin_memcpy(&v, scale + at, 16);
+    return v;
+}
 
-// gate and up of hidden channels of an expert, and their product: 16 channels a workgroup (own 0), or 64 `own` of them.
+// gate and up of hidden channels of an expert, and their product: 16 channels a workgroup, whose waves share them (!own), or 64. Workgroups of
+// `pass` n take the choices from 64 n (8 n) on, then those `passes` further.
 template <int DT>
-__global__ void __launch_bounds__(256, 2) experts_up(ExpertsArgs p, int own) {
+__global__ void __launch_bounds__(256, 2) experts_up(ExpertsArgs p, int own, int passes) {
     __shared__ __attribute__((aligned(1024))) uint8_t rings[4 * RING];
-    __shared__ float scales[2][64 * MOST_BLOCKS];
     __shared__ uint16_t list[MOST_LISTED];
-    const int channels = own ? 64 * own : 16, groups = (p.hidden + channels - 1) / channels;
-    const int slot = blockIdx.x / groups, f0 = (blockIdx.x % groups) * channels, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int expert = slot_expert(p, slot), here = min(channels, p.hidden - f0);
+    const int channels = own ? 64 : 16, groups = (p.hidden + channels - 1) / channels;
+    const int tiles = gridDim.x / passes, tile = blockIdx.x % tiles, pass = blockIdx.x / tiles;
+    const int slot = tile / groups, f0 = tile % groups * channels, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int expert = slot_expert(p, slot);
     if (uint32_t(expert) >= uint32_t(p.experts)) return;
-    const float* scale = p.gate_up_scale + int64_t(expert) * 2 * p.hidden + f0;
+    const float* scale = p.gate_up_scale + int64_t(expert) * 2 * p.hidden;
     const int64_t plane = int64_t(p.tokens) * p.top * p.hidden;
     const sgpr4 rw = buffer_rsrc(p.gate_up + int64_t(expert) * 2 * p.hidden * p.k, uint32_t(2 * p.hidden) * uint32_t(p.k));
     const sgpr4 rx = buffer_rsrc(p.x, uint32_t((p.tokens - 1) * p.ldx + p.k) * 2u);
     auto source = [&](int i) { return uint32_t(list[i] / p.top) * uint32_t(p.ldx) * 2u; };
-    // channels f0 + f .. + 3 of choice i
-    auto store4 = [&](int i, int f, v4f gate, v4f up) {
+    const int f = f0 + (own ? 16 * wave : 0) + 4 * (lane >> 4);  // the channels of this lane's sums
+    const v4f gate_scale = scales4(scale, f, p.hidden), up_scale = scales4(scale + p.hidden, f, p.hidden);
+    auto store4 = [&](int i, v4f gate, v4f up) {
         u32x2 hi, lo;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             uint32_t h0, l0, h1, l1;
-            split_hidden(wq_swiglu(gate[2 * j] * scales[0][f + 2 * j], up[2 * j] * scales[1][f + 2 * j]), h0, l0);
-            split_hidden(wq_swiglu(gate[2 * j + 1] * scales[0][f + 2 * j + 1], up[2 * j + 1] * scales[1][f + 2 * j + 1]), h1, l1);
+            split_hidden(wq_swiglu(gate[2 * j] * gate_scale[2 * j], up[2 * j] * up_scale[2 * j]), h0, l0);
+            split_hidden(wq_swiglu(gate[2 * j + 1] * gate_scale[2 * j + 1], up[2 * j + 1] * up_scale[2 * j + 1]), h1, l1);
             hi[j] = h0 | h1 << 16;
             lo[j] = l0 | l1 << 16;
         }
-        uint16_t* to = p.h + int64_t(list[i]) * p.hidden + f0 + f;
+        uint16_t* to = p.h + int64_t(list[i]) * p.hidden + f;
         *reinterpret_cast<u32x2*>(to) = hi;
         *reinterpret_cast<u32x2*>(to + plane) = lo;
     };
-    for (int f = threadIdx.x; f < here; f += 256) scales[0][f] = scale[f], scales[1][f] = scale[p.hidden + f];
-    const int lane = threadIdx.x & 63;
     const int most = own ? 64 : 8;
-    for (int first = 0;; first += most) {
+    for (int first = pass * most;; first += passes * most) {
         const int rest = find_choices(p, slot, expert, first, list) - first, left = min(rest, most);
         if (left <= 0) return;
         __syncthreads();
+        auto done = [&](v4f gate, v4f up) {
+            if ((lane & 15) < left && f < p.hidden) store4(lane & 15, gate, up);
+        };
         if (!own) {
-            auto store = [&](int i, int r, float gate, float up) {
-                uint32_t hi, lo;
-                split_hidden(wq_swiglu(gate * scales[0][r], up * scales[1][r]), hi, lo);
-                const int64_t at = int64_t(list[i]) * p.hidden + f0 + r;
-                p.h[at] = uint16_t(hi);
-                p.h[at + plane] = uint16_t(lo);
-            };
-            if (left <= 4) ring_rows<DT, 128, 4, 1>(rw, f0, p.hidden + f0, 2 * p.hidden, p.k, rx, 0, left, rings, source, store);
-            else ring_rows<DT, 128, 8, 1>(rw, f0, p.hidden + f0, 2 * p.hidden, p.k, rx, 0, left, rings, source, store);
-        } else if (left <= 8) {
-            const int mine = (here / 16 - wave + 3) / 4;
-            auto done = [&](int block, v4f gate, v4f up) {
-                const int f = 16 * (wave + 4 * block) + 4 * (lane >> 4);
-                if ((lane & 15) < left) store4(lane & 15, f, gate, up);
-            };
-            if (left <= 4) ring_blocks<DT, 128, 4, 1>(rw, f0 + 16 * wave, p.hidden + f0 + 16 * wave, 64, mine, p.k, rx, 0, left, rings, source, done);
-            else ring_blocks<DT, 128, 8, 1>(rw, f0 + 16 * wave, p.hidden + f0 + 16 * wave, 64, mine, p.k, rx, 0, left, rings, source, done);
+            if (left <= 4) ring_rows<DT, 128, 4, 1>(rw, f0, p.hidden + f0, p.k, rx, 0, left, rings, source, done);
+            else ring_rows<DT, 128, 8, 1>(rw, f0, p.hidden + f0, p.k, rx, 0, left, rings, source, done);
         } else {
-            for (int f = 0; f < here; f += 32) {
-                auto done = [&](int m, int c, v4f gate, v4f up) {
-                    const int i = 16 * m + (lane & 15), at = f + 16 * c;
-                    if (i < left && at < here) store4(i, at + 4 * (lane >> 4), gate, up);
-                };
-                if (f) __syncthreads();
-                if (left <= 16) shared_rows<DT, 1, 1>(rw, f0 + f, p.hidden + f0 + f, p.k, rx, 0, left, rings, source, done);
-                else if (left <= 32) shared_rows<DT, 2, 1>(rw, f0 + f, p.hidden + f0 + f, p.k, rx, 0, left, rings, source, done);
-                else shared_rows<DT, 4, 1>(rw, f0 + f, p.hidden + f0 + f, p.k, rx, 0, left, rings, source, done);
-            }
+            auto done_at = [&](int m, v4f gate, v4f up) {
+                if (16 * m + (lane & 15) < left && f < p.hidden) store4(16 * m + (lane & 15), gate, up);
+            };
+            if (left <= 16) shared_rows<DT, 128, 1, 1>(rw, f0, p.hidden + f0, p.k, rx, 0, left, rings, source, done_at);
+            else if (left <= 32) shared_rows<DT, 128, 2, 1>(rw, f0, p.hidden + f0, p.k, rx, 0, left, rings, source, done_at);
+            else shared_rows<DT, 64, 4, 1>(rw, f0, p.hidden + f0, p.k, rx, 0, left, rings, source, done_at);
         }
-        if (rest <= most) return;
+        if (rest <= passes * most) return;
         __syncthreads();
     }
 }
 
-// Output channels of an expert for its choices, weighted: 32 a workgroup (own 0), or 128 `own`.
-__global__ void __launch_bounds__(256, 2) experts_down(ExpertsArgs p, int own) {
+// Output channels of an expert for its choices: 32 a workgroup, whose waves share them (!own), or 128.
+__global__ void __launch_bounds__(256, 2) experts_down(ExpertsArgs p, int own, int passes) {
     __shared__ __attribute__((aligned(1024))) uint8_t rings[4 * RING];
-    __shared__ float scales[128 * MOST_BLOCKS], weights[MOST_LISTED];
     __shared__ uint16_t list[MOST_LISTED];
-    const int channels = own ? 128 * own : 32, groups = (p.k + channels - 1) / channels;
-    const int slot = blockIdx.x / groups, n0 = (blockIdx.x % groups) * channels, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int expert = slot_expert(p, slot), here = min(channels, p.k - n0);
+    const int channels = own ? 128 : 32, groups = (p.k + channels - 1) / channels;
+    const int tiles = gridDim.x / passes, tile = blockIdx.x % tiles, pass = blockIdx.x / tiles;
+    const int slot = tile / groups, n0 = tile % groups * channels, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int expert = slot_expert(p, slot);
     if (uint32_t(expert) >= uint32_t(p.experts)) return;
     const uint32_t plane = uint32_t(p.tokens) * uint32_t(p.top) * uint32_t(p.hidden) * 2u;
     const sgpr4 rw = buffer_rsrc(p.down + int64_t(expert) * p.k * p.hidden, uint32_t(p.k) * uint32_t(p.hidden));
     const sgpr4 rx = buffer_rsrc(p.h, 2u * plane);
     auto source = [&](int i) { return uint32_t(list[i]) * uint32_t(p.hidden) * 2u; };
-    // channels n0 + n .. + 3 of choice i
-    auto store4 = [&](int i, int n, v4f v) {
-        if (n >= here) return;
-        const float weight = weights[i];
-        v4f out;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) out[j] = v[j] * scales[n + j] * weight;
-        *reinterpret_cast<v4f*>(p.part + int64_t(list[i]) * p.k + n0 + n) = out;
+    const float* scale = p.down_scale + int64_t(expert) * p.k;
+    // the channels of this lane's sums: tiles of 16 in two runs, next to each other (!own) or 64 apart
+    const int n = n0 + (own ? 16 * wave : 0) + 4 * (lane >> 4), apart = own ? 64 : 16;
+    const v4f scale0 = scales4(scale, n, p.k), scale1 = scales4(scale, n + apart, p.k);
+    auto store4 = [&](int i, v4f a, v4f b) {
+        float* to = p.part + int64_t(list[i]) * p.k + n;
+        if (n < p.k) *reinterpret_cast<v4f*>(to) = a * scale0;
+        if (n + apart < p.k) *reinterpret_cast<v4f*>(to + apart) = b * scale1;
     };
-    for (int n = threadIdx.x; n < here; n += 256) scales[n] = p.down_scale[int64_t(expert) * p.k + n0 + n];
-    const int lane = threadIdx.x & 63;
-    const int most = own ? 32 : 8;
-    for (int first = 0;; first += most) {
+    const int most = own ? 64 : 8;
+    for (int first = pass * most;; first += passes * most) {
         const int rest = find_choices(p, slot, expert, first, list) - first, left = min(rest, most);
         if (left <= 0) return;
         __syncthreads();
-        if (threadIdx.x < left) weights[threadIdx.x] = p.weights[list[threadIdx.x]];
-        __syncthreads();
+        auto done = [&](v4f a, v4f b) {
+            if ((lane & 15) < left) store4(lane & 15, a, b);
+        };
         if (!own) {
-            auto store = [&](int i, int r, float a, float b) {
-                float* to = p.part + int64_t(list[i]) * p.k + n0 + r;
-                if (r < here) to[0] = a * scales[r] * weights[i];
-                if (16 + r < here) to[16] = b * scales[16 + r] * weights[i];
-            };
-            if (left <= 4) ring_rows<DT_BF16, 128, 4, 2>(rw, n0, n0 + 16, p.k, p.hidden, rx, plane, left, rings, source, store);
-            else ring_rows<DT_BF16, 64, 8, 2>(rw, n0, n0 + 16, p.k, p.hidden, rx, plane, left, rings, source, store);
-        } else if (left <= 8) {
-            const int mine = ((here + 31) / 32 - wave + 3) / 4;
-            auto done = [&](int block, v4f a, v4f b) {
-                const int n = 32 * (wave + 4 * block) + 4 * (lane >> 4);
-                if ((lane & 15) < left) store4(lane & 15, n, a), store4(lane & 15, n + 16, b);
-            };
-            if (left <= 4) ring_blocks<DT_BF16, 64, 4, 2>(rw, n0 + 32 * wave, n0 + 32 * wave + 16, 128, mine, p.hidden, rx, plane, left, rings, source, done);
-            else ring_blocks<DT_BF16, 64, 8, 2>(rw, n0 + 32 * wave, n0 + 32 * wave + 16, 128, mine, p.hidden, rx, plane, left, rings, source, done);
+            if (left <= 4) ring_rows<DT_BF16, 128, 4, 2>(rw, n0, n0 + 16, p.hidden, rx, plane, left, rings, source, done);
+            else ring_rows<DT_BF16, 64, 8, 2>(rw, n0, n0 + 16, p.hidden, rx, plane, left, rings, source, done);
         } else {
-            for (int n = 0; n < here; n += 64) {
-                auto done = [&](int m, int c, v4f a, v4f b) {
-                    const int i = 16 * m + (lane & 15), at = n + 16 * c + 4 * (lane >> 4);
-                    if (i < left) store4(i, at, a), store4(i, at + 32, b);
-                };
-                if (n) __syncthreads();
-                if (left <= 16) shared_rows<DT_BF16, 1, 2>(rw, n0 + n, n0 + n + 32, p.hidden, rx, plane, left, rings, source, done);
-                else shared_rows<DT_BF16, 2, 2>(rw, n0 + n, n0 + n + 32, p.hidden, rx, plane, left, rings, source, done);
-            }
+            auto done_at = [&](int m, v4f a, v4f b) {
+                if (16 * m + (lane & 15) < left) store4(16 * m + (lane & 15), a, b);
+            };
+            if (left <= 16) shared_rows<DT_BF16, 128, 1, 2>(rw, n0, n0 + 64, p.hidden, rx, plane, left, rings, source, done_at);
+            else if (left <= 32) shared_rows<DT_BF16, 64, 2, 2>(rw, n0, n0 + 64, p.hidden, rx, plane, left, rings, source, done_at);
+            else shared_rows<DT_BF16, 64, 4, 2>(rw, n0, n0 + 64, p.hidden, rx, plane, left, rings, source, done_at);
         }
-        if (rest <= most) return;
+        if (rest <= passes * most) return;
         __syncthreads();
     }
 }
@@ -627,7 +564,7 @@ template <int DT> WQ8_DEVICE float with_residual(const ExpertsArgs& p, int t, in
     return __builtin_fmaf(v, scale, Elem<DT>::to_f(static_cast<const raw*>(p.residual)[t * p.ldr + n]));
 }
 
-// A token's parts, added in the order of its choices.
+// A token's parts, weighted and added in the order of its choices.
 template <int DT>
 __global__ void __launch_bounds__(256) experts_join(ExpertsArgs p) {
     using raw = typename Elem<DT>::raw;
@@ -635,22 +572,108 @@ __global__ void __launch_bounds__(256) experts_join(ExpertsArgs p) {
     if (at >= p.tokens * quads) return;
     const int t = at / quads, n = at % quads * 4;
     v4f sum = {0, 0, 0, 0};
-    for (int j = 0; j < p.top; ++j) {
-        const int pair = t * p.top + j;
-        if (uint32_t(p.ids[pair]) >= uint32_t(p.experts)) continue;
-        sum += *reinterpret_cast<const v4f*>(p.part + int64_t(pair) * p.k + n);
+    for (int j0 = 0; j0 < p.top; j0 += 8) {
+        v4f part[8];
+        float weight[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int pair = t * p.top + min(j0 + j, p.top - 1);
+            const bool held = j0 + j < p.top && uint32_t(p.ids[pair]) < uint32_t(p.experts);  // the others' parts were not written
+            part[j] = *reinterpret_cast<const v4f*>(p.part + int64_t(pair) * p.k + n);
+            weight[j] = p.weights[pair];
+            if (!held) part[j] = v4f{0, 0, 0, 0}, weight[j] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(weight[j], part[j][i], sum[i]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) static_cast<raw*>(p.out)[t * p.ldo + n + i] = Elem<DT>::from_f(with_residual<DT>(p, t, n + i, sum[i]));
+}
+
+// One token: the second product and the sum over its choices in one launch. A workgroup has 8 output channels, a wave every eighth choice of the
+// token: 8 rows of 128 neighbouring bytes a load, 8 loads ahead, so that an expert's 8 x 1024 codes are asked for at once. One token leaves nothing
+// to share, and 16 rows of a matrix instruction would leave half the CUs idle: the products are FP32 on the vector unit, hidden values as FP32.
+template <int DT>
+__global__ void __launch_bounds__(512) experts_down_one(ExpertsArgs p) {
+    using raw = typename Elem<DT>::raw;
+    constexpr int STEP = 1024;
+    __shared__ __attribute__((aligned(16))) float hidden[8][STEP];
+    __shared__ float part[MOST_ONE][8];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n0 = blockIdx.x * 8, row = n0 + (lane >> 3), chunk = lane & 7;
+    for (int j = wave; j < p.top; j += 8) {
+        const int expert = p.ids[j];
+        float sum = 0.0f;
+        if (uint32_t(expert) < uint32_t(p.experts)) {
+            const int8_t* codes = p.down + (int64_t(expert) * p.k + row) * p.hidden;
+            const uint16_t* h = p.h + int64_t(j) * p.hidden;
+            const int64_t plane = int64_t(p.top) * p.hidden;
+            const float scale = p.down_scale[int64_t(expert) * p.k + row];
+            for (int begin = 0; begin < p.hidden; begin += STEP) {
+                u32x4 x[2][2], w[8];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int k = begin + 8 * (lane + 64 * i);
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) x[i][q] = k < p.hidden ? *reinterpret_cast<const u32x4*>(h + q * plane + k) : u32x4{0, 0, 0, 0};
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int k = begin + 128 * i + 16 * chunk;
+                    w[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(codes + (k < p.hidden ? k : 0)));  // past the row: against zeros
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        v4f v;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int word = 2 * half + (e >> 1), shift = 16 * (e & 1);
+                            v[e] = Elem<DT_BF16>::to_f(uint16_t(x[i][0][word] >> shift)) + Elem<DT_BF16>::to_f(uint16_t(x[i][1][word] >> shift));
+                        }
+                        *reinterpret_cast<v4f*>(&hidden[wave][8 * (lane + 64 * i) + 4 * half]) = v;
+                    }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (begin + 128 * i >= p.hidden) break;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const v4f v = *reinterpret_cast<const v4f*>(&hidden[wave][128 * i + 16 * chunk + 4 * c]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sum = __builtin_fmaf(float(int8_t(w[i][c] >> (8 * e))), v[e], sum);
+                    }
+                }
+            }
+            sum += lane_xor<1>(sum);
+            sum += lane_xor<2>(sum);
+            sum += lane_xor<4>(sum);
+            sum *= scale;
+        }
+        if (!chunk) part[j][lane >> 3] = sum;
+    }
+    __syncthreads();
+    if (threadIdx.x >= 8) return;
+    float total = 0.0f;
+    for (int j = 0; j < p.top; ++j)
+        if (uint32_t(p.ids[j]) < uint32_t(p.experts)) total = __builtin_fmaf(p.weights[j], part[j][threadIdx.x], total);
+    static_cast<raw*>(p.out)[n0 + threadIdx.x] = Elem<DT>::from_f(with_residual<DT>(p, 0, n0 + threadIdx.x, total));
 }
 
 }  // namespace wq8
 
 using namespace wq8;
 
+// Parts of K: as many as fill the CUs, of whole steps
+static int route_parts(int tokens, int experts, int k) {
+    const int64_t tiles = int64_t((experts + 15) / 16) * ((tokens + 15) / 16), steps = (k + ROUTE_STEP - 1) / ROUTE_STEP, fill = 512 / tiles;
+    return int(fill < 1 ? 1 : fill < steps ? fill : steps);
+}
+
 template <int XT>
 static void launch_logits(const RouteArgs& p, int router_dtype, hipStream_t stream) {
-    const dim3 grid((p.experts + 15) / 16, (p.tokens + 15) / 16);
+    const dim3 grid((p.experts + 15) / 16, (p.tokens + 15) / 16, p.parts);
     if (router_dtype == DT_F16) route_logits<XT, DT_F16><<<grid, 64 * ROUTE_WAVES, 0, stream>>>(p);
     else if (router_dtype == DT_BF16) route_logits<XT, DT_BF16><<<grid, 64 * ROUTE_WAVES, 0, stream>>>(p);
     else route_logits<XT, DT_F32><<<grid, 64 * ROUTE_WAVES, 0, stream>>>(p);
@@ -661,7 +684,9 @@ WQ8_API int wq8_route(const void* x, int64_t ldx, int dtype, const void* router,
     if (!tokens) return 0;
     if (dtype < 0 || dtype > 2 || router_dtype < 0 || router_dtype > 2 || score < 0 || score > 1) return -1;
     if (tokens < 0 || tokens > 65535 * 16 || experts < 1 || experts > 1024 || k < 8 || k % 8 || top < 1 || top > 64 || top > experts) return -2;
-    const RouteArgs p{x, router, bias, static_cast<double*>(logits), ids, weights, ldx, tokens, experts, k, top, score, normalise, factor};
+    const int wanted = route_parts(tokens, experts, k), steps = (k + ROUTE_STEP - 1) / ROUTE_STEP, part = (steps + wanted - 1) / wanted * ROUTE_STEP;
+    const RouteArgs p{x, router, bias, static_cast<double*>(logits), ids, weights, ldx, tokens, experts, k, top, score, normalise, (k + part - 1) / part, part,
+                      factor};
     if (dtype == DT_F16) launch_logits<DT_F16>(p, router_dtype, stream);
     else if (dtype == DT_BF16) launch_logits<DT_BF16>(p, router_dtype, stream);
     else launch_logits<DT_F32>(p, router_dtype, stream);
@@ -672,6 +697,11 @@ WQ8_API int wq8_route(const void* x, int64_t ldx, int dtype, const void* router,
     else if (experts <= 256) route_choose<4><<<groups, 256, 0, stream>>>(p);
     else route_choose<16><<<groups, 256, 0, stream>>>(p);
     return int(hipGetLastError());
+}
+
+WQ8_API void wq8_route_workspace(int tokens, int experts, int k, int64_t* sizes) {
+    sizes[0] = tokens > 0 && experts > 0 ? int64_t(route_parts(tokens, experts, k)) * tokens * experts * 8 : 0;
+    sizes[1] = 0;
 }
 
 WQ8_API int wq8_experts(const void* x, int64_t ldx, int dtype, const void* ids, const float* weights, const int8_t* gate_up, const float* gate_up_scale,
@@ -688,13 +718,20 @@ WQ8_API int wq8_experts(const void* x, int64_t ldx, int dtype, const void* ids, 
     const ExpertsArgs p{x, static_cast<const int32_t*>(ids), weights, gate_up, gate_up_scale, down, down_scale, static_cast<uint16_t*>(workspace),
                         reinterpret_cast<float*>(static_cast<char*>(workspace) + h_bytes), residual, rscale, out, ldx, ldr, ldo, tokens, top, experts, k, hidden};
     // tiles that waves share only where there are few, of 8 tokens at most
-    const auto own = [&](int64_t tiles, int waves) { return tokens <= 8 && slots * tiles <= 1024 ? 0 : slots * tiles <= 4096 ? 1 : slots * tiles <= 8192 ? 2 : MOST_BLOCKS; };
-    const int up = own(hidden / 16, 4), down_own = own((k + 31) / 32, 4);
-    const int up_groups = up ? (hidden + 64 * up - 1) / (64 * up) : hidden / 16, down_groups = down_own ? (k + 128 * down_own - 1) / (128 * down_own) : (k + 31) / 32;
-    if (dtype == DT_F16) experts_up<DT_F16><<<slots * up_groups, 256, 0, stream>>>(p, up);
-    else experts_up<DT_BF16><<<slots * up_groups, 256, 0, stream>>>(p, up);
+    const int up = tokens > 8 || slots * (hidden / 16) > 1024, down_own = tokens > 8 || slots * ((k + 31) / 32) > 1024;
+    const int up_groups = up ? (hidden + 63) / 64 : hidden / 16, down_groups = down_own ? (k + 127) / 128 : (k + 31) / 32;
+    // an expert of more tokens than a workgroup takes at once: other workgroups take the next ones
+    const auto passes = [&](int most) { return tokens <= most ? 1 : tokens <= 2 * most ? 2 : 4; };
+    const int up_passes = up ? passes(64) : 1, down_passes = down_own ? passes(64) : 1;
+    if (dtype == DT_F16) experts_up<DT_F16><<<slots * up_groups * up_passes, 256, 0, stream>>>(p, up, up_passes);
+    else experts_up<DT_BF16><<<slots * up_groups * up_passes, 256, 0, stream>>>(p, up, up_passes);
     if (const int rc = int(hipGetLastError())) return rc;
-    experts_down<<<slots * down_groups, 256, 0, stream>>>(p, down_own);
+    if (tokens == 1 && top <= MOST_ONE) {
+        if (dtype == DT_F16) experts_down_one<DT_F16><<<k / 8, 512, 0, stream>>>(p);
+        else experts_down_one<DT_BF16><<<k / 8, 512, 0, stream>>>(p);
+        return int(hipGetLastError());
+    }
+    experts_down<<<slots * down_groups * down_passes, 256, 0, stream>>>(p, down_own, down_passes);
     if (const int rc = int(hipGetLastError())) return rc;
     const int groups = (tokens * (k / 4) + 255) / 256;
     if (dtype == DT_F16) experts_join<DT_F16><<<groups, 256, 0, stream>>>(p);
