@@ -5,20 +5,22 @@
 // 64-bit definition but for borders within 2^-44 of each other. Tokens stand in the order of (logit, lowest index first), a 64-bit key:
 // top-k and top-p each keep the keys down to a last one, `cut`.
 //
-// Four launches, a row over up to 64 workgroups in the first three: the largest logit; a histogram (counts and weights) over (largest - logit) /
-// temperature; the keys of the histogram's bins in which the cuts lie, and the weights of what certainly stays; then a workgroup a row
-// finds the cut among those keys digit by digit, and the token whose running weight, in vocabulary order, passes draw * (weight kept).
+// Four launches, a row over up to 64 workgroups in the first three: the largest logit; a histogram over (largest - logit) / temperature (of counts
+// for top-k, of weights for top-p); the keys of the histogram's bins in which the cuts lie, and the weights of what certainly stays; then a
+// workgroup a row finds the cut among those keys, and the token whose running weight, in vocabulary order, passes draw * (weight kept). A top-k of at most
+// SMALL_K lists all of its keys: then no weight is taken of the rest of the row.
 #include "wq8_common.h"
 #include "wq8_abi.h"
+#include <type_traits>
 
 namespace wq8 {
 
-constexpr int SAMPLE_BINS = 1024, SAMPLE_SPLITS = 64, SAMPLE_LIST = 2048, SAMPLE_PIECE = 2048;
+constexpr int SAMPLE_BINS = 1024, SAMPLE_SPLITS = 64, SAMPLE_PARTS = 256, SAMPLE_LIST = 2048, SAMPLE_PIECE = 2048, SMALL_K = 1024, SHORT_LIST = 128;
 constexpr float BINS_PER_UNIT = 32.0f;  // the last bin begins at 31.97: weights below 2^-46, held as 0
 
 struct SampleRow {  // a row's workspace
     uint64_t largest[SAMPLE_SPLITS];
-    uint64_t kept[SAMPLE_SPLITS];
+    uint64_t kept[SAMPLE_PARTS];  // the weight kept of each part
     uint64_t mass[SAMPLE_BINS];
     uint32_t count[SAMPLE_BINS];
     uint64_t list[SAMPLE_LIST];
@@ -37,7 +39,7 @@ struct SampleArgs {
     int64_t* tokens;
     float temperature0, top_p0, min_p0;
     int top_k0;
-    int vocabulary, split, splits, shift;
+    int vocabulary, part, parts, split, splits, shift;  // parts of `part` tokens, splits of `split`, a multiple of that
 };
 
 // The order of a logit: larger numbers for larger logits, 0 for NaN; both zeros alike.
@@ -49,6 +51,19 @@ WQ8_DEVICE float order_logit(uint32_t o) { return __builtin_bit_cast(float, o >>
 WQ8_DEVICE uint64_t token_key(float l, int index) { return uint64_t(logit_order(l)) << 32 | (0xffffffffu - uint32_t(index)); }
 WQ8_DEVICE int key_index(uint64_t key) { return int(0xffffffffu - uint32_t(key)); }
 
+// exp(z) for z <= 0, 0 below -50 (and for NaN): z = n ln 2 + r with ln 2 in two parts, |r| <= 0.347, exp(r) by its series up to r^13 / 13!, whose rest is
+// below 2^-52 of it
+WQ8_DEVICE double exp_below_0(double z) {
+    const double n = __builtin_rint(z * 0x1.71547652b82fep+0);
+    double r = __builtin_fma(-n, 0x1.62e42fefa38p-1, z);  // 43 bits: n times it is exact
+    r = __builtin_fma(-n, 0x1.ef35793c7673p-45, r);
+    double e = 1.0 / 6227020800.0;
+    constexpr double INVERSE[13] = {1.0 / 479001600, 1.0 / 39916800, 1.0 / 3628800, 1.0 / 362880, 1.0 / 40320, 1.0 / 5040, 1.0 / 720, 1.0 / 120, 1.0 / 24, 1.0 / 6, 0.5, 1.0, 1.0};
+#pragma unroll
+    for (int i = 0; i < 13; ++i) e = __builtin_fma(e, r, INVERSE[i]);
+    return z > -50.0 ? __builtin_amdgcn_ldexp(e, int(n)) : 0.0;
+}
+
 // What a row is sampled by.
 struct Row {
     float top;         // its largest logit
@@ -58,14 +73,15 @@ struct Row {
     double scale, min_p;
     float top_p;
     int top_k;
-    bool greedy, nothing, by_p, by_k;
+    bool greedy, nothing, by_p, by_k, small_k;
 
     WQ8_DEVICE double weight(float l) const {
         if (l == top) return 1.0;
         const double z = (double(l) - double(top)) * inverse;
-        return z <= 0.0 ? exp(z) : 0.0;  // NaN: 0
+        return exp_below_0(z);
     }
-    WQ8_DEVICE uint64_t units(double w) const { return uint64_t(__builtin_rint(w * scale)); }
+    // the nearest whole number of w * scale <= 2^44, from the low bits of its sum with 2^52
+    WQ8_DEVICE uint64_t units(double w) const { return __builtin_bit_cast(uint64_t, __builtin_fma(w, scale, 0x1p52)) - 0x4330000000000000ull; }
     WQ8_DEVICE int bin(float l) const {
         if (l == top) return 0;
         const float b = (top - l) * bins;
@@ -74,10 +90,25 @@ struct Row {
 };
 
 WQ8_DEVICE uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
-template <typename T> WQ8_DEVICE T wave_total(T v) {
-#pragma unroll
-    for (int step = 32; step; step >>= 1) v += __shfl_xor(v, step);
-    return v;
+// The sum over the wave: rows of 16 lanes by DPP, then rows and halves by exchanges
+WQ8_DEVICE uint64_t sum64(uint64_t v) {
+    auto dpp = [](auto control, uint64_t u) {
+        constexpr int C = decltype(control)::value;
+        return uint64_t(dpp_u<C>(uint32_t(u >> 32))) << 32 | dpp_u<C>(uint32_t(u));
+    };
+    v += dpp(std::integral_constant<int, 0xB1>{}, v);
+    v += dpp(std::integral_constant<int, 0x4E>{}, v);
+    v += dpp(std::integral_constant<int, 0x141>{}, v);
+    v += dpp(std::integral_constant<int, 0x140>{}, v);
+    auto rows = [](uint64_t u) {
+        const auto low = __builtin_amdgcn_permlane16_swap(uint32_t(u), uint32_t(u), false, false), high = __builtin_amdgcn_permlane16_swap(uint32_t(u >> 32), uint32_t(u >> 32), false, false);
+        return (uint64_t(uint32_t(high[0])) << 32 | uint32_t(low[0])) + (uint64_t(uint32_t(high[1])) << 32 | uint32_t(low[1]));
+    };
+    auto halves = [](uint64_t u) {
+        const auto low = __builtin_amdgcn_permlane32_swap(uint32_t(u), uint32_t(u), false, false), high = __builtin_amdgcn_permlane32_swap(uint32_t(u >> 32), uint32_t(u >> 32), false, false);
+        return (uint64_t(uint32_t(high[0])) << 32 | uint32_t(low[0])) + (uint64_t(uint32_t(high[1])) << 32 | uint32_t(low[1]));
+    };
+    return halves(rows(v));
 }
 
 WQ8_DEVICE Row read_row(const SampleArgs& p, const SampleRow& state, int row) {
@@ -99,24 +130,39 @@ WQ8_DEVICE Row read_row(const SampleArgs& p, const SampleRow& state, int row) {
     r.top_k = p.top_k ? p.top_k[row] : p.top_k0;
     r.by_p = r.top_p < 1.0f;
     r.by_k = r.top_k > 0 && r.top_k < p.vocabulary;
+    r.small_k = r.by_k && r.top_k <= SMALL_K;
     return r;
 }
 
-// f(logit, index) for the row's values from begin to end, 8 neighbouring ones a thread at a time. Rows may begin at any value: the loads of 16 bytes
-// are as unaligned as the row is.
-template <int DT, typename F> WQ8_DEVICE void each_logit(const SampleArgs& p, int row, int begin, int end, const F& f) {
+// f(logit, index) for the row's values from begin to end, 8 neighbouring ones a thread at a time, four times that asked for together; after(i) behind
+// every 2048, i the first of them. Rows may begin at any value: the loads of 16 bytes are as unaligned as the row is.
+template <int DT, typename F, typename After> WQ8_DEVICE void each_logit(const SampleArgs& p, int row, int begin, int end, const F& f, const After& after) {
     using raw = typename Elem<DT>::raw;
+    constexpr int AHEAD = 4;
     const raw* values = static_cast<const raw*>(p.logits) + row * p.ld;
-    for (int i = begin + 8 * int(threadIdx.x); i < end; i += 8 * 256) {
-        raw v[8];
-        if (i + 8 <= end) __builtin_memcpy(v, values + i, sizeof(v));
-        else
+    for (int first = begin; first < end; first += AHEAD * SAMPLE_PIECE) {
+        raw v[AHEAD][8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = values[min(i + j, end - 1)];
+        for (int u = 0; u < AHEAD; ++u) {
+            const int i = first + u * SAMPLE_PIECE + 8 * int(threadIdx.x);
+            if (i + 8 <= end) __builtin_memcpy(v[u], values + i, sizeof(v[u]));
+            else if (i < end)
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (i + j < end) f(Elem<DT>::to_f(v[j]), i + j);
+                for (int j = 0; j < 8; ++j) v[u][j] = values[min(i + j, end - 1)];
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int i = first + u * SAMPLE_PIECE + 8 * int(threadIdx.x);
+            if (first + u * SAMPLE_PIECE >= end) break;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (i + j < end) f(Elem<DT>::to_f(v[u][j]), i + j);
+            after(first + u * SAMPLE_PIECE);
+        }
     }
+}
+template <int DT, typename F> WQ8_DEVICE void each_logit(const SampleArgs& p, int row, int begin, int end, const F& f) {
+    each_logit<DT>(p, row, begin, end, f, [](int) {});
 }
 
 // ---- 1: the largest logit of every part of a row -----------------------------------------------------------------------------
@@ -126,8 +172,13 @@ template <int DT> __global__ void __launch_bounds__(256) sample_largest(SampleAr
     SampleRow& state = p.rows[row];
     for (int b = s * 256 + threadIdx.x; b < SAMPLE_BINS; b += 256 * p.splits) state.mass[b] = 0, state.count[b] = 0;
     if (!s && !threadIdx.x) state.listed = 0;
-    uint64_t best = 0;
-    each_logit<DT>(p, row, s * p.split, min(p.vocabulary, (s + 1) * p.split), [&](float l, int i) { best = max64(best, token_key(l, i)); });
+    uint32_t most = 0;
+    int at = 0;
+    each_logit<DT>(p, row, s * p.split, min(p.vocabulary, (s + 1) * p.split), [&](float l, int i) {
+        const uint32_t o = logit_order(l);
+        if (o > most) most = o, at = i;  // (a thread's indices rise: the first of equal ones stays)
+    });
+    uint64_t best = uint64_t(most) << 32 | (0xffffffffu - uint32_t(at));
 #pragma unroll
     for (int step = 32; step; step >>= 1) best = max64(best, __shfl_xor(best, step));
     if (!(threadIdx.x & 63)) best4[threadIdx.x >> 6] = best;
@@ -146,15 +197,14 @@ template <int DT> __global__ void __launch_bounds__(256) sample_bins(SampleArgs 
     for (int b = threadIdx.x; b < SAMPLE_BINS; b += 256) mass[b] = 0, count[b] = 0;
     __syncthreads();
     each_logit<DT>(p, row, s * p.split, min(p.vocabulary, (s + 1) * p.split), [&](float l, int) {
-        if (l != l) return;
-        const int b = r.bin(l);
-        atomicAdd(&count[b], 1u);
-        if (b < SAMPLE_BINS - 1) atomicAdd(&mass[b], (unsigned long long)r.units(r.weight(l)));
+        const int b = r.bin(l);  // NaN: the last
+        if (b == SAMPLE_BINS - 1) return;
+        if (r.by_k) atomicAdd(&count[b], 1u);
+        if (!r.small_k) atomicAdd(&mass[b], (unsigned long long)r.units(r.weight(l)));
     });
     __syncthreads();
     for (int b = threadIdx.x; b < SAMPLE_BINS; b += 256) {
-        if (!count[b]) continue;
-        atomicAdd(&state.count[b], count[b]);
+        if (count[b]) atomicAdd(&state.count[b], count[b]);
         if (mass[b]) atomicAdd(reinterpret_cast<unsigned long long*>(&state.mass[b]), mass[b]);
     }
 }
@@ -184,7 +234,7 @@ struct Cut {
     uint64_t k_before;              // the weight before it
     int low, high;                  // the bins of top-p's last key (low > high: no top-p)
     uint64_t low_before;            // the weight before them
-    int certain;                    // bins below it stay whole
+    int certain;                    // bins below it stay whole (0 for a small k, whose bins are all listed)
     WQ8_DEVICE bool listed(int bin) const { return bin == k_bin || (bin >= low && bin <= high); }
 };
 
@@ -238,8 +288,8 @@ WQ8_DEVICE Cut find_cut(const Row& r, const SampleRow& state, CutScratch& sc) {
         uint64_t m = mass_before;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
-            // (the last bin's weights are 0: a k that reaches it leaves nothing out)
-            if (n < uint32_t(r.top_k) && n + count[i] >= uint32_t(r.top_k) && EACH * int(threadIdx.x) + i < SAMPLE_BINS - 1) {
+            // (the last bin's weights are 0 and it is not counted: a k that reaches it leaves nothing out)
+            if (n < uint32_t(r.top_k) && n + count[i] >= uint32_t(r.top_k)) {
                 sc.k_bin = EACH * threadIdx.x + i;
                 sc.k_left = r.top_k - n;
                 sc.k_before = m;
@@ -253,6 +303,14 @@ WQ8_DEVICE Cut find_cut(const Row& r, const SampleRow& state, CutScratch& sc) {
     c.k_bin = sc.k_bin;
     c.k_left = sc.k_left;
     c.k_before = sc.k_before;
+    if (r.small_k) {  // all up to the k's bin is listed; where the k reach the last bin, all but that
+        c.low = c.certain = 0;
+        c.high = min(c.k_bin, SAMPLE_BINS - 2);
+        c.low_before = c.k_before = 0;
+        c.k_left = r.top_k;
+        __syncthreads();
+        return c;
+    }
     if (r.by_p) {
         // the k's weight is known up to its bin: top-p's last key lies between those of the least and the most that it can be
         const bool some = c.k_bin < SAMPLE_BINS;
@@ -280,7 +338,7 @@ WQ8_DEVICE Cut find_cut(const Row& r, const SampleRow& state, CutScratch& sc) {
 // ---- 3: the keys of those bins, and the weights that certainly stay ------------------------------------------------------------
 template <int DT> __global__ void __launch_bounds__(256) sample_list(SampleArgs p) {
     __shared__ CutScratch scratch;
-    __shared__ uint64_t sums[4];
+    __shared__ unsigned long long kept[SAMPLE_PARTS];
     const int row = blockIdx.x / p.splits, s = blockIdx.x % p.splits;
     SampleRow& state = p.rows[row];
     const Row r = read_row(p, state, row);
@@ -288,24 +346,33 @@ template <int DT> __global__ void __launch_bounds__(256) sample_list(SampleArgs 
     const bool cutting = r.by_k || r.by_p;
     Cut c{};
     if (cutting) c = find_cut(r, state, scratch);
-    uint64_t sum = 0;
-    each_logit<DT>(p, row, s * p.split, min(p.vocabulary, (s + 1) * p.split), [&](float l, int i) {
-        if (l != l) return;
-        if (cutting) {
-            const int b = r.bin(l);
-            if (c.listed(b)) {
-                const uint32_t at = atomicAdd(&state.listed, 1u);
-                if (at < uint32_t(SAMPLE_LIST)) state.list[at] = token_key(l, i);
-            }
-            if (b >= c.certain) return;
-        }
-        const double w = r.weight(l);
-        if (w >= r.min_p) sum += r.units(w);
-    });
-    sum = wave_total(sum);
-    if (!(threadIdx.x & 63)) sums[threadIdx.x >> 6] = sum;
+    if (c.certain || !cutting)
+        for (int i = threadIdx.x; i < SAMPLE_PARTS; i += 256) kept[i] = 0;
     __syncthreads();
-    if (!threadIdx.x) state.kept[s] = sums[0] + sums[1] + sums[2] + sums[3];
+    uint64_t sum = 0;
+    each_logit<DT>(
+        p, row, s * p.split, min(p.vocabulary, (s + 1) * p.split),
+        [&](float l, int i) {
+            if (cutting) {
+                const int b = r.bin(l);
+                if (c.listed(b) && l == l) {
+                    const uint32_t at = atomicAdd(&state.listed, 1u);
+                    if (at < uint32_t(SAMPLE_LIST)) state.list[at] = token_key(l, i);
+                }
+                if (b >= c.certain) return;
+            }
+            const double w = r.weight(l);
+            if (w >= r.min_p) sum += r.units(w);
+        },
+        [&](int i) {
+            if (cutting && !c.certain) return;
+            sum = sum64(sum);
+            if (!(threadIdx.x & 63)) atomicAdd(&kept[i / p.part], (unsigned long long)sum);
+            sum = 0;
+        });
+    __syncthreads();
+    const int first = s * (p.split / p.part), last = min(p.parts, first + p.split / p.part);
+    for (int i = first + threadIdx.x; i < last; i += 256) state.kept[i] = cutting && !c.certain ? 0 : kept[i];
 }
 
 // ---- 4: the cut among the listed keys, and the token ---------------------------------------------------------------------------
@@ -314,10 +381,11 @@ struct PickScratch {
     uint64_t list[SAMPLE_LIST], units[SAMPLE_LIST];
     unsigned long long mass[256];
     uint32_t count[256];
-    unsigned long long kept[SAMPLE_SPLITS];
+    unsigned long long kept[SAMPLE_PARTS];
     unsigned long long lowest, highest, found, need, before;
     uint32_t in_digit;
-    int digit;
+    int digit, part;
+    uint64_t part_target;
     uint64_t waves64[4];
     uint32_t waves32[4];
 };
@@ -333,7 +401,13 @@ template <typename Each> WQ8_DEVICE uint64_t select_key(PickScratch& sc, const E
         low = key < low ? key : low;
         high = max64(high, key);
     });
-    if (low <= high) {
+#pragma unroll
+    for (int step = 32; step; step >>= 1) {
+        const uint64_t l = __shfl_xor(low, step);
+        low = l < low ? l : low;
+        high = max64(high, __shfl_xor(high, step));
+    }
+    if (!(tid & 63) && low <= high) {
         atomicMin(&sc.lowest, (unsigned long long)low);
         atomicMax(&sc.highest, (unsigned long long)high);
     }
@@ -396,7 +470,13 @@ template <int DT> __global__ void __launch_bounds__(256) sample_pick(SampleArgs 
         if (!tid) p.tokens[row] = r.nothing ? -1 : key_index(r.first);
         return;
     }
-    if (tid < p.splits) sc.kept[tid] = state.kept[tid];
+    sc.kept[tid] = tid < p.parts ? state.kept[tid] : 0;
+    const float u = p.draws[row];
+    // the kept weight that the token's running weight has to pass
+    auto drawn = [&](uint64_t total) {
+        const uint64_t target = u > 0.0f ? u < 1.0f ? share_of(u, total, false) : total - 1 : 0;
+        return target < total ? target : total - 1;
+    };
     uint64_t cut = 0;  // keys from it on stay
     if (r.by_k || r.by_p) {
         const Cut c = find_cut(r, state, sc.cut);
@@ -409,6 +489,35 @@ template <int DT> __global__ void __launch_bounds__(256) sample_pick(SampleArgs 
                 sc.units[i] = r.units(r.weight(order_logit(uint32_t(key >> 32))));
             }
         __syncthreads();
+        if (whole && listed <= uint32_t(SHORT_LIST) && r.small_k) {
+            // few keys, all that may stay: each against all others, for its place, the weight before it, and the weight up to it in the vocabulary's order
+            const int n = int(listed);
+            const uint64_t key = tid < n ? sc.list[tid] : 0, mine = tid < n ? sc.units[tid] : 0;
+            uint32_t place = 0;
+            uint64_t before = 0;
+            for (int j = 0; j < n; ++j)
+                if (sc.list[j] > key) ++place, before += sc.units[j];
+            bool stays = tid < n && place < uint32_t(r.top_k);
+            auto add = [&](uint64_t v) {
+                v = sum64(v);
+                __syncthreads();
+                if (!(tid & 63)) sc.waves64[tid >> 6] = v;
+                __syncthreads();
+                return sc.waves64[0] + sc.waves64[1] + sc.waves64[2] + sc.waves64[3];
+            };
+            uint64_t total = add(stays ? mine : 0);
+            if (r.by_p) stays = stays && before < wanted_mass(r.top_p, total);
+            stays = stays && r.weight(order_logit(uint32_t(key >> 32))) >= r.min_p;
+            total = add(stays ? mine : 0);
+            if (tid < n) sc.units[tid] = stays ? mine : 0;
+            __syncthreads();
+            const uint64_t target = drawn(total);
+            uint64_t upto = 0;
+            for (int j = 0; j < n; ++j)
+                if (uint32_t(sc.list[j]) >= uint32_t(key)) upto += sc.units[j];  // (the index's complement: lower ones, and itself)
+            if (stays && upto > target && upto - mine <= target) p.tokens[row] = key_index(key);
+            return;
+        }
         // the listed keys of some of the bins; where they are too many for the list (logits that are alike), the row is read again instead
         auto each = [&](int from, int to, const auto& f) {
             if (whole) {
@@ -425,7 +534,18 @@ template <int DT> __global__ void __launch_bounds__(256) sample_pick(SampleArgs 
             }
         };
         uint64_t total = 0, above;
-        if (c.k_bin < SAMPLE_BINS) {
+        if (r.small_k) {
+            uint64_t all = 0;
+            uint32_t n = 0;
+            each(c.low, c.high, [&](uint64_t, uint64_t units) { all += units, ++n; });
+            uint32_t counted;
+            scan256(all, sc.waves64, total);
+            scan256(n, sc.waves32, counted);
+            if (counted > uint32_t(r.top_k)) {
+                cut = select_key(sc, [&](const auto& f) { each(c.low, c.high, f); }, true, r.top_k, above);
+                total = above + r.units(r.weight(order_logit(uint32_t(cut >> 32))));
+            } else cut = 1;  // fewer than k weigh anything: all of them stay
+        } else if (c.k_bin < SAMPLE_BINS) {
             cut = select_key(sc, [&](const auto& f) { each(c.k_bin, c.k_bin, f); }, true, c.k_left, above);
             total = c.k_before + above + r.units(r.weight(order_logit(uint32_t(cut >> 32))));
         } else if (r.by_p) {
@@ -435,26 +555,28 @@ template <int DT> __global__ void __launch_bounds__(256) sample_pick(SampleArgs 
         }
         if (r.by_p) cut = select_key(sc, [&](const auto& f) { each(c.low, c.high, f); }, false, wanted_mass(r.top_p, total) - c.low_before, above);
         if (cut) {
-            const int from = c.certain, to = r.by_p ? c.high : c.k_bin;
+            const int from = c.certain, to = r.by_p || r.small_k ? c.high : c.k_bin;
             each(from, to, [&](uint64_t key, uint64_t units) {
-                if (key >= cut && r.weight(order_logit(uint32_t(key >> 32))) >= r.min_p) atomicAdd(&sc.kept[key_index(key) / p.split], (unsigned long long)units);
+                if (key >= cut && r.weight(order_logit(uint32_t(key >> 32))) >= r.min_p) atomicAdd(&sc.kept[key_index(key) / p.part], (unsigned long long)units);
             });
         }
     }
     __syncthreads();
     // the part of the row in which the running weight passes the drawn one
-    uint64_t total = 0;
-    for (int s = 0; s < p.splits; ++s) total += sc.kept[s];
-    const float u = p.draws[row];
-    uint64_t target = u > 0.0f ? u < 1.0f ? share_of(u, total, false) : total - 1 : 0;
-    if (target >= total) target = total - 1;
-    int s = 0;
-    while (s < p.splits - 1 && target >= sc.kept[s]) target -= sc.kept[s++];
+    uint64_t total;
+    const uint64_t here = sc.kept[tid], upto = scan256(here, sc.waves64, total), passes = drawn(total);
+    if (upto <= passes && passes < upto + here) {
+        sc.part = tid;
+        sc.part_target = passes - upto;
+    }
+    __syncthreads();
+    uint64_t target = sc.part_target;
+    const int s = sc.part;
     // in it, 8 neighbouring tokens a thread at a time
     using raw = typename Elem<DT>::raw;
     const raw* values = static_cast<const raw*>(p.logits) + row * p.ld;
-    const int end = min(p.vocabulary, (s + 1) * p.split);
-    for (int begin = s * p.split; begin < end; begin += 8 * 256) {
+    const int end = min(p.vocabulary, (s + 1) * p.part);
+    for (int begin = s * p.part; begin < end; begin += 8 * 256) {
         uint64_t units[8], mine = 0, piece;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -498,17 +620,18 @@ WQ8_API int wq8_sample(const void* logits, int64_t ld, int dtype, const float* d
     if (!rows) return 0;
     if (dtype < 0 || dtype > 2) return -1;
     if (rows < 0 || rows > (1 << 17) || vocabulary < 1 || vocabulary > (1 << 24)) return -2;
-    // parts of at least 2048 tokens, a thousand workgroups or so
-    const int pieces = (vocabulary + SAMPLE_PIECE - 1) / SAMPLE_PIECE;
+    // up to 256 parts of 2048 tokens or a multiple; splits of whole parts, a thousand workgroups or so
+    const int pieces = (vocabulary + SAMPLE_PIECE - 1) / SAMPLE_PIECE, part = (pieces + SAMPLE_PARTS - 1) / SAMPLE_PARTS * SAMPLE_PIECE;
+    const int parts = (vocabulary + part - 1) / part;
     int splits = (1023 + rows) / rows;
     splits = splits < SAMPLE_SPLITS ? splits : SAMPLE_SPLITS;
-    splits = splits < pieces ? splits : pieces;
-    const int split = (pieces + splits - 1) / splits * SAMPLE_PIECE;
+    splits = splits < parts ? splits : parts;
+    const int split = (parts + splits - 1) / splits * part;
     splits = (vocabulary + split - 1) / split;
     int bits = 0;
     while ((1 << bits) < vocabulary) ++bits;
     const SampleArgs p{logits, ld, draws, temperature, static_cast<const int32_t*>(top_k), top_p, min_p, static_cast<SampleRow*>(workspace), tokens,
-                       temperature0, top_p0, min_p0, top_k0, vocabulary, split, splits, bits <= 18 ? 44 : 62 - bits};
+                       temperature0, top_p0, min_p0, top_k0, vocabulary, part, parts, split, splits, bits <= 18 ? 44 : 62 - bits};
     if (dtype == DT_F16) return launch_sample<DT_F16>(p, rows, stream);
     if (dtype == DT_BF16) return launch_sample<DT_BF16>(p, rows, stream);
     return launch_sample<DT_F32>(p, rows, stream);
