@@ -39,7 +39,7 @@ struct SampleArgs {
     int64_t* tokens;
     float temperature0, top_p0, min_p0;
     int top_k0;
-    int vocabulary, part, parts, split, splits, shift;  // parts of `part` tokens, splits of `split`, a multiple of that
+    int vocabulary, bits, part, parts, split, splits, shift;  // indices have `bits`; parts of `part` tokens, splits of `split`, a multiple of that
 };
 
 // The order of a logit: larger numbers for larger logits, 0 for NaN; both zeros alike.
@@ -48,37 +48,52 @@ WQ8_DEVICE uint32_t logit_order(float l) {
     return l != l ? 0u : b >> 31 ? ~b : b | 0x80000000u;
 }
 WQ8_DEVICE float order_logit(uint32_t o) { return __builtin_bit_cast(float, o >> 31 ? o & 0x7fffffffu : ~o); }
-WQ8_DEVICE uint64_t token_key(float l, int index) { return uint64_t(logit_order(l)) << 32 | (0xffffffffu - uint32_t(index)); }
-WQ8_DEVICE int key_index(uint64_t key) { return int(0xffffffffu - uint32_t(key)); }
+// A token's key: its logit's order without the bits that 16-bit logits do not have (all 0, or all 1 below zero), then its index upside down.
+template <int DT> struct Key {
+    static constexpr int SPARE = DT == DT_BF16 ? 16 : DT == DT_F16 ? 13 : 0;
+    int bits;  // of an index
+    WQ8_DEVICE uint64_t of(float l, int index) const { return uint64_t(logit_order(l) >> SPARE) << bits | uint32_t((1 << bits) - 1 - index); }
+    WQ8_DEVICE int index(uint64_t key) const { return (1 << bits) - 1 - int(uint32_t(key) & ((1u << bits) - 1)); }
+    WQ8_DEVICE float logit(uint64_t key) const {
+        const uint32_t o = uint32_t(key >> bits) << SPARE;
+        return order_logit(o >> 31 ? o : o | ((1u << SPARE) - 1));
+    }
+};
 
-// exp(z) for z <= 0, 0 below -50 (and for NaN): z = n ln 2 + r with ln 2 in two parts, |r| <= 0.347, exp(r) by its series up to r^13 / 13!, whose rest is
-// below 2^-52 of it
-WQ8_DEVICE double exp_below_0(double z) {
-    const double n = __builtin_rint(z * 0x1.71547652b82fep+0);
-    double r = __builtin_fma(-n, 0x1.62e42fefa38p-1, z);  // 43 bits: n times it is exact
-    r = __builtin_fma(-n, 0x1.ef35793c7673p-45, r);
-    double e = 1.0 / 6227020800.0;
-    constexpr double INVERSE[13] = {1.0 / 479001600, 1.0 / 39916800, 1.0 / 3628800, 1.0 / 362880, 1.0 / 40320, 1.0 / 5040, 1.0 / 720, 1.0 / 120, 1.0 / 24, 1.0 / 6, 0.5, 1.0, 1.0};
+// 2^t for t <= 0, 0 below -72 (and for NaN): t = n + f, |f| <= 1/2, 2^f by the series of exp(f ln 2) up to its 12th power, whose rest is below 2^-52
+// of it. The sum with 1.5 2^52 holds n in its low bits, which are added to the exponent of 2^f.
+WQ8_DEVICE double power_of_2(double t) {
+    const double shifted = t + 0x1.8p52, f = t - (shifted - 0x1.8p52);
+    // ln(2)^i / i!, i = 12 .. 0
+    constexpr double LN2 = 0x1.62e42fefa39efp-1;
+    constexpr double POWER[13] = {1.0, LN2, LN2 * LN2, LN2 * LN2 * LN2, LN2 * LN2 * LN2 * LN2, LN2 * LN2 * LN2 * LN2 * LN2, LN2 * LN2 * LN2 * LN2 * LN2 * LN2,
+                                  LN2 * LN2 * LN2 * LN2 * LN2 * LN2 * LN2, LN2 * LN2 * LN2 * LN2 * LN2 * LN2 * LN2 * LN2,
+                                  LN2 * LN2 * LN2 * LN2 * LN2 * LN2 * LN2 * LN2 * LN2, LN2 * LN2 * LN2 * LN2 * LN2 * LN2 * LN2 * LN2 * LN2 * LN2,
+                                  LN2 * LN2 * LN2 * LN2 * LN2 * LN2 * LN2 * LN2 * LN2 * LN2 * LN2, LN2 * LN2 * LN2 * LN2 * LN2 * LN2 * LN2 * LN2 * LN2 * LN2 * LN2 * LN2};
+    constexpr double FACTORIAL[13] = {1, 1, 2, 6, 24, 120, 720, 5040, 40320, 362880, 3628800, 39916800, 479001600};
+    double e = POWER[12] / FACTORIAL[12];
 #pragma unroll
-    for (int i = 0; i < 13; ++i) e = __builtin_fma(e, r, INVERSE[i]);
-    return z > -50.0 ? __builtin_amdgcn_ldexp(e, int(n)) : 0.0;
+    for (int i = 11; i >= 0; --i) e = __builtin_fma(e, f, POWER[i] / FACTORIAL[i]);
+    const uint64_t bits = __builtin_bit_cast(uint64_t, e);
+    const uint32_t high = uint32_t(bits >> 32) + (uint32_t(__builtin_bit_cast(uint64_t, shifted)) << 20);
+    const double power = __builtin_bit_cast(double, uint64_t(high) << 32 | uint32_t(bits));
+    return t > -72.0 ? power : 0.0;
 }
 
 // What a row is sampled by.
 struct Row {
     float top;         // its largest logit
-    uint64_t first;    // the key of that
-    double inverse;    // of the temperature
+    int first;         // the first token that has it
+    double inverse;    // of the temperature, times log2(e)
     float bins;        // bins a unit of logit
     double scale, min_p;
     float top_p;
     int top_k;
-    bool greedy, nothing, by_p, by_k, small_k;
+    bool greedy, nothing, infinite, by_p, by_k, small_k;
 
+    WQ8_DEVICE double finite_weight(float l) const { return power_of_2((double(l) - double(top)) * inverse); }  // of a row whose largest logit is finite
     WQ8_DEVICE double weight(float l) const {
-        if (l == top) return 1.0;
-        const double z = (double(l) - double(top)) * inverse;
-        return exp_below_0(z);
+        return infinite ? l == top ? 1.0 : 0.0 : finite_weight(l);
     }
     // the nearest whole number of w * scale <= 2^44, from the low bits of its sum with 2^52
     WQ8_DEVICE uint64_t units(double w) const { return __builtin_bit_cast(uint64_t, __builtin_fma(w, scale, 0x1p52)) - 0x4330000000000000ull; }
@@ -111,19 +126,25 @@ WQ8_DEVICE uint64_t sum64(uint64_t v) {
     return halves(rows(v));
 }
 
+// The largest of the wave's values
+WQ8_DEVICE uint64_t wave_most(uint64_t v) {
+#pragma unroll
+    for (int step = 32; step; step >>= 1) v = max64(v, __shfl_xor(v, step));
+    return v;
+}
+
 WQ8_DEVICE Row read_row(const SampleArgs& p, const SampleRow& state, int row) {
     Row r;
     const int lane = threadIdx.x & 63;
-    uint64_t best = lane < p.splits ? state.largest[lane] : 0;
-#pragma unroll
-    for (int step = 32; step; step >>= 1) best = max64(best, __shfl_xor(best, step));
-    r.first = best;
+    const uint64_t best = wave_most(lane < p.splits ? state.largest[lane] : 0);  // order, and the index upside down
+    r.first = int(0xffffffffu - uint32_t(best));
     r.top = order_logit(uint32_t(best >> 32));
+    r.infinite = r.top == __builtin_inff();
     const float t = p.temperature ? p.temperature[row] : p.temperature0;
     r.greedy = !(t > 0.0f);
     r.nothing = uint32_t(best >> 32) <= logit_order(-__builtin_inff());
-    r.inverse = 1.0 / double(t);
-    r.bins = fminf(float(r.inverse) * BINS_PER_UNIT, 0x1.fffffep127f);  // (an infinity would part equal logits from others beside them)
+    r.inverse = 0x1.71547652b82fep+0 / double(t);
+    r.bins = fminf(float(1.0 / double(t)) * BINS_PER_UNIT, 0x1.fffffep127f);  // (an infinity would part equal logits from others beside them)
     r.scale = double(uint64_t(1) << p.shift);
     r.min_p = fmin(double(p.min_p ? p.min_p[row] : p.min_p0), 1.0);
     r.top_p = p.top_p ? p.top_p[row] : p.top_p0;
@@ -135,28 +156,30 @@ WQ8_DEVICE Row read_row(const SampleArgs& p, const SampleRow& state, int row) {
 }
 
 // f(logit, index) for the row's values from begin to end, 8 neighbouring ones a thread at a time, four times that asked for together; after(i) behind
-// every 2048, i the first of them. Rows may begin at any value: the loads of 16 bytes are as unaligned as the row is.
+// every 2048, i the first of them. Past the end f has NaN. Rows may begin at any value: the loads of 16 bytes are as unaligned as the row is.
 template <int DT, typename F, typename After> WQ8_DEVICE void each_logit(const SampleArgs& p, int row, int begin, int end, const F& f, const After& after) {
     using raw = typename Elem<DT>::raw;
     constexpr int AHEAD = 4;
     const raw* values = static_cast<const raw*>(p.logits) + row * p.ld;
+    raw none;
+    if constexpr (DT == DT_F32) none = __builtin_nanf("");
+    else none = 0x7fff;
     for (int first = begin; first < end; first += AHEAD * SAMPLE_PIECE) {
         raw v[AHEAD][8];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             const int i = first + u * SAMPLE_PIECE + 8 * int(threadIdx.x);
             if (i + 8 <= end) __builtin_memcpy(v[u], values + i, sizeof(v[u]));
-            else if (i < end)
+            else
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[u][j] = values[min(i + j, end - 1)];
+                for (int j = 0; j < 8; ++j) v[u][j] = i + j < end ? values[i + j] : none;
         }
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             const int i = first + u * SAMPLE_PIECE + 8 * int(threadIdx.x);
             if (first + u * SAMPLE_PIECE >= end) break;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (i + j < end) f(Elem<DT>::to_f(v[u][j]), i + j);
+            for (int j = 0; j < 8; ++j) f(Elem<DT>::to_f(v[u][j]), i + j);
             after(first + u * SAMPLE_PIECE);
         }
     }
@@ -179,8 +202,7 @@ template <int DT> __global__ void __launch_bounds__(256) sample_largest(SampleAr
         if (o > most) most = o, at = i;  // (a thread's indices rise: the first of equal ones stays)
     });
     uint64_t best = uint64_t(most) << 32 | (0xffffffffu - uint32_t(at));
-#pragma unroll
-    for (int step = 32; step; step >>= 1) best = max64(best, __shfl_xor(best, step));
+    best = wave_most(best);
     if (!(threadIdx.x & 63)) best4[threadIdx.x >> 6] = best;
     __syncthreads();
     if (!threadIdx.x) state.largest[s] = max64(max64(best4[0], best4[1]), max64(best4[2], best4[3]));
@@ -196,12 +218,22 @@ template <int DT> __global__ void __launch_bounds__(256) sample_bins(SampleArgs 
     if (r.greedy || r.nothing || !(r.by_k || r.by_p)) return;
     for (int b = threadIdx.x; b < SAMPLE_BINS; b += 256) mass[b] = 0, count[b] = 0;
     __syncthreads();
-    each_logit<DT>(p, row, s * p.split, min(p.vocabulary, (s + 1) * p.split), [&](float l, int) {
-        const int b = r.bin(l);  // NaN: the last
-        if (b == SAMPLE_BINS - 1) return;
-        if (r.by_k) atomicAdd(&count[b], 1u);
-        if (!r.small_k) atomicAdd(&mass[b], (unsigned long long)r.units(r.weight(l)));
-    });
+    const int begin = s * p.split, end = min(p.vocabulary, begin + p.split);
+    // (the last bin, NaN's too, weighs nothing and is not counted)
+    if (r.small_k)
+        each_logit<DT>(p, row, begin, end, [&](float l, int) {
+            const int b = r.bin(l);
+            if (b < SAMPLE_BINS - 1) atomicAdd(&count[b], 1u);
+        });
+    else
+        each_logit<DT>(p, row, begin, end, [&](float l, int) {
+            const int b = r.bin(l);
+            const uint64_t units = r.units(r.infinite ? 1.0 : r.finite_weight(l));
+            if (b < SAMPLE_BINS - 1) {
+                if (r.by_k) atomicAdd(&count[b], 1u);
+                atomicAdd(&mass[b], (unsigned long long)units);
+            }
+        });
     __syncthreads();
     for (int b = threadIdx.x; b < SAMPLE_BINS; b += 256) {
         if (count[b]) atomicAdd(&state.count[b], count[b]);
@@ -301,7 +333,7 @@ WQ8_DEVICE Cut find_cut(const Row& r, const SampleRow& state, CutScratch& sc) {
         __syncthreads();
     }
     c.k_bin = sc.k_bin;
-    c.k_left = sc.k_left;
+    c.k_left = c.k_bin < SAMPLE_BINS ? sc.k_left : ~0u;
     c.k_before = sc.k_before;
     if (r.small_k) {  // all up to the k's bin is listed; where the k reach the last bin, all but that
         c.low = c.certain = 0;
@@ -349,40 +381,53 @@ template <int DT> __global__ void __launch_bounds__(256) sample_list(SampleArgs 
     if (c.certain || !cutting)
         for (int i = threadIdx.x; i < SAMPLE_PARTS; i += 256) kept[i] = 0;
     __syncthreads();
+    const int begin = s * p.split, end = min(p.vocabulary, begin + p.split);
+    auto list = [&](float l, int i) {
+        const uint32_t at = atomicAdd(&state.listed, 1u);
+        if (at < uint32_t(SAMPLE_LIST)) state.list[at] = Key<DT>{p.bits}.of(l, i);
+    };
     uint64_t sum = 0;
-    each_logit<DT>(
-        p, row, s * p.split, min(p.vocabulary, (s + 1) * p.split),
-        [&](float l, int i) {
-            if (cutting) {
-                const int b = r.bin(l);
-                if (c.listed(b) && l == l) {
-                    const uint32_t at = atomicAdd(&state.listed, 1u);
-                    if (at < uint32_t(SAMPLE_LIST)) state.list[at] = token_key(l, i);
-                }
-                if (b >= c.certain) return;
-            }
-            const double w = r.weight(l);
-            if (w >= r.min_p) sum += r.units(w);
-        },
-        [&](int i) {
-            if (cutting && !c.certain) return;
-            sum = sum64(sum);
-            if (!(threadIdx.x & 63)) atomicAdd(&kept[i / p.part], (unsigned long long)sum);
-            sum = 0;
+    auto kept_of = [&](double w) { return w >= r.min_p ? r.units(w) : 0; };
+    auto after = [&](int i) {
+        sum = sum64(sum);
+        if (!(threadIdx.x & 63)) atomicAdd(&kept[i / p.part], (unsigned long long)sum);
+        sum = 0;
+    };
+    // a loop for each of what rows need, so that nothing parts the weights of one thread's values (each is a chain of 20 operations)
+    if (cutting && !c.certain)
+        each_logit<DT>(p, row, begin, end, [&](float l, int i) {
+            if (c.listed(r.bin(l)) && l == l) list(l, i);
         });
+    else if (cutting)
+        each_logit<DT>(
+            p, row, begin, end,
+            [&](float l, int i) {
+                const int b = r.bin(l);
+                const uint64_t units = kept_of(r.infinite ? 1.0 : r.finite_weight(l));
+                sum += b < c.certain ? units : 0;  // (of an infinite row, bins beside the first and the last are empty)
+                if (c.listed(b) && l == l) list(l, i);
+            },
+            after);
+    else if (r.infinite)
+        each_logit<DT>(p, row, begin, end, [&](float l, int) { sum += l == r.top ? kept_of(1.0) : 0; }, after);
+    else
+        each_logit<DT>(p, row, begin, end, [&](float l, int) { sum += kept_of(r.finite_weight(l)); }, after);
     __syncthreads();
     const int first = s * (p.split / p.part), last = min(p.parts, first + p.split / p.part);
     for (int i = first + threadIdx.x; i < last; i += 256) state.kept[i] = cutting && !c.certain ? 0 : kept[i];
 }
 
 // ---- 4: the cut among the listed keys, and the token ---------------------------------------------------------------------------
+struct __attribute__((aligned(16))) Listed {
+    uint64_t key, units;
+};
 struct PickScratch {
     CutScratch cut;
-    uint64_t list[SAMPLE_LIST], units[SAMPLE_LIST];
+    Listed list[SAMPLE_LIST];
     unsigned long long mass[256];
     uint32_t count[256];
     unsigned long long kept[SAMPLE_PARTS];
-    unsigned long long lowest, highest, found, need, before;
+    unsigned long long lowest, highest, found, need;
     uint32_t in_digit;
     int digit, part;
     uint64_t part_target;
@@ -391,8 +436,8 @@ struct PickScratch {
 };
 
 // The key at which the running count (by_count) or weight of `each`'s keys, from the largest on, reaches `need` (at least 1, at most their sum): digits of 8
-// bits from the first in which they differ, counts and weights of each digit's values. `above`: the weight of the larger keys.
-template <typename Each> WQ8_DEVICE uint64_t select_key(PickScratch& sc, const Each& each, bool by_count, uint64_t need, uint64_t& above) {
+// bits from the first in which they differ, counts and weights of each digit's values. 
+template <bool BY_COUNT, typename Each> WQ8_DEVICE uint64_t select_key(PickScratch& sc, const Each& each, uint64_t need) {
     const int tid = threadIdx.x;
     if (!tid) sc.lowest = ~0ull, sc.highest = 0;
     __syncthreads();
@@ -414,7 +459,6 @@ template <typename Each> WQ8_DEVICE uint64_t select_key(PickScratch& sc, const E
     __syncthreads();
     const uint64_t differ = sc.lowest ^ sc.highest;
     uint64_t key = sc.highest;
-    above = 0;
     int width = differ ? 64 - __builtin_clzll(differ) : 0;  // the bits above are settled
     while (width) {
         const int shift = max(0, width - 8);
@@ -426,25 +470,28 @@ template <typename Each> WQ8_DEVICE uint64_t select_key(PickScratch& sc, const E
             if ((width < 64 ? k >> width : 0) != settled) return;
             const int d = int(k >> shift) & ((1 << (width - shift)) - 1);
             atomicAdd(&sc.count[d], 1u);
-            atomicAdd(&sc.mass[d], (unsigned long long)units);
+            if (!BY_COUNT) atomicAdd(&sc.mass[d], (unsigned long long)units);
         });
         __syncthreads();
         const int d = 255 - tid;
         const uint32_t n = sc.count[d];
-        const uint64_t m = sc.mass[d];
-        uint32_t counts;
-        uint64_t masses;
-        const uint64_t n_before = scan256(n, sc.waves32, counts), m_before = scan256(m, sc.waves64, masses);
-        const uint64_t before = by_count ? n_before : m_before, here = by_count ? n : m;
+        uint64_t before, here;
+        if (BY_COUNT) {
+            uint32_t all;
+            before = scan256(n, sc.waves32, all);
+            here = n;
+        } else {
+            uint64_t all;
+            here = sc.mass[d];
+            before = scan256(here, sc.waves64, all);
+        }
         if (before < need && before + here >= need) {
             sc.digit = d;
             sc.in_digit = n;
             sc.need = need - before;
-            sc.before = m_before;
         }
         __syncthreads();
         need = sc.need;
-        above += sc.before;
         key = (settled << (width - shift) | uint64_t(sc.digit)) << shift;
         if (sc.in_digit == 1 && shift) {  // one key left: find it
             each([&](uint64_t k, uint64_t) {
@@ -467,7 +514,7 @@ template <int DT> __global__ void __launch_bounds__(256) sample_pick(SampleArgs 
     SampleRow& state = p.rows[row];
     const Row r = read_row(p, state, row);
     if (r.greedy || r.nothing) {
-        if (!tid) p.tokens[row] = r.nothing ? -1 : key_index(r.first);
+        if (!tid) p.tokens[row] = r.nothing ? -1 : r.first;
         return;
     }
     sc.kept[tid] = tid < p.parts ? state.kept[tid] : 0;
@@ -477,6 +524,14 @@ template <int DT> __global__ void __launch_bounds__(256) sample_pick(SampleArgs 
         const uint64_t target = u > 0.0f ? u < 1.0f ? share_of(u, total, false) : total - 1 : 0;
         return target < total ? target : total - 1;
     };
+    const Key<DT> keys{p.bits};
+    auto sum_of = [&](uint64_t v) {  // over the workgroup
+        v = sum64(v);
+        __syncthreads();
+        if (!(tid & 63)) sc.waves64[tid >> 6] = v;
+        __syncthreads();
+        return sc.waves64[0] + sc.waves64[1] + sc.waves64[2] + sc.waves64[3];
+    };
     uint64_t cut = 0;  // keys from it on stay
     if (r.by_k || r.by_p) {
         const Cut c = find_cut(r, state, sc.cut);
@@ -485,79 +540,77 @@ template <int DT> __global__ void __launch_bounds__(256) sample_pick(SampleArgs 
         if (whole)
             for (int i = tid; i < int(listed); i += 256) {
                 const uint64_t key = state.list[i];
-                sc.list[i] = key;
-                sc.units[i] = r.units(r.weight(order_logit(uint32_t(key >> 32))));
+                sc.list[i] = {key, r.units(r.weight(keys.logit(key)))};
             }
-        __syncthreads();
-        if (whole && listed <= uint32_t(SHORT_LIST) && r.small_k) {
-            // few keys, all that may stay: each against all others, for its place, the weight before it, and the weight up to it in the vocabulary's order
-            const int n = int(listed);
-            const uint64_t key = tid < n ? sc.list[tid] : 0, mine = tid < n ? sc.units[tid] : 0;
-            uint32_t place = 0;
-            uint64_t before = 0;
-            for (int j = 0; j < n; ++j)
-                if (sc.list[j] > key) ++place, before += sc.units[j];
-            bool stays = tid < n && place < uint32_t(r.top_k);
-            auto add = [&](uint64_t v) {
-                v = sum64(v);
-                __syncthreads();
-                if (!(tid & 63)) sc.waves64[tid >> 6] = v;
-                __syncthreads();
-                return sc.waves64[0] + sc.waves64[1] + sc.waves64[2] + sc.waves64[3];
-            };
-            uint64_t total = add(stays ? mine : 0);
-            if (r.by_p) stays = stays && before < wanted_mass(r.top_p, total);
-            stays = stays && r.weight(order_logit(uint32_t(key >> 32))) >= r.min_p;
-            total = add(stays ? mine : 0);
-            if (tid < n) sc.units[tid] = stays ? mine : 0;
-            __syncthreads();
-            const uint64_t target = drawn(total);
-            uint64_t upto = 0;
-            for (int j = 0; j < n; ++j)
-                if (uint32_t(sc.list[j]) >= uint32_t(key)) upto += sc.units[j];  // (the index's complement: lower ones, and itself)
-            if (stays && upto > target && upto - mine <= target) p.tokens[row] = key_index(key);
-            return;
-        }
-        // the listed keys of some of the bins; where they are too many for the list (logits that are alike), the row is read again instead
-        auto each = [&](int from, int to, const auto& f) {
-            if (whole) {
-                for (int i = tid; i < int(listed); i += 256) {
-                    const int b = r.bin(order_logit(uint32_t(sc.list[i] >> 32)));
-                    if (b >= from && b <= to) f(sc.list[i], sc.units[i]);
-                }
-            } else {
-                each_logit<DT>(p, row, 0, p.vocabulary, [&](float l, int i) {
-                    if (l != l) return;
-                    const int b = r.bin(l);
-                    if (b >= from && b <= to) f(token_key(l, i), r.units(r.weight(l)));
-                });
-            }
-        };
-        uint64_t total = 0, above;
-        if (r.small_k) {
-            uint64_t all = 0;
-            uint32_t n = 0;
-            each(c.low, c.high, [&](uint64_t, uint64_t units) { all += units, ++n; });
-            uint32_t counted;
-            scan256(all, sc.waves64, total);
-            scan256(n, sc.waves32, counted);
-            if (counted > uint32_t(r.top_k)) {
-                cut = select_key(sc, [&](const auto& f) { each(c.low, c.high, f); }, true, r.top_k, above);
-                total = above + r.units(r.weight(order_logit(uint32_t(cut >> 32))));
-            } else cut = 1;  // fewer than k weigh anything: all of them stay
-        } else if (c.k_bin < SAMPLE_BINS) {
-            cut = select_key(sc, [&](const auto& f) { each(c.k_bin, c.k_bin, f); }, true, c.k_left, above);
-            total = c.k_before + above + r.units(r.weight(order_logit(uint32_t(cut >> 32))));
-        } else if (r.by_p) {
+        uint64_t total = 0;  // of what top-p is taken
+        if (r.by_p && !r.by_k || r.by_p && !r.small_k && c.k_bin == SAMPLE_BINS) {
             uint64_t mass = 0;
             for (int b = tid; b < SAMPLE_BINS; b += 256) mass += state.mass[b];
-            scan256(mass, sc.waves64, total);
+            total = sum_of(mass);
         }
-        if (r.by_p) cut = select_key(sc, [&](const auto& f) { each(c.low, c.high, f); }, false, wanted_mass(r.top_p, total) - c.low_before, above);
-        if (cut) {
-            const int from = c.certain, to = r.by_p || r.small_k ? c.high : c.k_bin;
+        const int from = c.certain, to = r.by_p || r.small_k ? c.high : c.k_bin;  // the bins of the keys that may stay and are not certain to
+        if (c.k_bin == SAMPLE_BINS && !r.by_p && !r.small_k) {
+            // a k that leaves nothing out
+        } else if (whole && listed <= uint32_t(SHORT_LIST) && (r.small_k || c.k_bin == SAMPLE_BINS || !r.by_p)) {
+            // few keys, of one run of bins: each against all others, for its place and the weight before it
+            const int n = int(listed), padded = (n + 7) / 8 * 8;
+            if (tid >= n && tid < padded) sc.list[tid] = {0, 0};
+            __syncthreads();
+            const Listed mine = tid < n ? sc.list[tid] : Listed{0, 0};
+            uint32_t place = 0;
+            uint64_t before = 0;
+            for (int j = 0; j < padded; j += 8)
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const Listed other = sc.list[j + u];
+                    const bool ahead = other.key > mine.key;
+                    place += ahead;
+                    before += ahead ? other.units : 0;
+                }
+            bool stays = tid < n && (!r.by_k || place < c.k_left);
+            if (r.by_p) {
+                if (r.small_k) total = sum_of(stays ? mine.units : 0);
+                stays = stays && c.low_before + before < wanted_mass(r.top_p, total);
+            }
+            uint64_t last = stays ? ~mine.key : 0;  // the largest of these is the smallest key
+            last = wave_most(last);
+            __syncthreads();
+            if (!(tid & 63)) sc.waves64[tid >> 6] = last;
+            __syncthreads();
+            cut = ~max64(max64(sc.waves64[0], sc.waves64[1]), max64(sc.waves64[2], sc.waves64[3]));
+            __syncthreads();
+            if (stays && r.weight(keys.logit(mine.key)) >= r.min_p) atomicAdd(&sc.kept[keys.index(mine.key) / p.part], (unsigned long long)mine.units);
+        } else {
+            __syncthreads();
+            // the listed keys of some of the bins; where they are too many for the list (logits that are alike), the row is read again instead
+            auto each = [&](int low, int high, const auto& f) {
+                if (whole) {
+                    for (int i = tid; i < int(listed); i += 256) {
+                        const Listed one = sc.list[i];
+                        const int b = r.bin(keys.logit(one.key));
+                        if (b >= low && b <= high) f(one.key, one.units);
+                    }
+                } else {
+                    each_logit<DT>(p, row, 0, p.vocabulary, [&](float l, int i) {
+                        const int b = r.bin(l);
+                        if (l == l && b >= low && b <= high) f(keys.of(l, i), r.units(r.weight(l)));
+                    });
+                }
+            };
+            if (c.k_bin < SAMPLE_BINS) {
+                const int low = r.small_k ? 0 : c.k_bin;
+                cut = select_key<true>(sc, [&](const auto& f) { each(low, c.k_bin, f); }, c.k_left);
+                uint64_t upto = 0;
+                each(low, c.k_bin, [&](uint64_t key, uint64_t units) { upto += key >= cut ? units : 0; });
+                total = c.k_before + sum_of(upto);
+            } else if (r.small_k) {  // fewer than k weigh anything: all of them stay
+                uint64_t all = 0;
+                each(c.low, c.high, [&](uint64_t, uint64_t units) { all += units; });
+                total = sum_of(all);
+            }
+            if (r.by_p) cut = select_key<false>(sc, [&](const auto& f) { each(c.low, c.high, f); }, wanted_mass(r.top_p, total) - c.low_before);
             each(from, to, [&](uint64_t key, uint64_t units) {
-                if (key >= cut && r.weight(order_logit(uint32_t(key >> 32))) >= r.min_p) atomicAdd(&sc.kept[key_index(key) / p.part], (unsigned long long)units);
+                if (key >= cut && r.weight(keys.logit(key)) >= r.min_p) atomicAdd(&sc.kept[keys.index(key) / p.part], (unsigned long long)units);
             });
         }
     }
@@ -582,7 +635,7 @@ template <int DT> __global__ void __launch_bounds__(256) sample_pick(SampleArgs 
         for (int j = 0; j < 8; ++j) {
             const int i = begin + 8 * tid + j;
             const float l = Elem<DT>::to_f(values[min(i, end - 1)]);
-            const double w = i < end && l == l && token_key(l, i) >= cut ? r.weight(l) : 0.0;
+            const double w = i < end && l == l && keys.of(l, i) >= cut ? r.weight(l) : 0.0;
             units[j] = w >= r.min_p ? r.units(w) : 0;
             mine += units[j];
         }
@@ -631,7 +684,7 @@ WQ8_API int wq8_sample(const void* logits, int64_t ld, int dtype, const float* d
     int bits = 0;
     while ((1 << bits) < vocabulary) ++bits;
     const SampleArgs p{logits, ld, draws, temperature, static_cast<const int32_t*>(top_k), top_p, min_p, static_cast<SampleRow*>(workspace), tokens,
-                       temperature0, top_p0, min_p0, top_k0, vocabulary, part, parts, split, splits, bits <= 18 ? 44 : 62 - bits};
+                       temperature0, top_p0, min_p0, top_k0, vocabulary, bits, part, parts, split, splits, bits <= 18 ? 44 : 62 - bits};
     if (dtype == DT_F16) return launch_sample<DT_F16>(p, rows, stream);
     if (dtype == DT_BF16) return launch_sample<DT_BF16>(p, rows, stream);
     return launch_sample<DT_F32>(p, rows, stream);
