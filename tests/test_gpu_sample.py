@@ -190,3 +190,15 @@ def test_captured_and_on_two_streams(wq):
     torch.cuda.synchronize()
     for tokens, (l, u, _) in zip(found, inputs):
         assert torch.equal(tokens.cpu(), defined(l, u, top_k=50, top_p=0.9))
+
+
+@pytest.mark.parametrize("vocabulary", [1500, 9000, 20000])
+def test_lists_in_lds_in_memory_and_too_long(wq, vocabulary):
+    """All of a row's logits in two or three bins: lists of keys of up to 2048, up to 16384, and rows that are read again."""
+    g = torch.Generator(device="cuda").manual_seed(vocabulary)
+    logits = torch.rand(5, vocabulary, generator=g, device="cuda") * 0.05
+    draws = torch.rand(5, generator=g, device="cuda")
+    for dtype in (FP32, BF16, FP16):
+        l = logits.to(dtype)
+        for options in ({"top_k": vocabulary // 3}, {"top_k": 700, "top_p": 0.4}, {"top_p": 0.6}, {"top_k": vocabulary // 2, "top_p": 0.5, "min_p": 0.97}, {"top_k": 1000}):
+            assert torch.equal(wq.sample(l, draws, **options).cpu(), defined(l, draws, **options)), (dtype, options)

@@ -15,7 +15,7 @@
 
 namespace wq8 {
 
-constexpr int SAMPLE_BINS = 1024, SAMPLE_SPLITS = 64, SAMPLE_PARTS = 256, SAMPLE_LIST = 2048, SAMPLE_PIECE = 2048, SMALL_K = 1024, SHORT_LIST = 128;
+constexpr int SAMPLE_BINS = 1024, SAMPLE_SPLITS = 64, SAMPLE_PARTS = 256, SAMPLE_LIST = 2048, MOST_LISTED_KEYS = 16384, SAMPLE_PIECE = 2048, SMALL_K = 1024, SHORT_LIST = 128;
 constexpr float BINS_PER_UNIT = 32.0f;  // the last bin begins at 31.97: weights below 2^-46, held as 0
 
 struct SampleRow {  // a row's workspace
@@ -23,7 +23,6 @@ struct SampleRow {  // a row's workspace
     uint64_t kept[SAMPLE_PARTS];  // the weight kept of each part
     uint64_t mass[SAMPLE_BINS];
     uint32_t count[SAMPLE_BINS];
-    uint64_t list[SAMPLE_LIST];
     uint32_t listed, unused;
 };
 
@@ -36,10 +35,11 @@ struct SampleArgs {
     const float* top_p;
     const float* min_p;
     SampleRow* rows;
+    uint64_t* lists;   // `capacity` keys a row
     int64_t* tokens;
     float temperature0, top_p0, min_p0;
     int top_k0;
-    int vocabulary, bits, part, parts, split, splits, shift;  // indices have `bits`; parts of `part` tokens, splits of `split`, a multiple of that
+    int vocabulary, capacity, bits, part, parts, split, splits, shift;  // indices have `bits`; parts of `part` tokens, splits of `split`, a multiple of that
 };
 
 // The order of a logit: larger numbers for larger logits, 0 for NaN; both zeros alike.
@@ -384,7 +384,7 @@ template <int DT> __global__ void __launch_bounds__(256) sample_list(SampleArgs 
     const int begin = s * p.split, end = min(p.vocabulary, begin + p.split);
     auto list = [&](float l, int i) {
         const uint32_t at = atomicAdd(&state.listed, 1u);
-        if (at < uint32_t(SAMPLE_LIST)) state.list[at] = Key<DT>{p.bits}.of(l, i);
+        if (at < uint32_t(p.capacity)) p.lists[int64_t(row) * p.capacity + at] = Key<DT>{p.bits}.of(l, i);
     };
     uint64_t sum = 0;
     auto kept_of = [&](double w) { return w >= r.min_p ? r.units(w) : 0; };
@@ -536,10 +536,11 @@ template <int DT> __global__ void __launch_bounds__(256) sample_pick(SampleArgs 
     if (r.by_k || r.by_p) {
         const Cut c = find_cut(r, state, sc.cut);
         const uint32_t listed = state.listed;
-        const bool whole = listed <= uint32_t(SAMPLE_LIST);
+        const bool whole = listed <= uint32_t(SAMPLE_LIST);  // they fit into LDS
+        const uint64_t* keys_listed = p.lists + int64_t(row) * p.capacity;
         if (whole)
             for (int i = tid; i < int(listed); i += 256) {
-                const uint64_t key = state.list[i];
+                const uint64_t key = keys_listed[i];
                 sc.list[i] = {key, r.units(r.weight(keys.logit(key)))};
             }
         uint64_t total = 0;  // of what top-p is taken
@@ -582,13 +583,21 @@ template <int DT> __global__ void __launch_bounds__(256) sample_pick(SampleArgs 
             if (stays && r.weight(keys.logit(mine.key)) >= r.min_p) atomicAdd(&sc.kept[keys.index(mine.key) / p.part], (unsigned long long)mine.units);
         } else {
             __syncthreads();
-            // the listed keys of some of the bins; where they are too many for the list (logits that are alike), the row is read again instead
+            // the listed keys of some of the bins, from LDS or from memory; where they are too many for the list (logits that are alike), the row is read
+            // again instead
             auto each = [&](int low, int high, const auto& f) {
                 if (whole) {
                     for (int i = tid; i < int(listed); i += 256) {
                         const Listed one = sc.list[i];
                         const int b = r.bin(keys.logit(one.key));
                         if (b >= low && b <= high) f(one.key, one.units);
+                    }
+                } else if (listed <= uint32_t(p.capacity)) {
+                    for (int i = tid; i < int(listed); i += 256) {
+                        const uint64_t key = keys_listed[i];
+                        const float l = keys.logit(key);
+                        const int b = r.bin(l);
+                        if (b >= low && b <= high) f(key, r.units(r.weight(l)));
                     }
                 } else {
                     each_logit<DT>(p, row, 0, p.vocabulary, [&](float l, int i) {
@@ -656,6 +665,12 @@ template <int DT> __global__ void __launch_bounds__(256) sample_pick(SampleArgs 
 
 using namespace wq8;
 
+// Keys listed a row: as many as LDS holds, and more of few rows (1 GiB of lists in all)
+static int list_capacity(int rows) {
+    const int64_t fit = (int64_t(1) << 27) / (rows > 0 ? rows : 1);
+    return int(fit < SAMPLE_LIST ? SAMPLE_LIST : fit > MOST_LISTED_KEYS ? MOST_LISTED_KEYS : fit);
+}
+
 template <int DT> static int launch_sample(const SampleArgs& p, int rows, hipStream_t stream) {
     sample_largest<DT><<<rows * p.splits, 256, 0, stream>>>(p);
     if (const int rc = int(hipGetLastError())) return rc;
@@ -683,14 +698,15 @@ WQ8_API int wq8_sample(const void* logits, int64_t ld, int dtype, const float* d
     splits = (vocabulary + split - 1) / split;
     int bits = 0;
     while ((1 << bits) < vocabulary) ++bits;
-    const SampleArgs p{logits, ld, draws, temperature, static_cast<const int32_t*>(top_k), top_p, min_p, static_cast<SampleRow*>(workspace), tokens,
-                       temperature0, top_p0, min_p0, top_k0, vocabulary, bits, part, parts, split, splits, bits <= 18 ? 44 : 62 - bits};
+    const SampleArgs p{logits, ld, draws, temperature, static_cast<const int32_t*>(top_k), top_p, min_p, static_cast<SampleRow*>(workspace),
+                       reinterpret_cast<uint64_t*>(static_cast<SampleRow*>(workspace) + rows), tokens,
+                       temperature0, top_p0, min_p0, top_k0, vocabulary, list_capacity(rows), bits, part, parts, split, splits, bits <= 18 ? 44 : 62 - bits};
     if (dtype == DT_F16) return launch_sample<DT_F16>(p, rows, stream);
     if (dtype == DT_BF16) return launch_sample<DT_BF16>(p, rows, stream);
     return launch_sample<DT_F32>(p, rows, stream);
 }
 
 WQ8_API void wq8_sample_workspace(int rows, int64_t* sizes) {
-    sizes[0] = int64_t(rows) * int64_t(sizeof(SampleRow));
+    sizes[0] = int64_t(rows) * (int64_t(sizeof(SampleRow)) + int64_t(list_capacity(rows)) * 8);
     sizes[1] = 0;
 }
