@@ -97,6 +97,9 @@ EXPERTS = {
     "residual shape": {"residual": rows(1, 64)},
     "residual_scale alone": {"residual_scale": torch.zeros(64, dtype=BF16)},
     "residual_scale": {"residual": rows(3, 64), "residual_scale": torch.zeros(64)},
+    "spans 2 GiB": {"x": torch.zeros(3, 32768, dtype=BF16), "gate_up": torch.zeros(1, 65536, 32768, dtype=torch.int8, device="meta"),
+                    "gate_up_scale": torch.zeros(1, 65536, device="meta"), "down": torch.zeros(1, 32768, 32768, dtype=torch.int8, device="meta"),
+                    "down_scale": torch.zeros(1, 32768, device="meta")},
     "cpu": {},
 }
 
@@ -155,3 +158,35 @@ SAMPLE = {
 def test_sample_refuses(change):
     with pytest.raises(ValueError):
         wq.sample(**{"logits": torch.zeros(3, 5), "draws": torch.zeros(3), **SAMPLE[change]})
+
+
+def test_a_launch_has_its_device_current(monkeypatch):
+    """call_on() makes the tensors' GPU the current one around a call, and only where it is not."""
+    from wgpkernels_amd.int8 import _native
+    seen, entered = [], []
+
+    class Device:
+        def __init__(self, index):
+            entered.append(index)
+
+        def __enter__(self):
+            seen.append("in")
+
+        def __exit__(self, *_):
+            seen.append("out")
+
+    class Library:
+        def call(self, name, *args):
+            seen.append((name, args))
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    _native.call_on(Library(), 0, "a", 1)
+    _native.call_on(Library(), 1, "b", 2)
+    assert seen == [("a", (1,)), "in", ("b", (2,)), "out"] and entered == [1]
+
+
+def test_most_values_of_top_k():
+    """A top_k beyond the C interface's 32 bits is all of the vocabulary, not its low bits."""
+    from wgpkernels_amd.int8 import _sample
+    assert min(2 ** 32 + 3, _sample.MAX_VOCABULARY) == 2 ** 24 and _sample._pair(min(2 ** 32 + 3, _sample.MAX_VOCABULARY)) == (None, 2 ** 24)

@@ -22,7 +22,8 @@ linear() picks a path per GPU, shape and token-count bucket by timing the candid
 
 Next to the linears stands the attention side of a step (no counterpart in the reference): rotary() turns queries and keys
 by positions on one to three axes (_rotary.py), and a paged cache holds keys and values in 8 bits (_kvcache.py): kv_plan(),
-kv_write(), kv_read(), kv_attention().
+kv_write(), kv_read(), kv_attention(). The rest of a decode step: add_prepare() adds a branch to the residual stream on its way into
+a linear (_added.py), route() and experts() are a mixture-of-experts layer of INT8 weights (_experts.py), sample() draws the next tokens (_sample.py).
 """
 import ctypes
 import functools

@@ -92,8 +92,9 @@ def add_prepare(x, residual, residual_scale=None, group=0, path="block", act_wei
         values = x.new_empty((m, k), dtype=torch.int8)
         scale = x.new_empty(m if mode else (m, (k + 127) // 128), dtype=torch.float32)
         lo = torch.empty_like(values) if path == "exact" else None
-    library().call("wq8_add_prepare", x_at, ldx, residual_at, ldr, scale_at, out.data_ptr(), lds, mode, values.data_ptr(), _native.ptr(lo),
-                   _native.ptr(scale), m, k, dtype, group, weight_at, eps, _native.gpu(x).stream())
+    state = _native.gpu(x)
+    _native.call_on(library(), state.index, "wq8_add_prepare", x_at, ldx, residual_at, ldr, scale_at, out.data_ptr(), lds, mode, values.data_ptr(), _native.ptr(lo),
+                   _native.ptr(scale), m, k, dtype, group, weight_at, eps, state.stream())
     return Prepared(path, values, lo, scale, x.dtype), out
 
 
@@ -111,6 +112,7 @@ def prepared_values(prepared):
         raise ValueError("prepared codes must be 8-byte aligned")
     _check_devices(q, scale)
     out = torch.empty((m, k), dtype=prepared.dtype, device=q.device)
-    library().call("wq8_prepared_values", q.data_ptr(), _native.ptr(lo), scale.data_ptr(), out.data_ptr(), m, k, blocks, DTYPES[prepared.dtype],
-                   _native.gpu(q).stream())
+    state = _native.gpu(q)
+    _native.call_on(library(), state.index, "wq8_prepared_values", q.data_ptr(), _native.ptr(lo), scale.data_ptr(), out.data_ptr(), m, k, blocks, DTYPES[prepared.dtype],
+                   state.stream())
     return out

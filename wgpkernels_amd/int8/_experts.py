@@ -64,8 +64,9 @@ def route(x, router, top, score="softmax", bias=None, normalise=True, factor=1.0
     ids = x.new_empty((tokens, top), dtype=torch.int32)
     weights = x.new_empty((tokens, top), dtype=torch.float32)
     logits = x.new_empty(workspace_bytes, dtype=torch.uint8)
-    library().call("wq8_route", x_at, ldx, dtype, router_at, router_dtype, _native.ptr(bias), tokens, count, k, top, SCORES[score], normalise, factor,
-                   logits.data_ptr(), ids.data_ptr(), weights.data_ptr(), _native.gpu(x).stream())
+    state = _native.gpu(x)
+    _native.call_on(library(), state.index, "wq8_route", x_at, ldx, dtype, router_at, router_dtype, _native.ptr(bias), tokens, count, k, top, SCORES[score], normalise, factor,
+                   logits.data_ptr(), ids.data_ptr(), weights.data_ptr(), state.stream())
     return Routes(ids, weights)
 
 
@@ -102,6 +103,8 @@ def _check_experts(x, ids, weights, gate_up, gate_up_scale, down, down_scale, re
         raise ValueError("routes must be contiguous")
     if ids.shape[1] < 1 or ids.numel() > MAX_CHOICES:
         raise ValueError(f"experts() takes at most {MAX_CHOICES} choices (tokens x top) a call, not {tuple(ids.shape)}")
+    if both * k >= 2 ** 31 or ((x.shape[0] - 1) * _row_pitch(x) + k) * 2 >= 2 ** 31 or ids.numel() * both * 2 >= 2 ** 31:
+        raise ValueError("an expert's matrices, the rows as they lie and the hidden values must each span less than 2 GiB")
     _check_devices(*[t for t in (x, ids, weights, gate_up, gate_up_scale, down, down_scale, residual, residual_scale) if t is not None])
     tokens, top = ids.shape
     library().wq8_experts_workspace(tokens, top, k, both // 2, _sizes)
@@ -135,6 +138,7 @@ def experts(x, routes, gate_up, gate_up_scale, down, down_scale, residual=None, 
         _check_sum(out, x, x if residual is None else residual)
         ldo = _row_pitch(out)
     workspace = x.new_empty(workspace_bytes, dtype=torch.uint8)
-    library().call("wq8_experts", x_at, ldx, dtype, ids.data_ptr(), weights.data_ptr(), gate_up_at, gate_up_scale.data_ptr(), down_at, down_scale.data_ptr(),
-                   residual_at, ldr, _native.ptr(residual_scale), out.data_ptr(), ldo, tokens, top, count, k, hidden, workspace.data_ptr(), _native.gpu(x).stream())
+    state = _native.gpu(x)
+    _native.call_on(library(), state.index, "wq8_experts", x_at, ldx, dtype, ids.data_ptr(), weights.data_ptr(), gate_up_at, gate_up_scale.data_ptr(), down_at, down_scale.data_ptr(),
+                   residual_at, ldr, _native.ptr(residual_scale), out.data_ptr(), ldo, tokens, top, count, k, hidden, workspace.data_ptr(), state.stream())
     return out

@@ -109,6 +109,14 @@ class Library:
             raise_code(code, name)
 
 
+def call_on(library, index, name, *args):
+    """library.call() with GPU `index` the current one: a launch goes by the current device's code, whatever its stream."""
+    if torch._C._cuda_getDevice() == index:
+        return library.call(name, *args)
+    with torch.cuda.device(index):
+        return library.call(name, *args)
+
+
 def load_test_library(path=None):
     """libwgp_int8_test.so (built with `python -m wgpkernels_amd.build --library int8_test`): the test-only entry points
     of include/wq8_test.h, for the parity tests and bench.py."""

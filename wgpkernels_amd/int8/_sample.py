@@ -62,6 +62,7 @@ def sample(logits, draws, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     rows, vocabulary, ld, dtype, workspace_bytes = _layouts.get(key) or _layouts.keep(key, _check_sample(logits, draws, temperature, top_k, top_p, min_p))
     tokens = draws.new_empty(rows, dtype=torch.int64)
     workspace = draws.new_empty(workspace_bytes, dtype=torch.uint8)
-    library().call("wq8_sample", logits.data_ptr(), ld, dtype, draws.data_ptr(), *_pair(temperature), *_pair(top_k), *_pair(top_p), *_pair(min_p), rows,
-                   vocabulary, tokens.data_ptr(), workspace.data_ptr(), _native.gpu(logits).stream())
+    state = _native.gpu(logits)
+    _native.call_on(library(), state.index, "wq8_sample", logits.data_ptr(), ld, dtype, draws.data_ptr(), *_pair(temperature), *_pair(top_k if isinstance(top_k, torch.Tensor) else min(top_k, MAX_VOCABULARY)), *_pair(top_p), *_pair(min_p), rows,
+                   vocabulary, tokens.data_ptr(), workspace.data_ptr(), state.stream())
     return tokens

@@ -714,7 +714,6 @@ WQ8_API int wq8_experts(const void* x, int64_t ldx, int dtype, const void* ids, 
     if (int64_t(2) * hidden * k >= 1ll << 31 || ((tokens - 1) * ldx + k) * 2 >= 1ll << 31 || int64_t(tokens) * top * hidden * 4 >= 1ll << 31) return -2;
     const int pairs = tokens * top, slots = pairs <= experts ? pairs : experts;
     const int64_t h_bytes = (int64_t(pairs) * hidden * 4 + 255) / 256 * 256;
-    if (int64_t(slots) * (hidden / 16) > MAX_BLOCKS_256 || int64_t(slots) * ((k + 31) / 32) > MAX_BLOCKS_256 || int64_t(tokens) * (k / 4) > MAX_BLOCKS_256 * 64) return -2;
     const ExpertsArgs p{x, static_cast<const int32_t*>(ids), weights, gate_up, gate_up_scale, down, down_scale, static_cast<uint16_t*>(workspace),
                         reinterpret_cast<float*>(static_cast<char*>(workspace) + h_bytes), residual, rscale, out, ldx, ldr, ldo, tokens, top, experts, k, hidden};
     // tiles that waves share only where there are few, of 8 tokens at most
@@ -723,6 +722,9 @@ WQ8_API int wq8_experts(const void* x, int64_t ldx, int dtype, const void* ids, 
     // an expert of more tokens than a workgroup takes at once: other workgroups take the next ones
     const auto passes = [&](int most) { return tokens <= most ? 1 : tokens <= 2 * most ? 2 : 4; };
     const int up_passes = up ? passes(64) : 1, down_passes = down_own ? passes(64) : 1;
+    if (int64_t(slots) * up_groups * up_passes > MAX_BLOCKS_256 || int64_t(slots) * down_groups * down_passes > MAX_BLOCKS_256 ||
+        int64_t(tokens) * (k / 4) > 1ll << 30)
+        return -2;
     if (dtype == DT_F16) experts_up<DT_F16><<<slots * up_groups * up_passes, 256, 0, stream>>>(p, up, up_passes);
     else experts_up<DT_BF16><<<slots * up_groups * up_passes, 256, 0, stream>>>(p, up, up_passes);
     if (const int rc = int(hipGetLastError())) return rc;
