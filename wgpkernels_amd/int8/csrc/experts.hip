@@ -40,7 +40,8 @@ template <int DT> struct Eight {
 
 // Logits of 16 tokens x 16 experts over a part of K, in FP64 (the choice between near experts is a whole number: in FP32 one in some 10^4 tokens
 // would go by the order of the sum). 8 waves take 32 values of every row in turn; their sums are added in order, the parts by route_choose. Matrix
-// instructions of FP64 set the time (64 cycles for 4 values): parts short enough to fill the CUs.
+// instructions of FP64 set the time (64 cycles for 4 values): parts short enough to fill the CUs (64 experts over 2048
+// values 3.1 us, 7.3 with whole rows a workgroup).
 constexpr int ROUTE_WAVES = 8, ROUTE_STEP = 32 * ROUTE_WAVES;
 template <int XT, int RT>
 __global__ void __launch_bounds__(64 * ROUTE_WAVES) route_logits(RouteArgs p) {
@@ -108,7 +109,8 @@ WQ8_DEVICE double lane_value(double v, int lane) {  // lane the same for all
                                           uint32_t(__builtin_amdgcn_readlane(int(uint32_t(b)), lane)));
 }
 
-// Scores, choice and weights of a token a wave; a lane holds NE neighbouring experts.
+// Scores, choice and weights of a token a wave; a lane holds NE neighbouring experts. Bound by its chain of operations: 8 of 64 experts 3.7 us (6 with
+// exchanges through LDS).
 template <int NE>
 __global__ void __launch_bounds__(256) route_choose(RouteArgs p) {
     const int lane = threadIdx.x & 63, token = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -285,7 +287,8 @@ WQ8_DEVICE int find_choices(const ExpertsArgs& p, int slot, int expert, int firs
 
 // Two tiles of 16 weight rows on up to CAP tokens (PLANES rows each). The four waves of a workgroup take slices of SLICE values of the width in
 // turn, each through a ring of its own in LDS, filled by copies that pass the registers by: no wave waits for another one until the
-// end, where the four sums of every output are added in order. 16-byte chunks are placed by their row so that the 16 lanes that read one chunk of
+// end, where the four sums of every output are added in order. HBM bounds it, and at these sizes the latency of a workgroup's beginning: one token, 8 of 64 experts of
+// 2048 x 1024, gate and up 9.2 us for 33.6 MB (3.6 TB/s). 16-byte chunks are placed by their row so that the 16 lanes that read one chunk of
 // 16 rows meet different banks.
 constexpr int RING = 19 * 1024;  // a wave's: two workgroups a CU
 constexpr uint32_t OUT_OF_RANGE = 0x80000000u;
@@ -363,7 +366,9 @@ WQ8_DEVICE void ring_rows(sgpr4 rw, int row0, int row1, int width, sgpr4 rx, uin
     if (!wave) done(((a0 + red[0]) + red[128]) + red[256], ((a1 + red[64]) + red[192]) + red[320]);
 }
 
-// More tokens: 128 rows a workgroup, two runs of 64 of which each wave has a tile of 16, and the tokens' slices in LDS once for all of them.
+// More tokens or tiles: 128 rows a workgroup, two runs of 64 of which each wave has a tile of 16, and the tokens' slices in LDS once for all of them. HBM: 32
+// tokens, 8 of 128 experts of 2048 x 768 (78 chosen, up to 11 tokens each), gate and up 47 us for 245 MB (5.2 TB/s), down 30 for 123 MB (4.1 TB/s: short rows); 25
+// tokens on each of 16 experts of 5120 x 1536 58 and 48 (4.3 and 2.6 TB/s: copies of tokens beside the codes').
 // done(m, values of both tiles): element i is row 16 wave + 4 (lane / 16) + i of each run, token 16 m + lane % 16.
 template <int DT, int SLICE, int MT, int PLANES, typename Source, typename Done>
 WQ8_DEVICE void shared_rows(sgpr4 rw, int row0, int row1, int width, sgpr4 rx, uint32_t plane_bytes, int count, uint8_t* ring, const Source& source,
@@ -564,7 +569,7 @@ template <int DT> WQ8_DEVICE float with_residual(const ExpertsArgs& p, int t, in
     return __builtin_fmaf(v, scale, Elem<DT>::to_f(static_cast<const raw*>(p.residual)[t * p.ldr + n]));
 }
 
-// A token's parts, weighted and added in the order of its choices.
+// A token's parts, weighted and added in the order of its choices: 4.8 us for 32 tokens x 8 x 2048, the length of its loads' chain.
 template <int DT>
 __global__ void __launch_bounds__(256) experts_join(ExpertsArgs p) {
     using raw = typename Elem<DT>::raw;
@@ -592,7 +597,8 @@ __global__ void __launch_bounds__(256) experts_join(ExpertsArgs p) {
     for (int i = 0; i < 4; ++i) static_cast<raw*>(p.out)[t * p.ldo + n + i] = Elem<DT>::from_f(with_residual<DT>(p, t, n + i, sum[i]));
 }
 
-// One token: the second product and the sum over its choices in one launch. A workgroup has 8 output channels, a wave every eighth choice of the
+// One token: the second product and the sum over its choices in one launch (8 of 64 experts of 2048 x 1024: 9.0 us for 16.8 MB; by ring_rows and
+// experts_join 6.8 + 4.8). A workgroup has 8 output channels, a wave every eighth choice of the
 // token: 8 rows of 128 neighbouring bytes a load, 8 loads ahead, so that an expert's 8 x 1024 codes are asked for at once. One token leaves nothing
 // to share, and 16 rows of a matrix instruction would leave half the CUs idle: the products are FP32 on the vector unit, hidden values as FP32.
 template <int DT>
@@ -716,8 +722,12 @@ WQ8_API int wq8_experts(const void* x, int64_t ldx, int dtype, const void* ids, 
     const int64_t h_bytes = (int64_t(pairs) * hidden * 4 + 255) / 256 * 256;
     const ExpertsArgs p{x, static_cast<const int32_t*>(ids), weights, gate_up, gate_up_scale, down, down_scale, static_cast<uint16_t*>(workspace),
                         reinterpret_cast<float*>(static_cast<char*>(workspace) + h_bytes), residual, rscale, out, ldx, ldr, ldo, tokens, top, experts, k, hidden};
-    // tiles that waves share only where there are few, of 8 tokens at most
-    const int up = tokens > 8 || slots * (hidden / 16) > 1024, down_own = tokens > 8 || slots * ((k + 31) / 32) > 1024;
+    // Waves share tiles (ring_rows) in calls of up to 8 tokens with fewer than 1024 of them, of which the other form would make fewer workgroups than there
+    // are CUs, or 2048 where a tile is long, whose beginning weighs less. Both products, us (ring_rows, shared_rows), tokens x channels x hidden, experts, choices:
+    // 1 x 2048 x 1024, 64, 8 (512 tiles) 18.2, 21.6; 5 x 1552 x 592, 21, 3 (555, gate and up alone) 9.4, 12.2; 2 x 2048 x 1024, 64, 8 (1024) 32.1, 28.3; 8 x 1024 x 512, 32,
+    // 4 (1024) 22.4, 18.2; 4 x 2048 x 1024, 64, 8 (2048) 48.2, 38.6; 2 x 5120 x 1536, 16, 2 (384) 29.7, 39.3; 4 x 5120 x 1536, 16, 4 (1536, of 5120) 49, 62.
+    const auto shares = [&](int64_t tiles, int width) { return tokens <= 8 && slots * tiles < (width >= 4096 ? 2048 : 1024); };
+    const int up = !shares(hidden / 16, k), down_own = !shares((k + 31) / 32, hidden);
     const int up_groups = up ? (hidden + 63) / 64 : hidden / 16, down_groups = down_own ? (k + 127) / 128 : (k + 31) / 32;
     // an expert of more tokens than a workgroup takes at once: other workgroups take the next ones
     const auto passes = [&](int most) { return tokens <= most ? 1 : tokens <= 2 * most ? 2 : 4; };

@@ -392,7 +392,7 @@ static int launch_prep(const PrepArgs& p, int m, hipStream_t stream) {
 template <int DT, int MODE>
 static int launch_added(const PrepArgs& p, int m, hipStream_t stream) {
     const int chunks = p.k / 8, parts = (chunks + 255) / 256;
-    if (parts > 1 && parts <= 8 && m <= 256) {
+    if (parts > 1 && parts <= 8 && m <= 512) {
         if (parts == 2) prep_wide<DT, 2, 1, MODE, true><<<m, 512, 0, stream>>>(p);
         else if (parts == 3) prep_wide<DT, 3, 1, MODE, true><<<m, 768, 0, stream>>>(p);
         else if (parts == 4) prep_wide<DT, 4, 1, MODE, true><<<m, 1024, 0, stream>>>(p);
@@ -408,7 +408,7 @@ static int launch_added(const PrepArgs& p, int m, hipStream_t stream) {
 }
 
 // What prepared codes stand for, 8 a thread: code * scale, (hi + lo / 254) * scale, rounded once to the output's type. `per` is the scales of a
-// row (1, or one a 128-element block).
+// row (1, or one a 128-element block). HBM: 3 bytes a value of one byte; 32760 x 5120 98 us, 5.1 TB/s.
 template <int DT>
 __global__ void __launch_bounds__(256) prepared_values(const int8_t* q, const int8_t* lo, const float* scale, void* out, int64_t chunks, int row_chunks, int per) {
     const int64_t c = int64_t(blockIdx.x) * 256 + threadIdx.x;

@@ -15,7 +15,7 @@
 
 namespace wq8 {
 
-constexpr int SAMPLE_BINS = 1024, SAMPLE_SPLITS = 64, SAMPLE_PARTS = 256, SAMPLE_LIST = 2048, MOST_LISTED_KEYS = 16384, SAMPLE_PIECE = 2048, SMALL_K = 1024, SHORT_LIST = 128;
+constexpr int SAMPLE_BINS = 1024, SAMPLE_SPLITS = 64, SAMPLE_PARTS = 256, SAMPLE_LIST = 2048, MOST_LISTED_KEYS = 16384, SAMPLE_PIECE = 2048, SMALL_K = 1024, SHORT_LIST = 256;
 constexpr float BINS_PER_UNIT = 32.0f;  // the last bin begins at 31.97: weights below 2^-46, held as 0
 
 struct SampleRow {  // a row's workspace
@@ -189,6 +189,7 @@ template <int DT, typename F> WQ8_DEVICE void each_logit(const SampleArgs& p, in
 }
 
 // ---- 1: the largest logit of every part of a row -----------------------------------------------------------------------------
+// HBM and the launch: 64 rows of 131072 BF16 6 us (2.7 TB/s), one row of FP32 3.1.
 template <int DT> __global__ void __launch_bounds__(256) sample_largest(SampleArgs p) {
     __shared__ uint64_t best4[4];
     const int row = blockIdx.x / p.splits, s = blockIdx.x % p.splits;
@@ -209,6 +210,7 @@ template <int DT> __global__ void __launch_bounds__(256) sample_largest(SampleAr
 }
 
 // ---- 2: counts and weights over (largest - logit) / temperature ------------------------------------------------------------------
+// Bound by the additions in LDS and the exponentials: the same 64 rows, of options of their own, 12 us; one row 4.7.
 template <int DT> __global__ void __launch_bounds__(256) sample_bins(SampleArgs p) {
     __shared__ unsigned long long mass[SAMPLE_BINS];
     __shared__ uint32_t count[SAMPLE_BINS];
@@ -368,6 +370,7 @@ WQ8_DEVICE Cut find_cut(const Row& r, const SampleRow& state, CutScratch& sc) {
 }
 
 // ---- 3: the keys of those bins, and the weights that certainly stay ------------------------------------------------------------
+// Bound by the exponentials (30 operations of FP64 a value): 200 rows of 50001 FP16 17 us, the 64 rows 21; one row 5.8.
 template <int DT> __global__ void __launch_bounds__(256) sample_list(SampleArgs p) {
     __shared__ CutScratch scratch;
     __shared__ unsigned long long kept[SAMPLE_PARTS];
@@ -418,6 +421,8 @@ template <int DT> __global__ void __launch_bounds__(256) sample_list(SampleArgs 
 }
 
 // ---- 4: the cut among the listed keys, and the token ---------------------------------------------------------------------------
+// One workgroup a row, a chain of short steps: up to 256 keys (SHORT_LIST) each against all others, 8.6 us a row of top-k 50; more of them digit by digit, 24.
+// 200 keys in 32 rows (all of sample): 29.7 us compared, 33.0 by digits; 100 in one row 24.9 and 27.7.
 struct __attribute__((aligned(16))) Listed {
     uint64_t key, units;
 };
