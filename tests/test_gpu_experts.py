@@ -97,6 +97,28 @@ def test_any_number_of_tokens_an_expert(wq, counts, dtype):
     check(wq, x, ids, torch.rand(len(ids), 1, generator=g, device="cuda"), layer(g, len(counts), 336, 176))
 
 
+@pytest.mark.parametrize("tokens,k,hidden,count,top,dtype", [
+    (1, 256, 2064, 70, 65, BF16), (1, 512, 1552, 20, 17, FP16), (1, 4096, 48, 64, 64, BF16), (2, 2048, 528, 64, 8, FP16), (4, 4112, 272, 16, 4, BF16), (6, 304, 1040, 96, 12, BF16)])
+def test_forms_of_few_tokens(wq, tokens, k, hidden, count, top, dtype):
+    """One token of many choices and long rows; two to six around the borders between shared tiles and shared tokens."""
+    print(f"few {tokens} {k} {hidden} {count} {top} {dtype}", flush=True)
+    g = generator(k + hidden)
+    x, residual = (torch.randn(tokens, k, generator=g, device="cuda").to(dtype) for _ in range(2))
+    ids, weights = choices(g, tokens, top, count)
+    ids[0, top // 2] = -1
+    check(wq, x, ids, weights, layer(g, count, k, hidden), residual)
+
+
+def test_all_of_many_tokens_on_one_expert(wq):
+    g = generator(12)
+    parts = layer(g, 3, 128, 48)
+    x = torch.randn(333, 128, generator=g, device="cuda").to(BF16)
+    ids = torch.ones(333, 1, dtype=torch.int32, device="cuda")
+    check(wq, x, ids, torch.rand(333, 1, generator=g, device="cuda"), parts)
+    twice = torch.ones(8, 2, dtype=torch.int32, device="cuda")  # 16 choices of 8 tokens
+    check(wq, x[:8], twice, torch.rand(8, 2, generator=g, device="cuda"), parts)
+
+
 def test_experts_outside_and_twice(wq):
     g = generator(3)
     parts = layer(g, 6, 256, 64)

@@ -202,3 +202,13 @@ def test_lists_in_lds_in_memory_and_too_long(wq, vocabulary):
         l = logits.to(dtype)
         for options in ({"top_k": vocabulary // 3}, {"top_k": 700, "top_p": 0.4}, {"top_p": 0.6}, {"top_k": vocabulary // 2, "top_p": 0.5, "min_p": 0.97}, {"top_k": 1000}):
             assert torch.equal(wq.sample(l, draws, **options).cpu(), defined(l, draws, **options)), (dtype, options)
+
+
+def test_large_vocabulary(wq):
+    """3000001 tokens: weights in parts of 2^-40 (62 bits less 22 of an index), parts of several pieces. A part off by 2^-40 - 2^-44 moves the
+    token only where a draw falls so near a border: with this seed it does not."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    logits = torch.randn(2, 3_000_001, generator=g, device="cuda") * 3
+    draws = torch.rand(2, generator=g, device="cuda")
+    for options in ({}, {"top_k": 50}, {"top_p": 0.4}, {"top_k": 20000, "top_p": 0.9}, {"temperature": 0.0}):
+        assert torch.equal(wq.sample(logits, draws, **options).cpu(), defined(logits, draws, **options)), options

@@ -18,7 +18,6 @@ from ._rotary import Layouts, _check_devices
 SCORES = {"softmax": 0, "sigmoid": 1}
 MAX_EXPERTS, MAX_TOP, MAX_CHOICES = 1024, 64, 4096
 _route_layouts, _experts_layouts = Layouts(), Layouts()
-_sizes = (ctypes.c_int64 * 2)()
 
 
 class Routes(NamedTuple):
@@ -45,8 +44,9 @@ def _check_route(x, router, top, score, bias):
     if x.shape[0] > 65535 * 16:
         raise ValueError("a route is of 2^20 - 16 tokens at most")
     _check_devices(*[t for t in (x, router, bias) if t is not None])
-    library().wq8_route_workspace(x.shape[0], count, k, _sizes)
-    return x.shape[0], count, k, _row_pitch(x), DTYPES[x.dtype], DTYPES[router.dtype], _sizes[0]
+    sizes = (ctypes.c_int64 * 2)()
+    library().wq8_route_workspace(x.shape[0], count, k, sizes)
+    return x.shape[0], count, k, _row_pitch(x), DTYPES[x.dtype], DTYPES[router.dtype], sizes[0]
 
 
 def route(x, router, top, score="softmax", bias=None, normalise=True, factor=1.0):
@@ -107,8 +107,9 @@ def _check_experts(x, ids, weights, gate_up, gate_up_scale, down, down_scale, re
         raise ValueError("an expert's matrices, the rows as they lie and the hidden values must each span less than 2 GiB")
     _check_devices(*[t for t in (x, ids, weights, gate_up, gate_up_scale, down, down_scale, residual, residual_scale) if t is not None])
     tokens, top = ids.shape
-    library().wq8_experts_workspace(tokens, top, k, both // 2, _sizes)
-    return tokens, top, count, k, both // 2, _row_pitch(x), 0 if residual is None else _row_pitch(residual), DTYPES[x.dtype], _sizes[0]
+    sizes = (ctypes.c_int64 * 2)()
+    library().wq8_experts_workspace(tokens, top, k, both // 2, sizes)
+    return tokens, top, count, k, both // 2, _row_pitch(x), 0 if residual is None else _row_pitch(residual), DTYPES[x.dtype], sizes[0]
 
 
 def experts(x, routes, gate_up, gate_up_scale, down, down_scale, residual=None, residual_scale=None, out=None):

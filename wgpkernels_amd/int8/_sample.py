@@ -13,7 +13,6 @@ from ._rotary import Layouts, _check_devices
 
 MAX_VOCABULARY, MAX_ROWS = 2 ** 24, 2 ** 17
 _layouts = Layouts()
-_sizes = (ctypes.c_int64 * 2)()
 
 
 def _check_sample(logits, draws, temperature, top_k, top_p, min_p):
@@ -33,8 +32,9 @@ def _check_sample(logits, draws, temperature, top_k, top_p, min_p):
                 raise ValueError(f"{name} must be a number, or ({rows},) {str(dtype).removeprefix('torch.')}, contiguous")
             tensors.append(t)
     _check_devices(logits, draws, *tensors)
-    library().wq8_sample_workspace(rows, _sizes)
-    return rows, vocabulary, logits.stride(0) if rows > 1 else vocabulary, DTYPES[logits.dtype], _sizes[0]
+    sizes = (ctypes.c_int64 * 2)()
+    library().wq8_sample_workspace(rows, sizes)
+    return rows, vocabulary, logits.stride(0) if rows > 1 else vocabulary, DTYPES[logits.dtype], sizes[0]
 
 
 def _kind(option):

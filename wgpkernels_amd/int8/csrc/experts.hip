@@ -139,9 +139,7 @@ __global__ void __launch_bounds__(256) route_choose(RouteArgs p) {
                 if (first + s < p.parts) score[i] += more[s][i];
     }
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
-        top = __builtin_fmax(top, score[i]);
-    }
+    for (int i = 0; i < NE; ++i) top = __builtin_fmax(top, score[i]);
     if (p.score == 0) {
         top = __builtin_bit_cast(double, over_wave(__builtin_bit_cast(uint64_t, top), [](uint64_t a, uint64_t b) {
             return __builtin_bit_cast(uint64_t, __builtin_fmax(__builtin_bit_cast(double, a), __builtin_bit_cast(double, b)));
@@ -597,7 +595,13 @@ __global__ void __launch_bounds__(256) experts_join(ExpertsArgs p) {
     for (int i = 0; i < 4; ++i) static_cast<raw*>(p.out)[t * p.ldo + n + i] = Elem<DT>::from_f(with_residual<DT>(p, t, n + i, sum[i]));
 }
 
-// One token: the second product and the sum over its choices in one launch (8 of 64 experts of 2048 x 1024: 9.0 us for 16.8 MB; by ring_rows and
+// Orders a wave's LDS accesses, its lanes' to each other (they run in step and in order: nothing is waited for).
+WQ8_DEVICE void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// One token: the second product and the sum over its choices in one launch (8 of 64 experts of 2048 x 1024: 6.0 us for 16.8 MB; by ring_rows and
 // experts_join 6.8 + 4.8). A workgroup has 8 output channels, a wave every eighth choice of the
 // token: 8 rows of 128 neighbouring bytes a load, 8 loads ahead, so that an expert's 8 x 1024 codes are asked for at once. One token leaves nothing
 // to share, and 16 rows of a matrix instruction would leave half the CUs idle: the products are FP32 on the vector unit, hidden values as FP32.
@@ -641,6 +645,7 @@ __global__ void __launch_bounds__(512) experts_down_one(ExpertsArgs p) {
                         }
                         *reinterpret_cast<v4f*>(&hidden[wave][8 * (lane + 64 * i) + 4 * half]) = v;
                     }
+                wave_fence();  // every lane reads what others wrote
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     if (begin + 128 * i >= p.hidden) break;
@@ -651,6 +656,7 @@ __global__ void __launch_bounds__(512) experts_down_one(ExpertsArgs p) {
                         for (int e = 0; e < 4; ++e) sum = __builtin_fmaf(float(int8_t(w[i][c] >> (8 * e))), v[e], sum);
                     }
                 }
+                wave_fence();  // and has read before they write again
             }
             sum += lane_xor<1>(sum);
             sum += lane_xor<2>(sum);
