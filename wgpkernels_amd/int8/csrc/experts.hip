@@ -4,7 +4,6 @@
 // every chosen expert's weights read once from HBM for all of its tokens. No reference counterpart.
 #include "gemm_common.h"
 #include "wq8_abi.h"
-#include <type_traits>
 
 namespace wq8 {
 
@@ -77,23 +76,6 @@ __global__ void __launch_bounds__(64 * ROUTE_WAVES) route_logits(RouteArgs p) {
 WQ8_DEVICE uint64_t order_of(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
     return v != v ? 1 : b >> 63 ? ~b : b | (uint64_t(1) << 63);
-}
-// f(v, the value of another lane) until every lane has all 64: across the lanes of a row of 16 by DPP, then rows and halves by exchanges
-template <int CTRL> WQ8_DEVICE uint64_t dpp64(uint64_t v) {
-    return uint64_t(dpp_u<CTRL>(uint32_t(v >> 32))) << 32 | dpp_u<CTRL>(uint32_t(v));
-}
-template <typename F> WQ8_DEVICE uint64_t over_wave(uint64_t v, const F& f) {
-    v = f(v, dpp64<0xB1>(v));   // quad_perm [1,0,3,2]
-    v = f(v, dpp64<0x4E>(v));   // quad_perm [2,3,0,1]
-    v = f(v, dpp64<0x141>(v));  // row_half_mirror
-    v = f(v, dpp64<0x140>(v));  // row_mirror
-    auto exchange = [&](auto swap) {
-        const auto low = swap(uint32_t(v)), high = swap(uint32_t(v >> 32));
-        v = f(uint64_t(uint32_t(high[0])) << 32 | uint32_t(low[0]), uint64_t(uint32_t(high[1])) << 32 | uint32_t(low[1]));
-    };
-    exchange([](uint32_t u) { return __builtin_amdgcn_permlane16_swap(u, u, false, false); });
-    exchange([](uint32_t u) { return __builtin_amdgcn_permlane32_swap(u, u, false, false); });
-    return v;
 }
 WQ8_DEVICE uint64_t wave_max64(uint64_t v) {
     return over_wave(v, [](uint64_t a, uint64_t b) { return a > b ? a : b; });

@@ -11,7 +11,6 @@
 // SMALL_K lists all of its keys: then no weight is taken of the rest of the row.
 #include "wq8_common.h"
 #include "wq8_abi.h"
-#include <type_traits>
 
 namespace wq8 {
 
@@ -105,32 +104,14 @@ struct Row {
 };
 
 WQ8_DEVICE uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
-// The sum over the wave: rows of 16 lanes by DPP, then rows and halves by exchanges
+// The sum over the wave
 WQ8_DEVICE uint64_t sum64(uint64_t v) {
-    auto dpp = [](auto control, uint64_t u) {
-        constexpr int C = decltype(control)::value;
-        return uint64_t(dpp_u<C>(uint32_t(u >> 32))) << 32 | dpp_u<C>(uint32_t(u));
-    };
-    v += dpp(std::integral_constant<int, 0xB1>{}, v);
-    v += dpp(std::integral_constant<int, 0x4E>{}, v);
-    v += dpp(std::integral_constant<int, 0x141>{}, v);
-    v += dpp(std::integral_constant<int, 0x140>{}, v);
-    auto rows = [](uint64_t u) {
-        const auto low = __builtin_amdgcn_permlane16_swap(uint32_t(u), uint32_t(u), false, false), high = __builtin_amdgcn_permlane16_swap(uint32_t(u >> 32), uint32_t(u >> 32), false, false);
-        return (uint64_t(uint32_t(high[0])) << 32 | uint32_t(low[0])) + (uint64_t(uint32_t(high[1])) << 32 | uint32_t(low[1]));
-    };
-    auto halves = [](uint64_t u) {
-        const auto low = __builtin_amdgcn_permlane32_swap(uint32_t(u), uint32_t(u), false, false), high = __builtin_amdgcn_permlane32_swap(uint32_t(u >> 32), uint32_t(u >> 32), false, false);
-        return (uint64_t(uint32_t(high[0])) << 32 | uint32_t(low[0])) + (uint64_t(uint32_t(high[1])) << 32 | uint32_t(low[1]));
-    };
-    return halves(rows(v));
+    return over_wave(v, [](uint64_t a, uint64_t b) { return a + b; });
 }
 
 // The largest of the wave's values
 WQ8_DEVICE uint64_t wave_most(uint64_t v) {
-#pragma unroll
-    for (int step = 32; step; step >>= 1) v = max64(v, __shfl_xor(v, step));
-    return v;
+    return over_wave(v, [](uint64_t a, uint64_t b) { return max64(a, b); });
 }
 
 WQ8_DEVICE Row read_row(const SampleArgs& p, const SampleRow& state, int row) {
@@ -275,12 +256,7 @@ struct Cut {
 // Exclusive sums over the workgroup's 256 threads, and their total.
 template <typename T> WQ8_DEVICE T scan256(T v, T* waves, T& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    T upto = v;
-#pragma unroll
-    for (int step = 1; step < 64; step <<= 1) {
-        const T below = __shfl_up(upto, step);
-        if (lane >= step) upto += below;
-    }
+    const T upto = T(wave_upto(v));
     __syncthreads();
     if (lane == 63) waves[wave] = upto;
     __syncthreads();
@@ -451,12 +427,8 @@ template <bool BY_COUNT, typename Each> WQ8_DEVICE uint64_t select_key(PickScrat
         low = key < low ? key : low;
         high = max64(high, key);
     });
-#pragma unroll
-    for (int step = 32; step; step >>= 1) {
-        const uint64_t l = __shfl_xor(low, step);
-        low = l < low ? l : low;
-        high = max64(high, __shfl_xor(high, step));
-    }
+    low = ~wave_most(~low);
+    high = wave_most(high);
     if (!(tid & 63) && low <= high) {
         atomicMin(&sc.lowest, (unsigned long long)low);
         atomicMax(&sc.highest, (unsigned long long)high);

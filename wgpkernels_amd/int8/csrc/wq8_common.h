@@ -228,6 +228,38 @@ WQ8_DEVICE float wave_max(float v) {
     return fmaxf(p.a, p.b);
 }
 
+// f(v, the value of another lane) until every lane has all 64: across the lanes of a row of 16 by DPP, then rows and halves by exchanges
+template <int CTRL> WQ8_DEVICE uint64_t dpp64(uint64_t v) {
+    return uint64_t(dpp_u<CTRL>(uint32_t(v >> 32))) << 32 | dpp_u<CTRL>(uint32_t(v));
+}
+template <typename F> WQ8_DEVICE uint64_t over_wave(uint64_t v, const F& f) {
+    v = f(v, dpp64<0xB1>(v));   // quad_perm [1,0,3,2]
+    v = f(v, dpp64<0x4E>(v));   // quad_perm [2,3,0,1]
+    v = f(v, dpp64<0x141>(v));  // row_half_mirror
+    v = f(v, dpp64<0x140>(v));  // row_mirror
+    auto exchange = [&](auto swap) {
+        const auto low = swap(uint32_t(v)), high = swap(uint32_t(v >> 32));
+        v = f(uint64_t(uint32_t(high[0])) << 32 | uint32_t(low[0]), uint64_t(uint32_t(high[1])) << 32 | uint32_t(low[1]));
+    };
+    exchange([](uint32_t u) { return __builtin_amdgcn_permlane16_swap(u, u, false, false); });
+    exchange([](uint32_t u) { return __builtin_amdgcn_permlane32_swap(u, u, false, false); });
+    return v;
+}
+// Sums of 64-bit numbers over this lane and those below it: rows of 16 by DPP row shifts, then the last lanes of rows and halves handed on.
+template <int CTRL, int ROWS> WQ8_DEVICE uint64_t dpp_or_0(uint64_t v) {
+    const uint32_t low = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(v)), CTRL, ROWS, 0xF, true));
+    const uint32_t high = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(v >> 32)), CTRL, ROWS, 0xF, true));
+    return uint64_t(high) << 32 | low;
+}
+WQ8_DEVICE uint64_t wave_upto(uint64_t v) {
+    v += dpp_or_0<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
+    v += dpp_or_0<0x112, 0xF>(v);
+    v += dpp_or_0<0x114, 0xF>(v);
+    v += dpp_or_0<0x118, 0xF>(v);
+    v += dpp_or_0<0x142, 0xA>(v);  // row_bcast:15 to rows 1 and 3
+    return v + dpp_or_0<0x143, 0xC>(v);  // row_bcast:31 to rows 2 and 3
+}
+
 // ---- ConvRot rotation of one 8-element chunk -------------------------------------------------------------
 // A row is cut into 8-element chunks held one per lane, consecutive lanes holding consecutive chunks, so a
 // group of 256 elements spans 32 lanes (aligned). In-group index e = 8 * (lane % 32) + j, base-4 digits
