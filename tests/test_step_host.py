@@ -21,6 +21,7 @@ ADDED = {
     "width": lambda: (rows(k=252), rows(k=252), {}),
     "no channels": lambda: (rows(k=0), rows(k=0), {}),
     "columns": lambda: (torch.zeros(256, 4, dtype=BF16).t(), rows(), {}),
+    "many rows": lambda: (rows(1, 8).expand(2 ** 24, 8), rows(1, 8).expand(2 ** 24, 8), {}),
     "pitch": lambda: (rows(k=260)[:, :256], rows(), {}),
     "path": lambda: (rows(), rows(), {"path": "fast"}),
     "group": lambda: (rows(), rows(), {"group": 32}),
@@ -190,3 +191,27 @@ def test_most_values_of_top_k():
     """A top_k beyond the C interface's 32 bits is all of the vocabulary, not its low bits."""
     from wgpkernels_amd.int8 import _sample
     assert min(2 ** 32 + 3, _sample.MAX_VOCABULARY) == 2 ** 24 and _sample._pair(min(2 ** 32 + 3, _sample.MAX_VOCABULARY)) == (None, 2 ** 24)
+
+
+def test_entry_points_reject_before_a_launch():
+    """The C interface's own checks: codes without a GPU touched."""
+    lib = wq.library()
+    add = lambda m=4, k=64, dtype=1, path=0, group=0: lib.wq8_add_prepare(None, k, None, k, None, None, k, path, None, None, None, m, k, dtype, group, None, 0.0, None)
+    assert add(m=0) == 0
+    assert [add(dtype=2), add(path=3), add(group=32)] == [-1] * 3 and [add(k=60), add(k=0), add(m=-1), add(m=2 ** 24), add(k=24, group=16)] == [-2] * 5
+    assert lib.wq8_prepared_values(None, None, None, None, 0, 64, 0, 1, None) == 0
+    assert lib.wq8_prepared_values(None, None, None, None, 4, 64, 0, 3, None) == -1 and lib.wq8_prepared_values(None, None, None, None, 4, 60, 0, 1, None) == -2
+    route = lambda tokens=4, experts=8, k=64, top=2, dtype=1, score=0: lib.wq8_route(None, k, dtype, None, 1, None, tokens, experts, k, top, score, 1, 1.0, None, None,
+                                                                                      None, None)
+    assert route(tokens=0) == 0
+    assert [route(dtype=3), route(score=2)] == [-1] * 2
+    assert [route(experts=0), route(experts=1025), route(k=60), route(top=0), route(top=9), route(tokens=65535 * 16 + 1), route(tokens=-1)] == [-2] * 7
+    experts = lambda tokens=4, top=2, count=8, k=64, hidden=32, dtype=1, ldx=64: lib.wq8_experts(None, ldx, dtype, None, None, None, None, None, None, None, 0, None, None, k,
+                                                                                                tokens, top, count, k, hidden, None, None)
+    assert experts(tokens=0) == 0
+    assert experts(dtype=2) == -1
+    assert [experts(tokens=2049), experts(top=0), experts(count=0), experts(k=72), experts(hidden=24), experts(k=32768, hidden=32768), experts(ldx=2 ** 30),
+            experts(tokens=-1)] == [-2] * 8
+    sample = lambda rows=2, vocabulary=100, dtype=2: lib.wq8_sample(None, vocabulary, dtype, None, None, 1.0, None, 0, None, 1.0, None, 0.0, rows, vocabulary, None, None, None)
+    assert sample(rows=0) == 0
+    assert sample(dtype=3) == -1 and [sample(rows=-1), sample(rows=2 ** 17 + 1), sample(vocabulary=0), sample(vocabulary=2 ** 24 + 1)] == [-2] * 4

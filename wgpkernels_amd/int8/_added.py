@@ -31,6 +31,8 @@ def _check_added(x, residual, residual_scale, group, path, act_weight):
     m, k = x.shape
     if k < 8 or k % 8:
         raise ValueError(f"rows must have a multiple of 8 channels, not {k}")
+    if m >= 2 ** 24:
+        raise ValueError("add_prepare takes fewer than 2^24 rows")
     if group not in (0, 16, 64, 256) or (group and k % group):
         raise ValueError(f"ConvRot groups are of 16, 64 or 256 channels and divide the rows, not {group} of {k}")
     for t in (x, residual):

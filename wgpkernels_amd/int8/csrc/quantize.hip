@@ -512,6 +512,7 @@ WQ8_API int wq8_add_prepare(const void* x, int64_t ldx, const void* residual, in
     if (!m) return 0;
     if (dtype != DT_F16 && dtype != DT_BF16) return -1;
     if (path < PREP_BLOCKS || path > PREP_TRANSFORM) return -1;
+    if (m > MAX_BLOCKS_256) return -2;
     if (int rc = check_prep(m, k, dtype, group, ACT_RMS)) return rc;
     int8_t* q = path == PREP_TRANSFORM ? nullptr : static_cast<int8_t*>(out);
     PrepArgs p{x, q, path == PREP_ROWS ? lo : nullptr, scale, path == PREP_TRANSFORM ? out : nullptr, nullptr, act_weight, nullptr, 0, 0,

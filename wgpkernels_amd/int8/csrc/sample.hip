@@ -346,7 +346,7 @@ WQ8_DEVICE Cut find_cut(const Row& r, const SampleRow& state, CutScratch& sc) {
 }
 
 // ---- 3: the keys of those bins, and the weights that certainly stay ------------------------------------------------------------
-// Bound by the exponentials (30 operations of FP64 a value): 200 rows of 50001 FP16 17 us, the 64 rows 21; one row 5.8.
+// Bound by the exponentials (45 instructions a value, most of them FP64): 200 rows of 50001 FP16 17 us, the 64 rows 21; one row 5.6.
 template <int DT> __global__ void __launch_bounds__(256) sample_list(SampleArgs p) {
     __shared__ CutScratch scratch;
     __shared__ unsigned long long kept[SAMPLE_PARTS];
@@ -397,7 +397,7 @@ template <int DT> __global__ void __launch_bounds__(256) sample_list(SampleArgs 
 }
 
 // ---- 4: the cut among the listed keys, and the token ---------------------------------------------------------------------------
-// One workgroup a row, a chain of short steps: up to 256 keys (SHORT_LIST) each against all others, 8.6 us a row of top-k 50; more of them digit by digit, 24.
+// One workgroup a row, a chain of short steps: up to 256 keys (SHORT_LIST) each against all others, 7.8 us a row of top-k 50; more of them digit by digit, 22 the 64 rows.
 // 200 keys in 32 rows (all of sample): 29.7 us compared, 33.0 by digits; 100 in one row 24.9 and 27.7.
 struct __attribute__((aligned(16))) Listed {
     uint64_t key, units;
