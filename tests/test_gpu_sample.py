@@ -212,3 +212,21 @@ def test_large_vocabulary(wq):
     draws = torch.rand(2, generator=g, device="cuda")
     for options in ({}, {"top_k": 50}, {"top_p": 0.4}, {"top_k": 20000, "top_p": 0.9}, {"temperature": 0.0}):
         assert torch.equal(wq.sample(logits, draws, **options).cpu(), defined(logits, draws, **options)), options
+
+
+@pytest.mark.parametrize("dtype", [FP16, FP32])
+@pytest.mark.parametrize("options", [{}, {"top_k": 2000}, {"top_k": 4999}, {"top_k": 1025, "top_p": 0.6}, {"top_k": 3000, "min_p": 0.5}, {"top_k": 1000}, {"top_p": 0.5},
+                                     {"top_k": 2000, "temperature": math.inf}])
+def test_infinite_logits_share_all_weight(wq, dtype, options):
+    """One to all of a row's logits infinite, beside finite ones and NaN: as many as, fewer and more than top-k, options as numbers and as tensors."""
+    counts = [1, 2, 3, 10, 100, 1024, 1025, 1999, 2000, 2001, 4999, 5000]
+    logits, _, g = logits_of(len(counts), 5000, dtype, seed=11)
+    logits[::3, 5::7] = math.nan
+    for row, count in enumerate(counts):
+        logits[row, torch.randperm(5000, generator=g, device="cuda")[:count]] = math.inf
+    for draws in (torch.linspace(0, 0.999, len(counts), device="cuda"), torch.linspace(1 - 2.0 ** -24, 0.1, len(counts), device="cuda")):
+        want = defined(logits, draws, **options)
+        assert torch.equal(wq.sample(logits, draws, **options).cpu(), want)
+        tensors = {name: torch.full((len(counts),), value, dtype=torch.int32 if name == "top_k" else FP32, device="cuda") for name, value in options.items()}
+        assert torch.equal(wq.sample(logits, draws, **tensors).cpu(), want)
+        assert logits.cpu()[torch.arange(len(counts)), want].isinf().all()

@@ -249,7 +249,7 @@ struct Cut {
     uint64_t k_before;              // the weight before it
     int low, high;                  // the bins of top-p's last key (low > high: no top-p)
     uint64_t low_before;            // the weight before them
-    int certain;                    // bins below it stay whole (0 for a small k, whose bins are all listed)
+    int certain;                    // bins below it stay whole (0 for a small k, whose bins are all listed); at most the last one, which weighs nothing
     WQ8_DEVICE bool listed(int bin) const { return bin == k_bin || (bin >= low && bin <= high); }
 };
 
@@ -340,7 +340,7 @@ WQ8_DEVICE Cut find_cut(const Row& r, const SampleRow& state, CutScratch& sc) {
     c.low = sc.low;
     c.high = sc.high;
     c.low_before = sc.low_before;
-    c.certain = r.by_p ? c.low : c.k_bin;
+    c.certain = r.by_p ? c.low : min(c.k_bin, SAMPLE_BINS - 1);
     __syncthreads();
     return c;
 }
@@ -383,7 +383,7 @@ template <int DT> __global__ void __launch_bounds__(256) sample_list(SampleArgs 
             [&](float l, int i) {
                 const int b = r.bin(l);
                 const uint64_t units = kept_of(r.infinite ? 1.0 : r.finite_weight(l));
-                sum += b < c.certain ? units : 0;  // (of an infinite row, bins beside the first and the last are empty)
+                sum += b < c.certain ? units : 0;  // (an infinite row has its infinities in the first bin, all else in the last one, which stays out)
                 if (c.listed(b) && l == l) list(l, i);
             },
             after);
