@@ -230,3 +230,20 @@ def test_infinite_logits_share_all_weight(wq, dtype, options):
         tensors = {name: torch.full((len(counts),), value, dtype=torch.int32 if name == "top_k" else FP32, device="cuda") for name, value in options.items()}
         assert torch.equal(wq.sample(logits, draws, **tensors).cpu(), want)
         assert logits.cpu()[torch.arange(len(counts)), want].isinf().all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("temperature", [1e37, 5e37, 1e38, 3.4e38, math.inf])
+def test_logits_whose_differences_pass_fp32(wq, dtype, temperature):
+    """Logits over all of the type's range under temperatures alike: the largest one's distance to others is beyond FP32, their weights are not 0."""
+    most = torch.finfo(dtype).max
+    g = torch.Generator(device="cuda").manual_seed(12)
+    logits = ((2 * torch.rand(6, 4000, generator=g, device="cuda", dtype=torch.float64) - 1) * most).to(dtype)
+    logits[0, 17], logits[1, 3000], logits[2, 5] = most, most, -most
+    draws = torch.rand(6, generator=g, device="cuda")
+    for options in ({}, {"top_k": 40}, {"top_k": 3900}, {"top_p": 0.95}, {"top_p": 0.999, "top_k": 3990}, {"min_p": 0.01}):
+        assert torch.equal(wq.sample(logits, draws, temperature=temperature, **options).cpu(), defined(logits, draws, temperature=temperature, **options)), options
+    two = torch.tensor([[most, -most]], dtype=dtype, device="cuda")
+    for options in ({}, {"top_k": 1}, {"top_p": 0.9999}):
+        late = torch.tensor([1 - 2.0 ** -24], device="cuda")
+        assert torch.equal(wq.sample(two, late, temperature=temperature, **options).cpu(), defined(two, late, temperature=temperature, **options)), options

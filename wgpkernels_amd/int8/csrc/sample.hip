@@ -84,7 +84,8 @@ struct Row {
     float top;         // its largest logit
     int first;         // the first token that has it
     double inverse;    // of the temperature, times log2(e)
-    float bins;        // bins a unit of logit
+    float half;        // 1/2 where distances from the largest logit may pass FP32, else 1
+    float half_top, bins;  // half * top; bins a unit of half * logit
     double scale, min_p;
     float top_p;
     int top_k;
@@ -98,7 +99,7 @@ struct Row {
     WQ8_DEVICE uint64_t units(double w) const { return __builtin_bit_cast(uint64_t, __builtin_fma(w, scale, 0x1p52)) - 0x4330000000000000ull; }
     WQ8_DEVICE int bin(float l) const {
         if (l == top) return 0;
-        const float b = (top - l) * bins;
+        const float b = __builtin_fmaf(-half, l, half_top) * bins;
         return b < float(SAMPLE_BINS - 1) ? int(b) : SAMPLE_BINS - 1;
     }
 };
@@ -125,7 +126,9 @@ WQ8_DEVICE Row read_row(const SampleArgs& p, const SampleRow& state, int row) {
     r.greedy = !(t > 0.0f);
     r.nothing = uint32_t(best >> 32) <= logit_order(-__builtin_inff());
     r.inverse = 0x1.71547652b82fep+0 / double(t);
-    r.bins = fminf(float(1.0 / double(t)) * BINS_PER_UNIT, 0x1.fffffep127f);  // (an infinity would part equal logits from others beside them)
+    r.half = r.top >= 0x1p103f ? 0.5f : 1.0f;  // (2^103 above the lowest FP32: half a step past the largest)
+    r.half_top = r.half * r.top;
+    r.bins = fminf(float(double(BINS_PER_UNIT / r.half) / double(t)), 0x1.fffffep127f);  // (an infinity would part equal logits from others beside them)
     r.scale = double(uint64_t(1) << p.shift);
     r.min_p = fmin(double(p.min_p ? p.min_p[row] : p.min_p0), 1.0);
     r.top_p = p.top_p ? p.top_p[row] : p.top_p0;
