@@ -215,3 +215,23 @@ def test_entry_points_reject_before_a_launch():
     sample = lambda rows=2, vocabulary=100, dtype=2: lib.wq8_sample(None, vocabulary, dtype, None, None, 1.0, None, 0, None, 1.0, None, 0.0, rows, vocabulary, None, None, None)
     assert sample(rows=0) == 0
     assert sample(dtype=3) == -1 and [sample(rows=-1), sample(rows=2 ** 17 + 1), sample(vocabulary=0), sample(vocabulary=2 ** 24 + 1)] == [-2] * 4
+
+
+@pytest.mark.parametrize("given,kept", [(2 ** 32 + 3, 9), (2 ** 31, 9), (-2 ** 32 + 1, 9), (-2 ** 31 - 1, 9), (-2 ** 40 + 8, 9), (-1, 9), (0, 9), (9, 9), (7, 7)])
+def test_numbers_of_top_k_beyond_32_bits(monkeypatch, given, kept):
+    """How many of 9 tokens the C interface keeps, whose top_k has 32 bits, by what sample() hands to it."""
+    import ctypes
+    from types import SimpleNamespace
+
+    from wgpkernels_amd.int8 import _native, _sample
+    calls = []
+    monkeypatch.setattr(_sample, "_check_devices", lambda *tensors: None)
+    monkeypatch.setattr(_sample, "_layouts", _sample.Layouts())
+    monkeypatch.setattr(_native, "gpu", lambda x: SimpleNamespace(index=0, stream=lambda: None))
+    monkeypatch.setattr(_native, "call_on", lambda library, index, name, *args: calls.append((name, args)))
+    wq.sample(torch.zeros(3, 9), torch.zeros(3), top_k=given)
+    (name, args), = calls
+    # logits, pitch, type, draws, then an address and a number of each option: temperature, top_k
+    assert name == "wq8_sample" and args[6] is None
+    top_k = ctypes.c_int(args[7]).value
+    assert (top_k if 0 < top_k < 9 else 9) == kept

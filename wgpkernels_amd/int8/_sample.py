@@ -49,8 +49,8 @@ def _pair(option):
 def sample(logits, draws, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """A token of every row of logits (rows, vocabulary), BF16, FP16 or FP32 with unit column stride: (rows,) int64.
 
-    A token's weight is exp((logit - the row's largest) / temperature), in 64 bits. top_k keeps the k heaviest tokens (0, or the
-    vocabulary's size: all); of these top_p the fewest, heaviest first, whose weights reach top_p of their sum (1: all; always at least
+    A token's weight is exp((logit - the row's largest) / temperature), in 64 bits. top_k keeps the k heaviest tokens (0 or below, or
+    the vocabulary's size and above: all); of these top_p the fewest, heaviest first, whose weights reach top_p of their sum (1: all; always at least
     one); of these min_p those of at least min_p of the heaviest's weight. Equal logits go by the lowest index. The token drawn is the
     first, in the vocabulary's order, up to which the kept weights pass draws[row] (FP32, in [0, 1)) of their sum. A temperature of 0 (or below) takes
     the first largest logit. Each option is a number or a (rows,) tensor (FP32, top_k int32).
@@ -63,6 +63,8 @@ def sample(logits, draws, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     tokens = draws.new_empty(rows, dtype=torch.int64)
     workspace = draws.new_empty(workspace_bytes, dtype=torch.uint8)
     state = _native.gpu(logits)
-    _native.call_on(library(), state.index, "wq8_sample", logits.data_ptr(), ld, dtype, draws.data_ptr(), *_pair(temperature), *_pair(top_k if isinstance(top_k, torch.Tensor) else min(top_k, MAX_VOCABULARY)), *_pair(top_p), *_pair(min_p), rows,
-                   vocabulary, tokens.data_ptr(), workspace.data_ptr(), state.stream())
+    if not isinstance(top_k, torch.Tensor):
+        top_k = max(0, min(top_k, MAX_VOCABULARY))  # the C interface has 32 bits
+    _native.call_on(library(), state.index, "wq8_sample", logits.data_ptr(), ld, dtype, draws.data_ptr(), *_pair(temperature), *_pair(top_k), *_pair(top_p),
+                    *_pair(min_p), rows, vocabulary, tokens.data_ptr(), workspace.data_ptr(), state.stream())
     return tokens
