@@ -247,3 +247,42 @@ def test_logits_whose_differences_pass_fp32(wq, dtype, temperature):
     for options in ({}, {"top_k": 1}, {"top_p": 0.9999}):
         late = torch.tensor([1 - 2.0 ** -24], device="cuda")
         assert torch.equal(wq.sample(two, late, temperature=temperature, **options).cpu(), defined(two, late, temperature=temperature, **options)), options
+
+
+@pytest.mark.parametrize("vocabulary,above", [(131072, 28.0), (2 ** 18, 27.0), (2 ** 18 + 1, 28.0), (2 ** 20, 28.0), (3_000_001, 30.0), (2 ** 24, 28.0), (2 ** 24, 31.0), (2 ** 24, 2.0)])
+def test_a_peak_over_a_flat_tail(wq, vocabulary, above):
+    """One logit `above` all others, which are alike, against the weights themselves (the peak's 1, the others' exp(-above), not rounded): the running weights
+    beside the token drawn enclose the draw's. Every weight is rounded by half a unit, 2^-45 of the heaviest up to 2^18 tokens; above, 2^-53, or less than
+    2^-62 of the sum (units of 2^(ceil(log2 sum) - 62)): 2^-27 of the sum for all tokens of a row. The kept sum of a top-p is the
+    border's, off by as much again and a token."""
+    w, peak = math.exp(-above), vocabulary // 3
+    row = torch.zeros(1, vocabulary, device="cuda")
+    row[0, peak] = above
+    draws = torch.tensor([0.0, 0.5, 1 - 1000 * 2.0 ** -24, 1 - 200 * 2.0 ** -24, 1 - 100 * 2.0 ** -24, 1 - 30 * 2.0 ** -24, 1 - 2.0 ** -23, 1 - 2.0 ** -24], device="cuda")
+    n = len(draws)
+    weigh = lambda count: max(0.0, count) * w  # of that many tokens of the tail
+    upto = lambda t: weigh(t + 1 if t < peak else t) + (1.0 if t >= peak else 0.0)  # the running weight with token t
+    total = upto(vocabulary - 1)
+    bound = 2.0 ** -27 * total
+    for options, kept, slack in (({}, total, 0.0), ({"min_p": 0.9 * w}, total, 0.0), ({"top_k": vocabulary - 1}, total - w, 0.0),
+                                 ({"top_p": 1 - 2.0 ** -24}, total * (1 - 2.0 ** -24), w + bound)):
+        tokens = wq.sample(row.expand(n, vocabulary), draws, **options).tolist()
+        for u, t in zip(draws.tolist(), tokens):
+            assert upto(t - 1) - bound - slack <= u * kept <= upto(t) + bound + slack, (options, u, t)
+        assert tokens == sorted(tokens)
+
+
+def test_rows_of_all_kinds_over_a_large_vocabulary(wq):
+    """Above 2^18 tokens weights have a unit of their own in every row: equal logits, one above all, infinities, NaN, greedy rows and masked ones side by side."""
+    vocabulary = 2 ** 18 + 5
+    logits, draws, _ = logits_of(9, vocabulary, FP32, seed=13)
+    logits[0] = 2.5
+    logits[1, 77] = 1000.0
+    logits[2, 1000::5] = math.inf
+    logits[3, ::2] = math.nan
+    logits[4] = -math.inf
+    logits[5, 200000:] = -math.inf
+    logits[6] = math.nan
+    temperature = torch.tensor([1.0, 1.0, 0.7, 1.3, 1.0, 0.5, 1.0, 0.0, 1e30], device="cuda")
+    for options in ({}, {"top_k": 100000}, {"top_k": 30}, {"top_p": 0.7}, {"top_k": 5000, "top_p": 0.9, "min_p": 1e-4}):
+        assert torch.equal(wq.sample(logits, draws, temperature=temperature, **options).cpu(), defined(logits, draws, temperature=temperature, **options)), options

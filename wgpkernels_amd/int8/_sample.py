@@ -55,8 +55,9 @@ def sample(logits, draws, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     first, in the vocabulary's order, up to which the kept weights pass draws[row] (FP32, in [0, 1)) of their sum. A temperature of 0 (or below) takes
     the first largest logit. Each option is a number or a (rows,) tensor (FP32, top_k int32).
 
-    Weights are whole numbers of 2^-44 of the heaviest (vocabularies above 2^18: of 2^-38 at most), those below half of that 0: sums are exact, the same whatever order
-    they are taken in. NaN and -infinity are never drawn; infinities share all weight; a row with nothing else gives -1."""
+    Weights are held as whole numbers of units, so that their sums are the same whatever order they are taken in: 2^-44 of the heaviest, in vocabularies
+    above 2^18 2^-52 of it or less than 2^-60 of the sum. Those below half a unit are 0. Together a row's weights are off by at most 2^-27 of their sum, less than a
+    draw's last bit (2^-24). NaN and -infinity are never drawn; infinities share all weight; a row with nothing else gives -1."""
     key = (logits.shape, logits.stride(), logits.dtype, logits.get_device(), draws.shape, draws.stride(), draws.dtype, draws.get_device(), _kind(temperature),
            _kind(top_k), _kind(top_p), _kind(min_p))
     rows, vocabulary, ld, dtype, workspace_bytes = _layouts.get(key) or _layouts.keep(key, _check_sample(logits, draws, temperature, top_k, top_p, min_p))

@@ -1,27 +1,32 @@
 // A token of every row of logits by given random numbers, with temperature, top-k, top-p and min-p, on gfx950. No reference counterpart.
 //
-// A token's weight is exp((logit - largest) / temperature) in FP64, held as a whole number of 2^-44 (2^-shift): sums of weights are then the same
-// in whatever order they are taken, so a row may be spread over workgroups and added up by atomics, and the token drawn is that of the
-// 64-bit definition but for borders within 2^-44 of each other. Tokens stand in the order of (logit, lowest index first), a 64-bit key:
-// top-k and top-p each keep the keys down to a last one, `cut`.
+// A token's weight is exp((logit - largest) / temperature) in FP64, held as a whole number of units: sums of weights are then the same in whatever
+// order they are taken, so a row may be spread over workgroups and added up by atomics. A unit is 2^-44 of the heaviest weight in vocabularies of up
+// to 2^18 tokens, whose sums then fit 62 bits; above, a row's own (row_scale). Each weight is off by half a unit, all of a row's together by at most
+// 2^-27 of their sum (2^18 2^-45; above less than 2^-28): the token drawn is the 64-bit definition's wherever the draw, a number of 24 bits, is further from
+// a border between two tokens, or top-p's from one between two keys. Tokens stand in the order of (logit, lowest index first), a 64-bit key: top-k and top-p
+// each keep the keys down to a last one, `cut`.
 //
 // Four launches, a row over up to 64 workgroups in the first three: the largest logit; a histogram over (largest - logit) / temperature (of counts
 // for top-k, of weights for top-p); the keys of the histogram's bins in which the cuts lie, and the weights of what certainly stays; then a
 // workgroup a row finds the cut among those keys, and the token whose running weight, in vocabulary order, passes draw * (weight kept). A top-k of at most
-// SMALL_K lists all of its keys: then no weight is taken of the rest of the row.
+// SMALL_K lists all of its keys: then no weight is taken of the rest of the row. Vocabularies above 2^18 take a launch more, for their units.
 #include "wq8_common.h"
 #include "wq8_abi.h"
 
 namespace wq8 {
 
 constexpr int SAMPLE_BINS = 1024, SAMPLE_SPLITS = 64, SAMPLE_PARTS = 256, SAMPLE_LIST = 2048, MOST_LISTED_KEYS = 16384, SAMPLE_PIECE = 2048, SMALL_K = 1024, SHORT_LIST = 256;
-constexpr float BINS_PER_UNIT = 32.0f;  // the last bin begins at 31.97: weights below 2^-46, held as 0
+// The last bin begins at 31.97: weights below 2^-46, less than half of any unit. With units of a row's own, which are 2^-52 at least, at 37.9: below 2^-54.
+constexpr float BINS_PER_UNIT = 32.0f, LARGE_BINS_PER_UNIT = 27.0f;
+constexpr int UNIT_BITS = 44, MOST_UNIT_BITS = 52, UNIT_VOCABULARY_BITS = 18;  // 2^52: what FP64's sum with 2^52 holds
 
 struct SampleRow {  // a row's workspace
     uint64_t largest[SAMPLE_SPLITS];
     uint64_t kept[SAMPLE_PARTS];  // the weight kept of each part
     uint64_t mass[SAMPLE_BINS];
     uint32_t count[SAMPLE_BINS];
+    uint64_t weighed;  // of large vocabularies: the row's weights in parts of 2^-20, each rounded up
     uint32_t listed, unused;
 };
 
@@ -36,9 +41,9 @@ struct SampleArgs {
     SampleRow* rows;
     uint64_t* lists;   // `capacity` keys a row
     int64_t* tokens;
-    float temperature0, top_p0, min_p0;
+    float temperature0, top_p0, min_p0, bins_per_unit;
     int top_k0;
-    int vocabulary, capacity, bits, part, parts, split, splits, shift;  // indices have `bits`; parts of `part` tokens, splits of `split`, a multiple of that
+    int vocabulary, capacity, bits, part, parts, split, splits, shift;  // indices have `bits`; parts of `part` tokens, splits of `split`, a multiple of that; units of 2^-shift, 0: row_scale()
 };
 
 // The order of a logit: larger numbers for larger logits, 0 for NaN; both zeros alike.
@@ -59,8 +64,8 @@ template <int DT> struct Key {
     }
 };
 
-// 2^t for t <= 0, 0 below -72 (and for NaN): t = n + f, |f| <= 1/2, 2^f by the series of exp(f ln 2) up to its 12th power, whose rest is below 2^-52
-// of it. The sum with 1.5 2^52 holds n in its low bits, which are added to the exponent of 2^f.
+// 2^t for t <= 0, 0 below -72 (and for NaN): t = n + f, |f| <= 1/2, 2^f by the series of exp(f ln 2) up to its 12th power, whose rest is below 2^-51
+// of it (2.4e-16 at f = -1/2). The sum with 1.5 2^52 holds n in its low bits, which are added to the exponent of 2^f.
 WQ8_DEVICE double power_of_2(double t) {
     const double shifted = t + 0x1.8p52, f = t - (shifted - 0x1.8p52);
     // ln(2)^i / i!, i = 12 .. 0
@@ -95,7 +100,7 @@ struct Row {
     WQ8_DEVICE double weight(float l) const {
         return infinite ? l == top ? 1.0 : 0.0 : finite_weight(l);
     }
-    // the nearest whole number of w * scale <= 2^44, from the low bits of its sum with 2^52
+    // the nearest whole number of w * scale <= 2^52, from the low bits of its sum with 2^52
     WQ8_DEVICE uint64_t units(double w) const { return __builtin_bit_cast(uint64_t, __builtin_fma(w, scale, 0x1p52)) - 0x4330000000000000ull; }
     WQ8_DEVICE int bin(float l) const {
         if (l == top) return 0;
@@ -115,6 +120,15 @@ WQ8_DEVICE uint64_t wave_most(uint64_t v) {
     return over_wave(v, [](uint64_t a, uint64_t b) { return max64(a, b); });
 }
 
+// Units a weight of 1 of a row over a large vocabulary: as many as keep the row's sum below 2^62, the weights' rounding aside (an upper bound of the sum
+// is known), and 2^52 at most. All of a row's weights together are then off by less than 2^24 2^-53 of the heaviest, or by 2^23 units of less than 2^-60 of
+// their sum (sum < 2^(c - 20) < 2 (sum + 25) and sum > 2^8 there, a unit is 2^(c - 82)).
+WQ8_DEVICE double row_scale(uint64_t weighed) {
+    const int c = 64 - __builtin_clzll((weighed - 1) | 1);  // weighed <= 2^c
+    const int shift = min(MOST_UNIT_BITS, 82 - c);
+    return double(uint64_t(1) << shift);
+}
+
 WQ8_DEVICE Row read_row(const SampleArgs& p, const SampleRow& state, int row) {
     Row r;
     const int lane = threadIdx.x & 63;
@@ -128,8 +142,8 @@ WQ8_DEVICE Row read_row(const SampleArgs& p, const SampleRow& state, int row) {
     r.inverse = 0x1.71547652b82fep+0 / double(t);
     r.half = r.top >= 0x1p103f ? 0.5f : 1.0f;  // (2^103 above the lowest FP32: half a step past the largest)
     r.half_top = r.half * r.top;
-    r.bins = fminf(float(double(BINS_PER_UNIT / r.half) / double(t)), 0x1.fffffep127f);  // (an infinity would part equal logits from others beside them)
-    r.scale = double(uint64_t(1) << p.shift);
+    r.bins = fminf(float(double(p.bins_per_unit / r.half) / double(t)), 0x1.fffffep127f);  // (an infinity would part equal logits from others beside them)
+    r.scale = p.shift ? double(uint64_t(1) << p.shift) : row_scale(state.weighed);
     r.min_p = fmin(double(p.min_p ? p.min_p[row] : p.min_p0), 1.0);
     r.top_p = p.top_p ? p.top_p[row] : p.top_p0;
     r.top_k = p.top_k ? p.top_k[row] : p.top_k0;
@@ -179,7 +193,7 @@ template <int DT> __global__ void __launch_bounds__(256) sample_largest(SampleAr
     const int row = blockIdx.x / p.splits, s = blockIdx.x % p.splits;
     SampleRow& state = p.rows[row];
     for (int b = s * 256 + threadIdx.x; b < SAMPLE_BINS; b += 256 * p.splits) state.mass[b] = 0, state.count[b] = 0;
-    if (!s && !threadIdx.x) state.listed = 0;
+    if (!s && !threadIdx.x) state.listed = 0, state.weighed = 0;
     uint32_t most = 0;
     int at = 0;
     each_logit<DT>(p, row, s * p.split, min(p.vocabulary, (s + 1) * p.split), [&](float l, int i) {
@@ -191,6 +205,23 @@ template <int DT> __global__ void __launch_bounds__(256) sample_largest(SampleAr
     if (!(threadIdx.x & 63)) best4[threadIdx.x >> 6] = best;
     __syncthreads();
     if (!threadIdx.x) state.largest[s] = max64(max64(best4[0], best4[1]), max64(best4[2], best4[3]));
+}
+
+// ---- of large vocabularies: an upper bound of a row's weights ---------------------------------------------------------------------
+// Bound by the exponentials: 16 rows of 1000000 BF16 21 us, one of FP32 9.5.
+template <int DT> __global__ void __launch_bounds__(256) sample_weigh(SampleArgs p) {
+    const int row = blockIdx.x / p.splits, s = blockIdx.x % p.splits;
+    SampleRow& state = p.rows[row];
+    const Row r = read_row(p, state, row);  // (its scale is not known yet)
+    if (r.greedy || r.nothing) return;
+    const int begin = s * p.split, end = min(p.vocabulary, begin + p.split);
+    uint64_t sum = 0;
+    // (rounded, and one more: also for what weighs nothing, fewer than 2^25 of those)
+    auto add = [&](double w) { sum += __builtin_bit_cast(uint64_t, __builtin_fma(w, 0x1p20, 0x1p52 + 1.0)) - 0x4330000000000000ull; };
+    if (r.infinite) each_logit<DT>(p, row, begin, end, [&](float l, int) { add(l == r.top ? 1.0 : 0.0); });
+    else each_logit<DT>(p, row, begin, end, [&](float l, int) { add(r.finite_weight(l)); });
+    sum = sum64(sum);
+    if (!(threadIdx.x & 63)) atomicAdd(reinterpret_cast<unsigned long long*>(&state.weighed), (unsigned long long)sum);
 }
 
 // ---- 2: counts and weights over (largest - logit) / temperature ------------------------------------------------------------------
@@ -654,6 +685,8 @@ static int list_capacity(int rows) {
 template <int DT> static int launch_sample(const SampleArgs& p, int rows, hipStream_t stream) {
     sample_largest<DT><<<rows * p.splits, 256, 0, stream>>>(p);
     if (const int rc = int(hipGetLastError())) return rc;
+    if (!p.shift) sample_weigh<DT><<<rows * p.splits, 256, 0, stream>>>(p);
+    if (const int rc = int(hipGetLastError())) return rc;
     sample_bins<DT><<<rows * p.splits, 256, 0, stream>>>(p);
     if (const int rc = int(hipGetLastError())) return rc;
     sample_list<DT><<<rows * p.splits, 256, 0, stream>>>(p);
@@ -680,7 +713,8 @@ WQ8_API int wq8_sample(const void* logits, int64_t ld, int dtype, const float* d
     while ((1 << bits) < vocabulary) ++bits;
     const SampleArgs p{logits, ld, draws, temperature, static_cast<const int32_t*>(top_k), top_p, min_p, static_cast<SampleRow*>(workspace),
                        reinterpret_cast<uint64_t*>(static_cast<SampleRow*>(workspace) + rows), tokens,
-                       temperature0, top_p0, min_p0, top_k0, vocabulary, list_capacity(rows), bits, part, parts, split, splits, bits <= 18 ? 44 : 62 - bits};
+                       temperature0, top_p0, min_p0, bits <= UNIT_VOCABULARY_BITS ? BINS_PER_UNIT : LARGE_BINS_PER_UNIT, top_k0, vocabulary, list_capacity(rows),
+                       bits, part, parts, split, splits, bits <= UNIT_VOCABULARY_BITS ? UNIT_BITS : 0};
     if (dtype == DT_F16) return launch_sample<DT_F16>(p, rows, stream);
     if (dtype == DT_BF16) return launch_sample<DT_BF16>(p, rows, stream);
     return launch_sample<DT_F32>(p, rows, stream);
