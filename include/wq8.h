@@ -184,11 +184,14 @@ void wq8_experts_workspace(int tokens, int top, int k, int hidden, int64_t* size
 
 /* A token (int64) of every row of logits (rows, vocabulary), dtype 0-2, rows ld elements apart, any alignment; no counterpart in the
  * reference. draws (rows) f32 in [0, 1); temperature, top_k (int32), top_p and min_p per row, or null: then the value behind each for all
- * rows. -1 for a row without a logit above -infinity. vocabulary <= 2^24, rows <= 2^17; workspace: sizes[0] bytes, 16-byte aligned. */
+ * rows. -1 for a row without a logit above -infinity. vocabulary <= 2^24, rows <= 2^17; workspace: sizes[0] bytes of
+ * either query, 16-byte aligned; sizes[1] of the second one where top_k and top_p are null and cut nothing (top_k0 <= 0 or >= vocabulary, top_p0 >= 1).
+ * wq8_sample_workspace is for any vocabulary. */
 int wq8_sample(const void* logits, int64_t ld, int dtype, const float* draws, const float* temperature, float temperature0, const void* top_k, int top_k0,
                const float* top_p, float top_p0, const float* min_p, float min_p0, int rows, int vocabulary, int64_t* tokens, void* workspace,
                wq8_stream_t stream);
 void wq8_sample_workspace(int rows, int64_t* sizes);
+void wq8_sample_workspace_for(int rows, int vocabulary, int64_t* sizes);
 
 /* Cold-cache timing: reads `bytes` of a library-owned buffer on `stream` (nonzero if it cannot be allocated);
  * release frees it. Replace K8:1997-2016; bound at I:77-78. */

@@ -286,3 +286,43 @@ def test_rows_of_all_kinds_over_a_large_vocabulary(wq):
     temperature = torch.tensor([1.0, 1.0, 0.7, 1.3, 1.0, 0.5, 1.0, 0.0, 1e30], device="cuda")
     for options in ({}, {"top_k": 100000}, {"top_k": 30}, {"top_p": 0.7}, {"top_k": 5000, "top_p": 0.9, "min_p": 1e-4}):
         assert torch.equal(wq.sample(logits, draws, temperature=temperature, **options).cpu(), defined(logits, draws, temperature=temperature, **options)), options
+
+
+@pytest.mark.parametrize("rows,vocabulary", [(9001, 9000), (16384, 9000), (2 ** 17, 300)])
+@pytest.mark.parametrize("options", [{"top_k": 4000, "top_p": 0.7}, {"top_k": 700}, {"top_p": 0.9}, {"temperature": 0.0}])
+def test_many_rows(wq, rows, vocabulary, options):
+    """The most rows, and so many that lists of keys are shorter than a row's own: one flat row for all draws, of which every key lies in the cuts' bins."""
+    print(f"rows {rows} {vocabulary} {options}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    row = torch.rand(1, vocabulary, generator=g, device="cuda") * 0.01
+    draws = torch.rand(rows, generator=g, device="cuda")
+    tokens = wq.sample(row.expand(rows, vocabulary), draws, **options).cpu()
+    order = torch.sort(row[0].cpu(), descending=True, stable=True).indices
+    if options.get("temperature") == 0.0:
+        assert (tokens == order[0]).all()
+        return
+    weight = torch.round(torch.exp((row[0] - row.max()).cpu().double()) * 2.0 ** 44).long()
+    kept = weight[order]
+    kept[min(options.get("top_k", vocabulary), vocabulary):] = 0
+    mass = torch.cumsum(kept, 0)
+    if "top_p" in options:
+        kept[mass - kept >= math.ceil(Fraction(torch.tensor(options["top_p"]).item()) * mass[-1].item())] = 0
+    left = torch.zeros_like(weight)
+    left[order] = kept
+    upto = torch.cumsum(left, 0)
+    total = upto[-1].item()
+    targets = torch.tensor([math.floor(Fraction(u) * total) for u in draws.tolist()])
+    assert torch.equal(tokens, torch.searchsorted(upto, targets, right=True))
+
+
+def test_memory_of_a_call(wq):
+    """1024 rows over 300 tokens: 15 KB a row and 8 bytes a token, with nothing cut the first only."""
+    logits, draws, _ = logits_of(1024, 300, BF16, seed=14)
+    for options, most in (({"top_k": 40}, 1024 * (16384 + 8 * 300)), ({"top_p": torch.full((1024,), 0.9, device="cuda")}, 1024 * (16384 + 8 * 300)), ({}, 1024 * 16384),
+                          ({"temperature": 0.0, "top_k": 300}, 1024 * 16384)):
+        want = defined(logits[:64], draws[:64], **{name: option[:64] if isinstance(option, torch.Tensor) else option for name, option in options.items()})
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        tokens = wq.sample(logits, draws, **options)
+        assert torch.cuda.max_memory_allocated() - before <= most + 1024 * 8 + 2 ** 20
+        assert torch.equal(tokens[:64].cpu(), want)

@@ -235,3 +235,19 @@ def test_numbers_of_top_k_beyond_32_bits(monkeypatch, given, kept):
     assert name == "wq8_sample" and args[6] is None
     top_k = ctypes.c_int(args[7]).value
     assert (top_k if 0 < top_k < 9 else 9) == kept
+
+
+def test_workspace_of_a_sample():
+    """A row's state, and a list of keys that is no longer than the vocabulary; never more than the query for any vocabulary says."""
+    import ctypes
+    lib, sizes, most = wq.library(), (ctypes.c_int64 * 2)(), (ctypes.c_int64 * 2)()
+    lib.wq8_sample_workspace_for(1, 1, sizes)
+    state = sizes[1]
+    assert 14000 < state < 16384 and state % 16 == 0
+    for rows, vocabulary, keys in ((1, 131072, 16384), (1024, 300, 300), (8192, 20000, 16384), (16384, 20000, 8192), (16384, 5000, 5000), (2 ** 17, 300, 300), (2 ** 17, 2 ** 24, 2048)):
+        lib.wq8_sample_workspace_for(rows, vocabulary, sizes)
+        lib.wq8_sample_workspace(rows, most)
+        assert list(sizes) == [rows * (state + 8 * keys), rows * state] and sizes[0] <= most[0]
+    for rows, vocabulary in ((0, 100), (-1, 100), (5, 0)):
+        lib.wq8_sample_workspace_for(rows, vocabulary, sizes)
+        assert list(sizes) == [0, 0]

@@ -52,13 +52,15 @@ SIGNATURES = {
     "wq8_experts_workspace": ("-", "iiii" "p"),
     "wq8_sample": ("i", "pli" "p" "pfpipfpf" "ii" "pp" "p"),
     "wq8_sample_workspace": ("-", "i" "p"),
+    "wq8_sample_workspace_for": ("-", "ii" "p"),
     "wq8_l2_flush": ("i", "il" "p"),
     "wq8_l2_flush_release": ("-", ""),
 }
 # entry points an older or foreign build may lack: bound when present (segments_supported() reports the first)
 OPTIONAL = {"wq8_gemm_segments", "wq8_gemm_noalloc", "wq8_quantize_at", "wq8_quantize_blocks_at", "wq8_gemm_at", "wq8_gemv_line_act",
             "wq8_add_prepare", "wq8_prepared_values", "wq8_rotary", "wq8_kv_plan", "wq8_kv_write", "wq8_kv_read", "wq8_kv_attention", "wq8_kv_attention_workspace",
-            "wq8_route", "wq8_route_workspace", "wq8_experts", "wq8_experts_workspace", "wq8_sample", "wq8_sample_workspace"}
+            "wq8_route", "wq8_route_workspace", "wq8_experts", "wq8_experts_workspace", "wq8_sample", "wq8_sample_workspace",
+            "wq8_sample_workspace_for"}
 # the test library's entry points (include/wq8_test.h; libwgp_int8_test.so, not part of the product library)
 TEST_SIGNATURES = {
     "wq8_debug_block_sums": ("i", "ppp" "iii" "i" "p"),

@@ -16,7 +16,7 @@ _layouts = Layouts()
 
 
 def _check_sample(logits, draws, temperature, top_k, top_p, min_p):
-    """(rows, vocabulary, row pitch, dtype, workspace bytes, what of the options is a tensor)"""
+    """(rows, vocabulary, row pitch, dtype, workspace bytes, and those of a call that cuts nothing)"""
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1) or logits.dtype not in DTYPES:
         raise ValueError("logits must be (rows, vocabulary) FP16, BF16 or FP32 with unit column stride")
     rows, vocabulary = logits.shape
@@ -33,8 +33,8 @@ def _check_sample(logits, draws, temperature, top_k, top_p, min_p):
             tensors.append(t)
     _check_devices(logits, draws, *tensors)
     sizes = (ctypes.c_int64 * 2)()
-    library().wq8_sample_workspace(rows, sizes)
-    return rows, vocabulary, logits.stride(0) if rows > 1 else vocabulary, DTYPES[logits.dtype], sizes[0]
+    library().wq8_sample_workspace_for(rows, vocabulary, sizes)
+    return rows, vocabulary, logits.stride(0) if rows > 1 else vocabulary, DTYPES[logits.dtype], sizes[0], sizes[1]
 
 
 def _kind(option):
@@ -60,9 +60,10 @@ def sample(logits, draws, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     draw's last bit (2^-24). NaN and -infinity are never drawn; infinities share all weight; a row with nothing else gives -1."""
     key = (logits.shape, logits.stride(), logits.dtype, logits.get_device(), draws.shape, draws.stride(), draws.dtype, draws.get_device(), _kind(temperature),
            _kind(top_k), _kind(top_p), _kind(min_p))
-    rows, vocabulary, ld, dtype, workspace_bytes = _layouts.get(key) or _layouts.keep(key, _check_sample(logits, draws, temperature, top_k, top_p, min_p))
+    rows, vocabulary, ld, dtype, workspace_bytes, least_bytes = _layouts.get(key) or _layouts.keep(key, _check_sample(logits, draws, temperature, top_k, top_p, min_p))
+    cuts = isinstance(top_k, torch.Tensor) or isinstance(top_p, torch.Tensor) or 0 < top_k < vocabulary or not top_p >= 1
     tokens = draws.new_empty(rows, dtype=torch.int64)
-    workspace = draws.new_empty(workspace_bytes, dtype=torch.uint8)
+    workspace = draws.new_empty(workspace_bytes if cuts else least_bytes, dtype=torch.uint8)
     state = _native.gpu(logits)
     if not isinstance(top_k, torch.Tensor):
         top_k = max(0, min(top_k, MAX_VOCABULARY))  # the C interface has 32 bits

@@ -676,10 +676,11 @@ template <int DT> __global__ void __launch_bounds__(256) sample_pick(SampleArgs 
 
 using namespace wq8;
 
-// Keys listed a row: as many as LDS holds, and more of few rows (1 GiB of lists in all)
-static int list_capacity(int rows) {
+// Keys listed a row: as many as LDS holds, and more of few rows (1 GiB of lists in all, 2 GiB for 2^17 rows), but no more than there are tokens
+static int list_capacity(int rows, int vocabulary) {
     const int64_t fit = (int64_t(1) << 27) / (rows > 0 ? rows : 1);
-    return int(fit < SAMPLE_LIST ? SAMPLE_LIST : fit > MOST_LISTED_KEYS ? MOST_LISTED_KEYS : fit);
+    const int most = int(fit < SAMPLE_LIST ? SAMPLE_LIST : fit > MOST_LISTED_KEYS ? MOST_LISTED_KEYS : fit);
+    return most < vocabulary ? most : vocabulary;
 }
 
 template <int DT> static int launch_sample(const SampleArgs& p, int rows, hipStream_t stream) {
@@ -713,7 +714,8 @@ WQ8_API int wq8_sample(const void* logits, int64_t ld, int dtype, const float* d
     while ((1 << bits) < vocabulary) ++bits;
     const SampleArgs p{logits, ld, draws, temperature, static_cast<const int32_t*>(top_k), top_p, min_p, static_cast<SampleRow*>(workspace),
                        reinterpret_cast<uint64_t*>(static_cast<SampleRow*>(workspace) + rows), tokens,
-                       temperature0, top_p0, min_p0, bits <= UNIT_VOCABULARY_BITS ? BINS_PER_UNIT : LARGE_BINS_PER_UNIT, top_k0, vocabulary, list_capacity(rows),
+                       temperature0, top_p0, min_p0, bits <= UNIT_VOCABULARY_BITS ? BINS_PER_UNIT : LARGE_BINS_PER_UNIT, top_k0, vocabulary,
+                       list_capacity(rows, vocabulary),
                        bits, part, parts, split, splits, bits <= UNIT_VOCABULARY_BITS ? UNIT_BITS : 0};
     if (dtype == DT_F16) return launch_sample<DT_F16>(p, rows, stream);
     if (dtype == DT_BF16) return launch_sample<DT_BF16>(p, rows, stream);
@@ -721,6 +723,11 @@ WQ8_API int wq8_sample(const void* logits, int64_t ld, int dtype, const float* d
 }
 
 WQ8_API void wq8_sample_workspace(int rows, int64_t* sizes) {
-    sizes[0] = int64_t(rows) * (int64_t(sizeof(SampleRow)) + int64_t(list_capacity(rows)) * 8);
+    sizes[0] = int64_t(rows) * (int64_t(sizeof(SampleRow)) + int64_t(list_capacity(rows, 1 << 24)) * 8);
     sizes[1] = 0;
+}
+
+WQ8_API void wq8_sample_workspace_for(int rows, int vocabulary, int64_t* sizes) {
+    sizes[1] = rows > 0 && vocabulary > 0 ? int64_t(rows) * int64_t(sizeof(SampleRow)) : 0;
+    sizes[0] = sizes[1] ? sizes[1] + int64_t(rows) * list_capacity(rows, vocabulary) * 8 : 0;
 }
