@@ -172,3 +172,26 @@ def test_into_linear_prepared(wq):
     for path in ("block", "exact", "row"):
         prepared, total = wq.add_prepare(x, residual, scale, path=path, act_weight=weight, eps=1e-6)
         assert same(wq.linear_prepared(prepared, w, s), wq.linear(total, w, s, mode=path, act="rms_norm", act_weight=weight, eps=1e-6))
+
+
+@pytest.mark.parametrize("path", ["block", "exact", "row", "small"])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("m,k,group", [(7, 1024, 0), (7, 2056, 0), (7, 4096, 256), (7, 8200, 0), (600, 4104, 0), (7, 16392, 0)])
+def test_rows_of_infinities_and_nan_as_prepare_has_them(wq, path, dtype, m, k, group):
+    """Codes, remainders and scales of rows with NaN, one or two infinities, or nothing but zeros are prepare()'s of the sum too (NaN of any
+    payload alike)."""
+    print(f"not finite {path} {dtype} {m} {k} {group}", flush=True)
+    x, residual, scale, weight = inputs(m, k, dtype, seed=k)
+    x[1, 5], residual[2, k - 1] = float("nan"), float("inf")
+    residual[3, 0], residual[3, k // 2] = float("inf"), float("-inf")
+    x[4] = residual[4] = 0
+    residual[5] = float("nan")
+    residual[6] = torch.finfo(dtype).max
+    prepared, total = wq.add_prepare(x, residual, scale, group=group, path=path, act_weight=weight, eps=1e-6)
+    other = wq.prepare(total, group, path, "rms_norm", weight, 1e-6)
+    for a, b in ((prepared.x, other.x), (prepared.lo, other.lo), (prepared.scale, other.scale)):
+        assert (a is None) == (b is None)
+        if a is not None and a.is_floating_point():
+            assert torch.equal(a.isnan(), b.isnan())
+            a, b = (torch.where(t.isnan(), torch.zeros_like(t), t) for t in (a, b))
+        assert a is None or same(a, b)

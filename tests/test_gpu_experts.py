@@ -289,3 +289,19 @@ def test_whole_layer_captured(wq):
         other = step()
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(other, got)
+
+
+def test_most_tokens_of_a_route(wq):
+    """As many tokens as a route takes: rows at both ends and between them against the definition, all of them one expert each or more."""
+    tokens = 65535 * 16
+    g = generator(13)
+    x = torch.randn(tokens, 16, generator=g, device="cuda").to(BF16)
+    router = torch.randn(20, 16, generator=g, device="cuda").to(BF16)
+    ids, weights = wq.route(x, router, 3)
+    for at in (0, 1, 4000, 500_001, tokens - 33):
+        want_ids, want = routed(x[at:at + 33], router, 3)
+        assert torch.equal(ids[at:at + 33].cpu(), want_ids)
+        assert ((weights[at:at + 33].cpu().double() - want).abs() <= want * (2.0 ** -24 + 2.0 ** -40)).all()
+    assert ((ids >= 0) & (ids < 20)).all()
+    with pytest.raises(ValueError):
+        wq.route(torch.cat([x, x[:1]]), router, 3)
