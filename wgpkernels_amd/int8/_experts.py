@@ -4,7 +4,7 @@
     y = experts(x, routes, gate_up, gate_up_scales, down, down_scales, residual=stream, out=stream)
 
 The experts' weights are the checkpoint's INT8 matrices with FP32 scales per channel, stacked; they are used as stored, and each chosen
-expert's are read once for all of its tokens. Neither call reads anything on the host: a decode step with such layers can be captured.
+expert's are read once for up to 64 of its tokens. Activations are not rotated: weights of a ConvRot checkpoint are not what it takes. Neither call reads anything on the host: a decode step with such layers can be captured.
 """
 import ctypes
 from typing import NamedTuple

@@ -53,7 +53,7 @@ def sample(logits, draws, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     the vocabulary's size and above: all); of these top_p the fewest, heaviest first, whose weights reach top_p of their sum (1: all; always at least
     one); of these min_p those of at least min_p of the heaviest's weight. Equal logits go by the lowest index. The token drawn is the
     first, in the vocabulary's order, up to which the kept weights pass draws[row] (FP32, in [0, 1)) of their sum. A temperature of 0 (or below) takes
-    the first largest logit. Each option is a number or a (rows,) tensor (FP32, top_k int32).
+    the first largest logit. Each option is a number, held in FP32, or a (rows,) tensor (FP32, top_k int32).
 
     Weights are held as whole numbers of units, so that their sums are the same whatever order they are taken in: 2^-44 of the heaviest, in vocabularies
     above 2^18 2^-52 of it or less than 2^-60 of the sum. Those below half a unit are 0. Together a row's weights are off by at most 2^-27 of their sum, less than a

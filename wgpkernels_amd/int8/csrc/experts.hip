@@ -1,7 +1,8 @@
 // A mixture-of-experts layer of INT8 weights for a few tokens on gfx950: the router (its product in 64 bits, and its choice) and the chosen
 // experts' gated feed-forward blocks,
 //     y[t] = residual[t] + rscale * sum_j weights[t, j] * down_e(silu(gate_e(x[t])) * up_e(x[t])),   e = ids[t, j],
-// every chosen expert's weights read once from HBM for all of its tokens. No reference counterpart.
+// a chosen expert's weights read from memory once for up to 64 of its tokens (once for 8 choices in the form for the fewest tokens). No reference
+// counterpart. Times below are with the weights in the Infinity Cache where they fit it; cold ones are of copies of the weights taken in turn.
 #include "gemm_common.h"
 #include "wq8_abi.h"
 
@@ -268,7 +269,7 @@ WQ8_DEVICE int find_choices(const ExpertsArgs& p, int slot, int expert, int firs
 // Two tiles of 16 weight rows on up to CAP tokens (PLANES rows each). The four waves of a workgroup take slices of SLICE values of the width in
 // turn, each through a ring of its own in LDS, filled by copies that pass the registers by: no wave waits for another one until the
 // end, where the four sums of every output are added in order. HBM bounds it, and at these sizes the latency of a workgroup's beginning: one token, 8 of 64 experts of
-// 2048 x 1024, gate and up 9.2 us for 33.6 MB (3.6 TB/s). 16-byte chunks are placed by their row so that the 16 lanes that read one chunk of
+// 2048 x 1024, gate and up 9.9 us for 33.6 MB (3.4 TB/s; cold 11.1). 16-byte chunks are placed by their row so that the 16 lanes that read one chunk of
 // 16 rows meet different banks.
 constexpr int RING = 19 * 1024;  // a wave's: two workgroups a CU
 constexpr uint32_t OUT_OF_RANGE = 0x80000000u;
@@ -347,7 +348,7 @@ WQ8_DEVICE void ring_rows(sgpr4 rw, int row0, int row1, int width, sgpr4 rx, uin
 }
 
 // More tokens or tiles: 128 rows a workgroup, two runs of 64 of which each wave has a tile of 16, and the tokens' slices in LDS once for all of them. HBM: 32
-// tokens, 8 of 128 experts of 2048 x 768 (78 chosen, up to 11 tokens each), gate and up 47 us for 245 MB (5.2 TB/s), down 30 for 123 MB (4.1 TB/s: short rows); 25
+// tokens, 8 of 128 experts of 2048 x 768 (78 chosen, up to 11 tokens each), gate and up 47 us for 245 MB (5.2 TB/s; cold 50), down 30 for 123 MB (4.1 TB/s: short rows; cold 31); 25
 // tokens on each of 16 experts of 5120 x 1536 58 and 48 (4.3 and 2.6 TB/s: copies of tokens beside the codes').
 // done(m, values of both tiles): element i is row 16 wave + 4 (lane / 16) + i of each run, token 16 m + lane % 16.
 template <int DT, int SLICE, int MT, int PLANES, typename Source, typename Done>
@@ -549,7 +550,7 @@ template <int DT> WQ8_DEVICE float with_residual(const ExpertsArgs& p, int t, in
     return __builtin_fmaf(v, scale, Elem<DT>::to_f(static_cast<const raw*>(p.residual)[t * p.ldr + n]));
 }
 
-// A token's parts, weighted and added in the order of its choices: 4.8 us for 32 tokens x 8 x 2048, the length of its loads' chain.
+// A token's parts, weighted and added in the order of its choices: 5.0 us for 32 tokens x 8 x 2048, the length of its loads' chain.
 template <int DT>
 __global__ void __launch_bounds__(256) experts_join(ExpertsArgs p) {
     using raw = typename Elem<DT>::raw;
@@ -583,8 +584,8 @@ WQ8_DEVICE void wave_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// One token: the second product and the sum over its choices in one launch (8 of 64 experts of 2048 x 1024: 6.0 us for 16.8 MB; by ring_rows and
-// experts_join 6.8 + 4.8). A workgroup has 8 output channels, a wave every eighth choice of the
+// One token: the second product and the sum over its choices in one launch (8 of 64 experts of 2048 x 1024: 6.6 us for 16.8 MB, cold 7.1; by
+// ring_rows and experts_join 6.8 + 4.8). A workgroup has 8 output channels, a wave every eighth choice of the
 // token: 8 rows of 128 neighbouring bytes a load, 8 loads ahead, so that an expert's 8 x 1024 codes are asked for at once. One token leaves nothing
 // to share, and 16 rows of a matrix instruction would leave half the CUs idle: the products are FP32 on the vector unit, hidden values as FP32.
 template <int DT>

@@ -16,7 +16,15 @@
 
 namespace wq8 {
 
-constexpr int SAMPLE_BINS = 1024, SAMPLE_SPLITS = 64, SAMPLE_PARTS = 256, SAMPLE_LIST = 2048, MOST_LISTED_KEYS = 16384, SAMPLE_PIECE = 2048, SMALL_K = 1024, SHORT_LIST = 256;
+constexpr int SAMPLE_BINS = 1024, SAMPLE_SPLITS = 64, SAMPLE_PARTS = 256, SAMPLE_LIST = 2048, SAMPLE_PIECE = 2048, SHORT_LIST = 256;
+// Keys listed in memory, all of sample over 8 rows of 262144 BF16, top-p 0.95 at temperature 1.5: 69 us with 16384 of them or 131072, 739 with 2048 (the row is
+// read again); 64 flat rows of 131072 FP32, top-k 30000: 111 and 550 (2048); where 16384 are too few too, 4 flatter rows: 571, and 963 with 131072, which one
+// workgroup goes through in memory.
+constexpr int MOST_LISTED_KEYS = 16384;
+// A small top-k takes no weight of what it leaves out but orders all of its keys in one workgroup. All of sample, us, (small, as a large one) for top-k 50,
+// 200, 512, 1000 and top-p 0.9: 64 rows of 131072 BF16 30, 55; 34, 56; 46, 57; 58, 60. 32 rows: 27, 41; 31, 42; 41, 43; 49, 45. One of FP32: 21, 27; 25, 27; 34, 28;
+// 41, 29: the border is that of many rows, few would have it at 256.
+constexpr int SMALL_K = 1024;
 // The last bin begins at 31.97: weights below 2^-46, less than half of any unit. With units of a row's own, which are 2^-52 at least, at 37.9: below 2^-54.
 constexpr float BINS_PER_UNIT = 32.0f, LARGE_BINS_PER_UNIT = 27.0f;
 constexpr int UNIT_BITS = 44, MOST_UNIT_BITS = 52, UNIT_VOCABULARY_BITS = 18;  // 2^52: what FP64's sum with 2^52 holds
@@ -187,7 +195,7 @@ template <int DT, typename F> WQ8_DEVICE void each_logit(const SampleArgs& p, in
 }
 
 // ---- 1: the largest logit of every part of a row -----------------------------------------------------------------------------
-// HBM and the launch: 64 rows of 131072 BF16 6 us (2.7 TB/s), one row of FP32 3.1.
+// HBM and the launch: 64 rows of 131072 BF16 5.8 us (2.9 TB/s), one row of FP32 3.3.
 template <int DT> __global__ void __launch_bounds__(256) sample_largest(SampleArgs p) {
     __shared__ uint64_t best4[4];
     const int row = blockIdx.x / p.splits, s = blockIdx.x % p.splits;
@@ -225,7 +233,7 @@ template <int DT> __global__ void __launch_bounds__(256) sample_weigh(SampleArgs
 }
 
 // ---- 2: counts and weights over (largest - logit) / temperature ------------------------------------------------------------------
-// Bound by the additions in LDS and the exponentials: the same 64 rows, of options of their own, 12 us; one row 4.7.
+// Bound by the additions in LDS and the exponentials: the same 64 rows, of options of their own, 11 us; one row 4.8.
 template <int DT> __global__ void __launch_bounds__(256) sample_bins(SampleArgs p) {
     __shared__ unsigned long long mass[SAMPLE_BINS];
     __shared__ uint32_t count[SAMPLE_BINS];
@@ -380,7 +388,7 @@ WQ8_DEVICE Cut find_cut(const Row& r, const SampleRow& state, CutScratch& sc) {
 }
 
 // ---- 3: the keys of those bins, and the weights that certainly stay ------------------------------------------------------------
-// Bound by the exponentials (45 instructions a value, most of them FP64): 200 rows of 50001 FP16 17 us, the 64 rows 21; one row 5.6.
+// Bound by the exponentials (45 instructions a value, most of them FP64): 200 rows of 50001 FP16 17 us, the 64 rows 21; one row 5.7.
 template <int DT> __global__ void __launch_bounds__(256) sample_list(SampleArgs p) {
     __shared__ CutScratch scratch;
     __shared__ unsigned long long kept[SAMPLE_PARTS];
